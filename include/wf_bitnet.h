@@ -190,6 +190,29 @@ int wf_rope_kv_append(const void* qkv, int B, int H, const wf_kv_layout* kv, int
                       const int32_t* block_table, int max_blocks, const void* cos_tab, const void* sin_tab,
                       int max_pos, void* q_out, void* stream);
 
+/* Block tables and slot maps of a step, on the GPU: the free list of KVCacheManager (tests/test_kv_cache_cpp.py:44-70; pages come off the end of the list) as a
+ * stack in device memory, free_pages[0 .. *free_count) of pool_pages entries.  Request r (of rows <= 8192) has seq_lens[r] cached tokens, whose pages stand in
+ * block_table[r][0 .. ceil(seq_lens[r] / page_size)), and new_lens[r] >= 0 new ones.  The pages that it still needs are taken off the stack, request after
+ * request and block after block, and written to its row of block_table (the other entries stay).  For every new token t, requests one after another:
+ * token_rows[t], positions[t] (in its sequence), pages[t] and slots[t] (what wf_kv_scatter takes); entries from the last token up to max_tokens: -1, 0, -1, 0.
+ * offsets[rows + 1]: first token of each request and their number; lens_out = seq_lens + new_lens; free_count_out = *free_count - pages taken.  Nothing of the
+ * free list is written: a program goes on with free_count_out and lens_out.  status (one word): 0, or why the step cannot be planned as a whole (WF_PLAN_*
+ * bits); then nothing is: no token has a page, offsets are 0, lens_out = seq_lens, free_count_out = *free_count and block_table is as it was.
+ * page_size is any; the four token maps are 16-byte aligned; outputs overlap neither one another nor the inputs. */
+#define WF_PLAN_PAGES 1  /* more pages needed than there are */
+#define WF_PLAN_TOKENS 2 /* more than max_tokens new tokens */
+#define WF_PLAN_BLOCKS 4 /* a request needs more than max_blocks pages */
+#define WF_PLAN_LENGTH 8 /* a length is negative, or their sum beyond 2^31 - 1 */
+#define WF_PLAN_COUNT 16 /* *free_count is negative or beyond pool_pages */
+int wf_paged_plan(const int32_t* seq_lens, const int32_t* new_lens, int rows, int32_t* block_table, int max_blocks, const int32_t* free_pages, int pool_pages,
+                  const int32_t* free_count, int page_size, int max_tokens, int32_t* positions, int32_t* token_rows, int32_t* pages, int32_t* slots, int32_t* offsets,
+                  int32_t* lens_out, int32_t* free_count_out, int32_t* status, void* stream);
+/* The way back: the requests with done[r] != 0 hand their ceil(seq_lens[r] / page_size) pages back, request after request and block after block, on top of the
+ * stack (free_pages[*free_count ..]).  lens_out: 0 for them, seq_lens[r] for the others; free_count_out = *free_count + pages handed back.  Where the stack
+ * would not hold them, or a length or the count is out of range, nothing is done and lens_out and free_count_out are the inputs. */
+int wf_paged_release(const uint8_t* done, const int32_t* seq_lens, int rows, const int32_t* block_table, int max_blocks, int32_t* free_pages, int pool_pages,
+                     const int32_t* free_count, int page_size, int32_t* lens_out, int32_t* free_count_out, void* stream);
+
 /* attention_with_kv_cache (src/wrinklefree_inference/kv_cache/kv_cache.py:316-369) in its GQA form
  * (scripts/direct_inference_full.py:229-244): out[b,h,:] = softmax(q[b,h]·K[b,kvh]^T * scale) V[b,kvh]
  * over tokens [0, seq_lens[b]).  q bf16 [B,H,D]; out bf16 [B,H,D] (or f32).  Split-KV flash decode;
@@ -198,6 +221,14 @@ size_t wf_attn_workspace_bytes(int B, int H, int head_dim, int max_seq);
 int wf_paged_decode_attn(const void* q, const wf_kv_layout* kv, int layer, const int32_t* block_table,
                          int max_blocks, const int32_t* seq_lens, int B, int H, float scale, void* out,
                          int out_dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The same for a batch that shares a prefix: every sequence's keys are the first prefix_len tokens of the pages in prefix_table (ceil(prefix_len / page_size)
+ * entries), read once for all, and then its own seq_lens[b] tokens as above (block_table and seq_lens name the own tokens only; slots count from 0 again).
+ * prefix_len or max_blocks may be 0, seq_lens[b] too; a sequence without any key gets zeros.  q, out, the pool and the workspace are 16-byte aligned.  The workspace is
+ * free to be used again as soon as the stream has passed the call. */
+size_t wf_prefix_attn_workspace_bytes(int B, int H, int kv_heads, int head_dim, int max_seq, int prefix_len);
+int wf_paged_prefix_attn(const void* q, const wf_kv_layout* kv, int layer, const int32_t* prefix_table, int prefix_len, const int32_t* block_table, int max_blocks,
+                         const int32_t* seq_lens, int B, int H, float scale, void* out, int out_dtype, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- glue around the linears -------------------------------------------- */
 
@@ -216,6 +247,14 @@ int wf_embed(const void* table, const int32_t* tokens, int B, int H, void* out, 
 size_t wf_lm_head_workspace_bytes(int B, int V);
 int wf_lm_head_argmax(const void* h, const void* E, int B, int V, int K, float* logits_out, int32_t* next_out,
                       void* workspace, size_t workspace_bytes, void* stream);
+
+/* Log probabilities from logits [rows, vocab] (dtype WF_F32 / WF_BF16 / WF_F16, rows row_stride elements apart), z = logits / temperature, temperature > 0:
+ * logprob[r] = log softmax(z_r)[tokens[r]], entropy[r] = -sum p ln p (nats, in float whatever the dtype), and the `top` (0..64, at most vocab) largest logits of
+ * each row, largest first, equal ones by index: top_id, top_logprob [rows, top].  Logits of -inf have probability 0.  A row with nothing above -inf: logprobs
+ * -inf, entropy 0.  A row with +inf or NaN: all its floats NaN, NaN is no alternative (top_id -1 where the row has too few others).  A token outside
+ * [0, vocab): logprob NaN.  One launch, no workspace. */
+int wf_token_logprobs(const void* logits, int dtype, int rows, int vocab, long long row_stride, const int32_t* tokens, int top, float temperature, float* logprob,
+                      float* entropy, float* top_logprob, int32_t* top_id, void* stream);
 
 /* ---- decode engine (the whole step of scripts/direct_inference_full.py:267-302) --- */
 

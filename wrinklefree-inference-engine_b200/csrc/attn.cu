@@ -17,6 +17,7 @@
 //   exp2, O += P V.  Warps are merged through shared memory; chunks are merged by a second tiny kernel.
 #include <cuda_fp16.h>
 
+#include "attn_chunks.cuh"
 #include "fused_common.cuh"
 
 namespace wf {
@@ -24,8 +25,6 @@ namespace wf {
 constexpr int AT_WARPS = 4;
 constexpr int AT_EVEN_MAXB = 128;   // even work split (fused decode form): the per-sequence block counts are scanned by one CTA-wide pass
 constexpr int AT_STAGES = 3;
-constexpr int AT_BLK = 16;                              // tokens per stage
-constexpr int AT_D = 128;                               // head_dim (all supported shapes)
 constexpr int AT_ROW = AT_D * 2;                        // bytes per token row
 constexpr int AT_STAGE_BYTES = 2 * AT_BLK * AT_ROW;     // K + V
 constexpr int AT_SMEM = AT_WARPS * AT_STAGES * AT_STAGE_BYTES;   // 96 KB
@@ -157,17 +156,6 @@ __device__ __forceinline__ size_t kv_block_offset(int page, int layers, int laye
 
 __device__ __forceinline__ size_t kv_scale_offset(int page, int layers, int layer, int kv, int Hkv, int head, int page_size) {
     return ((((size_t)page * layers + layer) * 2 + kv) * Hkv + head) * (size_t)page_size;
-}
-
-// Blocks per chunk of a sequence with `nblocks` 16-token blocks.  The host sizes chunk_blocks from the length HINT of the captured graph
-// (a power of two >= the longest sequence); a sequence well below the hint would fill only the first chunks (2049 tokens under a 4096
-// hint: chunks of 128 + 1 blocks) — so every (sequence, kv head) pair cuts its own length evenly.  Same value in every CTA of the pair
-// and in the merge kernel (it depends on seq_lens only).
-__device__ __forceinline__ int chunk_blocks_of(int nblocks, int chunk_blocks, int max_chunks, int min_cb) {
-    if (min_cb <= 0 || max_chunks <= 1) return chunk_blocks;
-    int c = ((max(nblocks, 1) + max_chunks - 1) / max_chunks + 3) & ~3;
-    c = max(c, min_cb);
-    return min(c, chunk_blocks);
 }
 
 template <bool FUSED, bool I8>
@@ -979,7 +967,7 @@ int launch_rope_kv_append(const RopeParams& p, cudaStream_t s, bool pdl) {
 }
 
 // picks the chunking, launches attention (+ merge when sequences span several chunks)
-int launch_paged_decode_attn(AttnParams p, int max_seq_hint, void* workspace, size_t workspace_bytes, cudaStream_t s, bool pdl) {
+int launch_paged_decode_attn(AttnParams p, int max_seq_hint, void* workspace, size_t workspace_bytes, cudaStream_t s, bool pdl, AttnChunks* unmerged = nullptr) {
     static DevOnce attr;
     if (attr.need()) {
         if (cuda_check(cudaFuncSetAttribute(paged_decode_attn_kernel<false, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, AT_SMEM), "attn smem")) return WF_ERR_CUDA;
@@ -1074,7 +1062,7 @@ int launch_paged_decode_attn(AttnParams p, int max_seq_hint, void* workspace, si
     p.max_chunks = nchunks;
     p.page_shift = -1;
     if ((p.page_size & (p.page_size - 1)) == 0) { p.page_shift = 0; while ((1 << p.page_shift) < p.page_size) ++p.page_shift; }
-    p.direct = (nchunks <= 1);
+    p.direct = nchunks <= 1 && !unmerged;
     // Even work split (see the kernel): the fused decode form with at least 512 tokens of KV per CTA of one resident wave.
     const bool fused_form = p.qkv_acc != nullptr && p.merge_cnt != nullptr;
     const bool i8_pool = p.kv_scales != nullptr;
@@ -1155,7 +1143,9 @@ int launch_paged_decode_attn(AttnParams p, int max_seq_hint, void* workspace, si
         if (launch_check(le, "paged_decode_attn")) return WF_ERR_CUDA;
         if (fused) return WF_OK;
     }
-    if (!p.direct) {
+    if (unmerged) {
+        *unmerged = AttnChunks{p.part_o, p.part_ml, p.max_chunks, p.chunk_blocks, p.min_cb};
+    } else if (!p.direct) {
         MergeParams mp;
         mp.part_o = p.part_o; mp.part_ml = p.part_ml; mp.seq_lens = p.seq_lens;
         mp.H = p.H; mp.max_chunks = p.max_chunks; mp.chunk_blocks = p.chunk_blocks; mp.min_cb = p.min_cb;
@@ -1200,6 +1190,19 @@ int attn_decode(const void* q, const void* pool, int layers, int layer, int Hkv,
     return launch_paged_decode_attn(p, max_seq_hint, ws, ws_bytes, s, pdl);
 }
 
+int attn_decode_chunks(const void* q, const void* pool, int layers, int layer, int Hkv, int page_size, const int32_t* block_table, int max_blocks, const int32_t* seq_lens, int B, int H,
+                       float scale, void* ws, size_t ws_bytes, float* kv_scales, AttnChunks* out, cudaStream_t s) {
+    AttnParams p = {};
+    p.kv_scales = kv_scales;
+    p.q = (const __nv_bfloat16*)q; p.pool = (const __nv_bfloat16*)pool;
+    p.block_table = block_table; p.seq_lens = seq_lens;
+    p.B = B; p.H = H; p.Hkv = Hkv; p.G = H / Hkv;
+    p.layers = layers; p.layer = layer; p.page_size = page_size; p.max_blocks = max_blocks;
+    p.scale_log2e = scale * 1.4426950408889634f;
+    p.n_out = 1; p.signal_flag = -1;
+    return launch_paged_decode_attn(p, max_blocks * page_size, ws, ws_bytes, s, true, out);
+}
+
 // decode-engine form: q/k/v are dequantised from the qkv linear's raw accumulator inside the kernel (RoPE, KV append,
 // attention and the chunk merge are one launch)
 int attn_decode_fused(const FusedAttnArgs& a, cudaStream_t s, bool pdl) {
@@ -1230,12 +1233,14 @@ extern "C" size_t wf_kv_pool_bytes(int max_pages, int layers, int kv_heads, int 
     return elems * elt_size(dtype);
 }
 
+namespace wf {
 // scale region of an int8 pool
-static float* kv_scales_of(const wf_kv_layout* kv) {
+float* kv_scales_of(const wf_kv_layout* kv) {
     if (kv->dtype != WF_I8) return nullptr;
     return reinterpret_cast<float*>(reinterpret_cast<unsigned char*>(kv->pool) +
                                     (size_t)kv->max_pages * kv->layers * 2 * kv->kv_heads * kv->page_size * kv->head_dim);
 }
+}  // namespace wf
 
 static int check_kv(const wf_kv_layout* kv, const char* who) {
     if (!kv || !kv->pool) { set_error("%s: null kv layout/pool", who); return WF_ERR_INVALID; }
@@ -1291,18 +1296,22 @@ extern "C" size_t wf_attn_workspace_bytes(int B, int H, int head_dim, int max_se
     return legacy > even ? legacy : even;
 }
 
+int wf::check_decode_attn(const wf_kv_layout* kv, int layer, int H, int out_dtype, bool pointers, const char* who) {
+    if (int rc = check_kv(kv, who)) return rc;
+    if (!pointers) { set_error("%s: null pointer", who); return WF_ERR_INVALID; }
+    if (kv->dtype != WF_BF16 && kv->dtype != WF_I8) { set_error("%s: pool must be bf16 or int8", who); return WF_ERR_UNSUPPORTED; }
+    if (kv->head_dim != AT_D) { set_error("%s: head_dim must be 128 (got %d)", who, kv->head_dim); return WF_ERR_UNSUPPORTED; }
+    if (kv->page_size % AT_BLK) { set_error("%s: page_size must be a multiple of 16 (got %d)", who, kv->page_size); return WF_ERR_UNSUPPORTED; }
+    if (H % kv->kv_heads || H / kv->kv_heads > 8) { set_error("%s: H/Hkv must be an integer <= 8", who); return WF_ERR_UNSUPPORTED; }
+    if (layer < 0 || layer >= kv->layers) { set_error("%s: layer out of range", who); return WF_ERR_INVALID; }
+    if (out_dtype != WF_BF16 && out_dtype != WF_F32) { set_error("%s: out dtype", who); return WF_ERR_INVALID; }
+    return WF_OK;
+}
+
 extern "C" int wf_paged_decode_attn(const void* q, const wf_kv_layout* kv, int layer, const int32_t* block_table, int max_blocks,
                                     const int32_t* seq_lens, int B, int H, float scale, void* out, int out_dtype, void* workspace,
                                     size_t workspace_bytes, void* stream) {
-    int rc = check_kv(kv, "wf_paged_decode_attn");
-    if (rc) return rc;
-    if (!q || !block_table || !seq_lens || !out) { set_error("wf_paged_decode_attn: null pointer"); return WF_ERR_INVALID; }
-    if (kv->dtype != WF_BF16 && kv->dtype != WF_I8) { set_error("wf_paged_decode_attn: pool must be bf16 or int8"); return WF_ERR_UNSUPPORTED; }
-    if (kv->head_dim != AT_D) { set_error("wf_paged_decode_attn: head_dim must be 128 (got %d)", kv->head_dim); return WF_ERR_UNSUPPORTED; }
-    if (kv->page_size % AT_BLK) { set_error("wf_paged_decode_attn: page_size must be a multiple of 16 (got %d)", kv->page_size); return WF_ERR_UNSUPPORTED; }
-    if (H % kv->kv_heads || H / kv->kv_heads > 8) { set_error("wf_paged_decode_attn: H/Hkv must be an integer <= 8"); return WF_ERR_UNSUPPORTED; }
-    if (layer < 0 || layer >= kv->layers) { set_error("wf_paged_decode_attn: layer out of range"); return WF_ERR_INVALID; }
-    if (out_dtype != WF_BF16 && out_dtype != WF_F32) { set_error("wf_paged_decode_attn: out dtype"); return WF_ERR_INVALID; }
+    if (int rc = check_decode_attn(kv, layer, H, out_dtype, q && block_table && seq_lens && out, "wf_paged_decode_attn")) return rc;
     if (B <= 0) return WF_OK;
     return attn_decode(q, kv->pool, kv->layers, layer, kv->kv_heads, kv->page_size, block_table, max_blocks, seq_lens, B, H, scale, out,
                        out_dtype, max_blocks * kv->page_size, workspace, workspace_bytes, (cudaStream_t)stream, true, kv_scales_of(kv));

@@ -2,7 +2,7 @@
 //   sgl_kernel::bitnet_gemv_cpu / bitnet_gemm_cpu / bitnet_quantize_activations_cpu and their aliases (schemas: sgl_kernel/_ops.py; the names are the
 //   reference's, docs/research/sglang_optimization_plan.md:59-75): CUDA kernels of those ops;
 //   wf_native::linear, wf_native::mlp: the calls behind BitNetLinearNative and bitnet_mlp_forward (several launches each);
-//   wf_native::paged_decode_attn: wf_bitnet.ops.paged_decode_attn.
+//   wf_native::paged_decode_attn, paged_prefix_attn, paged_plan, paged_release, token_logprobs: the functions of these names in wf_bitnet.ops.
 // A call through ctypes spent 20 us of host time on what takes the GPU 6 (one token, 2560 x 2560), and the feed-forward op waited twice for a copy of
 // its weight scales to the device; here a call costs about 8 us and the scales travel as kernel parameters.
 #include <ATen/ATen.h>
@@ -206,6 +206,114 @@ Tensor paged_decode_attn(const Tensor& q, const Tensor& pool, int64_t max_pages,
     return out;
 }
 
+// an int32 tensor of `dim` dimensions on the device of `like`
+void need_i32(const Tensor& t, int64_t dim, const Tensor& like, const char* name) {
+    TORCH_CHECK_VALUE(t.scalar_type() == at::kInt, name, " must be int32");
+    TORCH_CHECK_VALUE(t.dim() == dim, name, " must have ", dim, " dimension", dim == 1 ? "" : "s");
+    TORCH_CHECK_VALUE(t.device() == like.device(), name, " must be on ", like.device());
+}
+int to_int(int64_t v, const char* name) {
+    TORCH_CHECK_VALUE(v >= 0 && v <= 0x7fffffff, name, " out of range");
+    return (int)v;
+}
+
+Tensor paged_prefix_attn(const Tensor& q, const Tensor& pool, int64_t max_pages, int64_t layers, int64_t kv_heads, int64_t page_size, int64_t head_dim, int64_t kv_dtype,
+                         int64_t layer, const Tensor& prefix_table, int64_t prefix_len, const Tensor& block_table, const Tensor& seq_lens, double scale, at::ScalarType out_dtype) {
+    need_gpu({&q, &pool, &prefix_table, &block_table, &seq_lens});
+    const c10::cuda::CUDAGuard guard(q.device());
+    TORCH_CHECK_VALUE(q.dim() == 3 && q.scalar_type() == at::kBFloat16, "q must be bf16 [B, H, D]");
+    TORCH_CHECK_VALUE(q.size(2) == head_dim, "q has heads of ", q.size(2), ", the cache of ", head_dim);
+    TORCH_CHECK_VALUE(pool.device() == q.device(), "the cache must be on ", q.device());
+    need_i32(prefix_table, 1, q, "prefix_table");
+    need_i32(block_table, 2, q, "block_table");
+    need_i32(seq_lens, 1, q, "seq_lens");
+    TORCH_CHECK_VALUE(block_table.size(0) == q.size(0) && seq_lens.size(0) == q.size(0), "block_table and seq_lens must have a row for each of ", q.size(0), " sequences");
+    TORCH_CHECK_VALUE(prefix_len >= 0 && prefix_len <= prefix_table.size(0) * page_size, "prefix_len (", prefix_len, ") beyond the ", prefix_table.size(0), " pages of prefix_table");
+    Tensor qc = q.contiguous();
+    if ((uintptr_t)qc.data_ptr() & 15) qc = qc.clone();
+    const Tensor pt = prefix_table.contiguous(), bt = block_table.contiguous(), sl = seq_lens.contiguous();
+    const int B = (int)q.size(0), H = (int)q.size(1), D = (int)q.size(2), blocks = to_int(bt.size(1), "block_table"), pre = to_int(prefix_len, "prefix_len");
+    to_int(bt.size(1) * page_size, "block_table");
+    Tensor out = at::empty({B, H, D}, q.options().dtype(out_dtype));
+    wf_kv_layout kv;
+    memset(&kv, 0, sizeof kv);
+    kv.pool = pool.data_ptr();
+    kv.max_pages = (int)max_pages; kv.layers = (int)layers; kv.kv_heads = (int)kv_heads; kv.page_size = (int)page_size; kv.head_dim = (int)head_dim; kv.dtype = (int)kv_dtype;
+    // memory of this call's own: calls on other streams and captured graphs do not share it
+    Tensor ws = at::empty({(int64_t)wf_prefix_attn_workspace_bytes(B, H, kv.kv_heads, D, blocks * kv.page_size, pre)}, q.options().dtype(at::kByte));
+    check(wf_paged_prefix_attn(qc.data_ptr(), &kv, (int)layer, (const int32_t*)pt.data_ptr(), pre, (const int32_t*)bt.data_ptr(), blocks, (const int32_t*)sl.data_ptr(), B, H, (float)scale,
+                               out.data_ptr(), code_of(out_dtype), ws.data_ptr(), (size_t)ws.numel(), stream()));
+    return out;
+}
+
+// rows, positions, pages, slots [max_tokens], offsets [B + 1], lens [B], free_count [1], status [1]: views of one buffer
+std::vector<Tensor> paged_plan(const Tensor& seq_lens, const Tensor& new_lens, Tensor block_table, const Tensor& free_pages, const Tensor& free_count, int64_t page_size,
+                               int64_t max_tokens) {
+    need_gpu({&seq_lens, &new_lens, &block_table, &free_pages, &free_count});
+    const c10::cuda::CUDAGuard guard(block_table.device());
+    need_i32(block_table, 2, block_table, "block_table");
+    need_i32(seq_lens, 1, block_table, "seq_lens");
+    need_i32(new_lens, 1, block_table, "new_lens");
+    need_i32(free_pages, 1, block_table, "free_pages");
+    need_i32(free_count, 1, block_table, "free_count");
+    const int64_t B = block_table.size(0);
+    TORCH_CHECK_VALUE(seq_lens.size(0) == B && new_lens.size(0) == B, "seq_lens and new_lens must have an entry for each of the ", B, " rows of block_table");
+    TORCH_CHECK_VALUE(free_count.size(0) == 1, "free_count must have one entry");
+    TORCH_CHECK_VALUE(block_table.is_contiguous(), "block_table must be contiguous (it is written in place)");
+    const Tensor sl = seq_lens.contiguous(), nl = new_lens.contiguous(), fp = free_pages.contiguous();
+    const int rows = to_int(B, "block_table"), cap = to_int(max_tokens, "max_tokens"), page = to_int(page_size, "page_size");
+    const int64_t cap4 = (max_tokens + 3) / 4 * 4;         // every map starts on 16 bytes
+    Tensor buf = at::empty({4 * cap4 + 2 * B + 3}, block_table.options());
+    const int64_t at[8] = {0, cap4, 2 * cap4, 3 * cap4, 4 * cap4, 4 * cap4 + B + 1, 4 * cap4 + 2 * B + 1, 4 * cap4 + 2 * B + 2};
+    const int64_t len[8] = {max_tokens, max_tokens, max_tokens, max_tokens, B + 1, B, 1, 1};
+    int32_t* base = (int32_t*)buf.data_ptr();
+    check(wf_paged_plan((const int32_t*)sl.data_ptr(), (const int32_t*)nl.data_ptr(), rows, (int32_t*)block_table.data_ptr(), to_int(block_table.size(1), "block_table"),
+                        (const int32_t*)fp.data_ptr(), to_int(fp.size(0), "free_pages"), (const int32_t*)free_count.data_ptr(), page, cap, base + at[1], base, base + at[2], base + at[3],
+                        base + at[4], base + at[5], base + at[6], base + at[7], stream()));
+    std::vector<Tensor> out;
+    out.reserve(8);
+    for (int i = 0; i < 8; ++i) out.push_back(buf.narrow(0, at[i], len[i]));
+    return out;
+}
+
+std::tuple<Tensor, Tensor> paged_release(const Tensor& done, const Tensor& seq_lens, const Tensor& block_table, Tensor free_pages, const Tensor& free_count, int64_t page_size) {
+    need_gpu({&done, &seq_lens, &block_table, &free_pages, &free_count});
+    const c10::cuda::CUDAGuard guard(block_table.device());
+    need_i32(block_table, 2, block_table, "block_table");
+    need_i32(seq_lens, 1, block_table, "seq_lens");
+    need_i32(free_pages, 1, block_table, "free_pages");
+    need_i32(free_count, 1, block_table, "free_count");
+    const int64_t B = block_table.size(0);
+    TORCH_CHECK_VALUE(done.scalar_type() == at::kBool && done.dim() == 1 && done.device() == block_table.device(), "done must be bool [B] on ", block_table.device());
+    TORCH_CHECK_VALUE(done.size(0) == B && seq_lens.size(0) == B, "done and seq_lens must have an entry for each of the ", B, " rows of block_table");
+    TORCH_CHECK_VALUE(free_count.size(0) == 1, "free_count must have one entry");
+    TORCH_CHECK_VALUE(free_pages.is_contiguous(), "free_pages must be contiguous (it is written in place)");
+    const Tensor dn = done.contiguous(), sl = seq_lens.contiguous(), bt = block_table.contiguous();
+    Tensor lens = at::empty({B}, sl.options()), count = at::empty({1}, sl.options());
+    check(wf_paged_release((const uint8_t*)dn.data_ptr(), (const int32_t*)sl.data_ptr(), to_int(B, "block_table"), (const int32_t*)bt.data_ptr(), to_int(bt.size(1), "block_table"),
+                           (int32_t*)free_pages.data_ptr(), to_int(free_pages.size(0), "free_pages"), (const int32_t*)free_count.data_ptr(), to_int(page_size, "page_size"),
+                           (int32_t*)lens.data_ptr(), (int32_t*)count.data_ptr(), stream()));
+    return {lens, count};
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor& logits, const Tensor& tokens, int64_t top, double temperature) {
+    need_gpu({&logits, &tokens});
+    const c10::cuda::CUDAGuard guard(logits.device());
+    TORCH_CHECK_VALUE(logits.dim() == 2, "logits must be [rows, vocab]");
+    need_i32(tokens, 1, logits, "tokens");
+    TORCH_CHECK_VALUE(tokens.size(0) == logits.size(0), "tokens must have an entry for each of the ", logits.size(0), " rows of logits");
+    const int dt = code_of(logits.scalar_type());
+    const Tensor x = logits.stride(1) == 1 || logits.size(1) <= 1 ? logits : logits.contiguous(), tk = tokens.contiguous();
+    const int n = to_int(x.size(0), "rows"), V = to_int(x.size(1), "vocab"), k = to_int(top, "top");
+    const int64_t ld = n > 1 ? x.stride(0) : V;
+    const Tensor& y = ld < V ? x.contiguous() : x;         // rows that overlap (an expanded row)
+    const auto f32 = x.options().dtype(at::kFloat);
+    Tensor lp = at::empty({n}, f32), ent = at::empty({n}, f32), tlp = at::empty({n, k}, f32), tid = at::empty({n, k}, x.options().dtype(at::kInt));
+    check(wf_token_logprobs(y.data_ptr(), dt, n, V, ld < V ? V : ld, (const int32_t*)tk.data_ptr(), k, (float)temperature, (float*)lp.data_ptr(), (float*)ent.data_ptr(),
+                            (float*)tlp.data_ptr(), (int32_t*)tid.data_ptr(), stream()));
+    return {lp, ent, tlp, tid};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(wf_native, m) {
@@ -213,6 +321,11 @@ TORCH_LIBRARY(wf_native, m) {
     m.def("mlp(Tensor x, Tensor gate_up_tile, int N2, Tensor down_w, float gate_scale, float up_scale, float down_scale, Tensor norm, float eps) -> Tensor");
     m.def("paged_decode_attn(Tensor q, Tensor pool, int max_pages, int layers, int kv_heads, int page_size, int head_dim, int kv_dtype, int layer, Tensor block_table, "
           "Tensor seq_lens, float scale, ScalarType out_dtype) -> Tensor");
+    m.def("paged_prefix_attn(Tensor q, Tensor pool, int max_pages, int layers, int kv_heads, int page_size, int head_dim, int kv_dtype, int layer, Tensor prefix_table, "
+          "int prefix_len, Tensor block_table, Tensor seq_lens, float scale, ScalarType out_dtype) -> Tensor");
+    m.def("paged_plan(Tensor seq_lens, Tensor new_lens, Tensor(a!) block_table, Tensor free_pages, Tensor free_count, int page_size, int max_tokens) -> Tensor[]");
+    m.def("paged_release(Tensor done, Tensor seq_lens, Tensor block_table, Tensor(a!) free_pages, Tensor free_count, int page_size) -> (Tensor, Tensor)");
+    m.def("token_logprobs(Tensor logits, Tensor tokens, int top, float temperature) -> (Tensor, Tensor, Tensor, Tensor)");
 }
 // CPU: the same functions, for their errors (a missing GPU, a tensor that is not on it).  Autograd: passed through, so that the outputs are plain tensors
 // whatever the inputs require, as behind the calls through ctypes.
@@ -221,6 +334,10 @@ TORCH_LIBRARY(wf_native, m) {
         m.impl("linear", linear);              \
         m.impl("mlp", mlp);                    \
         m.impl("paged_decode_attn", paged_decode_attn); \
+        m.impl("paged_prefix_attn", paged_prefix_attn); \
+        m.impl("paged_plan", paged_plan);      \
+        m.impl("paged_release", paged_release); \
+        m.impl("token_logprobs", token_logprobs); \
     }
 WF_NATIVE_IMPL(CUDA)
 WF_NATIVE_IMPL(CPU)
@@ -228,6 +345,10 @@ TORCH_LIBRARY_IMPL(wf_native, Autograd, m) {
     m.impl("linear", torch::CppFunction::makeFallthrough());
     m.impl("mlp", torch::CppFunction::makeFallthrough());
     m.impl("paged_decode_attn", torch::CppFunction::makeFallthrough());
+    m.impl("paged_prefix_attn", torch::CppFunction::makeFallthrough());
+    m.impl("paged_plan", torch::CppFunction::makeFallthrough());
+    m.impl("paged_release", torch::CppFunction::makeFallthrough());
+    m.impl("token_logprobs", torch::CppFunction::makeFallthrough());
 }
 TORCH_LIBRARY_IMPL(sgl_kernel, CUDA, m) {
     m.impl("bitnet_gemv_cpu", bitnet_gemv);

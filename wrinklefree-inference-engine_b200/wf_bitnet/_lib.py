@@ -84,6 +84,11 @@ SYMBOLS = {
     "wf_rope_kv_append": (_i, [_vp, _i, _i, C.POINTER(KvLayout), _i, _vp, _vp, _i, _vp, _vp, _i, _vp, _vp]),
     "wf_attn_workspace_bytes": (_sz, [_i, _i, _i, _i]),
     "wf_paged_decode_attn": (_i, [_vp, C.POINTER(KvLayout), _i, _vp, _i, _vp, _i, _i, _f, _vp, _i, _vp, _sz, _vp]),
+    "wf_paged_plan": (_i, [_vp, _vp, _i, _vp, _i, _vp, _i, _vp, _i, _i] + [_vp] * 9),
+    "wf_paged_release": (_i, [_vp, _vp, _i, _vp, _i, _vp, _i, _vp, _i, _vp, _vp, _vp]),
+    "wf_prefix_attn_workspace_bytes": (_sz, [_i] * 6),
+    "wf_paged_prefix_attn": (_i, [_vp, C.POINTER(KvLayout), _i, _vp, _i, _vp, _i, _vp, _i, _i, _f, _vp, _i, _vp, _sz, _vp]),
+    "wf_token_logprobs": (_i, [_vp, _i, _i, _i, C.c_longlong, _vp, _i, _f, _vp, _vp, _vp, _vp, _vp]),
     "wf_rmsnorm_quant": (_i, [_vp, _vp, _f, _i, _i, _vp, _vp, _vp, _vp, _vp]),
     "wf_embed": (_i, [_vp, _vp, _i, _i, _vp, _vp]),
     "wf_lm_head_workspace_bytes": (_sz, [_i, _i]),

@@ -7,7 +7,7 @@ raises `WfError`.
 from __future__ import annotations
 
 import ctypes as C
-from typing import Optional, Sequence, Tuple
+from typing import NamedTuple, Optional, Sequence, Tuple
 
 import torch
 
@@ -316,6 +316,50 @@ def paged_decode_attn(q: torch.Tensor, kv: PagedKV, layer: int, block_table: tor
                                            block_table, seq_lens, 1.0 / (q.shape[-1] ** 0.5) if scale is None else scale, out_dtype)
 
 
+def paged_prefix_attn(q: torch.Tensor, kv: PagedKV, layer: int, prefix_table: torch.Tensor, prefix_len: int, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                      scale: Optional[float] = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """Decode attention of a batch that shares a prefix: sequence b's keys are the first `prefix_len` tokens of the pages in prefix_table (int32 [pages]),
+    which are read once for the whole batch, and then seq_lens[b] tokens of its own pages, block_table[b] (int32 [B, blocks], blocks may be 0).
+    q: bf16 [B, H, D].  A sequence without any key gets zeros.  Otherwise as paged_decode_attn."""
+    if out_dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError("out_dtype must be bfloat16 or float32")
+    c = kv.c
+    return _native.ops().paged_prefix_attn(q, kv.raw if kv.dtype == torch.int8 else kv.pool, c.max_pages, c.layers, c.kv_heads, c.page_size, c.head_dim, c.dtype, layer,
+                                           prefix_table, prefix_len, block_table, seq_lens, 1.0 / (q.shape[-1] ** 0.5) if scale is None else scale, out_dtype)
+
+
+class PagedPlan(NamedTuple):
+    """A step's tokens in the paged cache, all int32 on the GPU.  Of every token, requests one after another (-1, 0, -1, 0 behind the last one):"""
+    rows: torch.Tensor          # [max_tokens] its request (row of block_table)
+    positions: torch.Tensor     # [max_tokens] its position in the sequence
+    pages: torch.Tensor         # [max_tokens] where it lies in the cache: what kv_scatter takes
+    slots: torch.Tensor         # [max_tokens]
+    offsets: torch.Tensor       # [B + 1] first token of each request, and the number of tokens
+    lens: torch.Tensor          # [B] seq_lens + new_lens
+    free_count: torch.Tensor    # [1] pages left
+    status: torch.Tensor        # [1] 0, or why nothing was planned (PLAN_*, ORed)
+
+
+PLAN_PAGES, PLAN_TOKENS, PLAN_BLOCKS, PLAN_LENGTH, PLAN_COUNT = 1, 2, 4, 8, 16
+
+
+def paged_plan(seq_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor, free_count: torch.Tensor, page_size: int,
+               max_tokens: int) -> PagedPlan:
+    """Block tables and slot maps of a step from its request lengths, without a word to the host: request b has seq_lens[b] cached tokens and brings new_lens[b]
+    (0: none).  Pages that it needs come off the end of the free list free_pages[:free_count] (the order of sgl_kernel.kvcache.PageAllocator) and are written to
+    its row of block_table; the free list itself stays.  Go on with the plan's `lens` and `free_count`.  A step that does not fit (pages, max_tokens, columns of
+    block_table; a length or the count out of range) is not planned at all: `status` says why, no token has a page, and `lens` and `free_count` are as before.
+    At most 8192 requests."""
+    return PagedPlan(*_native.ops().paged_plan(seq_lens, new_lens, block_table, free_pages, free_count, page_size, max_tokens))
+
+
+def paged_release(done: torch.Tensor, seq_lens: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor, free_count: torch.Tensor,
+                  page_size: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The requests with done[b] (bool [B]) hand their pages back, on top of the free list.  Returns (seq_lens with 0 for them, the new free_count); both as they
+    were, and nothing written, where the list would not hold the pages or a length is out of range."""
+    return _native.ops().paged_release(done, seq_lens, block_table, free_pages, free_count, page_size)
+
+
 # ----------------------------------------------------------------------------------------- glue
 def embed(table: torch.Tensor, tokens: torch.Tensor) -> torch.Tensor:
     _need_cuda(table, tokens)
@@ -335,3 +379,11 @@ def lm_head_argmax(h: torch.Tensor, E: torch.Tensor, want_logits: bool = True):
     check(lib().wf_lm_head_argmax(h.contiguous().data_ptr(), E.data_ptr(), B, V, K, logits.data_ptr() if want_logits else None,
                                   nxt.data_ptr(), ws.data_ptr(), ws.numel(), _stream()))
     return nxt, logits
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, temperature: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Of every row of logits (f32, bf16 or f16 [N, V], any row stride), softmax(logits / temperature): the log probability of tokens[n] (int32 [N]), the entropy,
+    and the `top` (at most 64) most likely tokens, most likely first, equal ones by id.  Returns (logprobs f32 [N], entropy f32 [N], top_logprobs f32 [N, top],
+    top_ids int32 [N, top]).  Logits of -inf have probability 0; a row of nothing else has logprobs -inf and entropy 0; a row with +inf or NaN has NaN; a token
+    outside [0, V) has NaN."""
+    return _native.ops().token_logprobs(logits, tokens, top, temperature)
