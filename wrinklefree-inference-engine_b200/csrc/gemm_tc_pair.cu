@@ -484,7 +484,7 @@ int check_wait_word(const char* who) {
     int* word = tc_wait_word();
     if (!word || !*(volatile int*)word) return WF_OK;
     if (const int role = __atomic_exchange_n(word, 0, __ATOMIC_ACQ_REL)) {
-        set_error("%s: a bounded wait of an earlier ternary product on this device ran out (%d); that product's output is not complete", who, role);
+        set_error("%s: a bounded wait of an earlier product on this device ran out (%d); that product's output is not complete", who, role);
         return WF_ERR_CUDA;
     }
     return WF_OK;
