@@ -30,8 +30,9 @@ def rows_of(kv, pages, layer, which, head, n):
 
 def check(q, kv, layer, ptable, prefix, table, lens, scale=None, out_dtype=torch.bfloat16):
     """Tolerance: weights enter the value product rounded to 16 bits (half a step 2^-8 of each, that of bf16, so 2^-8 of sum p |v|), the result is rounded once (2^-8 of it in
-    bf16, 2^-24 in float); scores are float sums of 128 products (130 half steps of sum |q k|, on p twice that), 2^x is off by 2^-22, and up to n weights and
-    n weighted values are added in float (2 n steps 2^-23)."""
+    bf16, 2^-24 in float); scores are float sums of 128 products (130 half steps of sum |q k|, on p twice that), 2^x is off by 2^-22, or by
+    7.5e-5 < 2^-13 where a polynomial gives it (in the weights and in their sum: 2^-12), and up to n weights and n weighted values are added in float
+    (2 n steps 2^-23)."""
     from wf_bitnet import ops
     out = ops.paged_prefix_attn(q, kv, layer, ptable, prefix, table, lens, scale, out_dtype)
     assert out.dtype == out_dtype and out.shape == q.shape
@@ -50,7 +51,7 @@ def check(q, kv, layer, ptable, prefix, table, lens, scale=None, out_dtype=torch
             qh = q[b, h * G:(h + 1) * G].to(F64)
             p = torch.softmax(qh @ k.T * sc, -1)
             want, mag = p @ v, p @ v.abs()
-            off = 2 * 130 * 2.0**-24 * float((qh.abs() @ k.abs().T).max()) * abs(sc) + 2.0**-21 + 2 * k.shape[0] * 2.0**-23
+            off = 2 * 130 * 2.0**-24 * float((qh.abs() @ k.abs().T).max()) * abs(sc) + 2.0**-12 + 2 * k.shape[0] * 2.0**-23
             tol = (2.0**-8 if out_dtype == torch.bfloat16 else 2.0**-24) * want.abs() + (2.0**-8 + off) * mag
             assert bool(((got - want).abs() <= tol * 1.01).all()), (b, h, ((got - want).abs() - tol).max())
 

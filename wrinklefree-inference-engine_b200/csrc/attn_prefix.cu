@@ -20,84 +20,46 @@ struct PxParams {
     int layers, layer, page_size;
     int splits, split_keys;        // keys of a split
     float scale_log2e;
-    float *part_o, *part_ml;       // [splits][B][H][AT_D], [splits][B][H][2]
+    float *part_o, *part_ml;       // [splits][Hkv][AT_D / 4][rows][4], [splits][Hkv][rows][2], rows = B * G up to the next multiple of 32
+    int rows_p;                    // those rows
     int wait_first;                // the kernel before is not this call's own
     int box, stages;               // keys per TMA box (a power of two that divides the page); key and value tiles in flight
     int* err;                      // the wait word
 };
 
-constexpr int PX_SIMPLE_WARPS = 4;
-// a warp per row and split: a lane per key for the scores, then a lane per 4 output columns
-__global__ void __launch_bounds__(PX_SIMPLE_WARPS * 32) prefix_attn_kernel(const __grid_constant__ PxParams p) {
-    const int lane = threadIdx.x & 31, row = blockIdx.x * PX_SIMPLE_WARPS + (threadIdx.x >> 5), split = blockIdx.y;
-    pdl_wait_prior();
-    pdl_launch_dependents();
-    if (row >= p.B * p.H) return;
-    const int kvh = row % p.H / p.G, j0 = split * p.split_keys, j1 = min(p.prefix, j0 + p.split_keys);
-    const __nv_bfloat16* q = p.q + (size_t)row * AT_D;
-    auto place = [&](int j, int kv) -> size_t {
-        const int pg = j / p.page_size;
-        return ((((size_t)p.table[pg] * p.layers + p.layer) * 2 + kv) * p.Hkv + kvh) * p.page_size + (j - pg * p.page_size);
-    };
-    float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int b = j0; b < j1; b += 32) {
-        const int j = b + lane;
-        float s = -INFINITY;
-        if (j < j1) {
-            const size_t at = place(j, 0);
-            float dot = 0.f;
-            for (int c = 0; c < AT_D; ++c) {
-                const float k = p.scales ? (float)((int)((const uint8_t*)p.pool)[at * AT_D + c] - 128) : __bfloat162float(((const __nv_bfloat16*)p.pool)[at * AT_D + c]);
-                dot = fmaf(__bfloat162float(q[c]), k, dot);
-            }
-            s = (p.scales ? dot * p.scales[at] : dot) * p.scale_log2e;
-        }
-        const float mn = fmaxf(m, warp_max(s)), f = m == -INFINITY ? 0.f : exp2f(m - mn), e = s == -INFINITY ? 0.f : exp2f(s - mn);
-        m = mn;
-        l = l * f + e;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) o[c] *= f;
-        for (int i = 0; i < min(32, j1 - b); ++i) {
-            const size_t at = place(b + i, 1);
-            const float w = __shfl_sync(0xffffffffu, e, i) * (p.scales ? p.scales[at] : 1.f);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const float v = p.scales ? (float)((int)((const uint8_t*)p.pool)[at * AT_D + 4 * lane + c] - 128) : __bfloat162float(((const __nv_bfloat16*)p.pool)[at * AT_D + 4 * lane + c]);
-                o[c] = fmaf(w, v, o[c]);
-            }
-        }
-    }
-    l = warp_sum(l);
-    const size_t at = (size_t)split * p.B * p.H + row;
-    *reinterpret_cast<float4*>(p.part_o + at * AT_D + 4 * lane) = make_float4(o[0], o[1], o[2], o[3]);
-    if (lane == 0) { p.part_ml[at * 2] = m; p.part_ml[at * 2 + 1] = l; }
-}
-
-// ---- the prefix part on the tensor cores (bf16 pools)
+// ---- the prefix part on the tensor cores
 //
-// A block owns one key/value head, a range of 128-key tiles and up to 256 query rows (a row = a sequence and one of the query heads that share the key/value
-// head).  Two softmax groups of four warps, a thread per row, take turns with the tensor cores, each with 128 TMEM columns of scores, overwritten in place by
-// the weights in bf16, and 128 columns of output:
-//   * more than 128 rows: a group per tile of 128 rows, and every key tile serves both;
-//   * up to 128 rows: both groups have the same rows and every other key tile; their results are joined in shared memory at the end.
-// Warp 8 loads keys and values by TMA (128 keys x 64 dims a box row of 128 bytes, a box per run of keys inside a page); one thread of warp 9 issues S = Q K^T
-// (both operands in shared memory) and O += P V (P in TMEM).  The output is rescaled only when a row's maximum has grown by more than 2^8 since the scale
-// was last fixed (exact: the sum carries the same scale).
+// A block owns one key/value head, a range of 64-key tiles and up to 256 query rows (a row = a sequence and one of the query heads that share the key/value
+// head).  Two softmax groups of four warps, a thread per row, each have two score buffers of 64 TMEM columns, which their weights (bf16) overwrite in place, and
+// 128 columns of output; the scores of a group's next tile are under way while a tile's weights are computed:
+//   * more than 128 rows: a group per 128 rows, and every tile serves both;
+//   * up to 128 rows: both groups have the same rows and every other tile; their results are joined in shared memory at the end.
+// Warp 8 loads keys and values by TMA into rings of 64-key tiles (a box of 64 dims per run of keys inside a page); one thread of warps 9 and 10 each issues a
+// group's S = Q K^T (both operands in shared memory) and O += P V (P in TMEM): a wait of one group leaves the other's products running.  The output is rescaled
+// only when a row's maximum has grown by more than 2^8 since the scale was last fixed (exact: the sum carries the same scale).
 // Every wait is bounded: one that runs out leaves a code in the device's wait word, and the block waits for its copies and products and leaves.
-constexpr int PX_KEYS = 128, PX_ROWS = 128;
-constexpr int PX_HALF = 128 * 128;                     // bytes of 128 rows x 64 bf16
-constexpr int PX_TILE = 2 * PX_HALF;
-constexpr int PX_RING = 7 * PX_TILE;                   // queries of one or two tiles, then three or two stages of keys and of values
-constexpr int PX_SMEM = PX_RING + 1024;
-constexpr int PX_THREADS = 10 * 32;
+constexpr int PX_KEYS = 64, PX_ROWS = 128;             // keys of a tile, rows of a group
+constexpr int PX_QHALF = PX_ROWS * 128, PX_QTILE = 2 * PX_QHALF;       // bytes of 128 rows x 64 bf16, and of both halves of the dims
+constexpr int PX_HALF = PX_KEYS * 128, PX_TILE = 2 * PX_HALF;          // the same of a tile of keys or values
+constexpr int PX_SMEM_USE = 224 * 1024;                // queries of one or two groups, then rings of six or five tiles of keys and of values
+constexpr int PX_SMEM = PX_SMEM_USE + 1024;
+constexpr int PX_STAGES = 6;
+constexpr int PX_THREADS = 11 * 32;
+// int8 pools: a ring of tiles as they lie in the pool, and one of converted tiles with their scales
+constexpr int PX_RAW = 3, PX_RAW_TILE = 2 * PX_KEYS * AT_D, PX_SC = 2 * PX_KEYS * 4, PX_STAGES8 = 3;
+constexpr int PX_CONV = 4;                             // converting warps
+constexpr int PX_SMEM8_USE = 2 * PX_QTILE + PX_STAGES8 * 2 * PX_TILE + PX_RAW * PX_RAW_TILE + PX_STAGES8 * PX_SC;
+constexpr int PX_SMEM8 = PX_SMEM8_USE + 1024;
+constexpr int PX_THREADS8 = PX_THREADS + PX_CONV * 32;
+static_assert(PX_SMEM <= 226 * 1024 && PX_SMEM8 <= 226 * 1024, "one block's shared memory");
 constexpr unsigned long long PX_LIMIT_NS = 1000000000ull;
 constexpr float PX_LAZY = 8.f;
 
 __device__ __forceinline__ uint64_t px_desc(uint32_t saddr, uint32_t lbo) {       // 128-byte rows, 128B swizzle, 8-row groups 1024 bytes apart
     return (uint64_t)((saddr & 0x3ffffu) >> 4) | (uint64_t)(lbo >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
-// D f32, A and B bf16, 128 x 128; b_mn: B is MN-major
-constexpr uint32_t px_idesc(int b_mn) { return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)b_mn << 16) | (16u << 17) | (8u << 24); }
+// D f32, A and B bf16, 128 x n; b_mn: B is MN-major
+constexpr uint32_t px_idesc(int n, int b_mn) { return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24); }
 __device__ __forceinline__ void px_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
                  ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
@@ -123,36 +85,60 @@ __device__ __forceinline__ bool px_wait_warp(uint64_t* bar, uint32_t parity) { r
 __device__ __forceinline__ uint64_t px_pair(uint32_t a, uint32_t b) { uint64_t v; asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(a), "r"(b)); return v; }
 __device__ __forceinline__ void px_unpair(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
 __device__ __forceinline__ uint64_t px_fma2(uint64_t a, uint64_t b, uint64_t c) { uint64_t v; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c)); return v; }
+__device__ __forceinline__ uint64_t px_mul2(uint64_t a, uint64_t b) { uint64_t v; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b)); return v; }
 __device__ __forceinline__ uint64_t px_add2(uint64_t a, uint64_t b) { uint64_t v; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b)); return v; }
 __device__ __forceinline__ float px_ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+__device__ __forceinline__ float px_max(float a, float b) { float y; asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b)); return y; }     // NaN stays NaN
+// 2^x of two numbers on the multiply-add units: x = i + f, |f| <= 1/2, by adding 1.5 * 2^23; 2^f by its minimax polynomial of degree 3 (Remez; off by 7.5e-5 at
+// most, a 26th of the rounding of a weight to bf16); i goes into the exponent.  Below 2^-126: 2^-126 or less.  The special function unit gives 16 values a
+// clock and SM, the products of a pair of groups ask for 25; one pair in PX_POLY takes this way.
+constexpr int PX_POLY = 4;
+__device__ __forceinline__ void px_exp2_poly(uint64_t x, float& e0, float& e1) {
+    const uint64_t magic = px_pair(0x4b400000u, 0x4b400000u), minus_magic = px_pair(0xcb400000u, 0xcb400000u), minus1 = px_pair(0xbf800000u, 0xbf800000u);
+    constexpr float c0 = 0.9999280571937561f, c1 = 0.6932609677314758f, c2 = 0.2426111251115799f, c3 = 0.0551716685295105f;
+    float x0, x1;
+    px_unpair(x, x0, x1);
+    x = px_pair(__float_as_uint(px_max(x0, -126.f)), __float_as_uint(px_max(x1, -126.f)));
+    const uint64_t t = px_add2(x, magic), f = px_fma2(px_add2(t, minus_magic), minus1, x);
+    uint64_t y = px_fma2(px_pair(__float_as_uint(c3), __float_as_uint(c3)), f, px_pair(__float_as_uint(c2), __float_as_uint(c2)));
+    y = px_fma2(y, f, px_pair(__float_as_uint(c1), __float_as_uint(c1)));
+    y = px_fma2(y, f, px_pair(__float_as_uint(c0), __float_as_uint(c0)));
+    e0 = __uint_as_float((uint32_t)y + ((uint32_t)t << 23));
+    e1 = __uint_as_float((uint32_t)(y >> 32) + ((uint32_t)(t >> 32) << 23));
+}
 __device__ __forceinline__ uint4 px_ldcg(const uint4* a) {
     uint4 r;
     asm volatile("ld.global.cg.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(a));
     return r;
 }
 
-__global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ PxParams p) {
+template <bool I8>
+__global__ void __launch_bounds__(I8 ? PX_THREADS8 : PX_THREADS, 1) prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ PxParams p) {
     extern __shared__ unsigned char smem_raw[];
-    __shared__ __align__(8) uint64_t q_full[2], k_full[3], k_empty[3], v_full[3], v_empty[3], v_fixed, s_full[2], p_full[2], o_full[2], drained;
+    __shared__ __align__(8) uint64_t q_full[2], kv_full[PX_STAGES], kv_empty[PX_STAGES], tail_full, raw_full[PX_RAW], raw_empty[PX_RAW], s_full[2][2], p_full[2][2], o_full[2], o_end[2], drained[2];
     __shared__ uint32_t tmem_base_s;
     __shared__ float2 other_ml[PX_ROWS];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int rows = p.B * p.G, pairs = (rows + 2 * PX_ROWS - 1) / (2 * PX_ROWS);
     const int pr = blockIdx.x % pairs, kvh = blockIdx.x / pairs % p.Hkv, split = blockIdx.x / pairs / p.Hkv;
     const int row0 = pr * 2 * PX_ROWS;
-    const bool alt = rows - row0 <= PX_ROWS;              // one tile of rows: the groups take every other key tile
+    const bool alt = rows - row0 <= PX_ROWS;              // the groups have the same rows and every other tile
     const int key0 = split * p.split_keys, key1 = min(p.prefix, key0 + p.split_keys);
     const int nt = (key1 - key0 + PX_KEYS - 1) / PX_KEYS;
     const int fix_row = key1 - key0 - (nt - 1) * PX_KEYS;  // rows of the last value tile from here on hold no key: zeroed (a weight of zero times NaN is NaN)
-    const int nst = p.stages;
+    const int nst = p.stages, hop = alt ? 2 : 1;           // tiles of a ring; from one tile of a group to its next
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    const uint32_t q_s = base, k_s = base + (7 - 2 * nst) * PX_TILE, v_s = k_s + nst * PX_TILE;
+    const uint32_t q_s = base, k_s = I8 ? base + 2 * PX_QTILE : base + PX_SMEM_USE - 2 * nst * PX_TILE, v_s = k_s + nst * PX_TILE;
+    const uint32_t raw_s = v_s + nst * PX_TILE, sc_s = raw_s + PX_RAW * PX_RAW_TILE;       // int8: the pool's tiles; 64 scales of keys and 64 of values of every converted tile
 
     if (tid == 0) {
-        for (int i = 0; i < 2; ++i) { mbar_init(&q_full[i], 4); mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); mbar_init(&o_full[i], 1); }
-        for (int i = 0; i < 3; ++i) { mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 1); mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 1); }
-        mbar_init(&v_fixed, 1);
-        mbar_init(&drained, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&q_full[i], 4); mbar_init(&o_full[i], 1); mbar_init(&o_end[i], 1); mbar_init(&drained[i], 1);
+            for (int u = 0; u < 2; ++u) { mbar_init(&s_full[i][u], 1); mbar_init(&p_full[i][u], 4); }
+        }
+        for (int u = 0; u < PX_STAGES; ++u) { mbar_init(&kv_full[u], I8 ? PX_CONV : 1); mbar_init(&kv_empty[u], alt ? 1 : 2); }
+        for (int u = 0; u < PX_RAW; ++u) { mbar_init(&raw_full[u], 1); mbar_init(&raw_empty[u], PX_CONV); }
+        mbar_init(&tail_full, 1);
         fence_mbar_init();
     }
     if (warp == 9) {
@@ -167,177 +153,240 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_tc_kernel(const __g
     pdl_launch_dependents();
 
     if (warp == 8) {
-        // ------------------------------------------------------------ producer
+        // ------------------------------------------------------------ producer: lanes 0..3 the boxes of keys, 4..7 of values
+        const int kv = lane >> 2 & 1, off = (lane & 3) * p.box;
+        const int depth = I8 ? PX_RAW : nst, step = I8 ? PX_RAW_TILE : PX_TILE;
+        const uint32_t ring = (I8 ? raw_s + kv * PX_KEYS * AT_D : kv ? v_s : k_s) + off * 128;
+        uint64_t *const fulls = I8 ? raw_full : kv_full, *const empties = I8 ? raw_empty : kv_empty;
+        auto here = [&](int i) { return lane < 8 && off < PX_KEYS && key0 + i * PX_KEYS + off < key1; };       // this lane's box of tile i holds keys
+        auto page_of = [&](int i) { return here(i) ? ldcg_i32(p.table + (key0 + i * PX_KEYS + off) / p.page_size) : 0; };
         bool ok = true;
-        int issued[2] = {0, 0};                           // tiles of keys and of values under way or landed
-        int st = 0, lap = 0;
-        for (int i = 0; i < nt && ok; ++i) {
-            const int j = key0 + i * PX_KEYS + lane * p.box;
-            const bool mine = lane * p.box < PX_KEYS && j < key1;
+        int st = 0, lap = 0, page = page_of(0), i = 0;
+        for (; i < nt; ++i) {
+            const int next = page_of(i + 1);
+            const bool mine = here(i), tail = !I8 && i == nt - 1 && fix_row < PX_KEYS;
             const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, mine));
-            int slot = 0, block = 0;
+            uint64_t* full = tail ? &tail_full : &fulls[st];
+            if (lap && !px_wait_warp(&empties[st], (uint32_t)((lap & 1) ^ 1))) { ok = false; break; }
+            if (lane == 0) mbar_expect_tx(full, boxes * (uint32_t)((I8 ? 1 : 2) * p.box * 128));
+            __syncwarp();
             if (mine) {
-                const int pg = j / p.page_size;
-                slot = j - pg * p.page_size;
-                block = ((ldcg_i32(p.table + pg) * p.layers + p.layer) * 2) * p.Hkv + kvh;
-            }
+                const int slot = (key0 + i * PX_KEYS + off) % p.page_size, block = ((page * p.layers + p.layer) * 2 + kv) * p.Hkv + kvh;
 #pragma unroll
-            for (int kv = 0; kv < 2; ++kv) {
-                uint64_t* full = kv ? &v_full[st] : &k_full[st];
-                if (lap && !px_wait_warp(kv ? &v_empty[st] : &k_empty[st], (uint32_t)((lap & 1) ^ 1))) { ok = false; break; }
-                if (lane == 0) mbar_expect_tx(full, boxes * (uint32_t)(2 * p.box * 128));
-                __syncwarp();
-                if (mine) {
-                    const uint32_t dst = (kv ? v_s : k_s) + st * PX_TILE + lane * p.box * 128;
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-                        asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-                                     ::"r"(dst + h * PX_HALF), "l"(&tmap), "r"(h * 64), "r"(slot), "r"(block + kv * p.Hkv), "r"(smem_u32(full)) : "memory");
-                }
-                __syncwarp();
-                issued[kv] = i + 1;
+                for (int h = 0; h < (I8 ? 1 : 2); ++h)
+                    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                                 ::"r"(ring + st * step + h * PX_HALF), "l"(&tmap), "r"(h * 64), "r"(slot), "r"(block), "r"(smem_u32(full)) : "memory");
             }
-            if (ok && i == nt - 1 && fix_row < PX_KEYS) {
-                if (!px_wait_warp(&v_full[st], (uint32_t)(lap & 1))) { ok = false; break; }
-                for (int c = lane; c < (PX_KEYS - fix_row) * 16; c += 32) {
+            __syncwarp();
+            page = next;
+            if (tail) {                                    // its keyless value rows are cleared before the tile is handed on
+                ok = px_wait_warp(&tail_full, 0);
+                for (int c = lane; ok && c < (PX_KEYS - fix_row) * 16; c += 32) {
                     const int h = c / ((PX_KEYS - fix_row) * 8), r = c - h * (PX_KEYS - fix_row) * 8;
                     asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(v_s + st * PX_TILE + h * PX_HALF + (fix_row * 8 + r) * 16), "r"(0u) : "memory");
                 }
                 fence_proxy_async();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&v_fixed);
+                if (ok && lane == 0) mbar_arrive(&kv_full[st]);
             }
-            if (++st == nst) { st = 0; ++lap; }
+            if (++st == depth) { st = 0; ++lap; }
         }
         if (!ok) {                                        // the block leaves early, but not before its copies have landed
             if (lane == 0) *(volatile int*)p.err = 16;
-            for (int kv = 0; kv < 2; ++kv)
-                for (int i = max(0, issued[kv] - nst); i < issued[kv]; ++i) px_wait_warp(kv ? &v_full[i % nst] : &k_full[i % nst], (uint32_t)((i / nst) & 1));
+            for (int u = max(0, i - depth); u < i; ++u)
+                if (I8 || u < nt - 1 || fix_row == PX_KEYS) px_wait_warp(&fulls[u % depth], (uint32_t)((u / depth) & 1));
         }
-    } else if (warp == 9) {
-        // ------------------------------------------------------------ MMA issuer
+    } else if (I8 && warp >= 11) {
+        // ------------------------------------------------------------ converters: codes to bf16 in the operands' layout, scales beside them
+        // A thread takes 16 codes of a row at a time.  A quarter of a warp takes four pieces of rows r and r ^ 5: both the swizzled pieces that it reads and those
+        // that it writes lie in different banks.
+        const int x = tid - 11 * 32, w = warp - 11;
+        const int pc = (lane & 3) + 4 * (lane >> 3 & 1), flip = lane >> 2 & 1 ? 5 : 0;
+        const int skv = x >> 6, sj = x & 63;               // this thread's scale: of keys or values, of which key
+        auto scale_of = [&](int i) {
+            const int j = key0 + i * PX_KEYS + sj;
+            if (i >= nt || j >= key1) return 0.f;
+            const int pg = j / p.page_size;
+            float v;
+            asm volatile("ld.global.cg.f32 %0, [%1];" : "=f"(v) : "l"(p.scales + ((((size_t)ldcg_i32(p.table + pg) * p.layers + p.layer) * 2 + skv) * p.Hkv + kvh) * p.page_size + (j - pg * p.page_size)));
+            return v;
+        };
+        bool ok = true;
+        int st = 0, lap = 0, rs = 0, rlap = 0;
+        float sc = scale_of(0);
+        for (int i = 0; i < nt; ++i) {
+            const float sc_next = scale_of(i + 1);
+            if (!px_wait_warp(&raw_full[rs], (uint32_t)(rlap & 1)) || (lap && !px_wait_warp(&kv_empty[st], (uint32_t)((lap & 1) ^ 1)))) { ok = false; break; }
+            asm volatile("st.shared.f32 [%0], %1;" ::"r"(sc_s + st * PX_SC + x * 4), "f"(sc) : "memory");
+#pragma unroll
+            for (int kv = 0; kv < 2; ++kv) {
+#pragma unroll
+                for (int it = 0; it < 4; ++it) {
+                    const int row = 2 * ((lane >> 4) | w << 1 | it << 3) ^ flip;
+                    uint32_t y[4], o[8];
+                    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(y[0]), "=r"(y[1]), "=r"(y[2]), "=r"(y[3])
+                                 : "r"(raw_s + rs * PX_RAW_TILE + kv * PX_KEYS * AT_D + row * 128 + ((pc ^ (row & 7)) << 4)) : "memory");
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {          // a byte above the mantissa of 2^23 is 2^23 + code + 128
+                        const uint64_t off2 = px_pair(0xcb000080u, 0xcb000080u);
+                        float a, b;
+                        px_unpair(px_add2(px_pair(__byte_perm(y[k], 0x4b000000u, 0x7440), __byte_perm(y[k], 0x4b000000u, 0x7441)), off2), a, b);
+                        o[2 * k] = pack_bf16x2(a, b);
+                        px_unpair(px_add2(px_pair(__byte_perm(y[k], 0x4b000000u, 0x7442), __byte_perm(y[k], 0x4b000000u, 0x7443)), off2), a, b);
+                        o[2 * k + 1] = pack_bf16x2(a, b);
+                    }
+                    const uint32_t dst = (kv ? v_s : k_s) + st * PX_TILE + (pc >> 2) * PX_HALF + row * 128;
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst + ((((pc & 3) * 2 + k) ^ (row & 7)) << 4)), "r"(o[4 * k]), "r"(o[4 * k + 1]), "r"(o[4 * k + 2]),
+                                     "r"(o[4 * k + 3]) : "memory");
+                }
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) { mbar_arrive(&kv_full[st]); mbar_arrive(&raw_empty[rs]); }
+            sc = sc_next;
+            if (++st == nst) { st = 0; ++lap; }
+            if (++rs == PX_RAW) { rs = 0; ++rlap; }
+        }
+        if (!ok && lane == 0) *(volatile int*)p.err = 19;
+    } else if (warp == 9 || warp == 10) {
+        // ------------------------------------------------------------ a group's products
+        const int t = warp - 9, tiles = alt ? (nt - t + 1) / 2 : nt;
         uint32_t elected;
         asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(elected));
-        if (elected) {
-            const uint32_t idesc_s = px_idesc(0), idesc_o = px_idesc(1);
-            uint32_t np[2] = {0, 0};                      // weight tiles consumed per group
-            bool ok = true, q_ready[2] = {false, false};
-            int kst = 0, klap = 0, vst = 0, vlap = 0;
-            auto scores = [&](int t) {                    // of the key tile in stage kst, for group t
-                const int qt = alt ? 0 : t;
-                if (!q_ready[qt]) { if (!px_wait(&q_full[qt], 0)) return false; q_ready[qt] = true; }
+        constexpr uint32_t idesc_s = px_idesc(PX_KEYS, 0), idesc_o = px_idesc(AT_D, 1);
+        const uint64_t qd = px_desc(q_s + (alt ? 0 : t) * PX_QTILE, 16), kd0 = px_desc(k_s, 16), vd0 = px_desc(v_s, PX_HALF);
+        const uint32_t s_t = tmem + t * 256, o_t = s_t + 128;
+        int kst = alt ? t : 0, vst = kst;
+        uint32_t par = 0;
+        bool ok = px_wait_warp(&q_full[alt ? 0 : t], 0);
+        for (int n = -1; n < tiles && ok; ++n) {
+            if (n + 1 < tiles) {                          // the next tile's scores, into the buffer that the values before last have left
+                if (!px_wait_warp(&kv_full[kst], par)) { ok = false; break; }
                 tc_fence_after();
-                const uint64_t qd = px_desc(q_s + qt * PX_TILE, 16), kd = px_desc(k_s + kst * PX_TILE, 16);
+                if (elected) {
+                    const uint64_t kd = kd0 + (uint64_t)(kst * (PX_TILE >> 4));
 #pragma unroll
-                for (int ks = 0; ks < 8; ++ks) {
-                    const uint64_t off = (uint64_t)((ks >> 2) * (PX_HALF >> 4) + (ks & 3) * 2);
-                    px_mma_ss(tmem + t * 256, qd + off, kd + off, idesc_s, ks ? 1u : 0u);
+                    for (int ks = 0; ks < 8; ++ks)
+                        px_mma_ss(s_t + ((n + 1) & 1) * PX_KEYS, qd + (uint64_t)((ks >> 2) * (PX_QHALF >> 4) + (ks & 3) * 2), kd + (uint64_t)((ks >> 2) * (PX_HALF >> 4) + (ks & 3) * 2), idesc_s,
+                                  ks ? 1u : 0u);
+                    px_commit(&s_full[t][(n + 1) & 1]);
                 }
-                px_commit(&s_full[t]);
-                return true;
-            };
-            auto values = [&](int t, bool last) {         // with the value tile in stage vst
-                if (!px_wait(&p_full[t], np[t] & 1)) return false;
-                tc_fence_after();
-                const uint64_t vd = px_desc(v_s + vst * PX_TILE, PX_HALF);
-#pragma unroll
-                for (int ks = 0; ks < 8; ++ks) px_mma_ts(tmem + t * 256 + 128, tmem + t * 256 + ks * 8, vd + (uint64_t)(ks * 128), idesc_o, np[t] || ks ? 1u : 0u);   // 16 keys = 2048 bytes
-                ++np[t];
-                if (last) px_commit(&o_full[t]);
-                return true;
-            };
-            for (int i = -1; i < nt && ok; ++i) {
-                const bool more = i + 1 < nt;
-                if (more && !px_wait(&k_full[kst], (uint32_t)(klap & 1))) { ok = false; break; }
-                auto next_k = [&]() { px_commit(&k_empty[kst]); if (++kst == nst) { kst = 0; ++klap; } };
-                if (alt && more) { ok = scores((i + 1) & 1); if (ok) next_k(); }
-                if (i >= 0 && ok) ok = px_wait(&v_full[vst], (uint32_t)(vlap & 1)) && !(i == nt - 1 && fix_row < PX_KEYS && !px_wait(&v_fixed, 0));
-                if (alt) {
-                    if (i >= 0 && ok) ok = values(i & 1, i >= nt - 2);
-                } else {
-                    for (int t = 0; t < 2 && ok; ++t) {
-                        if (i >= 0) ok = values(t, i == nt - 1);
-                        if (more && ok) ok = scores(t);
-                    }
-                }
-                if (!ok) break;
-                if (i >= 0) { px_commit(&v_empty[vst]); if (++vst == nst) { vst = 0; ++vlap; } }
-                if (more && !alt) next_k();
+                __syncwarp();
+                if ((kst += hop) >= nst) { kst -= nst; par ^= 1; }
             }
-            if (!ok) *(volatile int*)p.err = 17;
-            px_commit(&drained);                          // nor while a product still reads shared memory or TMEM
-            px_wait(&drained, 0);
+            if (n >= 0) {
+                if (!px_wait_warp(&p_full[t][n & 1], (uint32_t)((n >> 1) & 1))) { ok = false; break; }
+                tc_fence_after();
+                if (elected) {
+                    const uint64_t vd = vd0 + (uint64_t)(vst * (PX_TILE >> 4));
+#pragma unroll
+                    for (int ks = 0; ks < PX_KEYS / 16; ++ks) px_mma_ts(o_t, s_t + (n & 1) * PX_KEYS + ks * 8, vd + (uint64_t)(ks * 128), idesc_o, n || ks ? 1u : 0u);   // 16 keys = 2048 bytes
+                    px_commit(n == tiles - 1 ? &o_end[t] : &o_full[t]);
+                    px_commit(&kv_empty[vst]);
+                }
+                __syncwarp();
+                if ((vst += hop) >= nst) vst -= nst;
+            }
         }
+        if (!ok && lane == 0) *(volatile int*)p.err = 17;
         __syncwarp();
+        if (elected) px_commit(&drained[t]);              // nor while a product still reads shared memory or TMEM
+        px_wait_warp(&drained[t], 0);
     } else {
         // ------------------------------------------------------------ softmax: a thread per row
         const int t = warp >> 2, tr = (warp & 3) * 32 + lane, r = row0 + (alt ? 0 : t * PX_ROWS) + tr;
         const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t s_t = tmem + t * 256 + lane_base, o_t = s_t + 128;
         const bool r_ok = r < rows;
-        const int b = r_ok ? r / p.G : 0, row = b * p.H + kvh * p.G + (r_ok ? r - b * p.G : 0);
         const int tiles = alt ? (nt - t + 1) / 2 : nt;
         const bool flat = p.scale_log2e == 0.f;           // zero queries: every score is 0, but for the masked ones
         const float unit = flat ? 1.f : fabsf(p.scale_log2e);       // a negative scale turns the queries' signs
         if (t == 0 || !alt) {
-            // the row's query into the swizzled operand tile (zero where there is no row)
-            const uint32_t qrow = q_s + t * PX_TILE + tr * 128, sign = p.scale_log2e < 0.f ? 0x80008000u : 0u;
-            const uint4* src = reinterpret_cast<const uint4*>(p.q + (size_t)row * AT_D);
+            // the warp's 32 queries into the swizzled operand tile (zero where there is no row): two whole rows a load, all loads under way together
+            const uint32_t sign = p.scale_log2e < 0.f ? 0x80008000u : 0u;
+            const int q0 = (warp & 3) * 32 + (lane >> 4), c = lane & 15;
+            int x = row0 + (alt ? 0 : t * PX_ROWS) + q0, xb = x / p.G, xg = x - xb * p.G;
+            uint4 v[16];
 #pragma unroll
-            for (int c = 0; c < 16; ++c) {
-                uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                if (r_ok && !flat) v = px_ldcg(src + c);
-                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(qrow + (c >> 3) * PX_HALF + (((c & 7) ^ (tr & 7)) << 4)), "r"(v.x ^ sign), "r"(v.y ^ sign), "r"(v.z ^ sign),
-                             "r"(v.w ^ sign) : "memory");
+            for (int i = 0; i < 16; ++i, x += 2) {
+                v[i] = make_uint4(0u, 0u, 0u, 0u);
+                if (x < rows && !flat) v[i] = px_ldcg(reinterpret_cast<const uint4*>(p.q + ((size_t)xb * p.H + kvh * p.G + xg) * AT_D) + c);
+                for (xg += 2; xg >= p.G; xg -= p.G) ++xb;
             }
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(q_s + t * PX_QTILE + (c >> 3) * PX_QHALF + (q0 + 2 * i) * 128 + (((c & 7) ^ ((q0 + 2 * i) & 7)) << 4)),
+                             "r"(v[i].x ^ sign), "r"(v[i].y ^ sign), "r"(v[i].z ^ sign), "r"(v[i].w ^ sign) : "memory");
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(&q_full[t]);
         }
         float m_ref = -INFINITY, l = 0.f;                 // scores in units of log 2
+        int sst = alt ? t : 0;                             // int8: the converted tile that holds the scales
         bool ok = true;
-        for (int it = 0; it < tiles && ok; ++it) {
-            if (!px_wait_warp(&s_full[t], it & 1)) { ok = false; break; }     // also: every earlier product of this group is done
+        for (int n = 0; n < tiles && ok; ++n) {
+            const uint32_t s_n = s_t + (n & 1) * PX_KEYS;
+            if (!px_wait_warp(&s_full[t][n & 1], (uint32_t)((n >> 1) & 1))) { ok = false; break; }
             tc_fence_after();
-            uint32_t s[128];
-            TC_LD32(s_t, (s + 0));
-            TC_LD32(s_t + 32, (s + 32));
-            TC_LD32(s_t + 64, (s + 64));
-            TC_LD32(s_t + 96, (s + 96));
+            uint32_t s[PX_KEYS];
+            TC_LD32(s_n, (s + 0));
+            TC_LD32(s_n + 32, (s + 32));
             asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-            if ((alt ? 2 * it + t : it) == nt - 1 && fix_row < PX_KEYS) {
+            const uint32_t sc_n = sc_s + (I8 ? sst * PX_SC : 0);
+            if (I8) {                                     // the keys' scales; those of keys that are none are 0
 #pragma unroll
-                for (int c = 0; c < 128; ++c) if (c >= fix_row) s[c] = 0xff800000u;
+                for (int c = 0; c < PX_KEYS; c += 4) {
+                    uint32_t k[4];
+                    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(k[0]), "=r"(k[1]), "=r"(k[2]), "=r"(k[3]) : "r"(sc_n + c * 4) : "memory");
+                    const uint64_t a = px_mul2(px_pair(s[c], s[c + 1]), px_pair(k[0], k[1])), b = px_mul2(px_pair(s[c + 2], s[c + 3]), px_pair(k[2], k[3]));
+                    s[c] = (uint32_t)a; s[c + 1] = (uint32_t)(a >> 32); s[c + 2] = (uint32_t)b; s[c + 3] = (uint32_t)(b >> 32);
+                }
+                if ((sst += hop) >= nst) sst -= nst;
+            }
+            if (n * hop + (alt ? t : 0) == nt - 1 && fix_row < PX_KEYS) {
+#pragma unroll
+                for (int c = 0; c < PX_KEYS; ++c) if (c >= fix_row) s[c] = 0xff800000u;
             }
             float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int c = 0; c < 128; c += 8)
+            for (int c = 0; c < PX_KEYS; c += 8)
 #pragma unroll
-                for (int k = 0; k < 4; ++k) mx4[k] = fmaxf(fmaxf(mx4[k], __uint_as_float(s[c + k])), __uint_as_float(s[c + 4 + k]));
-            const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * unit;
+                for (int k = 0; k < 4; ++k) mx4[k] = px_max(px_max(mx4[k], __uint_as_float(s[c + k])), __uint_as_float(s[c + 4 + k]));
+            const float mx = px_max(px_max(mx4[0], mx4[1]), px_max(mx4[2], mx4[3])) * unit;
             float corr = 1.f;
-            if (mx > m_ref + PX_LAZY) {                   // also the first time anything is seen
+            if (!(mx <= m_ref + PX_LAZY)) {               // also the first time anything is seen, and NaN
                 corr = m_ref == -INFINITY ? 0.f : px_ex2(m_ref - mx);
                 m_ref = mx;
                 l *= corr;
             }
-            const uint32_t nm = __float_as_uint(m_ref == -INFINITY ? 0.f : -m_ref);
+            // a row with a score of +inf or NaN has no weights but NaN
+            const uint32_t nm = __float_as_uint(m_ref == -INFINITY ? 0.f : m_ref == INFINITY ? __uint_as_float(0x7fc00000u) : -m_ref);
             const uint64_t nm2 = px_pair(nm, nm), unit2 = px_pair(__float_as_uint(unit), __float_as_uint(unit));
             uint64_t ls[2] = {0ull, 0ull};
 #pragma unroll
-            for (int c = 0; c < 64; ++c) {                // columns (2c, 2c + 1) go to s[c], an entry whose score has been read
+            for (int c = 0; c < PX_KEYS / 2; ++c) {       // columns (2c, 2c + 1) go to s[c], an entry whose score has been read
+                const uint64_t x = px_fma2(px_pair(s[2 * c], s[2 * c + 1]), unit2, nm2);
                 float e0, e1;
-                px_unpair(px_fma2(px_pair(s[2 * c], s[2 * c + 1]), unit2, nm2), e0, e1);
-                e0 = px_ex2(e0); e1 = px_ex2(e1);
+                if (c % PX_POLY == PX_POLY - 1) {
+                    px_exp2_poly(x, e0, e1);
+                } else {
+                    px_unpair(x, e0, e1);
+                    e0 = px_ex2(e0); e1 = px_ex2(e1);
+                }
                 ls[c & 1] = px_add2(ls[c & 1], px_pair(__float_as_uint(e0), __float_as_uint(e1)));
+                if (I8) {                                 // the values' scales go into the weights
+                    uint32_t v0, v1;
+                    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v0), "=r"(v1) : "r"(sc_n + PX_KEYS * 4 + c * 8) : "memory");
+                    px_unpair(px_mul2(px_pair(__float_as_uint(e0), __float_as_uint(e1)), px_pair(v0, v1)), e0, e1);
+                }
                 s[c] = pack_bf16x2(e0, e1);
             }
-            float l0, l1;
-            px_unpair(px_add2(ls[0], ls[1]), l0, l1);
-            l += l0 + l1;
-            TC_ST32(s_t, (s + 0));
-            TC_ST32(s_t + 32, (s + 32));
-            if (it > 0 && __any_sync(0xffffffffu, corr != 1.f)) {
+            TC_ST32(s_n, s);
+            if (n > 0 && __any_sync(0xffffffffu, corr != 1.f)) {
+                if (!px_wait_warp(&o_full[t], (uint32_t)((n - 1) & 1))) { ok = false; break; }      // the scores above came behind all values but the last tile's
+                tc_fence_after();
 #pragma unroll 1
                 for (int c = 0; c < AT_D; c += 32) {
                     uint32_t o[32];
@@ -351,14 +400,17 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_tc_kernel(const __g
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[t]);
+            if (lane == 0) mbar_arrive(&p_full[t][n & 1]);
+            float l0, l1;
+            px_unpair(px_add2(ls[0], ls[1]), l0, l1);
+            l += l0 + l1;
         }
         // ---- the group's output: alone, or with that of the other group, whose half lies in the ring by then
-        if (ok && tiles > 0) ok = px_wait_warp(&o_full[t], 0);
-        bool joined = false;
+        if (ok && tiles > 0) ok = px_wait_warp(&o_end[t], 0);
         if (alt) {
             if (t == 1) {
-                if (ok) ok = px_wait_warp(&o_full[0], 0);  // the ring is read by neither group's products any more
+                // the ring is read by neither group's products any more
+                if (ok) ok = px_wait_warp(&o_end[0], 0);
                 other_ml[tr] = ok && tiles > 0 ? make_float2(m_ref, l) : make_float2(-INFINITY, 0.f);
             }
             if (t == 1 && ok && tiles > 0) {
@@ -375,11 +427,11 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_tc_kernel(const __g
                 }
             }
             asm volatile("bar.sync 1, 256;" ::: "memory");
-            joined = t == 0 && nt > 1;
         }
         if (ok && (t == 0 || !alt)) {
             tc_fence_after();
             float f0 = 1.f, f1 = 0.f;
+            const bool joined = alt && nt > 1;
             if (joined) {
                 const float2 ml = other_ml[tr];
                 const float m = fmaxf(m_ref, ml.x);
@@ -388,7 +440,8 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_tc_kernel(const __g
                 l = l * f0 + ml.y * f1;
                 m_ref = m;
             }
-            const size_t at = (size_t)split * p.B * p.H + row;
+            const size_t part = (size_t)split * p.Hkv + kvh;
+            float4* dst = reinterpret_cast<float4*>(p.part_o) + part * 32 * p.rows_p + r;      // rows side by side: a warp's stores are whole lines
 #pragma unroll 1
             for (int c = 0; c < AT_D; c += 32) {
                 uint32_t o[32];
@@ -403,10 +456,10 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_tc_kernel(const __g
                         asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(w.x), "=f"(w.y), "=f"(w.z), "=f"(w.w) : "r"(k_s + (((c + k) >> 2) * PX_ROWS + tr) * 16) : "memory");
                         v.x = fmaf(v.x, f0, w.x * f1); v.y = fmaf(v.y, f0, w.y * f1); v.z = fmaf(v.z, f0, w.z * f1); v.w = fmaf(v.w, f0, w.w * f1);
                     }
-                    if (r_ok) *reinterpret_cast<float4*>(p.part_o + at * AT_D + c + k) = v;
+                    if (r_ok) dst[(size_t)((c + k) >> 2) * p.rows_p] = v;
                 }
             }
-            if (r_ok) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(m_ref, l);
+            if (r_ok) reinterpret_cast<float2*>(p.part_ml)[part * p.rows_p + r] = make_float2(m_ref, l);
         }
         if (!ok && lane == 0) *(volatile int*)p.err = 18;
     }
@@ -422,15 +475,16 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_tc_kernel(const __g
 
 DevOnce g_px_attr;
 
-// [128][slot][page, layer, K | V, head], boxes of `box` slots x 64
+// [128][slot][page, layer, K | V, head], boxes of `box` slots x 128 bytes
 int px_encode(CUtensorMap* tm, const wf_kv_layout* kv, int box) {
     if (!tc_encoder()) gemm_tc_init_attrs();
     EncodeTiledFn fn = tc_encoder();
     if (!fn) { set_error("wf_paged_prefix_attn: cuTensorMapEncodeTiled unavailable"); return WF_ERR_CUDA; }
     const cuuint64_t gdim[3] = {AT_D, (cuuint64_t)kv->page_size, (cuuint64_t)kv->max_pages * kv->layers * 2 * kv->kv_heads};
-    const cuuint64_t gstride[2] = {AT_D * 2, (cuuint64_t)kv->page_size * AT_D * 2};
-    const cuuint32_t bx[3] = {64, (cuuint32_t)box, 1}, es[3] = {1, 1, 1};
-    const CUresult cr = fn(tm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, kv->pool, gdim, gstride, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+    const int es_ = kv->dtype == WF_I8 ? 1 : 2;
+    const cuuint64_t gstride[2] = {(cuuint64_t)AT_D * es_, (cuuint64_t)kv->page_size * AT_D * es_};
+    const cuuint32_t bx[3] = {(cuuint32_t)(128 / es_), (cuuint32_t)box, 1}, es[3] = {1, 1, 1};
+    const CUresult cr = fn(tm, es_ == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, kv->pool, gdim, gstride, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (cr != CUDA_SUCCESS) { set_error("wf_paged_prefix_attn: tensor map failed (%d)", (int)cr); return WF_ERR_CUDA; }
     return WF_OK;
@@ -439,52 +493,66 @@ int px_encode(CUtensorMap* tm, const wf_kv_layout* kv, int box) {
 struct PxMerge {
     AttnChunks own;                // part_o null: no own keys
     const int32_t* seq_lens;
-    const float *part_o, *part_ml;
-    int splits, rows, H;
+    const float *part_o, *part_ml; // as in PxParams
+    int splits, rows, rows_p, Hkv, G, H;
     void* out;
     int out_dtype;
 };
 
-// A warp per row (sequence and head), a lane per part for the maxima and factors and per 4 columns for the values.
-constexpr int PX_MERGE_WARPS = 4;
-__global__ void __launch_bounds__(PX_MERGE_WARPS * 32) prefix_merge_kernel(const __grid_constant__ PxMerge p) {
-    const int lane = threadIdx.x & 31, row = blockIdx.x * PX_MERGE_WARPS + (threadIdx.x >> 5);
+// A thread per row and 4 C columns: neighbouring threads are neighbouring rows, as the prefix part's results lie.  First the maximum of all parts, then their
+// factors and sums, several parts under way at a time.
+constexpr int PX_MERGE = 128;
+template <int C>
+__global__ void __launch_bounds__(PX_MERGE) prefix_merge_kernel(const __grid_constant__ PxMerge p) {
+    const int kvh = blockIdx.x % p.Hkv, r = blockIdx.x / p.Hkv * PX_MERGE + threadIdx.x, c0 = blockIdx.y * C;
     pdl_wait_prior();
     pdl_launch_dependents();
-    if (row >= p.rows) return;
+    if (r >= p.rows) return;
+    const int b = r / p.G, row = b * p.H + kvh * p.G + (r - b * p.G);
     int own = 0;
     if (p.own.part_o) {
-        const int nblocks = (p.seq_lens[row / p.H] + AT_BLK - 1) / AT_BLK;
+        const int nblocks = (p.seq_lens[b] + AT_BLK - 1) / AT_BLK;
         const int cb = chunk_blocks_of(nblocks, p.own.chunk_blocks, p.own.max_chunks, p.own.min_cb);
         own = (nblocks + cb - 1) / cb;
     }
-    auto slot = [&](int i) -> size_t { return i < p.splits ? (size_t)i * p.rows + row : (size_t)row * p.own.max_chunks + (i - p.splits); };
+    const size_t next = (size_t)p.Hkv * p.rows_p;         // from a split to the next
+    const float2 *ml = reinterpret_cast<const float2*>(p.part_ml) + (size_t)kvh * p.rows_p + r, *oml = reinterpret_cast<const float2*>(p.own.part_ml) + (size_t)row * p.own.max_chunks;
     float M = -INFINITY, L = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    const int n = p.splits + own;
-    for (int b = 0; b < n; b += 32) {
-        const int i = b + lane;
-        float2 ml = make_float2(-INFINITY, 0.f);
-        if (i < n) ml = reinterpret_cast<const float2*>(i < p.splits ? p.part_ml : p.own.part_ml)[slot(i)];
-        const float mn = fmaxf(M, warp_max(ml.x)), r = M == -INFINITY ? 0.f : exp2f(M - mn), f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - mn);
-        M = mn;
-        L = L * r + warp_sum(ml.y * f);
-        o.x *= r; o.y *= r; o.z *= r; o.w *= r;
-        for (int k = 0; k < min(32, n - b); ++k) {
-            const float fk = __shfl_sync(0xffffffffu, f, k);
-            const float4 v = reinterpret_cast<const float4*>((b + k < p.splits ? p.part_o : p.own.part_o) + slot(b + k) * AT_D)[lane];
-            o.x = fmaf(fk, v.x, o.x); o.y = fmaf(fk, v.y, o.y); o.z = fmaf(fk, v.z, o.z); o.w = fmaf(fk, v.w, o.w);
+#pragma unroll 8
+    for (int i = 0; i < p.splits; ++i) M = fmaxf(M, ml[i * next].x);
+    for (int i = 0; i < own; ++i) M = fmaxf(M, oml[i].x);
+    float4 o[C];
+#pragma unroll
+    for (int k = 0; k < C; ++k) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](const float2 x, const float4* v, size_t step) {
+        const float f = x.x == -INFINITY ? 0.f : exp2f(x.x - M);
+        L = fmaf(x.y, f, L);
+#pragma unroll
+        for (int k = 0; k < C; ++k) {
+            const float4 w = v[k * step];
+            o[k].x = fmaf(f, w.x, o[k].x); o[k].y = fmaf(f, w.y, o[k].y); o[k].z = fmaf(f, w.z, o[k].z); o[k].w = fmaf(f, w.w, o[k].w);
         }
-    }
+    };
+    const float4* v = reinterpret_cast<const float4*>(p.part_o) + ((size_t)kvh * 32 + c0) * p.rows_p + r;
+#pragma unroll 4
+    for (int i = 0; i < p.splits; ++i) add(ml[i * next], v + i * next * 32, p.rows_p);
+    const float4* w = reinterpret_cast<const float4*>(p.own.part_o) + (size_t)row * p.own.max_chunks * 32 + c0;
+    for (int i = 0; i < own; ++i) add(oml[i], w + (size_t)i * 32, 1);
     const float inv = L > 0.f ? 1.f / L : L == 0.f ? 0.f : L;      // no key: zeros; NaN stays
-    o.x *= inv; o.y *= inv; o.z *= inv; o.w *= inv;
-    if (p.out_dtype == WF_BF16) reinterpret_cast<uint2*>(p.out)[(size_t)row * 32 + lane] = make_uint2(pack_bf16x2(o.x, o.y), pack_bf16x2(o.z, o.w));
-    else reinterpret_cast<float4*>(p.out)[(size_t)row * 32 + lane] = o;
+#pragma unroll
+    for (int k = 0; k < C; ++k) {
+        const float4 y = make_float4(o[k].x * inv, o[k].y * inv, o[k].z * inv, o[k].w * inv);
+        const size_t at = (size_t)row * 32 + c0 + k;
+        if (p.out_dtype == WF_BF16) reinterpret_cast<uint2*>(p.out)[at] = make_uint2(pack_bf16x2(y.x, y.y), pack_bf16x2(y.z, y.w));
+        else reinterpret_cast<float4*>(p.out)[at] = y;
+    }
 }
+
+int px_rows_p(int B, int G) { return (B * G + 31) / 32 * 32; }
 
 // splits of the prefix and their keys
 void px_cut(int B, int H, int Hkv, int prefix, int* splits, int* keys) {
-    const int tiles = (prefix + PX_KEYS - 1) / PX_KEYS;
+    const int tiles = (prefix + 2 * PX_KEYS - 1) / (2 * PX_KEYS);        // pairs of tiles: one for each group
     const long long rows = (long long)B * (H / Hkv), units = Hkv * ((rows + 2 * PX_ROWS - 1) / (2 * PX_ROWS));
     int best = 1;
     long long least = -1;
@@ -492,7 +560,7 @@ void px_cut(int B, int H, int Hkv, int prefix, int* splits, int* keys) {
         const long long waves = (units * n + sm_count() - 1) / sm_count(), cost = waves * ((tiles + n - 1) / n + 3) * 100 + n * 20;
         if (least < 0 || cost < least) { least = cost; best = n; }
     }
-    *keys = (tiles + best - 1) / best * PX_KEYS;
+    *keys = (tiles + best - 1) / best * 2 * PX_KEYS;
     *splits = (prefix + *keys - 1) / *keys;
 }
 
@@ -500,7 +568,7 @@ size_t px_bytes(int B, int H, int Hkv, int prefix) {
     if (prefix <= 0) return 0;
     int splits, keys;
     px_cut(B, H, Hkv, prefix, &splits, &keys);
-    return ((size_t)splits * B * H * (AT_D + 2) * sizeof(float) + 255) / 256 * 256;      // the own chunks' vectors follow
+    return ((size_t)splits * Hkv * px_rows_p(B, H / Hkv) * (AT_D + 2) * sizeof(float) + 255) / 256 * 256;      // the own chunks' vectors follow
 }
 
 }  // namespace
@@ -528,7 +596,7 @@ extern "C" int wf_paged_prefix_attn(const void* q, const wf_kv_layout* kv, int l
     if ((uintptr_t)workspace & 15) { set_error("%s: the workspace must be 16-byte aligned", who); return WF_ERR_INVALID; }
     cudaStream_t s = (cudaStream_t)stream;
     PxMerge g = {};
-    g.seq_lens = seq_lens; g.rows = B * H; g.H = H; g.out = out; g.out_dtype = out_dtype;
+    g.seq_lens = seq_lens; g.Hkv = kv->kv_heads; g.G = H / kv->kv_heads; g.H = H; g.rows = B * g.G; g.rows_p = px_rows_p(B, g.G); g.out = out; g.out_dtype = out_dtype;
     if (max_blocks > 0)
         if (int rc = attn_decode_chunks(q, kv->pool, kv->layers, layer, kv->kv_heads, kv->page_size, block_table, max_blocks, seq_lens, B, H, scale, (char*)workspace + mine, workspace_bytes - mine,
                                         kv_scales_of(kv), &g.own, s)) return rc;
@@ -540,23 +608,26 @@ extern "C" int wf_paged_prefix_attn(const void* q, const wf_kv_layout* kv, int l
         p.scale_log2e = scale * 1.4426950408889634f;
         px_cut(B, H, kv->kv_heads, prefix_len, &p.splits, &p.split_keys);
         p.part_o = (float*)workspace;
-        p.part_ml = p.part_o + (size_t)p.splits * B * H * AT_D;
+        p.rows_p = g.rows_p;
+        p.part_ml = p.part_o + (size_t)p.splits * p.Hkv * p.rows_p * AT_D;
         p.wait_first = max_blocks == 0;
         g.part_o = p.part_o; g.part_ml = p.part_ml; g.splits = p.splits;
-        if (!p.scales) {
-            const int rows = B * p.G;
-            p.box = 16;
-            while (p.box < PX_KEYS && kv->page_size % (2 * p.box) == 0) p.box *= 2;
-            p.stages = rows <= PX_ROWS ? 3 : 2;
-            p.err = tc_wait_word();
-            if (!p.err) { set_error("%s: no wait word", who); return WF_ERR_CUDA; }
-            CUtensorMap tm;
-            if (int rc = px_encode(&tm, kv, p.box)) return rc;
-            if (g_px_attr.need() && cuda_check(cudaFuncSetAttribute(prefix_attn_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PX_SMEM), who)) return WF_ERR_CUDA;
-            const int pairs = (rows + 2 * PX_ROWS - 1) / (2 * PX_ROWS);
-            if (int rc = launch_check(launch_pdl(prefix_attn_tc_kernel, dim3((unsigned)(pairs * p.Hkv * p.splits)), PX_THREADS, PX_SMEM, s, tm, p), "prefix_attn_tc")) return rc;
-        } else
-            if (int rc = launch_check(launch_pdl(prefix_attn_kernel, dim3((B * H + PX_SIMPLE_WARPS - 1) / PX_SIMPLE_WARPS, p.splits), PX_SIMPLE_WARPS * 32, 0, s, p), "prefix_attn")) return rc;
+        const int rows = g.rows, pairs = (rows + 2 * PX_ROWS - 1) / (2 * PX_ROWS);
+        const bool i8 = p.scales != nullptr;
+        p.box = 16;
+        while (p.box < PX_KEYS && kv->page_size % (2 * p.box) == 0) p.box *= 2;
+        p.stages = i8 ? PX_STAGES8 : rows <= PX_ROWS ? 6 : 5;
+        p.err = tc_wait_word();
+        if (!p.err) { set_error("%s: no wait word", who); return WF_ERR_CUDA; }
+        CUtensorMap tm;
+        if (int rc = px_encode(&tm, kv, p.box)) return rc;
+        if (g_px_attr.need() && (cuda_check(cudaFuncSetAttribute(prefix_attn_tc_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, PX_SMEM), who) ||
+                                 cuda_check(cudaFuncSetAttribute(prefix_attn_tc_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, PX_SMEM8), who))) return WF_ERR_CUDA;
+        const dim3 grid((unsigned)(pairs * p.Hkv * p.splits));
+        const cudaError_t e = i8 ? launch_pdl(prefix_attn_tc_kernel<true>, grid, PX_THREADS8, PX_SMEM8, s, tm, p) : launch_pdl(prefix_attn_tc_kernel<false>, grid, PX_THREADS, PX_SMEM, s, tm, p);
+        if (int rc = launch_check(e, "prefix_attn_tc")) return rc;
     }
-    return launch_check(launch_pdl(prefix_merge_kernel, dim3((g.rows + PX_MERGE_WARPS - 1) / PX_MERGE_WARPS), PX_MERGE_WARPS * 32, 0, s, g), "prefix_merge");
+    const unsigned blocks = (unsigned)((g.rows + PX_MERGE - 1) / PX_MERGE) * g.Hkv;
+    if (blocks >= 64) return launch_check(launch_pdl(prefix_merge_kernel<4>, dim3(blocks, 8), PX_MERGE, 0, s, g), "prefix_merge");
+    return launch_check(launch_pdl(prefix_merge_kernel<1>, dim3(blocks, 32), PX_MERGE, 0, s, g), "prefix_merge");
 }
