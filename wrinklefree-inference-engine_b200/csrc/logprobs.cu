@@ -6,9 +6,11 @@
 // are taken before the scale, so that rows masked with a type's lowest value come out right too.
 //
 // The k largest (k <= 64) come out of the same pass.  An alternative is a 64-bit key, the number in an order-preserving form above the complement of its index, so
-// that keys differ and ties go to the lowest index.  A warp keeps its k largest sorted; what may belong to them is appended to its buffer in
-// shared memory, and a full buffer is sorted (bitonic, by shuffles) and merged into the list.  The warps of a block share the largest of their k-th keys as a
-// bound: below it a key has k larger ones.  On logits in no special order almost every vector fails one comparison of its largest entry with the bound.
+// that keys differ and ties go to the lowest index.  A bound, which k entries are known to reach, keeps almost all entries out: the k-th largest of the threads'
+// running maxima (of the ceil(k / 16) + 1 largest of each warp), taken after rounds 1, 4, 16, ... of loads.  What reaches it goes to a buffer of the block, some
+// k (1 + 3 log4 rounds) entries of a row in no special order; at the end a thread per candidate counts the larger ones: its place.  A row that fills the
+// buffer (rising, or of few different numbers) is read again: then every warp sorts what may belong to its k largest into a list of them (bitonic, by shuffles),
+// and the lists are merged.  Entries of -inf are not collected: where there are fewer than k others, the lowest of their indices are looked up at the end.
 //
 // A row is one block, or a cluster of 2 to 8 for few rows, whose results meet in distributed shared memory: one launch, no workspace.
 #include <cuda_fp16.h>
@@ -20,8 +22,8 @@ namespace wf {
 namespace {
 
 constexpr int LP_THREADS = 512, LP_WARPS = LP_THREADS / 32;
-constexpr int LP_VECS = 4;                            // 16-byte vectors a thread has in flight
-constexpr int LP_PEND = 64;                           // entries of a warp's buffer
+constexpr int LP_CAND = 2048;                         // candidates of a block
+constexpr int LP_PEND = 64;                           // entries of a warp's buffer where a row is read again
 constexpr float LP_LN2 = 0.6931471805599453f, LP_LOG2E = 1.4426950408889634f;
 constexpr float LP_FLOOR = -1000.f;                   // 2^LP_FLOOR is 0: what lies below (also -inf) is brought up to it, so that 0 times it is 0
 
@@ -92,8 +94,7 @@ __device__ __forceinline__ void lp_merge(u64 (&list)[R], const u64 (&other)[R], 
     }
 }
 
-// The n entries of a warp's buffer into its list, both in shared memory; the list's k-th key is returned and offered to the block's other warps.  Not inlined: the
-// streaming loop would hold a copy for every entry of a lane.
+// The n entries of a warp's buffer into its list, both in shared memory; the list's k-th key is returned and offered to the block's other warps
 template <int R>
 __device__ __noinline__ u64 lp_flush(u64* list, const u64* pend, int n, int k, u64* bound_s) {
     const int lane = threadIdx.x & 31;
@@ -164,66 +165,112 @@ __device__ __forceinline__ V lp_peer(const V* local, int rank) {       // the sa
     return v;
 }
 
+// A block's part of a row, entry by entry: every warp's k largest into its list, then all into list 0.  pend: LP_PEND entries a warp
+template <typename T, int R>
+__device__ __noinline__ void lp_again(const T* x, int i0, int i1, int k, u64 bound, u64* lists, u64* pend, u64* bound_s) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    u64 *const list = lists + warp * R * 32, *const buf = pend + warp * LP_PEND;
+    int npend = 0;
+    for (int r = 0; r < R; ++r) list[r * 32 + lane] = 0;
+    if (threadIdx.x == 0) *bound_s = bound;
+    __syncthreads();
+    for (int b = i0 + warp * 32; b < i1; b += LP_THREADS) {
+        const int i = b + lane;
+        const float v = i < i1 ? LpVec<T>::one(x[i]) : -INFINITY;
+        const u64 key = lp_key(v, i);
+        bound = lp_max(bound, *reinterpret_cast<volatile u64*>(bound_s));
+        const bool in = v > -INFINITY && key > bound;
+        const uint32_t who = __ballot_sync(0xffffffffu, in);
+        if (!who) continue;
+        if (npend + __popc(who) > LP_PEND) { bound = lp_max(bound, lp_flush<R>(list, buf, npend, k, bound_s)); npend = 0; }
+        if (in) buf[npend + __popc(who & ((1u << lane) - 1))] = key;
+        npend += __popc(who);
+    }
+    if (npend) lp_flush<R>(list, buf, npend, k, bound_s);
+    __syncthreads();
+    for (int half = LP_WARPS >> 1; half; half >>= 1) {
+        if (warp < half) {
+            u64 mine[R], other[R];
+#pragma unroll
+            for (int r = 0; r < R; ++r) { mine[r] = list[r * 32 + lane]; other[r] = list[(half * R + r) * 32 + lane]; }
+            lp_merge<R>(mine, other, lane);
+#pragma unroll
+            for (int r = 0; r < R; ++r) list[r * 32 + lane] = mine[r];
+        }
+        __syncthreads();
+    }
+}
+
 // R: 32-key parts of the lists of alternatives (0: none wanted)
 template <typename T, int R>
 __global__ void __launch_bounds__(LP_THREADS, 2) token_logprobs_kernel(const __grid_constant__ LpParams p) {
-    constexpr int VN = LpVec<T>::N, RL = R ? R : 1;
-    __shared__ u64 pend[R ? LP_WARPS : 1][LP_PEND];
-    __shared__ u64 lists[R ? LP_WARPS : 1][RL * 32];
+    constexpr int VN = LpVec<T>::N, VECS = 16 / VN, RL = R ? R : 1;      // 16 entries a thread and round, the next round's under way
+    constexpr int TOPS = LP_TOP_MAX / LP_WARPS + 1;
+    __shared__ u64 cand[R ? LP_CAND : 1];
+    __shared__ u64 lists[R ? LP_WARPS * RL * 32 : 1];
     __shared__ u64 bound_s;
+    __shared__ uint32_t tops[LP_WARPS * TOPS], bound_v;
+    __shared__ int ncand;
     __shared__ float part[LP_WARPS][3];
+    static_assert(!R || (LP_CAND >= LP_WARPS * LP_PEND && LP_CAND >= 8 * LP_TOP_MAX), "the candidates' space is used again");
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int cs = p.parts, rank = blockIdx.x % cs, row = blockIdx.x / cs;
+    if (R && tid == 0) { bound_v = 0; ncand = 0; }
+    if (R && tid < p.k) lists[tid] = 0;
+    if (R) __syncthreads();
     pdl_wait_prior();
     pdl_launch_dependents();
     const T* x = reinterpret_cast<const T*>(p.logits) + (long long)row * p.ld;
     const float c = p.inv_t * LP_LOG2E;
-    // the given token's logit, under way while the row is read
-    float x_tok = __uint_as_float(0x7fc00000u);
-    if (rank == 0 && tid == 0) { const int tok = p.tokens[row]; if (tok >= 0 && tok < p.V) x_tok = LpVec<T>::one(x[tok]); }
-    if (R) {
-#pragma unroll
-        for (int r = 0; r < RL; ++r) lists[warp][r * 32 + lane] = 0;
-        if (tid == 0) bound_s = 0;
-        __syncthreads();
-    }
     const int head = min(p.V, (int)(((16 - ((uintptr_t)x & 15)) & 15) / sizeof(T)));       // entries in front of the first whole vector
     const int nvec = (p.V - head) / VN, tail = p.V - head - nvec * VN;
     const uint4* xv = reinterpret_cast<const uint4*>(x + head);
     const int v0 = (int)((long long)nvec * rank / cs), v1 = (int)((long long)nvec * (rank + 1) / cs);
+    const uint4 none = make_uint4(0, 0, 0, 0);
+    uint4 w[VECS];
+    auto load = [&](int b) {
+#pragma unroll
+        for (int u = 0; u < VECS; ++u) { const int i = b + u * LP_THREADS + tid; w[u] = i < v1 ? lp_load(xv + i) : none; }
+    };
+    load(v0);
+    // the given token's logit, under way while the row is read
+    float x_tok = __uint_as_float(0x7fc00000u);
+    if (rank == 0 && tid == 0) { const int tok = p.tokens[row]; if (tok >= 0 && tok < p.V) x_tok = LpVec<T>::one(x[tok]); }
 
     Sums q = {-INFINITY, 0.f, 0.f};
-    u64 *const list = lists[R ? warp : 0], *const buf = pend[R ? warp : 0];
-    u64 bound = 0;                                     // keys up to here are not among the k largest
-    float bound_x = -INFINITY;
-    int npend = 0;
-    auto flush = [&]() {
-        bound = lp_max(bound, lp_flush<RL>(list, buf, npend, p.k, &bound_s));
-        npend = 0;
-    };
-    // N entries a lane; entry j has index i0 + (j / VN) * stride + j % VN and counts where that is below `end`
-    auto take = [&](auto& v, int n, int i0, int stride, int end) {
-        float m = v[0];
-#pragma unroll
-        for (int j = 1; j < LP_VECS * VN; ++j) if (j < n) m = fmaxf(m, v[j]);
-        if (R) {
-            bound = lp_max(bound, *reinterpret_cast<volatile u64*>(&bound_s));
-            bound_x = bound ? lp_value(bound) : -INFINITY;
-            if (__any_sync(0xffffffffu, m >= bound_x)) {
-#pragma unroll
-                for (int j = 0; j < LP_VECS * VN; ++j) {
-                    if (j >= n) break;
-                    const int i = i0 + (j / VN) * stride + j % VN;
-                    const u64 key = lp_key(v[j], i);
-                    const bool in = v[j] >= bound_x && key > bound && i < end;
-                    const uint32_t who = __ballot_sync(0xffffffffu, in);
-                    if (!who) continue;
-                    if (npend + __popc(who) > LP_PEND) flush();
-                    if (in) buf[npend + __popc(who & ((1u << lane) - 1))] = key;
-                    npend += __popc(who);
-                }
-            }
+    float bound_x = -INFINITY;                         // entries below are not among the k largest
+    // the k-th largest of the threads' numbers, in its ordered form: of each warp's ceil(k / 16) + 1 largest; 0 where there are not so many above -inf
+    auto kth_of = [&](float m) {
+        const int each = (p.k + LP_WARPS - 1) / LP_WARPS + 1;
+        uint32_t mine = m > -INFINITY ? (uint32_t)(lp_key(m, 0) >> 32) : 0;
+        for (int r = 0; r < each; ++r) {
+            const uint32_t top = __reduce_max_sync(0xffffffffu, mine);
+            if (lane == __ffs(__ballot_sync(0xffffffffu, mine == top)) - 1) mine = 0;
+            if (lane == 0) tops[r * LP_WARPS + warp] = top;
         }
+        __syncthreads();
+        const int n = each * LP_WARPS;
+        if (tid < n) {
+            const uint32_t top = tops[tid];
+            int larger = 0;
+#pragma unroll 8
+            for (int i = 0; i < n; ++i) larger += tops[i] >= top + (i >= tid ? 1u : 0u);      // equal ones: the first counts as larger
+            if (larger == p.k - 1) bound_v = top;
+        }
+        __syncthreads();
+        return bound_v;
+    };
+    auto value_of = [](uint32_t ordered) { return ordered ? lp_value((u64)ordered << 32) : -INFINITY; };
+    // entry j of n has index i0 + (j / VN) * stride + j % VN
+    auto offer = [&](auto& v, int n, int i0, int stride) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+            if (j < n && v[j] >= bound_x && v[j] > -INFINITY) {
+                const int at = atomicAdd(&ncand, 1);
+                if (at < LP_CAND) cand[R ? at : 0] = lp_key(v[j], i0 + (j / VN) * stride + j % VN);
+            }
+    };
+    auto add = [&](auto& v, int n, float m) {
         if (m > q.m) {
             const float d = lp_max_nan((q.m - m) * c, LP_FLOOR), r = lp_ex2(d);
             q.t = fmaf(q.s, d, q.t) * r;
@@ -232,36 +279,40 @@ __global__ void __launch_bounds__(LP_THREADS, 2) token_logprobs_kernel(const __g
         }
         const float m0 = q.m == -INFINITY ? 0.f : q.m;
 #pragma unroll
-        for (int j = 0; j < LP_VECS * VN; ++j) {
-            if (j >= n) break;
-            const float a = lp_max_nan((v[j] - m0) * c, LP_FLOOR), e = lp_ex2(a);
-            q.s += e;
-            q.t = fmaf(a, e, q.t);
-        }
+        for (int j = 0; j < 16; ++j)
+            if (j < n) {
+                const float a = lp_max_nan((v[j] - m0) * c, LP_FLOOR), e = lp_ex2(a);
+                q.s += e;
+                q.t = fmaf(a, e, q.t);
+            }
     };
 
-    const uint4 none = make_uint4(0, 0, 0, 0);
-    for (int b = v0; b < v1; b += LP_THREADS * LP_VECS) {
-        float v[LP_VECS * VN];
-        uint4 w[LP_VECS];
+    for (int b = v0, round = 1; b < v1; b += LP_THREADS * VECS, ++round) {
+        float v[16];
 #pragma unroll
-        for (int u = 0; u < LP_VECS; ++u) { const int i = b + u * LP_THREADS + tid; w[u] = i < v1 ? lp_load(xv + i) : none; }
-#pragma unroll
-        for (int u = 0; u < LP_VECS; ++u) {
+        for (int u = 0; u < VECS; ++u) {
             LpVec<T>::get(w[u], v + u * VN);
             if (b + u * LP_THREADS + tid >= v1) {
 #pragma unroll
                 for (int j = 0; j < VN; ++j) v[u * VN + j] = -INFINITY;
             }
         }
-        take(v, LP_VECS * VN, head + (b + tid) * VN, LP_THREADS * VN, head + v1 * VN);
+        load(b + LP_THREADS * VECS);
+        float m = v[0];
+#pragma unroll
+        for (int j = 1; j < 16; ++j) m = fmaxf(m, v[j]);
+        if (R) {
+            if (!(round & (round - 1)) && (round & 0x55555555)) bound_x = value_of(kth_of(fmaxf(m, q.m)));
+            if (m >= bound_x && m > -INFINITY) offer(v, 16, head + (b + tid) * VN, LP_THREADS * VN);
+        }
+        add(v, 16, m);
     }
     if (rank == 0 && warp == 0) {                      // the entries beside the whole vectors, one a lane
-        float v[LP_VECS * VN];
+        float v[16];
         const int i = lane < 16 ? lane : head + nvec * VN + lane - 16;
-        const bool in = lane < 16 ? lane < head : lane - 16 < tail;
-        v[0] = in ? LpVec<T>::one(x[i]) : -INFINITY;
-        take(v, 1, in ? i : p.V, 0, p.V);
+        v[0] = (lane < 16 ? lane < head : lane - 16 < tail) ? LpVec<T>::one(x[i]) : -INFINITY;
+        if (R) offer(v, 1, i, 0);
+        add(v, 1, v[0]);
     }
 
     // ---- a row's parts together: lanes, warps, blocks of the cluster
@@ -271,33 +322,52 @@ __global__ void __launch_bounds__(LP_THREADS, 2) token_logprobs_kernel(const __g
         q = lp_join(q, other, c);
     }
     if (lane == 0) { part[warp][0] = q.m; part[warp][1] = q.s; part[warp][2] = q.t; }
-    if (R && npend) flush();
     __syncthreads();
-    auto gather = [&](int n) {                         // lists 0 .. n-1 of this block into list 0
-        for (int half = n >> 1; half; half >>= 1) {
-            if (warp < half) {
-                u64 mine[RL], other[RL];
-#pragma unroll
-                for (int r = 0; r < RL; ++r) { mine[r] = list[r * 32 + lane]; other[r] = lists[R ? warp + half : 0][r * 32 + lane]; }
-                lp_merge<RL>(mine, other, lane);
-#pragma unroll
-                for (int r = 0; r < RL; ++r) list[r * 32 + lane] = mine[r];
-            }
-            __syncthreads();
-        }
-    };
     auto sums_of = [&](int n) {                        // the first n parts, in every lane of a warp
         Sums a = {-INFINITY, 0.f, 0.f};
         if (lane < n) a = {part[lane][0], part[lane][1], part[lane][2]};
 #pragma unroll
-        for (int o = 16; o; o >>= 1) {
+        for (int o = LP_WARPS / 2; o; o >>= 1) {
             const Sums other = {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o), __shfl_xor_sync(0xffffffffu, a.t, o)};
             a = lp_join(a, other, c);
         }
+        a.m = __shfl_sync(0xffffffffu, a.m, 0); a.s = __shfl_sync(0xffffffffu, a.s, 0); a.t = __shfl_sync(0xffffffffu, a.t, 0);
         return a;
     };
-    if (R) gather(LP_WARPS);
+    // the k largest of the first n candidates into list 0, a thread for each
+    auto place = [&](int n) {
+        for (int i = tid; i < n; i += LP_THREADS) {
+            const u64 key = cand[R ? i : 0];
+            int at = 0;
+#pragma unroll 8
+            for (int j = 0; j < n; ++j) at += cand[R ? j : 0] > key;
+            if (at < p.k) lists[R ? at : 0] = key;
+        }
+        __syncthreads();
+    };
     if (warp == 0) q = sums_of(LP_WARPS);
+    if (R) {
+        int n = ncand;
+        if (n > LP_CAND) {
+            const int i0 = rank ? head + v0 * VN : 0, i1 = rank == cs - 1 ? p.V : head + v1 * VN;
+            lp_again<T, RL>(x, i0, i1, p.k, bound_v ? ((u64)bound_v << 32) - 1 : 0, lists, cand, &bound_s);
+        } else {
+            if (n > 128) {                             // only those that reach the bound of all of them
+                u64 mine[LP_CAND / LP_THREADS], top = 0;
+#pragma unroll
+                for (int r = 0; r < LP_CAND / LP_THREADS; ++r) { mine[r] = r * LP_THREADS + tid < n ? cand[r * LP_THREADS + tid] : 0; top = lp_max(top, mine[r]); }
+                const uint32_t least = kth_of(top ? lp_value(top) : -INFINITY);
+                if (tid == 0) ncand = 0;
+                __syncthreads();
+#pragma unroll
+                for (int r = 0; r < LP_CAND / LP_THREADS; ++r)
+                    if (mine[r] && (uint32_t)(mine[r] >> 32) >= least) cand[atomicAdd(&ncand, 1)] = mine[r];
+                __syncthreads();
+                n = ncand;
+            }
+            place(n);
+        }
+    }
     if (cs > 1) {
         __syncthreads();
         if (tid == 0) { part[0][0] = q.m; part[0][1] = q.s; part[0][2] = q.t; }
@@ -305,14 +375,26 @@ __global__ void __launch_bounds__(LP_THREADS, 2) token_logprobs_kernel(const __g
         if (rank == 0) {
             Sums mine = {0.f, 0.f, 0.f};
             if (warp == 0 && lane < cs) mine = {lp_peer(&part[0][0], lane), lp_peer(&part[0][1], lane), lp_peer(&part[0][2], lane)};
-            if (R && warp > 0 && warp < cs) {
-#pragma unroll
-                for (int r = 0; r < RL; ++r) list[r * 32 + lane] = lp_peer(&lists[0][r * 32 + lane], warp);
-            }
+            // every block's list is sorted: a key's place is its own plus, of each other list, how many are larger
+            const int of = R ? tid / p.k : 0, own = R ? tid - of * p.k : 0;
+            if (R && tid < cs * p.k) cand[tid] = lp_peer(&lists[own], of);         // at most 8 x 64
             __syncwarp();
             if (warp == 0 && lane < cs) { part[lane][0] = mine.m; part[lane][1] = mine.s; part[lane][2] = mine.t; }
             __syncthreads();
-            if (R) gather(cs);
+            if (R) {
+                if (tid < p.k) lists[tid] = 0;         // (read by the copies above)
+                __syncthreads();
+                const u64 key = tid < cs * p.k ? cand[tid] : 0;
+                int at = own;
+                for (int r = 0; key && r < cs; ++r) {
+                    if (r == of) continue;
+                    int lo = 0, hi = p.k;
+                    while (lo < hi) { const int mid = (lo + hi) >> 1; if (cand[r * p.k + mid] > key) lo = mid + 1; else hi = mid; }
+                    at += lo;
+                }
+                if (key && at < p.k) lists[at] = key;
+                __syncthreads();
+            }
             if (warp == 0) q = sums_of(cs);
         }
         asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");   // nobody leaves while its shared memory may be read
@@ -326,14 +408,24 @@ __global__ void __launch_bounds__(LP_THREADS, 2) token_logprobs_kernel(const __g
         p.logprob[row] = bad || x_tok != x_tok ? nan : empty ? -INFINITY : LP_LN2 * ((x_tok - q.m) * c - ls);
     }
     if (R) {
+        int have = 0;
 #pragma unroll
         for (int r = 0; r < RL; ++r) {
             const int at = r * 32 + lane;
-            if (at >= p.k) continue;
-            const u64 key = list[at];
-            p.top_id[(size_t)row * p.k + at] = key ? (int)~(uint32_t)key : -1;
-            p.top_logprob[(size_t)row * p.k + at] = bad || !key ? nan : empty ? -INFINITY : LP_LN2 * ((lp_value(key) - q.m) * c - ls);
+            const u64 key = at < p.k ? lists[at] : 0;
+            have += __popc(__ballot_sync(0xffffffffu, key != 0));
+            if (!key) continue;
+            p.top_id[(size_t)row * p.k + at] = (int)~(uint32_t)key;
+            p.top_logprob[(size_t)row * p.k + at] = bad ? nan : LP_LN2 * ((lp_value(key) - q.m) * c - ls);
         }
+        for (int b = 0; have < p.k && b < p.V; b += 32) {      // the others are -inf: the lowest indices of those
+            const bool low = b + lane < p.V && LpVec<T>::one(x[b + lane]) == -INFINITY;
+            const uint32_t who = __ballot_sync(0xffffffffu, low);
+            const int at = have + __popc(who & ((1u << lane) - 1));
+            if (low && at < p.k) { p.top_id[(size_t)row * p.k + at] = b + lane; p.top_logprob[(size_t)row * p.k + at] = bad ? nan : -INFINITY; }
+            have += __popc(who);
+        }
+        for (int at = have + lane; at < p.k; at += 32) { p.top_id[(size_t)row * p.k + at] = -1; p.top_logprob[(size_t)row * p.k + at] = nan; }
     }
 }
 
