@@ -117,7 +117,6 @@ __global__ void __launch_bounds__(I8 ? PX_THREADS8 : PX_THREADS, 1) prefix_attn_
     extern __shared__ unsigned char smem_raw[];
     __shared__ __align__(8) uint64_t q_full[2], kv_full[PX_STAGES], kv_empty[PX_STAGES], tail_full, raw_full[PX_RAW], raw_empty[PX_RAW], s_full[2][2], p_full[2][2], o_full[2], o_end[2], drained[2];
     __shared__ uint32_t tmem_base_s;
-    __shared__ float2 other_ml[PX_ROWS];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int rows = p.B * p.G, pairs = (rows + 2 * PX_ROWS - 1) / (2 * PX_ROWS);
     const int pr = blockIdx.x % pairs, kvh = blockIdx.x / pairs % p.Hkv, split = blockIdx.x / pairs / p.Hkv;
@@ -145,6 +144,7 @@ __global__ void __launch_bounds__(I8 ? PX_THREADS8 : PX_THREADS, 1) prefix_attn_
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_s)), "n"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    if (tid == 8 * 32) asm volatile("prefetch.tensormap [%0];" ::"l"(&tmap) : "memory");
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -161,9 +161,10 @@ __global__ void __launch_bounds__(I8 ? PX_THREADS8 : PX_THREADS, 1) prefix_attn_
         auto here = [&](int i) { return lane < 8 && off < PX_KEYS && key0 + i * PX_KEYS + off < key1; };       // this lane's box of tile i holds keys
         auto page_of = [&](int i) { return here(i) ? ldcg_i32(p.table + (key0 + i * PX_KEYS + off) / p.page_size) : 0; };
         bool ok = true;
-        int st = 0, lap = 0, page = page_of(0), i = 0;
+        int st = 0, lap = 0, i = 0;
+        int page = page_of(0), page1 = page_of(1), page2 = page_of(2), page3 = page_of(3);      // a tile's entry is asked for four tiles ahead
         for (; i < nt; ++i) {
-            const int next = page_of(i + 1);
+            const int next = page_of(i + 4);
             const bool mine = here(i), tail = !I8 && i == nt - 1 && fix_row < PX_KEYS;
             const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, mine));
             uint64_t* full = tail ? &tail_full : &fulls[st];
@@ -178,7 +179,9 @@ __global__ void __launch_bounds__(I8 ? PX_THREADS8 : PX_THREADS, 1) prefix_attn_
                                  ::"r"(ring + st * step + h * PX_HALF), "l"(&tmap), "r"(h * 64), "r"(slot), "r"(block), "r"(smem_u32(full)) : "memory");
             }
             __syncwarp();
-            page = next;
+            page = page1; page1 = page2; page2 = page3; page3 = next;
+            // the other tiles wait until the queries are there, which would queue behind them (the ring's first filling takes all SMs' bandwidth)
+            if (i == 1) { px_wait_warp(&q_full[0], 0); if (!alt) px_wait_warp(&q_full[1], 0); }
             if (tail) {                                    // its keyless value rows are cleared before the tile is handed on
                 ok = px_wait_warp(&tail_full, 0);
                 for (int c = lane; ok && c < (PX_KEYS - fix_row) * 16; c += 32) {
@@ -301,6 +304,7 @@ __global__ void __launch_bounds__(I8 ? PX_THREADS8 : PX_THREADS, 1) prefix_attn_
         const uint32_t s_t = tmem + t * 256 + lane_base, o_t = s_t + 128;
         const bool r_ok = r < rows;
         const int tiles = alt ? (nt - t + 1) / 2 : nt;
+        const bool idle = r - lane >= rows;               // none of the warp's rows exists: it only keeps the others company
         const bool flat = p.scale_log2e == 0.f;           // zero queries: every score is 0, but for the masked ones
         const float unit = flat ? 1.f : fabsf(p.scale_log2e);       // a negative scale turns the queries' signs
         if (t == 0 || !alt) {
@@ -330,6 +334,10 @@ __global__ void __launch_bounds__(I8 ? PX_THREADS8 : PX_THREADS, 1) prefix_attn_
             const uint32_t s_n = s_t + (n & 1) * PX_KEYS;
             if (!px_wait_warp(&s_full[t][n & 1], (uint32_t)((n >> 1) & 1))) { ok = false; break; }
             tc_fence_after();
+            if (idle) {
+                if (lane == 0) mbar_arrive(&p_full[t][n & 1]);
+                continue;
+            }
             uint32_t s[PX_KEYS];
             TC_LD32(s_n, (s + 0));
             TC_LD32(s_n + 32, (s + 32));
@@ -405,61 +413,61 @@ __global__ void __launch_bounds__(I8 ? PX_THREADS8 : PX_THREADS, 1) prefix_attn_
             px_unpair(px_add2(ls[0], ls[1]), l0, l1);
             l += l0 + l1;
         }
-        // ---- the group's output: alone, or with that of the other group, whose half lies in the ring by then
+        // ---- the group's output.  Groups of the same rows hand each other a half of the columns through the ring, when no product reads it any more, and each
+        // finishes the half that it keeps
+        const bool joined = alt && nt > 1;
         if (ok && tiles > 0) ok = px_wait_warp(&o_end[t], 0);
-        if (alt) {
-            if (t == 1) {
-                // the ring is read by neither group's products any more
-                if (ok) ok = px_wait_warp(&o_end[0], 0);
-                other_ml[tr] = ok && tiles > 0 ? make_float2(m_ref, l) : make_float2(-INFINITY, 0.f);
-            }
-            if (t == 1 && ok && tiles > 0) {
-                tc_fence_after();
-#pragma unroll 1
-                for (int c = 0; c < AT_D; c += 32) {
-                    uint32_t o[32];
-                    __syncwarp();
-                    TC_LD32(o_t + c, o);
-                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        if (joined && ok) ok = px_wait_warp(&o_end[1 - t], 0);
+        tc_fence_after();
+        const uint32_t ml_s = k_s + 2 * PX_ROWS * 256 + tr * 8;
+        const uint32_t mine = k_s + (uint32_t)t * PX_ROWS * 256 + tr * 16, theirs = k_s + (uint32_t)(1 - t) * PX_ROWS * 256 + tr * 16;
+        if (joined && ok && !idle) {
+            uint32_t o[64];
+            TC_LD32(o_t + (1 - t) * 64, (o + 0));
+            TC_LD32(o_t + (1 - t) * 64 + 32, (o + 32));
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-                    for (int k = 0; k < 32; k += 4)
-                        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(k_s + (((c + k) >> 2) * PX_ROWS + tr) * 16), "r"(o[k]), "r"(o[k + 1]), "r"(o[k + 2]), "r"(o[k + 3]) : "memory");
-                }
-            }
-            asm volatile("bar.sync 1, 256;" ::: "memory");
+            for (int k = 0; k < 64; k += 4)
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(mine + (k >> 2) * PX_ROWS * 16), "r"(o[k]), "r"(o[k + 1]), "r"(o[k + 2]), "r"(o[k + 3]) : "memory");
+            asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(ml_s + t * PX_ROWS * 8), "f"(m_ref), "f"(l) : "memory");
         }
-        if (ok && (t == 0 || !alt)) {
-            tc_fence_after();
+        if (joined) asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (ok && !idle && (t == 0 || joined || !alt)) {
+            const size_t part = (size_t)split * p.Hkv + kvh;
+            float4* dst = reinterpret_cast<float4*>(p.part_o) + part * 32 * p.rows_p + r;      // rows side by side: a warp's stores are whole lines
             float f0 = 1.f, f1 = 0.f;
-            const bool joined = alt && nt > 1;
             if (joined) {
-                const float2 ml = other_ml[tr];
+                float2 ml;
+                asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(ml.x), "=f"(ml.y) : "r"(ml_s + (1 - t) * PX_ROWS * 8) : "memory");
                 const float m = fmaxf(m_ref, ml.x);
                 f0 = m_ref == -INFINITY ? 0.f : px_ex2(m_ref - m);
                 f1 = ml.x == -INFINITY ? 0.f : px_ex2(ml.x - m);
                 l = l * f0 + ml.y * f1;
                 m_ref = m;
             }
-            const size_t part = (size_t)split * p.Hkv + kvh;
-            float4* dst = reinterpret_cast<float4*>(p.part_o) + part * 32 * p.rows_p + r;      // rows side by side: a warp's stores are whole lines
 #pragma unroll 1
-            for (int c = 0; c < AT_D; c += 32) {
-                uint32_t o[32];
+            for (int c = joined ? t * 64 : 0; c < (joined ? t * 64 + 64 : AT_D); c += 64) {
+                uint32_t o[64];
                 __syncwarp();
-                TC_LD32(o_t + c, o);
+                TC_LD32(o_t + c, (o + 0));
+                TC_LD32(o_t + c + 32, (o + 32));
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                if (joined) {
 #pragma unroll
-                for (int k = 0; k < 32; k += 4) {
-                    float4 v = make_float4(__uint_as_float(o[k]), __uint_as_float(o[k + 1]), __uint_as_float(o[k + 2]), __uint_as_float(o[k + 3]));
-                    if (joined) {
+                    for (int k = 0; k < 64; k += 4) {
                         float4 w;
-                        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(w.x), "=f"(w.y), "=f"(w.z), "=f"(w.w) : "r"(k_s + (((c + k) >> 2) * PX_ROWS + tr) * 16) : "memory");
-                        v.x = fmaf(v.x, f0, w.x * f1); v.y = fmaf(v.y, f0, w.y * f1); v.z = fmaf(v.z, f0, w.z * f1); v.w = fmaf(v.w, f0, w.w * f1);
+                        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(w.x), "=f"(w.y), "=f"(w.z), "=f"(w.w) : "r"(theirs + (k >> 2) * PX_ROWS * 16) : "memory");
+                        o[k] = __float_as_uint(fmaf(__uint_as_float(o[k]), f0, w.x * f1));
+                        o[k + 1] = __float_as_uint(fmaf(__uint_as_float(o[k + 1]), f0, w.y * f1));
+                        o[k + 2] = __float_as_uint(fmaf(__uint_as_float(o[k + 2]), f0, w.z * f1));
+                        o[k + 3] = __float_as_uint(fmaf(__uint_as_float(o[k + 3]), f0, w.w * f1));
                     }
-                    if (r_ok) dst[(size_t)((c + k) >> 2) * p.rows_p] = v;
                 }
+#pragma unroll
+                for (int k = 0; k < 64; k += 4)
+                    if (r_ok) dst[(size_t)((c + k) >> 2) * p.rows_p] = make_float4(__uint_as_float(o[k]), __uint_as_float(o[k + 1]), __uint_as_float(o[k + 2]), __uint_as_float(o[k + 3]));
             }
-            if (r_ok) reinterpret_cast<float2*>(p.part_ml)[part * p.rows_p + r] = make_float2(m_ref, l);
+            if (r_ok && (t == 0 || !alt)) reinterpret_cast<float2*>(p.part_ml)[part * p.rows_p + r] = make_float2(m_ref, l);
         }
         if (!ok && lane == 0) *(volatile int*)p.err = 18;
     }
@@ -550,14 +558,15 @@ __global__ void __launch_bounds__(PX_MERGE) prefix_merge_kernel(const __grid_con
 
 int px_rows_p(int B, int G) { return (B * G + 31) / 32 * 32; }
 
-// splits of the prefix and their keys
+// Splits of the prefix and their keys, in units of a hundredth of what two tiles take a block (1.95 us): a block costs 300 beside its tiles (queries in, results out),
+// and every split what the merge reads of it.
 void px_cut(int B, int H, int Hkv, int prefix, int* splits, int* keys) {
     const int tiles = (prefix + 2 * PX_KEYS - 1) / (2 * PX_KEYS);        // pairs of tiles: one for each group
     const long long rows = (long long)B * (H / Hkv), units = Hkv * ((rows + 2 * PX_ROWS - 1) / (2 * PX_ROWS));
     int best = 1;
     long long least = -1;
-    for (int n = 1; n <= tiles && n <= 148; ++n) {
-        const long long waves = (units * n + sm_count() - 1) / sm_count(), cost = waves * ((tiles + n - 1) / n + 3) * 100 + n * 20;
+    for (int n = 1; n <= tiles && n <= sm_count(); ++n) {
+        const long long waves = (units * n + sm_count() - 1) / sm_count(), cost = waves * ((tiles + n - 1) / n + 3) * 100 + n * (5 + (long long)B * H / 60);
         if (least < 0 || cost < least) { least = cost; best = n; }
     }
     *keys = (tiles + best - 1) / best * 2 * PX_KEYS;

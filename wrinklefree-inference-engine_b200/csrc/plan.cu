@@ -16,7 +16,7 @@ namespace wf {
 namespace {
 
 constexpr int PL_THREADS = 512, PL_SMALL = 128;
-constexpr int PL_MAX_ROWS = 8192;                     // two sums and a length of every request: 96 KB of shared memory
+constexpr int PL_MAX_ROWS = 8192;                     // four numbers of every request: 128 KB of shared memory
 
 struct PlanParams {
     const int32_t *seq, *fresh;    // cached and new tokens of each request
@@ -24,11 +24,12 @@ struct PlanParams {
     int32_t* table;
     int32_t* free_pages;
     const int32_t* free_count;
-    int rows, max_blocks, pool_pages, page, shift, cap;   // shift: log2(page), or -1
+    int rows, max_blocks, pool_pages, page, cap;
+    uint32_t mul, shift;           // x / page = x * mul >> shift for x below 2^31
     int32_t *positions, *token_rows, *pages, *slots, *offsets, *lens_out, *count_out, *status;
 };
 
-__device__ __forceinline__ int pl_div(const PlanParams& p, int x) { return p.shift >= 0 ? x >> p.shift : (int)((unsigned)x / (unsigned)p.page); }
+__device__ __forceinline__ int pl_div(const PlanParams& p, int x) { return (int)((unsigned long long)(unsigned)x * p.mul >> p.shift); }
 __device__ __forceinline__ int pl_blocks(const PlanParams& p, int x) { return x > 0 ? pl_div(p, x - 1) + 1 : 0; }
 __device__ __forceinline__ long long pl_warp_scan(long long v, int lane) {
 #pragma unroll
@@ -42,10 +43,10 @@ __device__ __forceinline__ int pl_find(const int* first, int n, int x) {
     return lo;
 }
 
-// Sums over the requests.  tok[i], blk[i]: tokens and pages in front of request i (entry `rows`: all of them); seq[i]: its cached tokens.  Returns the status,
-// the same in every thread; with a status the sums mean nothing.
+// Sums over the requests.  tok[i], blk[i]: tokens and pages in front of request i (entry `rows`: all of them); seq[i], old[i]: its cached tokens and their pages.
+// Returns the status, the same in every thread; with a status the sums mean nothing.
 template <bool RELEASE>
-__device__ __forceinline__ int pl_sums(const PlanParams& p, int count, int* tok, int* blk, int* seq) {
+__device__ __forceinline__ int pl_sums(const PlanParams& p, int count, int* tok, int* blk, int* seq, int* old) {
     __shared__ long long w_tok[32], w_blk[32];
     __shared__ int w_status[32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5;
@@ -65,7 +66,8 @@ __device__ __forceinline__ int pl_sums(const PlanParams& p, int count, int* tok,
             const int n = p.fresh[r];
             if (s < 0 || n < 0 || s > 0x7fffffff - n) status |= WF_PLAN_LENGTH;
             else {
-                const int after = pl_blocks(p, s + n), need = after - pl_blocks(p, s);
+                const int before = pl_blocks(p, s), after = pl_blocks(p, s + n), need = after - before;
+                old[r] = before;
                 if (after > p.max_blocks) status |= WF_PLAN_BLOCKS;
                 tok[r] = n;
                 blk[r] = need;
@@ -98,10 +100,10 @@ __device__ __forceinline__ int pl_sums(const PlanParams& p, int count, int* tok,
 
 __global__ void __launch_bounds__(PL_THREADS) paged_plan_kernel(const __grid_constant__ PlanParams p) {
     extern __shared__ int pl_smem[];
-    int *tok = pl_smem, *blk = tok + p.rows + 1, *seq = blk + p.rows + 1;
+    int *tok = pl_smem, *blk = tok + p.rows + 1, *seq = blk + p.rows + 1, *old = seq + p.rows + 1;
     pdl_wait_prior();
     pdl_launch_dependents();
-    const int count = *p.free_count, status = pl_sums<false>(p, count, tok, blk, seq);
+    const int count = *p.free_count, status = pl_sums<false>(p, count, tok, blk, seq, old);
     const int total = status || !p.rows ? 0 : tok[p.rows], n_pages = status || !p.rows ? 0 : blk[p.rows];
     const int first = blockIdx.x * blockDim.x + threadIdx.x, step = gridDim.x * blockDim.x;
     if (blockIdx.x == gridDim.x - 1) {
@@ -121,10 +123,10 @@ __global__ void __launch_bounds__(PL_THREADS) paged_plan_kernel(const __grid_con
                 if (t >= total) break;
                 while (t >= tok[r + 1]) ++r;           // requests without new tokens are passed over
                 pos[k] = seq[r] + (t - tok[r]);
-                const int b = pl_div(p, pos[k]), old = pl_blocks(p, seq[r]);
+                const int b = pl_div(p, pos[k]), fresh = b - old[r];
                 row[k] = r;
                 slot[k] = pos[k] - b * p.page;
-                page[k] = b < old ? p.table[(size_t)r * p.max_blocks + b] : p.free_pages[count - 1 - (blk[r] + b - old)];
+                page[k] = fresh < 0 ? p.table[(size_t)r * p.max_blocks + b] : p.free_pages[count - 1 - (blk[r] + fresh)];
             }
         }
         if (4 * q + 4 <= p.cap) {
@@ -140,7 +142,7 @@ __global__ void __launch_bounds__(PL_THREADS) paged_plan_kernel(const __grid_con
     }
     for (int k = first; k < n_pages; k += step) {
         const int r = pl_find(blk, p.rows, k);
-        p.table[(size_t)r * p.max_blocks + pl_blocks(p, seq[r]) + (k - blk[r])] = p.free_pages[count - 1 - k];
+        p.table[(size_t)r * p.max_blocks + old[r] + (k - blk[r])] = p.free_pages[count - 1 - k];
     }
 }
 
@@ -149,7 +151,7 @@ __global__ void __launch_bounds__(PL_THREADS) paged_release_kernel(const __grid_
     int *blk = pl_smem, *seq = blk + p.rows + 1;
     pdl_wait_prior();
     pdl_launch_dependents();
-    const int count = *p.free_count, status = pl_sums<true>(p, count, nullptr, blk, seq);
+    const int count = *p.free_count, status = pl_sums<true>(p, count, nullptr, blk, seq, nullptr);
     const int n_pages = status || !p.rows ? 0 : blk[p.rows];
     if (blockIdx.x == gridDim.x - 1) {
         for (int r = threadIdx.x; r < p.rows; r += blockDim.x) p.lens_out[r] = !status && p.done[r] ? 0 : seq[r];
@@ -165,8 +167,12 @@ int pl_check(const char* who, PlanParams& p) {
     if (p.rows < 0 || p.max_blocks < 0 || p.pool_pages < 0 || p.cap < 0) { set_error("%s: negative size", who); return WF_ERR_INVALID; }
     if (p.page <= 0) { set_error("%s: page_size must be positive (got %d)", who, p.page); return WF_ERR_INVALID; }
     if (p.rows > PL_MAX_ROWS) { set_error("%s: at most %d requests (got %d)", who, PL_MAX_ROWS, p.rows); return WF_ERR_UNSUPPORTED; }
-    p.shift = -1;
-    if (!(p.page & (p.page - 1))) { p.shift = 0; while ((1 << p.shift) < p.page) ++p.shift; }
+    // with 2^(l-1) < page <= 2^l, mul = ceil(2^(31+l) / page) is below 2^32 and exceeds 2^(31+l) / page by less than 1: x * mul / 2^(31+l) is above x / page by less
+    // than 2^-l <= 1 / page, which does not reach the next whole number
+    uint32_t l = 0;
+    while (l < 31 && (1u << l) < (uint32_t)p.page) ++l;
+    p.shift = 31 + l;
+    p.mul = (uint32_t)(((1ull << p.shift) + p.page - 1) / p.page);
     return WF_OK;
 }
 
@@ -174,7 +180,7 @@ DevOnce g_pl_attr;
 
 int pl_attrs() {
     if (!g_pl_attr.need()) return WF_OK;
-    if (cuda_check(cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 3 * (PL_MAX_ROWS + 1) * 4), "wf_paged_plan")) return WF_ERR_CUDA;
+    if (cuda_check(cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * (PL_MAX_ROWS + 1) * 4), "wf_paged_plan")) return WF_ERR_CUDA;
     return cuda_check(cudaFuncSetAttribute(paged_release_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * (PL_MAX_ROWS + 1) * 4), "wf_paged_release");
 }
 int pl_threads(const PlanParams& p, long long items) { return p.rows <= PL_SMALL && items <= PL_SMALL ? PL_SMALL : PL_THREADS; }
@@ -202,7 +208,7 @@ extern "C" int wf_paged_plan(const int32_t* seq_lens, const int32_t* new_lens, i
     if (((uintptr_t)positions | (uintptr_t)token_rows | (uintptr_t)pages | (uintptr_t)slots) & 15) { set_error("wf_paged_plan: the token maps must be 16-byte aligned"); return WF_ERR_INVALID; }
     if (int rc = pl_attrs()) return rc;
     const long long items = ((long long)max_tokens + 3) / 4;
-    return launch_check(launch_pdl(paged_plan_kernel, pl_grid(p, items), pl_threads(p, items), 3 * (rows + 1) * 4, (cudaStream_t)stream, p), "wf_paged_plan");
+    return launch_check(launch_pdl(paged_plan_kernel, pl_grid(p, items), pl_threads(p, items), 4 * (rows + 1) * 4, (cudaStream_t)stream, p), "wf_paged_plan");
 }
 
 extern "C" int wf_paged_release(const uint8_t* done, const int32_t* seq_lens, int rows, const int32_t* block_table, int max_blocks, int32_t* free_pages, int pool_pages,

@@ -217,6 +217,15 @@ int to_int(int64_t v, const char* name) {
     return (int)v;
 }
 
+// A contiguous tensor over part of `buf`, `at` entries of its own type from the start: the outputs of a call share one allocation (1.6 us each otherwise, and a
+// slice through the dispatcher 0.9 us)
+Tensor part_of(const Tensor& buf, at::ScalarType type, int64_t at, at::IntArrayRef sizes) {
+    auto impl = c10::make_intrusive<c10::TensorImpl>(c10::TensorImpl::VIEW, c10::Storage(buf.storage()), buf.key_set(), c10::scalarTypeToTypeMeta(type));
+    impl->set_storage_offset(at);
+    impl->set_sizes_contiguous(sizes);
+    return Tensor(std::move(impl));
+}
+
 Tensor paged_prefix_attn(const Tensor& q, const Tensor& pool, int64_t max_pages, int64_t layers, int64_t kv_heads, int64_t page_size, int64_t head_dim, int64_t kv_dtype,
                          int64_t layer, const Tensor& prefix_table, int64_t prefix_len, const Tensor& block_table, const Tensor& seq_lens, double scale, at::ScalarType out_dtype) {
     need_gpu({&q, &pool, &prefix_table, &block_table, &seq_lens});
@@ -263,7 +272,7 @@ std::vector<Tensor> paged_plan(const Tensor& seq_lens, const Tensor& new_lens, T
     const Tensor sl = seq_lens.contiguous(), nl = new_lens.contiguous(), fp = free_pages.contiguous();
     const int rows = to_int(B, "block_table"), cap = to_int(max_tokens, "max_tokens"), page = to_int(page_size, "page_size");
     const int64_t cap4 = (max_tokens + 3) / 4 * 4;         // every map starts on 16 bytes
-    Tensor buf = at::empty({4 * cap4 + 2 * B + 3}, block_table.options());
+    const Tensor buf = at::empty({4 * cap4 + 2 * B + 3}, block_table.options());
     const int64_t at[8] = {0, cap4, 2 * cap4, 3 * cap4, 4 * cap4, 4 * cap4 + B + 1, 4 * cap4 + 2 * B + 1, 4 * cap4 + 2 * B + 2};
     const int64_t len[8] = {max_tokens, max_tokens, max_tokens, max_tokens, B + 1, B, 1, 1};
     int32_t* base = (int32_t*)buf.data_ptr();
@@ -272,7 +281,7 @@ std::vector<Tensor> paged_plan(const Tensor& seq_lens, const Tensor& new_lens, T
                         base + at[4], base + at[5], base + at[6], base + at[7], stream()));
     std::vector<Tensor> out;
     out.reserve(8);
-    for (int i = 0; i < 8; ++i) out.push_back(buf.narrow(0, at[i], len[i]));
+    for (int i = 0; i < 8; ++i) out.push_back(part_of(buf, at::kInt, at[i], {len[i]}));
     return out;
 }
 
@@ -289,7 +298,8 @@ std::tuple<Tensor, Tensor> paged_release(const Tensor& done, const Tensor& seq_l
     TORCH_CHECK_VALUE(free_count.size(0) == 1, "free_count must have one entry");
     TORCH_CHECK_VALUE(free_pages.is_contiguous(), "free_pages must be contiguous (it is written in place)");
     const Tensor dn = done.contiguous(), sl = seq_lens.contiguous(), bt = block_table.contiguous();
-    Tensor lens = at::empty({B}, sl.options()), count = at::empty({1}, sl.options());
+    const Tensor buf = at::empty({B + 1}, sl.options());
+    Tensor lens = part_of(buf, at::kInt, 0, {B}), count = part_of(buf, at::kInt, B, {1});
     check(wf_paged_release((const uint8_t*)dn.data_ptr(), (const int32_t*)sl.data_ptr(), to_int(B, "block_table"), (const int32_t*)bt.data_ptr(), to_int(bt.size(1), "block_table"),
                            (int32_t*)free_pages.data_ptr(), to_int(free_pages.size(0), "free_pages"), (const int32_t*)free_count.data_ptr(), to_int(page_size, "page_size"),
                            (int32_t*)lens.data_ptr(), (int32_t*)count.data_ptr(), stream()));
@@ -307,8 +317,9 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor& logits, 
     const int n = to_int(x.size(0), "rows"), V = to_int(x.size(1), "vocab"), k = to_int(top, "top");
     const int64_t ld = n > 1 ? x.stride(0) : V;
     const Tensor& y = ld < V ? x.contiguous() : x;         // rows that overlap (an expanded row)
-    const auto f32 = x.options().dtype(at::kFloat);
-    Tensor lp = at::empty({n}, f32), ent = at::empty({n}, f32), tlp = at::empty({n, k}, f32), tid = at::empty({n, k}, x.options().dtype(at::kInt));
+    const int64_t m = n, mk = m * k;
+    const Tensor buf = at::empty({2 * (m + mk)}, x.options().dtype(at::kFloat));
+    Tensor lp = part_of(buf, at::kFloat, 0, {m}), ent = part_of(buf, at::kFloat, m, {m}), tlp = part_of(buf, at::kFloat, 2 * m, {m, k}), tid = part_of(buf, at::kInt, 2 * m + mk, {m, k});
     check(wf_token_logprobs(y.data_ptr(), dt, n, V, ld < V ? V : ld, (const int32_t*)tk.data_ptr(), k, (float)temperature, (float*)lp.data_ptr(), (float*)ent.data_ptr(),
                             (float*)tlp.data_ptr(), (int32_t*)tid.data_ptr(), stream()));
     return {lp, ent, tlp, tid};
