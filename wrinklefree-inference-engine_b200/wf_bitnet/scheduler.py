@@ -60,7 +60,7 @@ def execute(model, entries: Sequence[Tuple[int, Sequence[int]]], want: Sequence[
     cursor = [0] * len(entries)
     done, last_rows = 0, 0
     while done < total:
-        slots, counts, toks, w_local, w_global, room = [], [], [], [], [], limit
+        slots, counts, toks, wanted, room = [], [], [], [], limit
         for ei, (slot, t) in enumerate(entries):
             if room == 0:
                 break
@@ -74,15 +74,15 @@ def execute(model, entries: Sequence[Tuple[int, Sequence[int]]], want: Sequence[
             toks.extend(int(x) for x in t[lo:hi])
             for ti, k in want_at.get(ei, ()):
                 if lo <= ti < hi:
-                    w_local.append(base + ti - lo)
-                    w_global.append(k)
+                    wanted.append((k, base + ti - lo))
             cursor[ei] = hi
             room -= hi - lo
-        out = model.step(slots, counts, toks, w_local, fetch)
-        if rows is not None and w_global:
-            rows[w_global] = out
+        wanted.sort()                                              # the rows that stay on the device stand in the order of `want`, too
+        out = model.step(slots, counts, toks, [i for _, i in wanted], fetch)
+        if rows is not None and wanted:
+            rows[[k for k, _ in wanted]] = out
         done += len(toks)
-        last_rows = len(w_local)
+        last_rows = len(wanted)
     return rows if fetch else last_rows
 
 
