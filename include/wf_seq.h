@@ -207,6 +207,11 @@ int wf_seq_step(wf_seq_engine* e, int nseq, const int32_t* slots, const int32_t*
 /* Draw one token per wanted row of the last step: temperature <= 0 is greedy; else softmax(logits / temperature) limited to the top_k
  * most likely (0: all) and to the smallest set whose mass reaches top_p (>= 1: all); uniforms: one number in [0, 1) per row. */
 int wf_seq_sample(wf_seq_engine* e, int nwant, float temperature, int top_k, float top_p, const float* uniforms_host, int32_t* next_host);
+/* Of each wanted row of the last step, softmax(logits / temperature) (temperature > 0): the log probability of tokens_host[row] (a token outside the vocabulary:
+ * NaN), the entropy (nats), and the `top` (0..64) most likely tokens, most likely first, equal ones by id (top_logprob_host, top_id_host [nwant, top], null for
+ * top = 0).  Logits of -inf have probability 0.  Synchronous. */
+int wf_seq_logprobs(wf_seq_engine* e, int nwant, const int32_t* tokens_host, int top, float temperature, float* logprob_host, float* entropy_host,
+                    float* top_logprob_host, int32_t* top_id_host);
 void* wf_seq_logits_device(wf_seq_engine* e);
 int wf_seq_launches_last_step(const wf_seq_engine* e);
 

@@ -315,3 +315,12 @@ def test_the_same_through_ctypes(monkeypatch):
                 lambda: ops.paged_release(lens, lens, lens.view(3, 1), lens, count, 16), lambda: ops.paged_plan(lens, new, lens.view(3, 1).cpu(), lens, count, 16, 4)):
         with pytest.raises(ValueError):
             bad()
+
+
+@pytest.mark.parametrize("int8", [False, True])
+def test_tables_far_wider_than_the_sequences(int8):
+    """sequences are cut by their own lengths, whatever the table has room for"""
+    q, kv, layer, pt, prefix, table, lens = case(3, 8, 2, 300, [30, 0, 290], 16, int8)
+    wide = torch.zeros(3, 5000, dtype=torch.int32, device="cuda")
+    wide[:, :table.shape[1]] = table
+    check(q, kv, layer, pt, prefix, wide, lens)

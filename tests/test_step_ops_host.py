@@ -61,12 +61,16 @@ def test_prefix_attention_refusals():
 
 def test_prefix_workspace_holds_both_parts():
     L = _lib.lib()
-    assert L.wf_prefix_attn_workspace_bytes(0, 8, 2, 128, 100, 100) == 0
-    assert L.wf_prefix_attn_workspace_bytes(3, 20, 5, 128, 4096, 0) == L.wf_attn_workspace_bytes(3, 20, 128, 4096)
-    for prefix in (1, 128, 5000, 1 << 20):
-        own = L.wf_attn_workspace_bytes(33, 1, 128, 64)
-        both = L.wf_prefix_attn_workspace_bytes(33, 1, 1, 128, 64, prefix)
-        assert both >= own + 33 * 130 * 4 and (both - own) % 256 == 0        # the own chunks start on a vector's boundary
+    assert L.wf_prefix_attn_workspace_bytes(0, 8, 2, 100, 100) == 0
+    for B, H, Hkv in ((1, 1, 1), (33, 1, 1), (3, 20, 5), (128, 32, 8)):
+        row = 130 * 4                                     # a row's partial result
+        for seq in (16, 256, 257, 4096, 131072):
+            own = L.wf_prefix_attn_workspace_bytes(B, H, Hkv, seq, 0)
+            assert B * H * row * min(64, -(-seq // 256)) <= own <= L.wf_attn_workspace_bytes(B, H, 128, max(seq, 512))
+        own = L.wf_prefix_attn_workspace_bytes(B, H, Hkv, 64, 0)
+        for prefix in (1, 128, 5000, 1 << 20):
+            both = L.wf_prefix_attn_workspace_bytes(B, H, Hkv, 64, prefix)
+            assert both >= own + B * H * row and (both - own) % 256 == 0      # the own chunks start on a vector's boundary
 
 
 def test_logprob_refusals():

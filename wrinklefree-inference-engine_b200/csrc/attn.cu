@@ -16,6 +16,7 @@
 //   head form the (padded) M=16 rows of mma.m16n8k16 bf16: S = Q K^T (fp32), online softmax in fp32 with
 //   exp2, O += P V.  Warps are merged through shared memory; chunks are merged by a second tiny kernel.
 #include <cuda_fp16.h>
+#include <algorithm>
 
 #include "attn_chunks.cuh"
 #include "fused_common.cuh"
@@ -1188,6 +1189,13 @@ int attn_decode(const void* q, const void* pool, int layers, int layer, int Hkv,
     p.out = out; p.out_dtype = out_dtype;
     p.n_out = 1; p.out_ld = H * AT_D; p.out_col0 = 0; p.signal_flag = -1;
     return launch_paged_decode_attn(p, max_seq_hint, ws, ws_bytes, s, pdl);
+}
+
+// launch_paged_decode_attn cuts a sequence into chunks of 256 tokens and more, at most 64 of them or 8 blocks an SM in all
+size_t attn_chunks_bytes(int B, int H, int Hkv, int max_seq) {
+    if (B <= 0 || max_seq <= 0) return 0;
+    const long long pairs = (long long)B * Hkv, most = 8LL * sm_count() / pairs + 1, cut = ((long long)max_seq + 255) / 256 + 1;
+    return (size_t)B * H * (size_t)std::min(cut, std::max(64LL, most)) * (AT_D + 2) * sizeof(float);
 }
 
 int attn_decode_chunks(const void* q, const void* pool, int layers, int layer, int Hkv, int page_size, const int32_t* block_table, int max_blocks, const int32_t* seq_lens, int B, int H,

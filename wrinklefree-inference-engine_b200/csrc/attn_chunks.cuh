@@ -24,7 +24,8 @@ struct AttnChunks {
     const float *part_o, *part_ml;
     int max_chunks, chunk_blocks, min_cb;
 };
-// workspace: wf_attn_workspace_bytes
+// workspace: attn_chunks_bytes
+size_t attn_chunks_bytes(int B, int H, int Hkv, int max_seq);
 int attn_decode_chunks(const void* q, const void* pool, int layers, int layer, int Hkv, int page_size, const int32_t* block_table, int max_blocks, const int32_t* seq_lens, int B, int H,
                        float scale, void* ws, size_t ws_bytes, float* kv_scales, AttnChunks* out, cudaStream_t s);
 

@@ -558,26 +558,26 @@ __global__ void __launch_bounds__(PX_MERGE) prefix_merge_kernel(const __grid_con
 
 int px_rows_p(int B, int G) { return (B * G + 31) / 32 * 32; }
 
-// Splits of the prefix and their keys, in units of a hundredth of what two tiles take a block (1.95 us): a block costs 300 beside its tiles (queries in, results out),
-// and every split what the merge reads of it.
-void px_cut(int B, int H, int Hkv, int prefix, int* splits, int* keys) {
-    const int tiles = (prefix + 2 * PX_KEYS - 1) / (2 * PX_KEYS);        // pairs of tiles: one for each group
-    const long long rows = (long long)B * (H / Hkv), units = Hkv * ((rows + 2 * PX_ROWS - 1) / (2 * PX_ROWS));
+struct PxCut { int splits, keys; size_t bytes; };      // splits of the prefix, their keys, and the bytes of the partial results
+
+// In units of a hundredth of what two tiles take a block (1.95 us): a block costs 300 beside its tiles (queries in, results out), and every split what the
+// merge reads of it.
+PxCut px_cut(int B, int H, int Hkv, int prefix) {
+    if (prefix <= 0) return PxCut{0, 0, 0};
+    const int G = H / Hkv, sms = sm_count(), tiles = (int)(((long long)prefix + 2 * PX_KEYS - 1) / (2 * PX_KEYS));       // pairs of tiles: one for each group
+    const long long rows = (long long)B * G, units = Hkv * ((rows + 2 * PX_ROWS - 1) / (2 * PX_ROWS));
     int best = 1;
     long long least = -1;
-    for (int n = 1; n <= tiles && n <= sm_count(); ++n) {
-        const long long waves = (units * n + sm_count() - 1) / sm_count(), cost = waves * ((tiles + n - 1) / n + 3) * 100 + n * (5 + (long long)B * H / 60);
+    // more than two blocks an SM are for those who have them without splits
+    for (int n = 1; n <= tiles && (n == 1 || units * n <= 2 * sms); ++n) {
+        const long long waves = (units * n + sms - 1) / sms, cost = waves * ((tiles + n - 1) / n + 3) * 100 + n * (5 + rows * Hkv / 60);
         if (least < 0 || cost < least) { least = cost; best = n; }
     }
-    *keys = (tiles + best - 1) / best * 2 * PX_KEYS;
-    *splits = (prefix + *keys - 1) / *keys;
-}
-
-size_t px_bytes(int B, int H, int Hkv, int prefix) {
-    if (prefix <= 0) return 0;
-    int splits, keys;
-    px_cut(B, H, Hkv, prefix, &splits, &keys);
-    return ((size_t)splits * Hkv * px_rows_p(B, H / Hkv) * (AT_D + 2) * sizeof(float) + 255) / 256 * 256;      // the own chunks' vectors follow
+    PxCut c;
+    c.keys = (tiles + best - 1) / best * 2 * PX_KEYS;
+    c.splits = (int)(((long long)prefix + c.keys - 1) / c.keys);
+    c.bytes = ((size_t)c.splits * Hkv * px_rows_p(B, G) * (AT_D + 2) * sizeof(float) + 255) / 256 * 256;                // the own chunks' vectors follow
+    return c;
 }
 
 }  // namespace
@@ -586,21 +586,23 @@ size_t px_bytes(int B, int H, int Hkv, int prefix) {
 
 using namespace wf;
 
-extern "C" size_t wf_prefix_attn_workspace_bytes(int B, int H, int kv_heads, int head_dim, int max_seq, int prefix_len) {
+extern "C" size_t wf_prefix_attn_workspace_bytes(int B, int H, int kv_heads, int max_seq, int prefix_len) {
     if (B <= 0 || H <= 0 || kv_heads <= 0) return 0;
-    return px_bytes(B, H, kv_heads, prefix_len) + (max_seq > 0 ? wf_attn_workspace_bytes(B, H, head_dim, max_seq) : 0);
+    return px_cut(B, H, kv_heads, prefix_len).bytes + attn_chunks_bytes(B, H, kv_heads, max_seq);
 }
 
 extern "C" int wf_paged_prefix_attn(const void* q, const wf_kv_layout* kv, int layer, const int32_t* prefix_table, int prefix_len, const int32_t* block_table, int max_blocks,
                                     const int32_t* seq_lens, int B, int H, float scale, void* out, int out_dtype, void* workspace, size_t workspace_bytes, void* stream) {
     const char* who = "wf_paged_prefix_attn";
-    if (prefix_len < 0 || max_blocks < 0 || B < 0) { set_error("%s: negative size", who); return WF_ERR_INVALID; }
+    if (prefix_len < 0 || max_blocks < 0 || B < 0 || H <= 0) { set_error("%s: bad size (B %d, H %d, prefix %d, blocks %d)", who, B, H, prefix_len, max_blocks); return WF_ERR_INVALID; }
     const bool pointers = B == 0 || (q && out && (prefix_len == 0 || prefix_table) && (max_blocks == 0 || (block_table && seq_lens)));
     if (int rc = check_decode_attn(kv, layer, H, out_dtype, pointers, who)) return rc;
     if (B == 0) return WF_OK;
+    if ((long long)max_blocks * kv->page_size > 0x7fffffff || (long long)B * H > (1 << 24)) { set_error("%s: a row of block_table spans 2^31 tokens, or 2^24 heads", who); return WF_ERR_UNSUPPORTED; }
     if (int rc = check_wait_word(who)) return rc;
     if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)kv->pool) & 15) { set_error("%s: q, out and the pool must be 16-byte aligned", who); return WF_ERR_INVALID; }
-    const size_t mine = px_bytes(B, H, kv->kv_heads, prefix_len), need = wf_prefix_attn_workspace_bytes(B, H, kv->kv_heads, AT_D, max_blocks * kv->page_size, prefix_len);
+    const PxCut cut = px_cut(B, H, kv->kv_heads, prefix_len);
+    const size_t mine = cut.bytes, need = mine + attn_chunks_bytes(B, H, kv->kv_heads, max_blocks * kv->page_size);
     if (need && (!workspace || workspace_bytes < need)) { set_error("%s: workspace too small (%zu < %zu)", who, workspace_bytes, need); return WF_ERR_INVALID; }
     if ((uintptr_t)workspace & 15) { set_error("%s: the workspace must be 16-byte aligned", who); return WF_ERR_INVALID; }
     cudaStream_t s = (cudaStream_t)stream;
@@ -615,7 +617,7 @@ extern "C" int wf_paged_prefix_attn(const void* q, const wf_kv_layout* kv, int l
         p.prefix = prefix_len; p.B = B; p.H = H; p.Hkv = kv->kv_heads; p.G = H / kv->kv_heads;
         p.layers = kv->layers; p.layer = layer; p.page_size = kv->page_size;
         p.scale_log2e = scale * 1.4426950408889634f;
-        px_cut(B, H, kv->kv_heads, prefix_len, &p.splits, &p.split_keys);
+        p.splits = cut.splits; p.split_keys = cut.keys;
         p.part_o = (float*)workspace;
         p.rows_p = g.rows_p;
         p.part_ml = p.part_o + (size_t)p.splits * p.Hkv * p.rows_p * AT_D;

@@ -2,6 +2,7 @@
 // all cached layers, fixed-size state slots (convolution tails, recurrent matrices), and the step function over a ragged batch of
 // prompt portions and single decoded tokens.  The host side decides WHAT runs in a step (scheduler, trace replay); everything that
 // computes is a kernel launched from here.
+#include "../logprobs.cuh"
 #include "seq_kernels.cuh"
 #include "../pager.h"
 #include "wf_seq.h"
@@ -154,6 +155,8 @@ struct wf_seq_engine {
     float* d_uniform = nullptr;
     int32_t* d_next = nullptr;
     size_t sample_rows = 0;
+    void* d_logprob = nullptr;     // tokens, log probabilities, entropies and alternatives of wf_seq_logprobs
+    size_t logprob_bytes = 0;
     float* layer_tap = nullptr;
     // decode-only steps (one token per sequence) replay a CUDA graph captured per (sequences, wanted rows): their launch parameters depend
     // on nothing else.  A shape runs eagerly the first time (one-time kernel attributes are set then) and is captured the second time.
@@ -1694,6 +1697,7 @@ extern "C" void wf_seq_destroy(wf_seq_engine* e) {
     if (e->logits) cudaFree(e->logits);
     if (e->d_uniform) cudaFree(e->d_uniform);
     if (e->d_next) cudaFree(e->d_next);
+    if (e->d_logprob) cudaFree(e->d_logprob);
     if (e->h_meta) cudaFreeHost(e->h_meta);
     for (auto& ev : e->out_ev) if (ev) cudaEventDestroy(ev);
     if (e->stream) cudaStreamDestroy(e->stream);
@@ -1874,6 +1878,30 @@ extern "C" int wf_seq_sample(wf_seq_engine* e, int nwant, float temperature, int
     if (int rc = launch_sample(e->logits, nwant, e->cfg.vocab, temperature, top_k, top_p, e->d_uniform, e->d_next, e->stream)) return rc;
     if (cuda_check(cudaMemcpyAsync(next_host, e->d_next, (size_t)nwant * 4, cudaMemcpyDeviceToHost, e->stream), "next D2H")) return WF_ERR_CUDA;
     return cuda_check(cudaStreamSynchronize(e->stream), "wf_seq_sample");
+}
+
+extern "C" int wf_seq_logprobs(wf_seq_engine* e, int nwant, const int32_t* tokens_host, int top, float temperature, float* logprob_host, float* entropy_host,
+                               float* top_logprob_host, int32_t* top_id_host) {
+    if (!e || nwant <= 0 || (size_t)nwant > e->logits_rows) { set_error("wf_seq_logprobs: no logits for %d rows", nwant); return WF_ERR_INVALID; }
+    if (!tokens_host || !logprob_host || !entropy_host || (top > 0 && (!top_logprob_host || !top_id_host))) { set_error("wf_seq_logprobs: null pointer"); return WF_ERR_INVALID; }
+    if (top < 0 || top > LP_TOP_MAX || top > e->cfg.vocab) { set_error("wf_seq_logprobs: top (%d) is 0 to %d, and at most the vocabulary", top, LP_TOP_MAX); return WF_ERR_INVALID; }
+    const size_t n = (size_t)nwant, bytes = n * (3 + 2 * (size_t)top) * 4;
+    if (bytes > e->logprob_bytes) {
+        if (e->d_logprob) cudaFree(e->d_logprob);
+        e->d_logprob = nullptr; e->logprob_bytes = 0;
+        if (cuda_check(cudaMalloc(&e->d_logprob, bytes), "cudaMalloc")) return WF_ERR_CUDA;
+        e->logprob_bytes = bytes;
+    }
+    int32_t* tok = (int32_t*)e->d_logprob;
+    float *lp = (float*)(tok + n), *ent = lp + n, *tlp = ent + n;
+    int32_t* tid = (int32_t*)(tlp + n * top);
+    if (cuda_check(cudaMemcpyAsync(tok, tokens_host, n * 4, cudaMemcpyHostToDevice, e->stream), "tokens H2D")) return WF_ERR_CUDA;
+    if (int rc = launch_token_logprobs(e->logits, 0, nwant, e->cfg.vocab, e->cfg.vocab, tok, top, temperature, lp, ent, tlp, tid, e->stream)) return rc;
+    if (cuda_check(cudaMemcpyAsync(logprob_host, lp, n * 4, cudaMemcpyDeviceToHost, e->stream), "logprobs D2H") ||
+        cuda_check(cudaMemcpyAsync(entropy_host, ent, n * 4, cudaMemcpyDeviceToHost, e->stream), "logprobs D2H")) return WF_ERR_CUDA;
+    if (top > 0 && (cuda_check(cudaMemcpyAsync(top_logprob_host, tlp, n * top * 4, cudaMemcpyDeviceToHost, e->stream), "logprobs D2H") ||
+                    cuda_check(cudaMemcpyAsync(top_id_host, tid, n * top * 4, cudaMemcpyDeviceToHost, e->stream), "logprobs D2H"))) return WF_ERR_CUDA;
+    return cuda_check(cudaStreamSynchronize(e->stream), "wf_seq_logprobs");
 }
 
 extern "C" int wf_seq_run_part(wf_seq_engine* e, int layer, int part, int nseq, const int32_t* slots, const int32_t* counts, const float* in_host,

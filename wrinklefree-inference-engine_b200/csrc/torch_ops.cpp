@@ -249,7 +249,7 @@ Tensor paged_prefix_attn(const Tensor& q, const Tensor& pool, int64_t max_pages,
     kv.pool = pool.data_ptr();
     kv.max_pages = (int)max_pages; kv.layers = (int)layers; kv.kv_heads = (int)kv_heads; kv.page_size = (int)page_size; kv.head_dim = (int)head_dim; kv.dtype = (int)kv_dtype;
     // memory of this call's own: calls on other streams and captured graphs do not share it
-    Tensor ws = at::empty({(int64_t)wf_prefix_attn_workspace_bytes(B, H, kv.kv_heads, D, blocks * kv.page_size, pre)}, q.options().dtype(at::kByte));
+    Tensor ws = at::empty({(int64_t)wf_prefix_attn_workspace_bytes(B, H, kv.kv_heads, blocks * kv.page_size, pre)}, q.options().dtype(at::kByte));
     check(wf_paged_prefix_attn(qc.data_ptr(), &kv, (int)layer, (const int32_t*)pt.data_ptr(), pre, (const int32_t*)bt.data_ptr(), blocks, (const int32_t*)sl.data_ptr(), B, H, (float)scale,
                                out.data_ptr(), code_of(out_dtype), ws.data_ptr(), (size_t)ws.numel(), stream()));
     return out;

@@ -211,6 +211,13 @@ class BitNetForCausalLM(nn.Module):
             raise NotImplementedError("the BitNet engine samples greedily")
         return np.array([int(r.argmax()) for r in self._last_rows[:nrows]], dtype=np.int32)
 
+    def logprobs(self, nrows: int, tokens, top: int = 0, temperature: float = 1.0):
+        import numpy as np
+        rows = torch.from_numpy(np.stack(self._last_rows[:nrows])).cuda()
+        from wf_bitnet import ops
+        out = ops.token_logprobs(rows, torch.tensor([int(t) for t in tokens], dtype=torch.int32, device="cuda"), top, temperature)
+        return tuple(t.cpu().numpy() for t in out)
+
     def close(self) -> None:
         self.engine.close()
 

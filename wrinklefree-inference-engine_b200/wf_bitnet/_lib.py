@@ -86,7 +86,7 @@ SYMBOLS = {
     "wf_paged_decode_attn": (_i, [_vp, C.POINTER(KvLayout), _i, _vp, _i, _vp, _i, _i, _f, _vp, _i, _vp, _sz, _vp]),
     "wf_paged_plan": (_i, [_vp, _vp, _i, _vp, _i, _vp, _i, _vp, _i, _i] + [_vp] * 9),
     "wf_paged_release": (_i, [_vp, _vp, _i, _vp, _i, _vp, _i, _vp, _i, _vp, _vp, _vp]),
-    "wf_prefix_attn_workspace_bytes": (_sz, [_i] * 6),
+    "wf_prefix_attn_workspace_bytes": (_sz, [_i] * 5),
     "wf_paged_prefix_attn": (_i, [_vp, C.POINTER(KvLayout), _i, _vp, _i, _vp, _i, _vp, _i, _i, _f, _vp, _i, _vp, _sz, _vp]),
     "wf_token_logprobs": (_i, [_vp, _i, _i, _i, C.c_longlong, _vp, _i, _f, _vp, _vp, _vp, _vp, _vp]),
     "wf_rmsnorm_quant": (_i, [_vp, _vp, _f, _i, _i, _vp, _vp, _vp, _vp, _vp]),
@@ -194,6 +194,7 @@ SEQ_SYMBOLS = {
     "wf_seq_free_slots": (_i, [_vp]),
     "wf_seq_step": (_i, [_vp, _i, _vp, _vp, _vp, _i, _vp, _vp]),
     "wf_seq_sample": (_i, [_vp, _i, _f, _i, _f, _vp, _vp]),
+    "wf_seq_logprobs": (_i, [_vp, _i, _vp, _i, _f, _vp, _vp, _vp, _vp]),
     "wf_seq_logits_device": (_vp, [_vp]),
     "wf_seq_launches_last_step": (_i, [_vp]),
     "wf_seq_set_layer_tap": (_i, [_vp, _vp]),

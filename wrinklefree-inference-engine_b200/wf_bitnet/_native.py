@@ -65,7 +65,7 @@ class _Ctypes:
             qc = q.contiguous()
             qc = qc.clone() if qc.data_ptr() % 16 else qc
             out = torch.empty(B, H, D, dtype=out_dtype, device=q.device)
-            ws = torch.empty(int(_lib.lib().wf_prefix_attn_workspace_bytes(B, H, kv_heads, D, bt.shape[1] * page_size, prefix_len)), dtype=torch.uint8, device=q.device)
+            ws = torch.empty(int(_lib.lib().wf_prefix_attn_workspace_bytes(B, H, kv_heads, bt.shape[1] * page_size, prefix_len)), dtype=torch.uint8, device=q.device)
             layout = _lib.KvLayout(pool.data_ptr(), max_pages, layers, kv_heads, page_size, head_dim, kv_dtype)
             _lib.check(_lib.lib().wf_paged_prefix_attn(qc.data_ptr(), C.byref(layout), layer, pt.data_ptr(), prefix_len, bt.data_ptr(), bt.shape[1], sl.data_ptr(), B, H, float(scale),
                                                        out.data_ptr(), ops._DT[out_dtype], ws.data_ptr(), ws.numel(), ops._stream()))

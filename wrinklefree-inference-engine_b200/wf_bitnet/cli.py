@@ -1,9 +1,10 @@
 """Command line of the serving stack.
 
-  python -m wf_bitnet.cli generate --model DIR --prompt-ids 5,17,3 [--prompt-ids ...] --max-new-tokens 16 [--temperature T --top-k K --top-p P]
+  python -m wf_bitnet.cli generate --model DIR --prompt-ids 5,17,3 [--prompt-ids ...] --max-new-tokens 16 [--temperature T --top-k K --top-p P] [--logprobs N]
   python -m wf_bitnet.cli trace    --model DIR --dtype bfloat16|float32 --out DIR --max-tokens N     (bin/trace_run)
 
-`generate` queues the prompts on the scheduler and prints one JSON line per finished request.  `trace` replays a schedule given on
+`generate` queues the prompts on the scheduler and prints one JSON line per finished request; with --logprobs N the line also has every output token's log
+probability, the entropy of its distribution and the N most likely tokens ([id, log probability] pairs).  `trace` replays a schedule given on
 standard input, one JSON object per line — {"step": n, "entries": [{"id", "tokens", "want"}], "end": [ids]} — through the same model,
 cache manager and batch execution, writes the logits of the wanted positions to OUT/<step>.f32 (little-endian float32 [wanted, vocab])
 and answers `done <step>` after every step.  Both pick the model class from config.json through the registry.
@@ -35,9 +36,12 @@ def cmd_generate(a) -> int:
     model = load_model(a.model, a.dtype, a.max_tokens or need, a.slots, a.page_size, a.max_step_tokens)
     sched = Scheduler(model, max_prefill_chunk=a.prefill_chunk or None)
     for i, p in enumerate(prompts):
-        sched.add(Request(f"r{i}", p, a.max_new_tokens, SamplingParams(a.temperature, a.top_k, a.top_p, a.seed + i)))
+        sched.add(Request(f"r{i}", p, a.max_new_tokens, SamplingParams(a.temperature, a.top_k, a.top_p, a.seed + i), logprobs=a.logprobs))
     for r in sorted(sched.run(), key=lambda r: r.rid):
-        print(json.dumps({"id": r.rid, "prompt_tokens": len(r.prompt), "output_ids": r.output}), flush=True)
+        line = {"id": r.rid, "prompt_tokens": len(r.prompt), "output_ids": r.output}
+        if a.logprobs is not None:
+            line.update(logprobs=r.token_logprobs, entropy=r.entropies, top_logprobs=r.top_logprobs)
+        print(json.dumps(line), flush=True)
     model.close()
     return 0
 
@@ -96,6 +100,7 @@ def main(argv=None) -> int:
             p.add_argument("--top-p", type=float, default=1.0)
             p.add_argument("--seed", type=int, default=0)
             p.add_argument("--prefill-chunk", type=int, default=0)
+            p.add_argument("--logprobs", type=int, default=None, help="log probabilities of the output tokens, and of this many alternatives each (0 to 64)")
         else:
             p.add_argument("--out", required=True)
     a = ap.parse_args(argv)

@@ -1,5 +1,5 @@
-"""Continuous-batching scheduler for models that expose the ragged step interface (admit / release / step / sample, as
-sglang.srt.models.karusun.KarusunForCausalLM does): every step runs the single next tokens of the sequences that are decoding together
+"""Continuous-batching scheduler for models that expose the ragged step interface (admit / release / step / sample, and logprobs for requests that
+ask for them, as sglang.srt.models.karusun.KarusunForCausalLM does): every step runs the single next tokens of the sequences that are decoding together
 with portions of the prompts that are still being read, under one token budget.  Slots and cache pages are reserved at admission and
 handed back when a request finishes, so later requests run in pages and slots that earlier ones used.
 
@@ -32,10 +32,14 @@ class Request:
     max_new_tokens: int = 16
     sampling: SamplingParams = field(default_factory=SamplingParams)
     stop_ids: Tuple[int, ...] = ()
+    logprobs: Optional[int] = None        # not None: log probabilities of the drawn tokens, and of this many alternatives each (0..64)
     # filled by the scheduler
     slot: int = -1
     fed: int = 0                          # prompt tokens already run
     output: List[int] = field(default_factory=list)
+    token_logprobs: List[float] = field(default_factory=list)                    # of output[i], from the model's distribution itself (temperature 1, no limits)
+    entropies: List[float] = field(default_factory=list)
+    top_logprobs: List[List[Tuple[int, float]]] = field(default_factory=list)    # (token, log probability), most likely first
     reserved_pages: int = 0
     finished: bool = False
     _rng: Optional[np.random.Generator] = None
@@ -100,6 +104,11 @@ class Scheduler:
         if not req.prompt:
             raise ValueError("empty prompt")
         longest = int(getattr(self.model, "max_positions", 0))          # models with a table of positions end where it ends
+        if req.logprobs is not None:
+            if not 0 <= req.logprobs <= min(64, int(self.model.vocab)):
+                raise ValueError(f"request {req.rid!r} asks for {req.logprobs} alternatives, 0 to {min(64, int(self.model.vocab))} can be had")
+            if not hasattr(self.model, "logprobs"):
+                raise NotImplementedError(f"{type(self.model).__name__} gives no log probabilities")
         if longest and len(req.prompt) + req.max_new_tokens - 1 > longest:      # the last drawn token is not fed back
             raise ValueError(f"request {req.rid!r} needs {len(req.prompt) + req.max_new_tokens - 1} positions, the model has {longest}")
         self.waiting.append(req)
@@ -152,6 +161,7 @@ class Scheduler:
         finished = []
         if want:
             nxt = self._draw(logits, owners)
+            self._note_logprobs(owners, nxt)
             for r, t in zip(owners, nxt):
                 r.output.append(int(t))
                 if len(r.output) >= r.max_new_tokens or int(t) in r.stop_ids:
@@ -162,6 +172,17 @@ class Scheduler:
             self.running.remove(r)
             finished.append(r)
         return finished
+
+    def _note_logprobs(self, owners: List[Request], nxt: np.ndarray) -> None:
+        asked = [r.logprobs for r in owners if r.logprobs is not None]
+        if not asked:
+            return
+        lp, ent, tlp, tid = self.model.logprobs(len(owners), nxt, max(asked))
+        for k, r in enumerate(owners):
+            if r.logprobs is not None:
+                r.token_logprobs.append(float(lp[k]))
+                r.entropies.append(float(ent[k]))
+                r.top_logprobs.append([(int(tid[k, j]), float(tlp[k, j])) for j in range(r.logprobs)])
 
     def _draw(self, logits: np.ndarray, owners: List[Request]) -> np.ndarray:
         """The model's sampling kernel works on the rows the last batch left on the device, in order; groups of equal parameters are

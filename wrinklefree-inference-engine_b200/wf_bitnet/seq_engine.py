@@ -107,6 +107,18 @@ class SeqEngine:
         seq_check(seq_lib().wf_seq_sample(self._h, nrows, float(temperature), int(top_k), float(top_p), u.ctypes.data if u is not None else None, nxt.ctypes.data))
         return nxt
 
+    def logprobs(self, nrows: int, tokens: Sequence[int], top: int = 0, temperature: float = 1.0) -> Tuple[np.ndarray, np.ndarray, np.ndarray, np.ndarray]:
+        """Of each wanted row of the last step: the log probability of tokens[row], the entropy, and the `top` most likely tokens' log probabilities and ids.
+        Returns (float32 [nrows], float32 [nrows], float32 [nrows, top], int32 [nrows, top])."""
+        t = _i32(tokens)
+        if t.shape != (nrows,):
+            raise ValueError(f"{t.size} tokens for {nrows} rows")
+        lp, ent = np.empty(nrows, dtype=np.float32), np.empty(nrows, dtype=np.float32)
+        tlp, tid = np.empty((nrows, max(top, 0)), dtype=np.float32), np.empty((nrows, max(top, 0)), dtype=np.int32)
+        seq_check(seq_lib().wf_seq_logprobs(self._h, nrows, t.ctypes.data, int(top), float(temperature), lp.ctypes.data, ent.ctypes.data, tlp.ctypes.data if top > 0 else None,
+                                            tid.ctypes.data if top > 0 else None))
+        return lp, ent, tlp, tid
+
     def launches_last_step(self) -> int:
         return int(seq_lib().wf_seq_launches_last_step(self._h))
 

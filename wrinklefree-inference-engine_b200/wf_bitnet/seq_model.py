@@ -1,5 +1,5 @@
 """Model-class base of the layer-stack sequence models served by the native engine (libwf_seq.so): weight loading by checkpoint name
-and the step interface (admit / release / step / sample) that the scheduler, `generate` and the trace replay drive.  A design's module
+and the step interface (admit / release / step / sample / logprobs) that the scheduler, `generate` and the trace replay drive.  A design's module
 supplies the configuration reader that turns config.json into the engine's native structs; it computes nothing itself."""
 from __future__ import annotations
 
@@ -115,6 +115,9 @@ class SeqCausalLM:
 
     def sample(self, nrows: int, temperature: float = 0.0, top_k: int = 0, top_p: float = 1.0, uniforms=None) -> np.ndarray:
         return self.engine.sample(nrows, temperature, top_k, top_p, uniforms)
+
+    def logprobs(self, nrows: int, tokens: Sequence[int], top: int = 0, temperature: float = 1.0):
+        return self.engine.logprobs(nrows, tokens, top, temperature)
 
     def close(self) -> None:
         self.engine.close()
