@@ -206,36 +206,43 @@ __global__ void __launch_bounds__(I8 ? PX_THREADS8 : PX_THREADS, 1) prefix_attn_
         const int x = tid - 11 * 32, w = warp - 11;
         const int pc = (lane & 3) + 4 * (lane >> 3 & 1), flip = lane >> 2 & 1 ? 5 : 0;
         const int skv = x >> 6, sj = x & 63;               // this thread's scale: of keys or values, of which key
-        auto scale_of = [&](int i) {
-            const int j = key0 + i * PX_KEYS + sj;
-            if (i >= nt || j >= key1) return 0.f;
-            const int pg = j / p.page_size;
-            float v;
-            asm volatile("ld.global.cg.f32 %0, [%1];" : "=f"(v) : "l"(p.scales + ((((size_t)ldcg_i32(p.table + pg) * p.layers + p.layer) * 2 + skv) * p.Hkv + kvh) * p.page_size + (j - pg * p.page_size)));
+        auto page_of = [&](int i) { const int j = key0 + i * PX_KEYS + sj; return i < nt && j < key1 ? ldcg_i32(p.table + j / p.page_size) : -1; };
+        auto scale_of = [&](int i, int page) {
+            float v = 0.f;
+            if (page >= 0)
+                asm volatile("ld.global.cg.f32 %0, [%1];" : "=f"(v) : "l"(p.scales + ((((size_t)page * p.layers + p.layer) * 2 + skv) * p.Hkv + kvh) * p.page_size + (key0 + i * PX_KEYS + sj) % p.page_size));
             return v;
         };
         bool ok = true;
         int st = 0, lap = 0, rs = 0, rlap = 0;
-        float sc = scale_of(0);
+        // a scale is asked for one tile ahead, its page two tiles before that
+        int page1 = page_of(1), page2 = page_of(2);
+        float sc = scale_of(0, page_of(0));
         for (int i = 0; i < nt; ++i) {
-            const float sc_next = scale_of(i + 1);
+            const float sc_next = scale_of(i + 1, page1);
+            page1 = page2; page2 = page_of(i + 3);
             if (!px_wait_warp(&raw_full[rs], (uint32_t)(rlap & 1)) || (lap && !px_wait_warp(&kv_empty[st], (uint32_t)((lap & 1) ^ 1)))) { ok = false; break; }
             asm volatile("st.shared.f32 [%0], %1;" ::"r"(sc_s + st * PX_SC + x * 4), "f"(sc) : "memory");
 #pragma unroll
             for (int kv = 0; kv < 2; ++kv) {
+                uint32_t y[4][4];
 #pragma unroll
                 for (int it = 0; it < 4; ++it) {
                     const int row = 2 * ((lane >> 4) | w << 1 | it << 3) ^ flip;
-                    uint32_t y[4], o[8];
-                    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(y[0]), "=r"(y[1]), "=r"(y[2]), "=r"(y[3])
+                    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(y[it][0]), "=r"(y[it][1]), "=r"(y[it][2]), "=r"(y[it][3])
                                  : "r"(raw_s + rs * PX_RAW_TILE + kv * PX_KEYS * AT_D + row * 128 + ((pc ^ (row & 7)) << 4)) : "memory");
+                }
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {          // a byte above the mantissa of 2^23 is 2^23 + code + 128
+                for (int it = 0; it < 4; ++it) {
+                    const int row = 2 * ((lane >> 4) | w << 1 | it << 3) ^ flip;
+                    uint32_t o[8];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {          // a byte below the exponent of 2^23 is 2^23 + code + 128
                         const uint64_t off2 = px_pair(0xcb000080u, 0xcb000080u);
                         float a, b;
-                        px_unpair(px_add2(px_pair(__byte_perm(y[k], 0x4b000000u, 0x7440), __byte_perm(y[k], 0x4b000000u, 0x7441)), off2), a, b);
+                        px_unpair(px_add2(px_pair(__byte_perm(y[it][k], 0x4b000000u, 0x7440), __byte_perm(y[it][k], 0x4b000000u, 0x7441)), off2), a, b);
                         o[2 * k] = pack_bf16x2(a, b);
-                        px_unpair(px_add2(px_pair(__byte_perm(y[k], 0x4b000000u, 0x7442), __byte_perm(y[k], 0x4b000000u, 0x7443)), off2), a, b);
+                        px_unpair(px_add2(px_pair(__byte_perm(y[it][k], 0x4b000000u, 0x7442), __byte_perm(y[it][k], 0x4b000000u, 0x7443)), off2), a, b);
                         o[2 * k + 1] = pack_bf16x2(a, b);
                     }
                     const uint32_t dst = (kv ? v_s : k_s) + st * PX_TILE + (pc >> 2) * PX_HALF + row * 128;
@@ -373,6 +380,7 @@ __global__ void __launch_bounds__(I8 ? PX_THREADS8 : PX_THREADS, 1) prefix_attn_
             const uint32_t nm = __float_as_uint(m_ref == -INFINITY ? 0.f : m_ref == INFINITY ? __uint_as_float(0x7fc00000u) : -m_ref);
             const uint64_t nm2 = px_pair(nm, nm), unit2 = px_pair(__float_as_uint(unit), __float_as_uint(unit));
             uint64_t ls[2] = {0ull, 0ull};
+            uint32_t vs[4];
 #pragma unroll
             for (int c = 0; c < PX_KEYS / 2; ++c) {       // columns (2c, 2c + 1) go to s[c], an entry whose score has been read
                 const uint64_t x = px_fma2(px_pair(s[2 * c], s[2 * c + 1]), unit2, nm2);
@@ -385,9 +393,8 @@ __global__ void __launch_bounds__(I8 ? PX_THREADS8 : PX_THREADS, 1) prefix_attn_
                 }
                 ls[c & 1] = px_add2(ls[c & 1], px_pair(__float_as_uint(e0), __float_as_uint(e1)));
                 if (I8) {                                 // the values' scales go into the weights
-                    uint32_t v0, v1;
-                    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v0), "=r"(v1) : "r"(sc_n + PX_KEYS * 4 + c * 8) : "memory");
-                    px_unpair(px_mul2(px_pair(__float_as_uint(e0), __float_as_uint(e1)), px_pair(v0, v1)), e0, e1);
+                    if (!(c & 1)) asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(vs[0]), "=r"(vs[1]), "=r"(vs[2]), "=r"(vs[3]) : "r"(sc_n + PX_KEYS * 4 + c * 8) : "memory");
+                    px_unpair(px_mul2(px_pair(__float_as_uint(e0), __float_as_uint(e1)), px_pair(vs[2 * (c & 1)], vs[2 * (c & 1) + 1])), e0, e1);
                 }
                 s[c] = pack_bf16x2(e0, e1);
             }
