@@ -22,7 +22,7 @@ def test_plan_refusals():
                 dict(pos=None), dict(tok=None), dict(pages=None), dict(slots=None), dict(off=None), dict(lens=None), dict(cout=None), dict(status=None), dict(pos=P + 4), dict(slots=P + 8)):
         assert call(**bad) == _lib.WF_ERR_INVALID, bad
         assert b"wf_paged_plan" in L.wf_last_error()
-    assert call(rows=8193) == _lib.WF_ERR_UNSUPPORTED
+    assert call(rows=8193) == call(cap=(1 << 30) + 1) == _lib.WF_ERR_UNSUPPORTED
 
 
 def test_release_refusals():
@@ -50,11 +50,12 @@ def test_prefix_attention_refusals():
         a["kv"] = None if k.get("kv_null") else C.byref(layout)
         a.pop("kv_null", None)
         return L.wf_paged_prefix_attn(*a.values(), None)
-    for bad in (dict(q=None), dict(pt=None), dict(table=None), dict(lens=None), dict(out=None), dict(ws=None), dict(ws_bytes=16), dict(prefix=-1), dict(blocks=-1), dict(B=-1), dict(layer=1),
+    for bad in (dict(q=None), dict(pt=None), dict(table=None), dict(lens=None), dict(out=None), dict(ws=None), dict(ws_bytes=16), dict(prefix=-1), dict(blocks=-1), dict(B=-1), dict(H=0), dict(H=-2), dict(layer=1),
                 dict(layer=-1), dict(dt=_lib.WF_F16), dict(q=P + 2), dict(out=P + 8), dict(ws=P + 8), dict(kv=dict(pool=None)), dict(kv=dict(pool=P + 2)), dict(kv=dict(kv_heads=0)), dict(kv_null=True)):
         assert call(**bad) == _lib.WF_ERR_INVALID, bad
         assert b"wf_paged_prefix_attn" in L.wf_last_error()
-    for bad in (dict(kv=dict(head_dim=64)), dict(kv=dict(page_size=24)), dict(kv=dict(kv_heads=3)), dict(H=18), dict(kv=dict(dtype=_lib.WF_F32))):
+    for bad in (dict(kv=dict(head_dim=64)), dict(kv=dict(page_size=24)), dict(kv=dict(kv_heads=3)), dict(H=18), dict(kv=dict(dtype=_lib.WF_F32)), dict(prefix=(1 << 30) + 1),
+                dict(blocks=1 << 27), dict(B=1 << 22)):
         assert call(**bad) == _lib.WF_ERR_UNSUPPORTED, bad
     assert call(B=0, q=None, out=None) == _lib.WF_OK
 

@@ -17,7 +17,7 @@ struct PxParams {
     const float* scales;           // int8 pool
     const int32_t* table;          // pages of the prefix
     int prefix, B, H, Hkv, G;
-    int layers, layer, page_size;
+    int layers, layer, page_size, max_pages;
     int splits, split_keys;        // keys of a split
     float scale_log2e;
     float *part_o, *part_ml;       // [splits][Hkv][AT_D / 4][rows][4], [splits][Hkv][rows][2], rows = B * G up to the next multiple of 32
@@ -209,7 +209,7 @@ __global__ void __launch_bounds__(I8 ? PX_THREADS8 : PX_THREADS, 1) prefix_attn_
         auto page_of = [&](int i) { const int j = key0 + i * PX_KEYS + sj; return i < nt && j < key1 ? ldcg_i32(p.table + j / p.page_size) : -1; };
         auto scale_of = [&](int i, int page) {
             float v = 0.f;
-            if (page >= 0)
+            if (page >= 0 && page < p.max_pages)           // what is no page reads as zeros, as the copies do
                 asm volatile("ld.global.cg.f32 %0, [%1];" : "=f"(v) : "l"(p.scales + ((((size_t)page * p.layers + p.layer) * 2 + skv) * p.Hkv + kvh) * p.page_size + (key0 + i * PX_KEYS + sj) % p.page_size));
             return v;
         };
@@ -488,7 +488,7 @@ __global__ void __launch_bounds__(I8 ? PX_THREADS8 : PX_THREADS, 1) prefix_attn_
     if (!p.wait_first) pdl_wait_prior();                  // the own part's kernel: whoever waits for this one has waited for that one
 }
 
-DevOnce g_px_attr;
+DevMade g_px_attr;
 
 // [128][slot][page, layer, K | V, head], boxes of `box` slots x 128 bytes
 int px_encode(CUtensorMap* tm, const wf_kv_layout* kv, int box) {
@@ -528,7 +528,7 @@ __global__ void __launch_bounds__(PX_MERGE) prefix_merge_kernel(const __grid_con
     if (p.own.part_o) {
         const int nblocks = (p.seq_lens[b] + AT_BLK - 1) / AT_BLK;
         const int cb = chunk_blocks_of(nblocks, p.own.chunk_blocks, p.own.max_chunks, p.own.min_cb);
-        own = (nblocks + cb - 1) / cb;
+        own = min((nblocks + cb - 1) / cb, p.own.max_chunks);      // (a length beyond the table's)
     }
     const size_t next = (size_t)p.Hkv * p.rows_p;         // from a split to the next
     const float2 *ml = reinterpret_cast<const float2*>(p.part_ml) + (size_t)kvh * p.rows_p + r, *oml = reinterpret_cast<const float2*>(p.own.part_ml) + (size_t)row * p.own.max_chunks;
@@ -605,7 +605,7 @@ extern "C" int wf_paged_prefix_attn(const void* q, const wf_kv_layout* kv, int l
     const bool pointers = B == 0 || (q && out && (prefix_len == 0 || prefix_table) && (max_blocks == 0 || (block_table && seq_lens)));
     if (int rc = check_decode_attn(kv, layer, H, out_dtype, pointers, who)) return rc;
     if (B == 0) return WF_OK;
-    if ((long long)max_blocks * kv->page_size > 0x7fffffff || (long long)B * H > (1 << 24)) { set_error("%s: a row of block_table spans 2^31 tokens, or 2^24 heads", who); return WF_ERR_UNSUPPORTED; }
+    if ((long long)max_blocks * kv->page_size > 0x7fffffff || prefix_len > 1 << 30 || (long long)B * H > (1 << 24)) { set_error("%s: a row of block_table of 2^31 tokens, a prefix of more than 2^30, or 2^24 rows of queries", who); return WF_ERR_UNSUPPORTED; }
     if (int rc = check_wait_word(who)) return rc;
     if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)kv->pool) & 15) { set_error("%s: q, out and the pool must be 16-byte aligned", who); return WF_ERR_INVALID; }
     const PxCut cut = px_cut(B, H, kv->kv_heads, prefix_len);
@@ -622,7 +622,7 @@ extern "C" int wf_paged_prefix_attn(const void* q, const wf_kv_layout* kv, int l
         PxParams p = {};
         p.q = (const __nv_bfloat16*)q; p.pool = kv->pool; p.scales = kv_scales_of(kv); p.table = prefix_table;
         p.prefix = prefix_len; p.B = B; p.H = H; p.Hkv = kv->kv_heads; p.G = H / kv->kv_heads;
-        p.layers = kv->layers; p.layer = layer; p.page_size = kv->page_size;
+        p.layers = kv->layers; p.layer = layer; p.page_size = kv->page_size; p.max_pages = kv->max_pages;
         p.scale_log2e = scale * 1.4426950408889634f;
         p.splits = cut.splits; p.split_keys = cut.keys;
         p.part_o = (float*)workspace;
@@ -639,8 +639,10 @@ extern "C" int wf_paged_prefix_attn(const void* q, const wf_kv_layout* kv, int l
         if (!p.err) { set_error("%s: no wait word", who); return WF_ERR_CUDA; }
         CUtensorMap tm;
         if (int rc = px_encode(&tm, kv, p.box)) return rc;
-        if (g_px_attr.need() && (cuda_check(cudaFuncSetAttribute(prefix_attn_tc_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, PX_SMEM), who) ||
-                                 cuda_check(cudaFuncSetAttribute(prefix_attn_tc_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, PX_SMEM8), who))) return WF_ERR_CUDA;
+        if (int rc = g_px_attr.once([&]() -> int {
+                return cuda_check(cudaFuncSetAttribute(prefix_attn_tc_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, PX_SMEM), who) ||
+                               cuda_check(cudaFuncSetAttribute(prefix_attn_tc_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, PX_SMEM8), who) ? WF_ERR_CUDA : WF_OK;
+            })) return rc;
         const dim3 grid((unsigned)(pairs * p.Hkv * p.splits));
         const cudaError_t e = i8 ? launch_pdl(prefix_attn_tc_kernel<true>, grid, PX_THREADS8, PX_SMEM8, s, tm, p) : launch_pdl(prefix_attn_tc_kernel<false>, grid, PX_THREADS, PX_SMEM, s, tm, p);
         if (int rc = launch_check(e, "prefix_attn_tc")) return rc;

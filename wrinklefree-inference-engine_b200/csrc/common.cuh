@@ -1,6 +1,8 @@
 // Shared device helpers for the sm_100a BitNet kernels (inline PTX wrappers, bf16 rounding
 // helpers that mirror the reference's torch-CPU rounding points, small reductions).
 #pragma once
+#include <atomic>
+#include <mutex>
 #include <utility>
 #include <cuda_runtime.h>
 #include <cuda_bf16.h>
@@ -34,6 +36,22 @@ struct DevOnce {
         if ((done >> d) & 1ull) return false;
         done |= 1ull << d;
         return true;
+    }
+};
+
+// The same where calls may come from several threads: `make` runs under a lock, and counts as done when it has succeeded.
+struct DevMade {
+    std::atomic<unsigned long long> done{0};
+    std::mutex mu;
+    template <typename F> int once(F make) {
+        int d = 0;
+        if (cudaGetDevice(&d) != cudaSuccess || d < 0 || d > 63) return make();
+        if ((done.load(std::memory_order_acquire) >> d) & 1ull) return WF_OK;
+        std::lock_guard<std::mutex> lk(mu);
+        if ((done.load(std::memory_order_acquire) >> d) & 1ull) return WF_OK;
+        const int rc = make();
+        if (rc == WF_OK) done.fetch_or(1ull << d, std::memory_order_release);
+        return rc;
     }
 };
 

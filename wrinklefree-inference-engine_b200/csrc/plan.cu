@@ -166,6 +166,7 @@ __global__ void __launch_bounds__(PL_THREADS) paged_release_kernel(const __grid_
 int pl_check(const char* who, PlanParams& p) {
     if (p.rows < 0 || p.max_blocks < 0 || p.pool_pages < 0 || p.cap < 0) { set_error("%s: negative size", who); return WF_ERR_INVALID; }
     if (p.page <= 0) { set_error("%s: page_size must be positive (got %d)", who, p.page); return WF_ERR_INVALID; }
+    if (p.cap > 1 << 30) { set_error("%s: max_tokens is at most 2^30 (got %d)", who, p.cap); return WF_ERR_UNSUPPORTED; }
     if (p.rows > PL_MAX_ROWS) { set_error("%s: at most %d requests (got %d)", who, PL_MAX_ROWS, p.rows); return WF_ERR_UNSUPPORTED; }
     // with 2^(l-1) < page <= 2^l, mul = ceil(2^(31+l) / page) is below 2^32 and exceeds 2^(31+l) / page by less than 1: x * mul / 2^(31+l) is above x / page by less
     // than 2^-l <= 1 / page, which does not reach the next whole number
@@ -176,12 +177,13 @@ int pl_check(const char* who, PlanParams& p) {
     return WF_OK;
 }
 
-DevOnce g_pl_attr;
+DevMade g_pl_attr;
 
 int pl_attrs() {
-    if (!g_pl_attr.need()) return WF_OK;
-    if (cuda_check(cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * (PL_MAX_ROWS + 1) * 4), "wf_paged_plan")) return WF_ERR_CUDA;
-    return cuda_check(cudaFuncSetAttribute(paged_release_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * (PL_MAX_ROWS + 1) * 4), "wf_paged_release");
+    return g_pl_attr.once([]() -> int {
+        if (cuda_check(cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * (PL_MAX_ROWS + 1) * 4), "wf_paged_plan")) return WF_ERR_CUDA;
+        return cuda_check(cudaFuncSetAttribute(paged_release_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * (PL_MAX_ROWS + 1) * 4), "wf_paged_release");
+    });
 }
 int pl_threads(const PlanParams& p, long long items) { return p.rows <= PL_SMALL && items <= PL_SMALL ? PL_SMALL : PL_THREADS; }
 int pl_grid(const PlanParams& p, long long items) {

@@ -6,6 +6,7 @@ does not load (another torch), the same calls go through ctypes: the same kernel
 from __future__ import annotations
 
 import ctypes as C
+import threading
 import warnings
 
 import torch
@@ -14,6 +15,7 @@ from . import _lib
 
 TORCH_LIB_PATH = _lib.LIB_PATH.parent / "libwf_torch.so"
 _ops = None
+_loading = threading.Lock()
 
 
 class _Ctypes:
@@ -215,7 +217,9 @@ def ops():
     """torch.ops.wf_native, or the same functions through ctypes; raises when libwf_bitnet.so has not been built."""
     global _ops
     if _ops is None:
-        _ops = _load()
+        with _loading:
+            if _ops is None:
+                _ops = _load()
     return _ops
 
 
