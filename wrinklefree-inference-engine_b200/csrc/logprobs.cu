@@ -385,16 +385,13 @@ __global__ void __launch_bounds__(LP_THREADS, 2) token_logprobs_kernel(const __g
                 if (tid < p.k) lists[tid] = 0;         // (read by the copies above)
                 __syncthreads();
                 const u64 key = tid < cs * p.k ? cand[tid] : 0;
-                int lo[8], at = own;                       // the lists side by side: their steps do not wait for one another
-#pragma unroll
-                for (int r = 0; r < 8; ++r) lo[r] = 0;
-                for (int step = 1 << (31 - __clz(p.k)); key && step; step >>= 1) {
-#pragma unroll
-                    for (int r = 0; r < 8; ++r)
-                        if (r < cs && r != of && lo[r] + step <= p.k && cand[r * p.k + lo[r] + step - 1] > key) lo[r] += step;
+                int at = own;
+                for (int r = 0; key && r < cs; ++r) {
+                    if (r == of) continue;
+                    int lo = 0, hi = p.k;
+                    while (lo < hi) { const int mid = (lo + hi) >> 1; if (cand[r * p.k + mid] > key) lo = mid + 1; else hi = mid; }
+                    at += lo;
                 }
-#pragma unroll
-                for (int r = 0; r < 8; ++r) at += lo[r];
                 if (key && at < p.k) lists[at] = key;
                 __syncthreads();
             }
