@@ -248,7 +248,7 @@ size_t wf_lm_head_workspace_bytes(int B, int V);
 int wf_lm_head_argmax(const void* h, const void* E, int B, int V, int K, float* logits_out, int32_t* next_out,
                       void* workspace, size_t workspace_bytes, void* stream);
 
-/* Log probabilities from logits [rows, vocab] (dtype WF_F32 / WF_BF16 / WF_F16, rows row_stride elements apart), z = logits / temperature, temperature > 0:
+/* Log probabilities from logits [rows, vocab] (dtype WF_F32 / WF_BF16 / WF_F16, rows row_stride elements apart), z = logits / temperature, temperature > 0, vocab at most 2^30:
  * logprob[r] = log softmax(z_r)[tokens[r]], entropy[r] = -sum p ln p (nats, in float whatever the dtype), and the `top` (0..64, at most vocab) largest logits of
  * each row, largest first, equal ones by index: top_id, top_logprob [rows, top].  Logits of -inf have probability 0.  A row with nothing above -inf: logprobs
  * -inf, entropy 0.  A row with +inf or NaN: all its floats NaN, NaN is no alternative (top_id -1 where the row has too few others).  A token outside

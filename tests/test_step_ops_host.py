@@ -89,6 +89,12 @@ def test_logprob_refusals():
     assert call(rows=0, x=None, tok=None, lp=None, ent=None, tlp=None, tid=None) == _lib.WF_OK
 
 
+def test_logprobs_columns_beyond_their_index():
+    # a block's indices run past the last column by a step: they are 32-bit
+    rc = _lib.lib().wf_token_logprobs(P, _lib.WF_BF16, 1, (1 << 30) + 1, (1 << 30) + 1, P, 0, 1.0, P, P, None, None, None)
+    assert rc == _lib.WF_ERR_UNSUPPORTED
+
+
 def test_torch_ops_and_their_fakes():
     import sgl_kernel  # noqa: F401
     from wf_bitnet import _native

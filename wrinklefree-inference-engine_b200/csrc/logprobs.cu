@@ -458,6 +458,7 @@ cudaError_t lp_launch(const LpParams& p, int n, cudaStream_t s) {
 int launch_token_logprobs(const void* logits, int dtype, int n, int V, long long ld, const int32_t* tokens, int k, float temperature, float* logprob, float* entropy,
                           float* top_logprob, int32_t* top_id, cudaStream_t s) {
     if (n < 0 || V <= 0) { set_error("wf_token_logprobs: bad shape [%d, %d]", n, V); return WF_ERR_INVALID; }
+    if (V > 1 << 30) { set_error("wf_token_logprobs: at most 2^30 columns (got %d)", V); return WF_ERR_UNSUPPORTED; }       // indices of a step beyond the last column fit too
     if (n > 1 && ld < V) { set_error("wf_token_logprobs: row stride %lld below %d columns", ld, V); return WF_ERR_INVALID; }
     if (k < 0 || k > V) { set_error("wf_token_logprobs: top (%d) of %d", k, V); return WF_ERR_INVALID; }
     if (k > LP_TOP_MAX) { set_error("wf_token_logprobs: top is at most %d (got %d)", LP_TOP_MAX, k); return WF_ERR_UNSUPPORTED; }
