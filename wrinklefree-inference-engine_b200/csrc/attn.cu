@@ -45,6 +45,8 @@ constexpr int AT8_STAGES = 4;                                    // 67.6 KB per 
 constexpr int AT8_SCALE_OFF = 2 * AT_BLK * AT8_ROW;                 // 16 K scales | 16 V scales
 constexpr int AT8_STAGE_BYTES = AT8_SCALE_OFF + 2 * AT_BLK * 4;     // 4224
 constexpr int AT8_SMEM = AT_WARPS * AT8_STAGES * AT8_STAGE_BYTES;   // 101,376
+// beside another kernel's blocks (BESIDE below): 64 KB
+constexpr int AT_BESIDE_STAGES = 2, AT_BESIDE_SMEM = AT_WARPS * AT_BESIDE_STAGES * AT_STAGE_BYTES;
 constexpr float AT8_PV_UP = 256.f, AT8_PV_DOWN = 1.f / 256.f;
 
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
@@ -159,9 +161,13 @@ __device__ __forceinline__ size_t kv_scale_offset(int page, int layers, int laye
     return ((((size_t)page * layers + layer) * 2 + kv) * Hkv + head) * (size_t)page_size;
 }
 
-template <bool FUSED, bool I8>
-__global__ void __launch_bounds__(AT_WARPS * 32, I8 ? 3 : 2) paged_decode_attn_kernel(const AttnParams p) {
-    constexpr int ST = I8 ? AT8_STAGES : AT_STAGES;
+// BESIDE: the kernel before is a part of the same call, has waited for all that this one reads, and goes on while this one's blocks take what it leaves of each SM:
+// 64 KB of shared memory and 168 registers a thread.  So no block waits but the last one, at its end: who waits for this kernel has waited for that one.  Loads go
+// to L2: without the wait nothing says that L1 holds none of an earlier step's lines.
+template <bool FUSED, bool I8, bool BESIDE = false>
+__global__ void __launch_bounds__(AT_WARPS * 32, I8 || BESIDE ? 3 : 2) paged_decode_attn_kernel(const AttnParams p) {
+    static_assert(!BESIDE || (!FUSED && !I8), "the form beside another kernel is made for bf16 pools");
+    constexpr int ST = BESIDE ? AT_BESIDE_STAGES : I8 ? AT8_STAGES : AT_STAGES;
     constexpr int SB = I8 ? AT8_STAGE_BYTES : AT_STAGE_BYTES;
     constexpr int ROW = I8 ? AT8_ROW : AT_ROW;
     // the even form (opt-in, measured slower) is not compiled into the int8 kernel: its range state pushed that instantiation over the
@@ -175,7 +181,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32, I8 ? 3 : 2) paged_decode_attn_k
 
     const bool tr = FUSED && !I8 && p.trace && bid == 0 && threadIdx.x == 0;
     if (tr) p.trace[0] = gtimer();
-    if (FUSED) pdl_launch_dependents();
+    if (FUSED || BESIDE) pdl_launch_dependents();
     else { pdl_wait_prior(); pdl_launch_dependents(); }   // queries, lengths, table and cache may all be the work of the kernel before
 
     // ---- work decomposition.
@@ -236,7 +242,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32, I8 ? 3 : 2) paged_decode_attn_k
             b = pair / p.Hkv; kvh = pair - b * p.Hkv;
         } else if (!I8 && p.chunk_major) { kvh = blockIdx.x; b = blockIdx.y; chunk = blockIdx.z; }
         else { chunk = blockIdx.x; kvh = blockIdx.y; b = blockIdx.z; }
-        seq_len = p.seq_lens[b];
+        seq_len = BESIDE ? ldcg_i32(p.seq_lens + b) : p.seq_lens[b];
         nblocks = (seq_len + AT_BLK - 1) / AT_BLK;
         cbk = chunk_blocks_of(nblocks, cbk, p.max_chunks, p.min_cb);
         if (whole) cbk = max(nblocks, 1);
@@ -286,7 +292,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32, I8 ? 3 : 2) paged_decode_attn_k
     auto page_of = [&](int i) -> int {
         const int tokf = (blk0 + warp + AT_WARPS * i) * AT_BLK;
         const int pi = p.page_shift >= 0 ? (tokf >> p.page_shift) : tokf / p.page_size;
-        return bt[min(pi, p.max_blocks - 1)];
+        return BESIDE ? ldcg_i32(bt + min(pi, p.max_blocks - 1)) : bt[min(pi, p.max_blocks - 1)];
     };
     int pg_q0 = page_of(0), pg_q1 = page_of(1), pg_q2 = page_of(2);
     auto issue = [&](int i) {   // i-th block of this warp -> stage i % AT_STAGES
@@ -339,7 +345,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32, I8 ? 3 : 2) paged_decode_attn_k
     int pre = 0;   // stages issued before the dependency wait (first segment only)
     if (!waited) {
         while (pre < ST - 1 && (pre >= my_n || blk0 + warp + AT_WARPS * pre < blk_pos)) { issue(pre); ++pre; }
-        pdl_wait_prior();
+        if (!BESIDE) pdl_wait_prior();
         waited = true;
         if (tr) p.trace[1] = gtimer();
         if (FUSED && p.zero0) {
@@ -355,7 +361,10 @@ __global__ void __launch_bounds__(AT_WARPS * 32, I8 ? 3 : 2) paged_decode_attn_k
         const __nv_bfloat16* qrow = p.q + ((size_t)b * p.H + (size_t)kvh * p.G + g) * AT_D;
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) {
-            if (!I8) {
+            if (BESIDE) {
+                qa[ks][0] = g < p.G ? (uint32_t)ldcg_i32(reinterpret_cast<const int32_t*>(qrow + ks * 16 + 2 * t)) : 0u;
+                qa[ks][1] = g < p.G ? (uint32_t)ldcg_i32(reinterpret_cast<const int32_t*>(qrow + ks * 16 + 8 + 2 * t)) : 0u;
+            } else if (!I8) {
                 qa[ks][0] = (g < p.G) ? *reinterpret_cast<const uint32_t*>(qrow + ks * 16 + 2 * t) : 0u;
                 qa[ks][1] = (g < p.G) ? *reinterpret_cast<const uint32_t*>(qrow + ks * 16 + 8 + 2 * t) : 0u;
             } else {   // d = 16 ks + 4t .. 4t+3 (the order the int8 K bytes come out of ldmatrix), bf16 -> f16 is exact here
@@ -766,7 +775,8 @@ __global__ void __launch_bounds__(AT_WARPS * 32, I8 ? 3 : 2) paged_decode_attn_k
     if (tr) p.trace[5] = gtimer();
     __syncthreads();   // the next segment's K/V ring (and its q fragments) reuse the shared memory the merge just read
     }   // segment loop
-    if (!waited) {     // a CTA without work (legacy form: chunk past the sequence; even form: empty range) still owes the dependency
+    if (BESIDE && bid == nctas - 1) pdl_wait_prior();
+    if (!BESIDE && !waited) {     // a CTA without work (legacy form: chunk past the sequence; even form: empty range) still owes the dependency
         pdl_wait_prior();   // wait and its share of the accumulator clearing
         if (FUSED && p.zero0) {
             for (int i = (bid * AT_WARPS * 32 + tid) * 4; i < p.zero0_n; i += nctas * AT_WARPS * 32 * 4)
@@ -968,13 +978,16 @@ int launch_rope_kv_append(const RopeParams& p, cudaStream_t s, bool pdl) {
 }
 
 // picks the chunking, launches attention (+ merge when sequences span several chunks)
-int launch_paged_decode_attn(AttnParams p, int max_seq_hint, void* workspace, size_t workspace_bytes, cudaStream_t s, bool pdl, AttnChunks* unmerged = nullptr) {
+int launch_paged_decode_attn(AttnParams p, int max_seq_hint, void* workspace, size_t workspace_bytes, cudaStream_t s, bool pdl, AttnChunks* unmerged = nullptr, bool beside = false) {
     static DevOnce attr;
     if (attr.need()) {
         if (cuda_check(cudaFuncSetAttribute(paged_decode_attn_kernel<false, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, AT_SMEM), "attn smem")) return WF_ERR_CUDA;
         if (cuda_check(cudaFuncSetAttribute(paged_decode_attn_kernel<true, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, AT_SMEM), "attn smem")) return WF_ERR_CUDA;
         if (cuda_check(cudaFuncSetAttribute(paged_decode_attn_kernel<false, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, AT8_SMEM), "attn smem")) return WF_ERR_CUDA;
         if (cuda_check(cudaFuncSetAttribute(paged_decode_attn_kernel<true, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, AT8_SMEM), "attn smem")) return WF_ERR_CUDA;
+        // (left to itself the driver gives an SM the shared memory that one of its kernels asks for, and the other's blocks wait)
+        if (cuda_check(cudaFuncSetAttribute(paged_decode_attn_kernel<false, false, true>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared), "attn smem") ||
+            cuda_check(cudaFuncSetAttribute(paged_decode_attn_kernel<false, false, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, AT_BESIDE_SMEM), "attn smem")) return WF_ERR_CUDA;
     }
     const int max_blocks16 = (max_seq_hint + AT_BLK - 1) / AT_BLK;
     // Chunking of a sequence's KV stream over CTAs (large grids; small ones take the cluster form below).  Cost model, calibrated on
@@ -1011,6 +1024,9 @@ int launch_paged_decode_attn(AttnParams p, int max_seq_hint, void* workspace, si
         // 2B bs32/2K one chunk 2.81 ms, two 2.45; bs48/4K one 4.09, three 3.77; bs64/4K and bs64/2K one chunk (320 CTAs on 444 slots) best
         const long long R = p.kv_scales ? slots : slots * 3 / 8;
         auto model = [&](int nn, int cb) -> long long {
+            // beside another kernel a block starts whenever one has ended, and the last one runs by itself: 16 sequences of 2048 beside a prefix of 2048 take 32.6 us at
+            // n = 1, 26.0 at 2, 27.8 at 4; 64 of 4096 beside 1024 152.6, 137.9 and 134.6; 32 of 4096 beside 8192 94.2, 86.6 and 84.8; 128 of 1024 beside 8192 103, 107 and 117
+            if (beside) return pairs * nn * (cb + cm_c0) * 10 / (3LL * sm_count() * 3 / 8) + (cb + cm_c0) * 10 + (nn > 1 ? 14 * nn : 0);
             const long long J = pairs * nn, L = cb + (p.kv_scales && !getenv("WF_ATTN_C0") ? 30 : cm_c0);   // int8: n = 4 at bs64/4K predicted 14 % ahead of n = 1 with C0 = 10, measured 3 % behind
             const long long full = J / slots, rem = J % slots;
             auto wave = [&](long long m) -> long long { return m >= R ? m * L * 10 / R : (m > 0 ? L * 10 : 0); };
@@ -1026,7 +1042,7 @@ int launch_paged_decode_attn(AttnParams p, int max_seq_hint, void* workspace, si
             const long long cost = model(nn, cb);
             if (best < 0 || cost < best) { best = cost; chunk_blocks = cb; nchunks = nn; }
         }
-        if (!p.kv_scales && model(old_n, old_cb) * 100 <= best * 104) { chunk_blocks = old_cb; nchunks = old_n; }   // (a bf16 calibration)
+        if (!p.kv_scales && !beside && model(old_n, old_cb) * 100 <= best * 104) { chunk_blocks = old_cb; nchunks = old_n; }   // (a bf16 calibration)
     }
     {   // experiments: WF_ATTN_NCHUNKS forces the chunk count of the large-grid form
         static const int force_n = getenv("WF_ATTN_NCHUNKS") ? atoi(getenv("WF_ATTN_NCHUNKS")) : 0;
@@ -1129,7 +1145,7 @@ int launch_paged_decode_attn(AttnParams p, int max_seq_hint, void* workspace, si
                              : (p.chunk_major ? dim3(p.Hkv, p.B, nchg) : dim3(nchg, p.Hkv, p.B));
         cfg.blockDim = dim3(AT_WARPS * 32);
         const bool i8 = p.kv_scales != nullptr;
-        cfg.dynamicSmemBytes = i8 ? AT8_SMEM : AT_SMEM;
+        cfg.dynamicSmemBytes = i8 ? AT8_SMEM : beside ? AT_BESIDE_SMEM : AT_SMEM;
         cfg.stream = s;
         cudaLaunchAttribute la[2];
         int na = 0;
@@ -1139,7 +1155,8 @@ int launch_paged_decode_attn(AttnParams p, int max_seq_hint, void* workspace, si
         cfg.numAttrs = na;
         const bool fused = p.qkv_acc != nullptr;
         cudaError_t le;
-        if (i8) le = fused ? cudaLaunchKernelEx(&cfg, paged_decode_attn_kernel<true, true>, p) : cudaLaunchKernelEx(&cfg, paged_decode_attn_kernel<false, true>, p);
+        if (beside) le = cudaLaunchKernelEx(&cfg, paged_decode_attn_kernel<false, false, true>, p);
+        else if (i8) le = fused ? cudaLaunchKernelEx(&cfg, paged_decode_attn_kernel<true, true>, p) : cudaLaunchKernelEx(&cfg, paged_decode_attn_kernel<false, true>, p);
         else le = fused ? cudaLaunchKernelEx(&cfg, paged_decode_attn_kernel<true, false>, p) : cudaLaunchKernelEx(&cfg, paged_decode_attn_kernel<false, false>, p);
         if (launch_check(le, "paged_decode_attn")) return WF_ERR_CUDA;
         if (fused) return WF_OK;
@@ -1199,7 +1216,7 @@ size_t attn_chunks_bytes(int B, int H, int Hkv, int max_seq) {
 }
 
 int attn_decode_chunks(const void* q, const void* pool, int layers, int layer, int Hkv, int page_size, const int32_t* block_table, int max_blocks, const int32_t* seq_lens, int B, int H,
-                       float scale, void* ws, size_t ws_bytes, float* kv_scales, AttnChunks* out, cudaStream_t s) {
+                       float scale, void* ws, size_t ws_bytes, float* kv_scales, bool beside, AttnChunks* out, cudaStream_t s) {
     AttnParams p = {};
     p.kv_scales = kv_scales;
     p.q = (const __nv_bfloat16*)q; p.pool = (const __nv_bfloat16*)pool;
@@ -1208,7 +1225,7 @@ int attn_decode_chunks(const void* q, const void* pool, int layers, int layer, i
     p.layers = layers; p.layer = layer; p.page_size = page_size; p.max_blocks = max_blocks;
     p.scale_log2e = scale * 1.4426950408889634f;
     p.n_out = 1; p.signal_flag = -1;
-    return launch_paged_decode_attn(p, max_blocks * page_size, ws, ws_bytes, s, true, out);
+    return launch_paged_decode_attn(p, max_blocks * page_size, ws, ws_bytes, s, true, out, beside && !kv_scales);
 }
 
 // decode-engine form: q/k/v are dequantised from the qkv linear's raw accumulator inside the kernel (RoPE, KV append,

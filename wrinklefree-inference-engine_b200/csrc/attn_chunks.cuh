@@ -24,10 +24,11 @@ struct AttnChunks {
     const float *part_o, *part_ml;
     int max_chunks, chunk_blocks, min_cb;
 };
-// workspace: attn_chunks_bytes
+// workspace: attn_chunks_bytes.  beside (bf16 pools): the kernel launched before has waited for all that this part reads, lets the next one start at once and leaves it 64 KB
+// of shared memory and 168 x 128 registers of every SM
 size_t attn_chunks_bytes(int B, int H, int Hkv, int max_seq);
 int attn_decode_chunks(const void* q, const void* pool, int layers, int layer, int Hkv, int page_size, const int32_t* block_table, int max_blocks, const int32_t* seq_lens, int B, int H,
-                       float scale, void* ws, size_t ws_bytes, float* kv_scales, AttnChunks* out, cudaStream_t s);
+                       float scale, void* ws, size_t ws_bytes, float* kv_scales, bool beside, AttnChunks* out, cudaStream_t s);
 
 // what the decode attention entry points ask of their cache, heads and output (pointers: none of theirs is null)
 int check_decode_attn(const wf_kv_layout* kv, int layer, int H, int out_dtype, bool pointers, const char* who);

@@ -2,7 +2,11 @@
 //
 // Softmax over (prefix, own) keys is the merge of two: each part leaves its running maximum m, sum l of 2^(s - m) and weighted values o, and the row's result is
 // sum o_i 2^(m_i - M) / sum l_i 2^(m_i - M).  The own part is paged decode attention (attn.cu) with its chunks left unmerged.  The prefix part is a dense
-// product per key/value head, B * H / Hkv rows of queries against the prefix's keys, cut over the keys into splits.
+// product per key/value head, B * H / Hkv rows of queries against the prefix's keys, cut over the keys into splits.  The first part is bound by memory, the
+// second by the tensor cores' operand reads and the exponentials between their products: with a bf16 pool the prefix part is launched first and keeps to 161 KB of
+// shared memory and 3/4 of the registers, so that blocks of the own part run beside it on the same SMs (128 sequences, 32 and 8 heads, a prefix of 32768 and 700 own
+// tokens: 95.6 us against 109 one after another; 64, 8192 and 400: 22.9 and 27.3; 256, 2048 and 100: 47 and 56; never slower from prefixes of 512 to 65536).
+// With an int8 pool both are bound by instructions and the own part goes first.
 #include "attn_chunks.cuh"
 #include "gemm_tc_common.cuh"
 #include "wf_bitnet.h"
@@ -22,8 +26,8 @@ struct PxParams {
     float scale_log2e;
     float *part_o, *part_ml;       // [splits][Hkv][AT_D / 4][rows][4], [splits][Hkv][rows][2], rows = B * G up to the next multiple of 32
     int rows_p;                    // those rows
-    int wait_first;                // the kernel before is not this call's own
     int box, stages;               // keys per TMA box (a power of two that divides the page); key and value tiles in flight
+    int behind_own;                // the kernel before is this call's own part, which has waited for what both read
     int* err;                      // the wait word
 };
 
@@ -37,20 +41,29 @@ struct PxParams {
 // Warp 8 loads keys and values by TMA into rings of 64-key tiles (a box of 64 dims per run of keys inside a page); one thread of warps 9 and 10 each issues a
 // group's S = Q K^T (both operands in shared memory) and O += P V (P in TMEM): a wait of one group leaves the other's products running.  The output is rescaled
 // only when a row's maximum has grown by more than 2^8 since the scale was last fixed (exact: the sum carries the same scale).
+// Weights are rounded to bf16, as the products' operands (half a step is 2^-9 of a weight; sums, maxima and outputs are fp32).
 // Every wait is bounded: one that runs out leaves a code in the device's wait word, and the block waits for its copies and products and leaves.
+//
+// What bounds it: with 256 rows a 64-key tile takes 1720 clocks, of which the tensor core works for 1280 (S reads 4 KB of queries and 2 KB of keys in 48 clocks where
+// its products take 32; P V is bound by its products, 2 x 256) and the special function units for 768; the rest are the waits between a group's products and its
+// softmax, 150 clocks and more each beside the products' reads.  128 sequences, 32 and 8 heads, 32768 keys (69 GFLOP): 63 us in place, 1.1 PFLOP/s, 65 % of a library
+// product's rate.  Two threads a row, tiles of 128 keys, one issuing thread for both groups: 4 to 22 % slower.
 constexpr int PX_KEYS = 64, PX_ROWS = 128;             // keys of a tile, rows of a group
 constexpr int PX_QHALF = PX_ROWS * 128, PX_QTILE = 2 * PX_QHALF;       // bytes of 128 rows x 64 bf16, and of both halves of the dims
 constexpr int PX_HALF = PX_KEYS * 128, PX_TILE = 2 * PX_HALF;          // the same of a tile of keys or values
-constexpr int PX_SMEM_USE = 224 * 1024;                // queries of one or two groups, then rings of six or five tiles of keys and of values
+constexpr int PX_SMEM_USE = 160 * 1024;                // queries of one or two groups, then rings of four or three tiles of keys and of values (five of six: as fast)
 constexpr int PX_SMEM = PX_SMEM_USE + 1024;
-constexpr int PX_STAGES = 6;
-constexpr int PX_THREADS = 11 * 32;
+constexpr int PX_STAGES = 4;
+// A block of the own part wants 64 KB and 168 registers a thread of the same SM.  Registers are had from quarters of an SM, three warps of this kernel and one of that
+// on each: (3 x 112 + 168) x 32 of 16384.  The softmax warps take 16 of what the others leave (at 112 for all they spill, 84 us instead of 73).
+constexpr int PX_THREADS = 12 * 32, PX_REGS = 112, PX_REGS_SOFTMAX = 128, PX_REGS_OTHERS = 80;         // (warp 11 only fills its warpgroup)
+static_assert(2 * PX_REGS_SOFTMAX + PX_REGS_OTHERS == 3 * PX_REGS, "the softmax warpgroups take what the third one gives");
 // int8 pools: a ring of tiles as they lie in the pool, and one of converted tiles with their scales
 constexpr int PX_RAW = 3, PX_RAW_TILE = 2 * PX_KEYS * AT_D, PX_SC = 2 * PX_KEYS * 4, PX_STAGES8 = 3;
 constexpr int PX_CONV = 4;                             // converting warps
 constexpr int PX_SMEM8_USE = 2 * PX_QTILE + PX_STAGES8 * 2 * PX_TILE + PX_RAW * PX_RAW_TILE + PX_STAGES8 * PX_SC;
 constexpr int PX_SMEM8 = PX_SMEM8_USE + 1024;
-constexpr int PX_THREADS8 = PX_THREADS + PX_CONV * 32;
+constexpr int PX_THREADS8 = (11 + PX_CONV) * 32;
 static_assert(PX_SMEM <= 226 * 1024 && PX_SMEM8 <= 226 * 1024, "one block's shared memory");
 constexpr unsigned long long PX_LIMIT_NS = 1000000000ull;
 constexpr float PX_LAZY = 8.f;
@@ -91,7 +104,7 @@ __device__ __forceinline__ float px_ex2(float x) { float y; asm("ex2.approx.ftz.
 __device__ __forceinline__ float px_max(float a, float b) { float y; asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b)); return y; }     // NaN stays NaN
 // 2^x of two numbers on the multiply-add units: x = i + f, |f| <= 1/2, by adding 1.5 * 2^23; 2^f by its minimax polynomial of degree 3 (Remez; off by 7.5e-5 at
 // most, a 26th of the rounding of a weight to bf16); i goes into the exponent.  Below 2^-126: 2^-126 or less.  The special function unit gives 16 values a
-// clock and SM, the products of a pair of groups ask for 25; one pair in PX_POLY takes this way.
+// clock and SM; one pair in PX_POLY takes this way: 74.4 us for a prefix of 32768 under 128 sequences with one in 8, 71.5 in 4, 71.7 in 3, 72.3 in 2, 79 without.
 constexpr int PX_POLY = 4;
 __device__ __forceinline__ void px_exp2_poly(uint64_t x, float& e0, float& e1) {
     const uint64_t magic = px_pair(0x4b400000u, 0x4b400000u), minus_magic = px_pair(0xcb400000u, 0xcb400000u), minus1 = px_pair(0xbf800000u, 0xbf800000u);
@@ -106,6 +119,8 @@ __device__ __forceinline__ void px_exp2_poly(uint64_t x, float& e0, float& e1) {
     e0 = __uint_as_float((uint32_t)y + ((uint32_t)t << 23));
     e1 = __uint_as_float((uint32_t)(y >> 32) + ((uint32_t)(t >> 32) << 23));
 }
+template <int N> __device__ __forceinline__ void px_regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N) : "memory"); }
+template <int N> __device__ __forceinline__ void px_regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ uint4 px_ldcg(const uint4* a) {
     uint4 r;
     asm volatile("ld.global.cg.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(a));
@@ -113,7 +128,7 @@ __device__ __forceinline__ uint4 px_ldcg(const uint4* a) {
 }
 
 template <bool I8>
-__global__ void __launch_bounds__(I8 ? PX_THREADS8 : PX_THREADS, 1) prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ PxParams p) {
+__global__ void __launch_bounds__(I8 ? PX_THREADS8 : PX_THREADS, 1) __maxnreg__(I8 ? 128 : PX_REGS) prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ PxParams p) {
     extern __shared__ unsigned char smem_raw[];
     __shared__ __align__(8) uint64_t q_full[2], kv_full[PX_STAGES], kv_empty[PX_STAGES], tail_full, raw_full[PX_RAW], raw_empty[PX_RAW], s_full[2][2], p_full[2][2], o_full[2], o_end[2], drained[2];
     __shared__ uint32_t tmem_base_s;
@@ -149,10 +164,13 @@ __global__ void __launch_bounds__(I8 ? PX_THREADS8 : PX_THREADS, 1) prefix_attn_
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_base_s;
-    if (p.wait_first) pdl_wait_prior();
+    if (!p.behind_own) pdl_wait_prior();
     pdl_launch_dependents();
 
-    if (warp == 8) {
+    if (!I8 && warp == 11) {
+        if (!I8) px_regs_dec<PX_REGS_OTHERS>();
+    } else if (warp == 8) {
+        if (!I8) px_regs_dec<PX_REGS_OTHERS>();
         // ------------------------------------------------------------ producer: lanes 0..3 the boxes of keys, 4..7 of values
         const int kv = lane >> 2 & 1, off = (lane & 3) * p.box;
         const int depth = I8 ? PX_RAW : nst, step = I8 ? PX_RAW_TILE : PX_TILE;
@@ -261,6 +279,7 @@ __global__ void __launch_bounds__(I8 ? PX_THREADS8 : PX_THREADS, 1) prefix_attn_
         }
         if (!ok && lane == 0) *(volatile int*)p.err = 19;
     } else if (warp == 9 || warp == 10) {
+        if (!I8) px_regs_dec<PX_REGS_OTHERS>();
         // ------------------------------------------------------------ a group's products
         const int t = warp - 9, tiles = alt ? (nt - t + 1) / 2 : nt;
         uint32_t elected;
@@ -305,6 +324,7 @@ __global__ void __launch_bounds__(I8 ? PX_THREADS8 : PX_THREADS, 1) prefix_attn_
         if (elected) px_commit(&drained[t]);              // nor while a product still reads shared memory or TMEM
         px_wait_warp(&drained[t], 0);
     } else {
+        if (!I8) px_regs_inc<PX_REGS_SOFTMAX>();
         // ------------------------------------------------------------ softmax: a thread per row
         const int t = warp >> 2, tr = (warp & 3) * 32 + lane, r = row0 + (alt ? 0 : t * PX_ROWS) + tr;
         const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
@@ -485,7 +505,7 @@ __global__ void __launch_bounds__(I8 ? PX_THREADS8 : PX_THREADS, 1) prefix_attn_
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
     }
-    if (!p.wait_first) pdl_wait_prior();                  // the own part's kernel: whoever waits for this one has waited for that one
+    if (p.behind_own) pdl_wait_prior();                   // whoever waits for this kernel has waited for that one
 }
 
 DevMade g_px_attr;
@@ -514,45 +534,91 @@ struct PxMerge {
     int out_dtype;
 };
 
-// A thread per row and 4 C columns: neighbouring threads are neighbouring rows, as the prefix part's results lie.  First the maximum of all parts, then their
-// factors and sums, several parts under way at a time.
+// Bound by a few rounds of latency: of 128 sequences with 9 splits of 2.1 MB 9 us, of which the launch takes 2.  A thread per row and 4 C columns: neighbouring threads are neighbouring rows, as the prefix part's results lie.  The results of several parts, with their maxima
+// and sums, are under way at a time; the first own chunks' too, before it is known how many of them there are (every slot is memory of the workspace).
 constexpr int PX_MERGE = 128;
 template <int C>
 __global__ void __launch_bounds__(PX_MERGE) prefix_merge_kernel(const __grid_constant__ PxMerge p) {
+    constexpr int AT_ONCE = C == 1 ? 12 : 4, OWN = C == 1 ? 4 : 2;
     const int kvh = blockIdx.x % p.Hkv, r = blockIdx.x / p.Hkv * PX_MERGE + threadIdx.x, c0 = blockIdx.y * C;
     pdl_wait_prior();
     pdl_launch_dependents();
     if (r >= p.rows) return;
     const int b = r / p.G, row = b * p.H + kvh * p.G + (r - b * p.G);
-    int own = 0;
-    if (p.own.part_o) {
-        const int nblocks = (p.seq_lens[b] + AT_BLK - 1) / AT_BLK;
-        const int cb = chunk_blocks_of(nblocks, p.own.chunk_blocks, p.own.max_chunks, p.own.min_cb);
-        own = min((nblocks + cb - 1) / cb, p.own.max_chunks);      // (a length beyond the table's)
-    }
     const size_t next = (size_t)p.Hkv * p.rows_p;         // from a split to the next
     const float2 *ml = reinterpret_cast<const float2*>(p.part_ml) + (size_t)kvh * p.rows_p + r, *oml = reinterpret_cast<const float2*>(p.own.part_ml) + (size_t)row * p.own.max_chunks;
+    const float4* v = reinterpret_cast<const float4*>(p.part_o) + ((size_t)kvh * 32 + c0) * p.rows_p + r;
+    const float4* w = reinterpret_cast<const float4*>(p.own.part_o) + (size_t)row * p.own.max_chunks * 32 + c0;
+    const float2 none = make_float2(-INFINITY, 0.f);
+    const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
     float M = -INFINITY, L = 0.f;
-#pragma unroll 8
-    for (int i = 0; i < p.splits; ++i) M = fmaxf(M, ml[i * next].x);
-    for (int i = 0; i < own; ++i) M = fmaxf(M, oml[i].x);
     float4 o[C];
 #pragma unroll
-    for (int k = 0; k < C; ++k) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-    auto add = [&](const float2 x, const float4* v, size_t step) {
-        const float f = x.x == -INFINITY ? 0.f : exp2f(x.x - M);
-        L = fmaf(x.y, f, L);
+    for (int k = 0; k < C; ++k) o[k] = zero;
+    auto join = [&](auto& x, auto& y) {                   // parts with their maxima and sums x, and values y
+        constexpr int N = sizeof(x) / sizeof(x[0]);
+        float m = M;
 #pragma unroll
-        for (int k = 0; k < C; ++k) {
-            const float4 w = v[k * step];
-            o[k].x = fmaf(f, w.x, o[k].x); o[k].y = fmaf(f, w.y, o[k].y); o[k].z = fmaf(f, w.z, o[k].z); o[k].w = fmaf(f, w.w, o[k].w);
+        for (int u = 0; u < N; ++u) m = fmaxf(m, x[u].x);
+        const float f0 = M == -INFINITY ? 0.f : exp2f(M - m);
+        L *= f0;
+#pragma unroll
+        for (int k = 0; k < C; ++k) { o[k].x *= f0; o[k].y *= f0; o[k].z *= f0; o[k].w *= f0; }
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+            const float f = x[u].x == -INFINITY ? 0.f : exp2f(x[u].x - m);
+            L = fmaf(x[u].y, f, L);
+#pragma unroll
+            for (int k = 0; k < C; ++k) {
+                o[k].x = fmaf(f, y[u][k].x, o[k].x); o[k].y = fmaf(f, y[u][k].y, o[k].y); o[k].z = fmaf(f, y[u][k].z, o[k].z); o[k].w = fmaf(f, y[u][k].w, o[k].w);
+            }
         }
+        M = m;
     };
-    const float4* v = reinterpret_cast<const float4*>(p.part_o) + ((size_t)kvh * 32 + c0) * p.rows_p + r;
-#pragma unroll 4
-    for (int i = 0; i < p.splits; ++i) add(ml[i * next], v + i * next * 32, p.rows_p);
-    const float4* w = reinterpret_cast<const float4*>(p.own.part_o) + (size_t)row * p.own.max_chunks * 32 + c0;
-    for (int i = 0; i < own; ++i) add(oml[i], w + (size_t)i * 32, 1);
+    int own = 0;
+    const int slots = p.own.part_o ? p.own.max_chunks : 0;
+    const int len = slots ? p.seq_lens[b] : 0;
+    float2 ox[OWN];
+    float4 oy[OWN][C];
+#pragma unroll
+    for (int u = 0; u < OWN; ++u) {
+        ox[u] = u < slots ? oml[u] : none;
+#pragma unroll
+        for (int k = 0; k < C; ++k) oy[u][k] = u < slots ? w[(size_t)u * 32 + k] : zero;
+    }
+    for (int i = 0; i < p.splits; i += AT_ONCE) {
+        float2 x[AT_ONCE];
+        float4 y[AT_ONCE][C];
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u) {
+            x[u] = i + u < p.splits ? ml[(i + u) * next] : none;
+#pragma unroll
+            for (int k = 0; k < C; ++k) y[u][k] = i + u < p.splits ? v[(i + u) * next * 32 + (size_t)k * p.rows_p] : zero;
+        }
+        join(x, y);
+    }
+    if (slots) {
+        const int nblocks = (len + AT_BLK - 1) / AT_BLK;
+        const int cb = chunk_blocks_of(nblocks, p.own.chunk_blocks, p.own.max_chunks, p.own.min_cb);
+        own = min((nblocks + cb - 1) / cb, slots);        // (a length beyond the table's)
+    }
+#pragma unroll
+    for (int u = 0; u < OWN; ++u)
+        if (u >= own) {
+            ox[u] = none;
+#pragma unroll
+            for (int k = 0; k < C; ++k) oy[u][k] = zero;
+        }
+    join(ox, oy);
+    for (int i = OWN; i < own; i += OWN) {
+#pragma unroll
+        for (int u = 0; u < OWN; ++u) {
+            ox[u] = i + u < own ? oml[i + u] : none;
+#pragma unroll
+            for (int k = 0; k < C; ++k) oy[u][k] = i + u < own ? w[(size_t)(i + u) * 32 + k] : zero;
+        }
+        join(ox, oy);
+    }
     const float inv = L > 0.f ? 1.f / L : L == 0.f ? 0.f : L;      // no key: zeros; NaN stays
 #pragma unroll
     for (int k = 0; k < C; ++k) {
@@ -568,7 +634,7 @@ int px_rows_p(int B, int G) { return (B * G + 31) / 32 * 32; }
 struct PxCut { int splits, keys; size_t bytes; };      // splits of the prefix, their keys, and the bytes of the partial results
 
 // In units of a hundredth of what two tiles take a block (1.95 us): a block costs 300 beside its tiles (queries in, results out), and every split what the
-// merge reads of it.
+// merge reads of it.  Twice or half of the latter moves 64 sequences over 8192 keys by -0.2 and +1.8 us of 22.8, 4 over 2048 not at all.
 PxCut px_cut(int B, int H, int Hkv, int prefix) {
     if (prefix <= 0) return PxCut{0, 0, 0};
     const int G = H / Hkv, sms = sm_count(), tiles = (int)(((long long)prefix + 2 * PX_KEYS - 1) / (2 * PX_KEYS));       // pairs of tiles: one for each group
@@ -615,9 +681,13 @@ extern "C" int wf_paged_prefix_attn(const void* q, const wf_kv_layout* kv, int l
     cudaStream_t s = (cudaStream_t)stream;
     PxMerge g = {};
     g.seq_lens = seq_lens; g.Hkv = kv->kv_heads; g.G = H / kv->kv_heads; g.H = H; g.rows = B * g.G; g.rows_p = px_rows_p(B, g.G); g.out = out; g.out_dtype = out_dtype;
-    if (max_blocks > 0)
-        if (int rc = attn_decode_chunks(q, kv->pool, kv->layers, layer, kv->kv_heads, kv->page_size, block_table, max_blocks, seq_lens, B, H, scale, (char*)workspace + mine, workspace_bytes - mine,
-                                        kv_scales_of(kv), &g.own, s)) return rc;
+    auto own_part = [&](bool beside) -> int {
+        return attn_decode_chunks(q, kv->pool, kv->layers, layer, kv->kv_heads, kv->page_size, block_table, max_blocks, seq_lens, B, H, scale, (char*)workspace + mine, workspace_bytes - mine,
+                                  kv_scales_of(kv), beside, &g.own, s);
+    };
+    const bool own_first = max_blocks > 0 && kv->dtype == WF_I8;
+    if (own_first)
+        if (int rc = own_part(false)) return rc;
     if (prefix_len > 0) {
         PxParams p = {};
         p.q = (const __nv_bfloat16*)q; p.pool = kv->pool; p.scales = kv_scales_of(kv); p.table = prefix_table;
@@ -627,26 +697,29 @@ extern "C" int wf_paged_prefix_attn(const void* q, const wf_kv_layout* kv, int l
         p.splits = cut.splits; p.split_keys = cut.keys;
         p.part_o = (float*)workspace;
         p.rows_p = g.rows_p;
+        p.behind_own = own_first;
         p.part_ml = p.part_o + (size_t)p.splits * p.Hkv * p.rows_p * AT_D;
-        p.wait_first = max_blocks == 0;
         g.part_o = p.part_o; g.part_ml = p.part_ml; g.splits = p.splits;
         const int rows = g.rows, pairs = (rows + 2 * PX_ROWS - 1) / (2 * PX_ROWS);
         const bool i8 = p.scales != nullptr;
         p.box = 16;
         while (p.box < PX_KEYS && kv->page_size % (2 * p.box) == 0) p.box *= 2;
-        p.stages = i8 ? PX_STAGES8 : rows <= PX_ROWS ? 6 : 5;
+        p.stages = i8 ? PX_STAGES8 : (PX_SMEM_USE - (rows <= PX_ROWS ? 1 : 2) * PX_QTILE) / (2 * PX_TILE);
         p.err = tc_wait_word();
         if (!p.err) { set_error("%s: no wait word", who); return WF_ERR_CUDA; }
         CUtensorMap tm;
         if (int rc = px_encode(&tm, kv, p.box)) return rc;
         if (int rc = g_px_attr.once([&]() -> int {
-                return cuda_check(cudaFuncSetAttribute(prefix_attn_tc_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, PX_SMEM), who) ||
+                return cuda_check(cudaFuncSetAttribute(prefix_attn_tc_kernel<false>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared), who) ||
+                               cuda_check(cudaFuncSetAttribute(prefix_attn_tc_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, PX_SMEM), who) ||
                                cuda_check(cudaFuncSetAttribute(prefix_attn_tc_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, PX_SMEM8), who) ? WF_ERR_CUDA : WF_OK;
             })) return rc;
         const dim3 grid((unsigned)(pairs * p.Hkv * p.splits));
         const cudaError_t e = i8 ? launch_pdl(prefix_attn_tc_kernel<true>, grid, PX_THREADS8, PX_SMEM8, s, tm, p) : launch_pdl(prefix_attn_tc_kernel<false>, grid, PX_THREADS, PX_SMEM, s, tm, p);
         if (int rc = launch_check(e, "prefix_attn_tc")) return rc;
     }
+    if (max_blocks > 0 && !own_first)
+        if (int rc = own_part(prefix_len > 0)) return rc;
     const unsigned blocks = (unsigned)((g.rows + PX_MERGE - 1) / PX_MERGE) * g.Hkv;
     if (blocks >= 64) return launch_check(launch_pdl(prefix_merge_kernel<4>, dim3(blocks, 8), PX_MERGE, 0, s, g), "prefix_merge");
     return launch_check(launch_pdl(prefix_merge_kernel<1>, dim3(blocks, 32), PX_MERGE, 0, s, g), "prefix_merge");
