@@ -248,6 +248,52 @@ def test_graphs_and_streams_side_by_side(int8):
     assert all(torch.equal(x, y) for x, y in zip(outs, want))
 
 
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("B, H, Hkv, prefix, lens", [(3, 32, 8, 500, [6000, 300, 0]), (2, 8, 1, 3000, [20000, 16385]), (1, 4, 4, 40, [5121])])
+def test_long_own_parts(B, H, Hkv, prefix, lens, int8):
+    """sequences of many chunks: more of them than the merge asks for at once"""
+    check(*case(B, H, Hkv, prefix, lens, 16, int8, 4))
+
+
+@pytest.mark.parametrize("B, own", [(256, 300), (300, 40)])
+def test_wide_merges(B, own):
+    """many rows: the merge takes 16 columns a thread"""
+    q, kv, layer, pt, prefix, table, lens = case(B, 32, 8, 700, [(7 * b) % own for b in range(B)], 16, False, 6, layers=1, layer=0)
+    some = [0, 1, B // 2, B - 1]
+    from wf_bitnet import ops
+    out = ops.paged_prefix_attn(q, kv, layer, pt, prefix, table, lens)
+    for b in some:                                       # a sequence by itself: held against 64 bits by check
+        check(q[b:b + 1], kv, layer, pt, prefix, table[b:b + 1], lens[b:b + 1])
+        alone = ops.paged_prefix_attn(q[b:b + 1], kv, layer, pt, prefix, table[b:b + 1], lens[b:b + 1])
+        # both are within 2^-8 |result| + (2^-8 + small) of the weighted values, |v| < 6 here, of the same number
+        assert float((out[b] - alone[0]).abs().max()) < 4 * 2.0**-8 * 6
+
+
+@pytest.mark.parametrize("int8", [False, True])
+def test_replays_see_what_the_step_before_them_wrote(int8):
+    """queries, tables and lengths written by the kernels right before the call, others at each replay"""
+    from wf_bitnet import ops
+    q, kv, layer, pt, prefix, table, lens = case(24, 8, 2, 900, [16 * (b % 20 + 1) for b in range(24)], 16, int8, 8)
+    order = [torch.randperm(24, device="cuda") for _ in range(6)]
+    turned = [pt[torch.arange(pt.numel() - 1, device="cuda").roll(i)] for i in range(6)]     # (the last page is not full)
+    src = [(q[o].contiguous(), torch.cat([t, pt[-1:]]), table[o].contiguous(), lens[o].contiguous()) for o, t in zip(order, turned)]
+    want = [ops.paged_prefix_attn(a, kv, layer, b, prefix, c, d) for a, b, c, d in src]
+    held = [t.clone() for t in src[0]]
+    feed = [t.clone() for t in src[0]]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for h, f in zip(held, feed):
+            h.copy_(f)
+        out = ops.paged_prefix_attn(held[0], kv, layer, held[1], prefix, held[2], held[3])
+    for _ in range(3):
+        for s, w in zip(src, want):
+            for f, t in zip(feed, s):
+                f.copy_(t)
+            graph.replay()
+            assert torch.equal(out, w)
+
+
 def test_one_serving_step_after_another():
     """plan -> cache -> attention behind the prefix -> logits -> log probabilities, the same as with everything computed in 64 bits; pages go back at the end"""
     from wf_bitnet import ops

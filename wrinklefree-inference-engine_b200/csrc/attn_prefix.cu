@@ -41,7 +41,7 @@ struct PxParams {
 // Warp 8 loads keys and values by TMA into rings of 64-key tiles (a box of 64 dims per run of keys inside a page); one thread of warps 9 and 10 each issues a
 // group's S = Q K^T (both operands in shared memory) and O += P V (P in TMEM): a wait of one group leaves the other's products running.  The output is rescaled
 // only when a row's maximum has grown by more than 2^8 since the scale was last fixed (exact: the sum carries the same scale).
-// Weights are rounded to bf16, as the products' operands (half a step is 2^-9 of a weight; sums, maxima and outputs are fp32).
+// Weights are rounded to bf16, as the products' operands (off by 2^-8 of a weight at most; sums, maxima and outputs are fp32).
 // Every wait is bounded: one that runs out leaves a code in the device's wait word, and the block waits for its copies and products and leaves.
 //
 // What bounds it: with 256 rows a 64-key tile takes 1720 clocks, of which the tensor core works for 1280 (S reads 4 KB of queries and 2 KB of keys in 48 clocks where
@@ -103,7 +103,7 @@ __device__ __forceinline__ uint64_t px_add2(uint64_t a, uint64_t b) { uint64_t v
 __device__ __forceinline__ float px_ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ float px_max(float a, float b) { float y; asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b)); return y; }     // NaN stays NaN
 // 2^x of two numbers on the multiply-add units: x = i + f, |f| <= 1/2, by adding 1.5 * 2^23; 2^f by its minimax polynomial of degree 3 (Remez; off by 7.5e-5 at
-// most, a 26th of the rounding of a weight to bf16); i goes into the exponent.  Below 2^-126: 2^-126 or less.  The special function unit gives 16 values a
+// most, a 50th of what the rounding of a weight to bf16 may be); i goes into the exponent.  Below 2^-126: 2^-126 or less.  The special function unit gives 16 values a
 // clock and SM; one pair in PX_POLY takes this way: 74.4 us for a prefix of 32768 under 128 sequences with one in 8, 71.5 in 4, 71.7 in 3, 72.3 in 2, 79 without.
 constexpr int PX_POLY = 4;
 __device__ __forceinline__ void px_exp2_poly(uint64_t x, float& e0, float& e1) {
