@@ -60,7 +60,7 @@ constexpr int PX_THREADS = 12 * 32, PX_REGS = 112, PX_REGS_SOFTMAX = 128, PX_REG
 static_assert(2 * PX_REGS_SOFTMAX + PX_REGS_OTHERS == 3 * PX_REGS, "the softmax warpgroups take what the third one gives");
 // int8 pools: a ring of tiles as they lie in the pool, and one of converted tiles with their scales
 constexpr int PX_RAW = 3, PX_RAW_TILE = 2 * PX_KEYS * AT_D, PX_SC = 2 * PX_KEYS * 4, PX_STAGES8 = 3;
-constexpr int PX_CONV = 4;                             // converting warps
+constexpr int PX_CONV = 4;                             // converting warps (eight: as fast, at 34.4 us for 31 sequences of 64 and 8 heads over 16384 keys: shared memory is what is busy)
 constexpr int PX_SMEM8_USE = 2 * PX_QTILE + PX_STAGES8 * 2 * PX_TILE + PX_RAW * PX_RAW_TILE + PX_STAGES8 * PX_SC;
 constexpr int PX_SMEM8 = PX_SMEM8_USE + 1024;
 constexpr int PX_THREADS8 = (11 + PX_CONV) * 32;
