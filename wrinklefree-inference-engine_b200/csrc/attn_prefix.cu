@@ -128,7 +128,7 @@ __device__ __forceinline__ uint4 px_ldcg(const uint4* a) {
 }
 
 template <bool I8>
-__global__ void __launch_bounds__(I8 ? PX_THREADS8 : PX_THREADS, 1) __maxnreg__(I8 ? 128 : PX_REGS) prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ PxParams p) {
+__maxnreg__(I8 ? 128 : PX_REGS) __global__ void __launch_bounds__(I8 ? PX_THREADS8 : PX_THREADS, 1) prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ PxParams p) {
     extern __shared__ unsigned char smem_raw[];
     __shared__ __align__(8) uint64_t q_full[2], kv_full[PX_STAGES], kv_empty[PX_STAGES], tail_full, raw_full[PX_RAW], raw_empty[PX_RAW], s_full[2][2], p_full[2][2], o_full[2], o_end[2], drained[2];
     __shared__ uint32_t tmem_base_s;
