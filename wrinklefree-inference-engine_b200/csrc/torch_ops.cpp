@@ -6,6 +6,7 @@
 // A call through ctypes spent 20 us of host time on what takes the GPU 6 (one token, 2560 x 2560), and the feed-forward op waited twice for a copy of
 // its weight scales to the device; here a call costs about 8 us and the scales travel as kernel parameters.
 #include <ATen/ATen.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <pybind11/pybind11.h>
@@ -217,6 +218,17 @@ int to_int(int64_t v, const char* name) {
     return (int)v;
 }
 
+// A contiguous tensor in new memory of the current device and stream, straight from torch's allocator: an at::empty takes 1.6 us, most of it on its way there
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType type) {
+    size_t bytes = c10::elementSize(type);
+    for (int64_t s : sizes) bytes *= (size_t)s;
+    auto* from = c10::cuda::CUDACachingAllocator::get();
+    auto impl = c10::make_intrusive<c10::TensorImpl>(c10::Storage(c10::Storage::use_byte_size_t(), bytes, from->allocate(bytes), from, true), c10::DispatchKeySet(c10::DispatchKey::CUDA),
+                                                     c10::scalarTypeToTypeMeta(type));
+    impl->set_sizes_contiguous(sizes);
+    return Tensor(std::move(impl));
+}
+
 // A contiguous tensor over part of `buf`, `at` entries of its own type from the start: the outputs of a call share one allocation (1.6 us each otherwise, and a
 // slice through the dispatcher 0.9 us)
 Tensor part_of(const Tensor& buf, at::ScalarType type, int64_t at, at::IntArrayRef sizes) {
@@ -243,13 +255,13 @@ Tensor paged_prefix_attn(const Tensor& q, const Tensor& pool, int64_t max_pages,
     const Tensor pt = prefix_table.contiguous(), bt = block_table.contiguous(), sl = seq_lens.contiguous();
     const int B = (int)q.size(0), H = (int)q.size(1), D = (int)q.size(2), blocks = to_int(bt.size(1), "block_table"), pre = to_int(prefix_len, "prefix_len");
     to_int(bt.size(1) * page_size, "block_table");
-    Tensor out = at::empty({B, H, D}, q.options().dtype(out_dtype));
+    Tensor out = fresh({B, H, D}, out_dtype);
     wf_kv_layout kv;
     memset(&kv, 0, sizeof kv);
     kv.pool = pool.data_ptr();
     kv.max_pages = (int)max_pages; kv.layers = (int)layers; kv.kv_heads = (int)kv_heads; kv.page_size = (int)page_size; kv.head_dim = (int)head_dim; kv.dtype = (int)kv_dtype;
     // memory of this call's own: calls on other streams and captured graphs do not share it
-    Tensor ws = at::empty({(int64_t)wf_prefix_attn_workspace_bytes(B, H, kv.kv_heads, blocks * kv.page_size, pre)}, q.options().dtype(at::kByte));
+    Tensor ws = fresh({(int64_t)wf_prefix_attn_workspace_bytes(B, H, kv.kv_heads, blocks * kv.page_size, pre)}, at::kByte);
     check(wf_paged_prefix_attn(qc.data_ptr(), &kv, (int)layer, (const int32_t*)pt.data_ptr(), pre, (const int32_t*)bt.data_ptr(), blocks, (const int32_t*)sl.data_ptr(), B, H, (float)scale,
                                out.data_ptr(), code_of(out_dtype), ws.data_ptr(), (size_t)ws.numel(), stream()));
     return out;
@@ -272,7 +284,7 @@ std::vector<Tensor> paged_plan(const Tensor& seq_lens, const Tensor& new_lens, T
     const Tensor sl = seq_lens.contiguous(), nl = new_lens.contiguous(), fp = free_pages.contiguous();
     const int rows = to_int(B, "block_table"), cap = to_int(max_tokens, "max_tokens"), page = to_int(page_size, "page_size");
     const int64_t cap4 = (max_tokens + 3) / 4 * 4;         // every map starts on 16 bytes
-    const Tensor buf = at::empty({4 * cap4 + 2 * B + 3}, block_table.options());
+    const Tensor buf = fresh({4 * cap4 + 2 * B + 3}, at::kInt);
     const int64_t at[8] = {0, cap4, 2 * cap4, 3 * cap4, 4 * cap4, 4 * cap4 + B + 1, 4 * cap4 + 2 * B + 1, 4 * cap4 + 2 * B + 2};
     const int64_t len[8] = {max_tokens, max_tokens, max_tokens, max_tokens, B + 1, B, 1, 1};
     int32_t* base = (int32_t*)buf.data_ptr();
@@ -298,7 +310,7 @@ std::tuple<Tensor, Tensor> paged_release(const Tensor& done, const Tensor& seq_l
     TORCH_CHECK_VALUE(free_count.size(0) == 1, "free_count must have one entry");
     TORCH_CHECK_VALUE(free_pages.is_contiguous(), "free_pages must be contiguous (it is written in place)");
     const Tensor dn = done.contiguous(), sl = seq_lens.contiguous(), bt = block_table.contiguous();
-    const Tensor buf = at::empty({B + 1}, sl.options());
+    const Tensor buf = fresh({B + 1}, at::kInt);
     Tensor lens = part_of(buf, at::kInt, 0, {B}), count = part_of(buf, at::kInt, B, {1});
     check(wf_paged_release((const uint8_t*)dn.data_ptr(), (const int32_t*)sl.data_ptr(), to_int(B, "block_table"), (const int32_t*)bt.data_ptr(), to_int(bt.size(1), "block_table"),
                            (int32_t*)free_pages.data_ptr(), to_int(free_pages.size(0), "free_pages"), (const int32_t*)free_count.data_ptr(), to_int(page_size, "page_size"),
@@ -318,7 +330,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor& logits, 
     const int64_t ld = n > 1 ? x.stride(0) : V;
     const Tensor& y = ld < V ? x.contiguous() : x;         // rows that overlap (an expanded row)
     const int64_t m = n, mk = m * k;
-    const Tensor buf = at::empty({2 * (m + mk)}, x.options().dtype(at::kFloat));
+    const Tensor buf = fresh({2 * (m + mk)}, at::kFloat);
     Tensor lp = part_of(buf, at::kFloat, 0, {m}), ent = part_of(buf, at::kFloat, m, {m}), tlp = part_of(buf, at::kFloat, 2 * m, {m, k}), tid = part_of(buf, at::kInt, 2 * m + mk, {m, k});
     check(wf_token_logprobs(y.data_ptr(), dt, n, V, ld < V ? V : ld, (const int32_t*)tk.data_ptr(), k, (float)temperature, (float*)lp.data_ptr(), (float*)ent.data_ptr(),
                             (float*)tlp.data_ptr(), (int32_t*)tid.data_ptr(), stream()));
