@@ -47,7 +47,8 @@ struct PxParams {
 // What bounds it: with 256 rows a 64-key tile takes 1720 clocks, of which the tensor core works for 1280 (S reads 4 KB of queries and 2 KB of keys in 48 clocks where
 // its products take 32; P V is bound by its products, 2 x 256) and the special function units for 768; the rest are the waits between a group's products and its
 // softmax, 150 clocks and more each beside the products' reads.  128 sequences, 32 and 8 heads, 32768 keys (69 GFLOP): 63 us in place, 1.1 PFLOP/s, 65 % of a library
-// product's rate.  Two threads a row, tiles of 128 keys, one issuing thread for both groups: 4 to 22 % slower.
+// product's rate.  Two threads a row, tiles of 128 keys (one score buffer a group, whose
+// softmax and products wait for one another), one issuing thread for both groups: 4 to 22 % slower.
 constexpr int PX_KEYS = 64, PX_ROWS = 128;             // keys of a tile, rows of a group
 constexpr int PX_QHALF = PX_ROWS * 128, PX_QTILE = 2 * PX_QHALF;       // bytes of 128 rows x 64 bf16, and of both halves of the dims
 constexpr int PX_HALF = PX_KEYS * 128, PX_TILE = 2 * PX_HALF;          // the same of a tile of keys or values
