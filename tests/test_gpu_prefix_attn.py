@@ -255,9 +255,9 @@ def test_long_own_parts(B, H, Hkv, prefix, lens, int8):
     check(*case(B, H, Hkv, prefix, lens, 16, int8, 4))
 
 
-@pytest.mark.parametrize("B, own", [(256, 300), (300, 40)])
+@pytest.mark.parametrize("B, own", [(128, 120), (256, 300), (300, 40)])
 def test_wide_merges(B, own):
-    """many rows: the merge takes 16 columns a thread"""
+    """many rows: the merge takes 8 or 16 columns a thread"""
     q, kv, layer, pt, prefix, table, lens = case(B, 32, 8, 700, [(7 * b) % own for b in range(B)], 16, False, 6, layers=1, layer=0)
     some = [0, 1, B // 2, B - 1]
     from wf_bitnet import ops

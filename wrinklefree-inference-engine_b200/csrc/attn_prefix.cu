@@ -5,7 +5,7 @@
 // product per key/value head, B * H / Hkv rows of queries against the prefix's keys, cut over the keys into splits.  The first part is bound by memory, the
 // second by the tensor cores' operand reads and the exponentials between their products: with a bf16 pool the prefix part is launched first and keeps to 161 KB of
 // shared memory and 3/4 of the registers, so that blocks of the own part run beside it on the same SMs (128 sequences, 32 and 8 heads, a prefix of 32768 and 700 own
-// tokens: 95.6 us against 109 one after another; 64, 8192 and 400: 22.9 and 27.3; 256, 2048 and 100: 47 and 56; never slower from prefixes of 512 to 65536).
+// tokens: 95.6 us against 109 one after another; 64, 8192 and 400: 22.9 and 27.3; 256, 2048 and 100: 50 and 56; nowhere more than 1 % slower from prefixes of 512 to 65536).
 // With an int8 pool both are bound by instructions and the own part goes first.
 #include "attn_chunks.cuh"
 #include "gemm_tc_common.cuh"
@@ -535,12 +535,13 @@ struct PxMerge {
     int out_dtype;
 };
 
-// Bound by a few rounds of latency: of 128 sequences with 9 splits of 2.1 MB 9 us, of which the launch takes 2.  A thread per row and 4 C columns: neighbouring threads are neighbouring rows, as the prefix part's results lie.  The results of several parts, with their maxima
-// and sums, are under way at a time; the first own chunks' too, before it is known how many of them there are (every slot is memory of the workspace).
+// Bound by a few rounds of latency: of 128 sequences with 9 splits of 2.1 MB 8 us, of which the launch takes 2.  A thread per row and 4 C columns: neighbouring
+// threads are neighbouring rows, as the prefix part's results lie.  The results of several parts, with their maxima and sums, are under way at a time; the first own
+// chunks' too, before it is known how many of them there are (every slot is memory of the workspace).
 constexpr int PX_MERGE = 128;
 template <int C>
-__global__ void __launch_bounds__(PX_MERGE) prefix_merge_kernel(const __grid_constant__ PxMerge p) {
-    constexpr int AT_ONCE = C == 1 ? 12 : 4, OWN = C == 1 ? 4 : 2;
+__global__ void __launch_bounds__(PX_MERGE, 4) prefix_merge_kernel(const __grid_constant__ PxMerge p) {
+    constexpr int AT_ONCE = C == 1 ? 8 : C == 2 ? 9 : 4, OWN = C == 1 ? 4 : 2;
     const int kvh = blockIdx.x % p.Hkv, r = blockIdx.x / p.Hkv * PX_MERGE + threadIdx.x, c0 = blockIdx.y * C;
     pdl_wait_prior();
     pdl_launch_dependents();
@@ -722,6 +723,8 @@ extern "C" int wf_paged_prefix_attn(const void* q, const wf_kv_layout* kv, int l
     if (max_blocks > 0 && !own_first)
         if (int rc = own_part(prefix_len > 0)) return rc;
     const unsigned blocks = (unsigned)((g.rows + PX_MERGE - 1) / PX_MERGE) * g.Hkv;
-    if (blocks >= 64) return launch_check(launch_pdl(prefix_merge_kernel<4>, dim3(blocks, 8), PX_MERGE, 0, s, g), "prefix_merge");
-    return launch_check(launch_pdl(prefix_merge_kernel<1>, dim3(blocks, 32), PX_MERGE, 0, s, g), "prefix_merge");
+    // one wave of four blocks an SM, with as many columns a thread as that takes (128 sequences of 32 and 8 heads, prefix 32768: 97.2 us with 8, 98.9 with 4, 1.7 waves)
+    if (blocks * 32 <= 4 * (unsigned)sm_count()) return launch_check(launch_pdl(prefix_merge_kernel<1>, dim3(blocks, 32), PX_MERGE, 0, s, g), "prefix_merge");
+    if (blocks * 16 <= 4 * (unsigned)sm_count()) return launch_check(launch_pdl(prefix_merge_kernel<2>, dim3(blocks, 16), PX_MERGE, 0, s, g), "prefix_merge");
+    return launch_check(launch_pdl(prefix_merge_kernel<4>, dim3(blocks, 8), PX_MERGE, 0, s, g), "prefix_merge");
 }
