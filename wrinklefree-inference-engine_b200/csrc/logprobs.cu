@@ -15,7 +15,8 @@
 // A row is one block, or a cluster of 2 to 8 for few rows, whose results meet in distributed shared memory: one launch, no workspace.
 //
 // Bound by memory where there is much to read: 2000 rows of 128256 in float 153 us, 6.7 TB/s.  A small call is a chain of latencies: one row 3.9 us without
-// alternatives, 6.2 with one, 9.4 with 20 (bounds, ranks and the meeting of the blocks, a barrier or two each); 64 rows in bf16 11.3, of which 2.5 are its bytes.
+// alternatives, 6.1 with one, 8.3 with 20 (bounds, ranks and the meeting of the blocks, a barrier or two each); 64 rows in bf16 with five 11.1, of which 2.5 are its
+// bytes.
 #include <cuda_fp16.h>
 
 #include "logprobs.cuh"
@@ -26,6 +27,9 @@ namespace {
 
 constexpr int LP_THREADS = 512, LP_WARPS = LP_THREADS / 32;
 constexpr int LP_CAND = 2048;                         // candidates of a block
+// Blocks' lists of up to so many keys are joined by counting (n^2 / 32 reads of shared memory an SM), longer ones by bisection in each other list (a chain of reads):
+// eight lists of 20 take one row from 9.4 to 8.4 us, four of 64 took 33 rows from 8.8 to 10.3.
+constexpr int LP_FEW = 20;
 constexpr int LP_PEND = 64;                           // entries of a warp's buffer where a row is read again
 constexpr float LP_LN2 = 0.6931471805599453f, LP_LOG2E = 1.4426950408889634f;
 constexpr float LP_FLOOR = -1000.f;                   // 2^LP_FLOOR is 0: what lies below (also -inf) is brought up to it, so that 0 times it is 0
@@ -213,13 +217,14 @@ __global__ void __launch_bounds__(LP_THREADS, 2) token_logprobs_kernel(const __g
     __shared__ u64 lists[R ? LP_WARPS * RL * 32 : 1];
     __shared__ u64 bound_s;
     __shared__ uint32_t tops[LP_WARPS * TOPS], bound_v;
-    __shared__ int ncand;
+    __shared__ int ncand, ranks[R ? 8 * LP_FEW : 1];
     __shared__ float part[LP_WARPS][3];
     static_assert(!R || (LP_CAND >= LP_WARPS * LP_PEND && LP_CAND >= 8 * LP_TOP_MAX), "the candidates' space is used again");
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int cs = p.parts, rank = blockIdx.x % cs, row = blockIdx.x / cs;
     if (R && tid == 0) { bound_v = 0; ncand = 0; }
     if (R && tid < p.k) lists[tid] = 0;
+    if (R && tid < 8 * LP_FEW) ranks[tid] = 0;
     if (R) __syncthreads();
     pdl_wait_prior();
     pdl_launch_dependents();
@@ -337,7 +342,7 @@ __global__ void __launch_bounds__(LP_THREADS, 2) token_logprobs_kernel(const __g
         a.m = __shfl_sync(0xffffffffu, a.m, 0); a.s = __shfl_sync(0xffffffffu, a.s, 0); a.t = __shfl_sync(0xffffffffu, a.t, 0);
         return a;
     };
-    // the k largest of the first n candidates into list 0, a thread for each
+    // the k largest of the first n candidates into list 0, a thread for each: its place is how many are larger
     auto place = [&](int n) {
         for (int i = tid; i < n; i += LP_THREADS) {
             const u64 key = cand[R ? i : 0];
@@ -378,13 +383,26 @@ __global__ void __launch_bounds__(LP_THREADS, 2) token_logprobs_kernel(const __g
         if (rank == 0) {
             Sums mine = {0.f, 0.f, 0.f};
             if (warp == 0 && lane < cs) mine = {lp_peer(&part[0][0], lane), lp_peer(&part[0][1], lane), lp_peer(&part[0][2], lane)};
-            // every block's list is sorted: a key's place is its own plus, of each other list, how many are larger
             const int of = R ? tid / p.k : 0, own = R ? tid - of * p.k : 0;
             if (R && tid < cs * p.k) cand[tid] = lp_peer(&lists[own], of);         // at most 8 x 64
             __syncwarp();
             if (warp == 0 && lane < cs) { part[lane][0] = mine.m; part[lane][1] = mine.s; part[lane][2] = mine.t; }
             __syncthreads();
-            if (R) {
+            if (R && p.k <= LP_FEW) {
+                // a key's place is how many are larger, counted by as many threads as there are for each (places beyond the keys that there are hold 0 already)
+                const int n = cs * p.k, per = LP_THREADS / n, i = tid / per;
+                if (i < n) {
+                    const u64 key = cand[i];
+                    int at = 0;
+#pragma unroll 4
+                    for (int j = tid - i * per; j < n; j += per) at += cand[j] > key;
+                    if (at) atomicAdd(&ranks[i], at);
+                }
+                __syncthreads();
+                if (tid < n && ranks[tid] < p.k) lists[ranks[tid]] = cand[tid];
+                __syncthreads();
+            } else if (R) {
+                // every block's list is sorted: a key's place is its own plus, of each other list, how many are larger
                 if (tid < p.k) lists[tid] = 0;         // (read by the copies above)
                 __syncthreads();
                 const u64 key = tid < cs * p.k ? cand[tid] : 0;
@@ -473,8 +491,8 @@ int launch_token_logprobs(const void* logits, int dtype, int n, int V, long long
     LpParams p;
     p.logits = logits; p.ld = ld; p.tokens = tokens; p.V = V; p.k = k; p.inv_t = 1.f / temperature;
     p.logprob = logprob; p.entropy = entropy; p.top_logprob = top_logprob; p.top_id = top_id;
-    // blocks of a row: as many as there are SMs for, while every thread of them has two vectors to read.  One row of 128256 in float with 20 alternatives 9.4 us, 10.9 on
-    // four blocks, 13.3 on two, 16.7 on one.  Two blocks an SM: 37 rows with 5 alternatives 16.3 for 12.1, 64 rows of 32064 7.8 for 6.9, 75 rows of 128256 15.8 for 15.4
+    // blocks of a row: as many as there are SMs for, while every thread of them has two vectors to read.  One row of 128256 in float with 20 alternatives, lists
+    // joined by bisection: 9.4 us, 10.9 on four blocks, 13.3 on two, 16.7 on one.  Two blocks an SM: 37 rows with 5 alternatives 16.3 for 12.1, 64 rows of 32064 7.8 for 6.9, 75 rows of 128256 15.8 for 15.4
     // (with 20 alternatives 19.2 for 20.1); four: 64 rows in bf16 18.3 for 11.3.
     int cs = 1;
     while (cs < 8 && (long long)n * cs * 2 <= sm_count() && (long long)V * es >= 16LL * LP_THREADS * cs * 2) cs *= 2;
