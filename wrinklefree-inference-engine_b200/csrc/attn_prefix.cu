@@ -64,7 +64,7 @@ constexpr int PX_RAW = 3, PX_RAW_TILE = 2 * PX_KEYS * AT_D, PX_SC = 2 * PX_KEYS 
 constexpr int PX_CONV = 4;                             // converting warps (eight: as fast, at 34.4 us for 31 sequences of 64 and 8 heads over 16384 keys: shared memory is what is busy)
 constexpr int PX_SMEM8_USE = 2 * PX_QTILE + PX_STAGES8 * 2 * PX_TILE + PX_RAW * PX_RAW_TILE + PX_STAGES8 * PX_SC;
 constexpr int PX_SMEM8 = PX_SMEM8_USE + 1024;
-constexpr int PX_THREADS8 = (11 + PX_CONV) * 32;
+constexpr int PX_THREADS8 = (11 + PX_CONV) * 32, PX_REGS8 = 128;
 static_assert(PX_SMEM <= 226 * 1024 && PX_SMEM8 <= 226 * 1024, "one block's shared memory");
 constexpr unsigned long long PX_LIMIT_NS = 1000000000ull;
 constexpr float PX_LAZY = 8.f;
@@ -129,7 +129,7 @@ __device__ __forceinline__ uint4 px_ldcg(const uint4* a) {
 }
 
 template <bool I8>
-__maxnreg__(I8 ? 128 : PX_REGS) __global__ void __launch_bounds__(I8 ? PX_THREADS8 : PX_THREADS, 1) prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ PxParams p) {
+__maxnreg__(I8 ? PX_REGS8 : PX_REGS) __global__ void prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ PxParams p) {
     extern __shared__ unsigned char smem_raw[];
     __shared__ __align__(8) uint64_t q_full[2], kv_full[PX_STAGES], kv_empty[PX_STAGES], tail_full, raw_full[PX_RAW], raw_empty[PX_RAW], s_full[2][2], p_full[2][2], o_full[2], o_end[2], drained[2];
     __shared__ uint32_t tmem_base_s;
