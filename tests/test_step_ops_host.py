@@ -60,6 +60,12 @@ def test_prefix_attention_refusals():
     assert call(B=0, q=None, out=None) == _lib.WF_OK
 
 
+def test_more_sequences_than_a_grid_holds():
+    layout = _lib.KvLayout(P, 8, 1, 1, 16, 128, _lib.WF_BF16)
+    assert _lib.lib().wf_paged_prefix_attn(P, C.byref(layout), 0, P, 40, P, 2, P, 65536, 1, 0.1, P, _lib.WF_BF16, P, 1 << 60, None) == _lib.WF_ERR_UNSUPPORTED
+    assert b"65535" in _lib.lib().wf_last_error()
+
+
 def test_prefix_workspace_holds_both_parts():
     L = _lib.lib()
     assert L.wf_prefix_attn_workspace_bytes(0, 8, 2, 100, 100) == 0

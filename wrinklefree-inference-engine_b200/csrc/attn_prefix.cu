@@ -675,6 +675,7 @@ extern "C" int wf_paged_prefix_attn(const void* q, const wf_kv_layout* kv, int l
     if (int rc = check_decode_attn(kv, layer, H, out_dtype, pointers, who)) return rc;
     if (B == 0) return WF_OK;
     if ((long long)max_blocks * kv->page_size > 0x7fffffff || prefix_len > 1 << 30 || (long long)B * H > (1 << 24)) { set_error("%s: a row of block_table of 2^31 tokens, a prefix of more than 2^30, or 2^24 rows of queries", who); return WF_ERR_UNSUPPORTED; }
+    if (max_blocks > 0 && B > 65535) { set_error("%s: at most 65535 sequences with keys of their own (got %d)", who, B); return WF_ERR_UNSUPPORTED; }       // a grid's third dimension
     if (int rc = check_wait_word(who)) return rc;
     if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)kv->pool) & 15) { set_error("%s: q, out and the pool must be 16-byte aligned", who); return WF_ERR_INVALID; }
     const PxCut cut = px_cut(B, H, kv->kv_heads, prefix_len);
