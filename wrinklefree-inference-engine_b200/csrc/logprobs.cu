@@ -315,10 +315,11 @@ __global__ void __launch_bounds__(LP_THREADS, 2) token_logprobs_kernel(const __g
         }
         add(v, 16, m);
     }
-    if (rank == 0 && warp == 0) {                      // the entries beside the whole vectors, one a lane
+    // the entries beside the whole vectors, one a lane: those in front belong to the first block, those behind to the last, as where a block reads its part again
+    if (warp == 0 && (rank == 0 || rank == cs - 1)) {
         float v[16];
         const int i = lane < 16 ? lane : head + nvec * VN + lane - 16;
-        v[0] = (lane < 16 ? lane < head : lane - 16 < tail) ? LpVec<T>::one(x[i]) : -INFINITY;
+        v[0] = (lane < 16 ? rank == 0 && lane < head : rank == cs - 1 && lane - 16 < tail) ? LpVec<T>::one(x[i]) : -INFINITY;
         if (R) offer(v, 1, i, 0);
         add(v, 1, v[0]);
     }
