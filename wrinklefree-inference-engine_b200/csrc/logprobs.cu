@@ -1,7 +1,7 @@
 // Log probabilities of given tokens, with the entropy of their distributions and the most likely alternatives, from a batch's logits in ONE pass.
 //
 // With z = x / T, m the row's largest logit, a_i = (x_i - m) / T (in log 2), s = sum 2^a_i and t = sum a_i 2^a_i:
-//   log p(tok) = ln 2 (a_tok - log2 s),   H = -sum p ln p = ln 2 (log2 s - t / s);
+//   log p(tok) = (x_tok - m) / T - ln 2 log2 s,   H = -sum p ln p = ln 2 (log2 s - t / s);
 // both sums follow the running maximum (s' = s r, t' = (t + s log2 r) r, r = 2^((m - m') / T)).  Logits of -inf have probability 0 and add nothing; differences
 // are taken before the scale, so that rows masked with a type's lowest value come out right too.
 //
@@ -427,10 +427,12 @@ __global__ void __launch_bounds__(LP_THREADS, 2) token_logprobs_kernel(const __g
     }
     if (warp) return;
     const float ls = log2f(q.s), nan = __uint_as_float(0x7fc00000u);
+    // not ln 2 ((x - m) c - ls): the lowest float under a mask times log2 e is beyond float
+    auto log_p = [&](float v) { return fmaf(v - q.m, p.inv_t, -LP_LN2 * ls); };
     const bool empty = q.m == -INFINITY, bad = !(q.s >= 0.f) || q.m == INFINITY;     // no entry above -inf; NaN or +inf among them
     if (lane == 0) {
         p.entropy[row] = bad ? nan : empty ? 0.f : fmaxf(LP_LN2 * (ls - q.t / q.s), 0.f);
-        p.logprob[row] = bad || x_tok != x_tok ? nan : empty ? -INFINITY : LP_LN2 * ((x_tok - q.m) * c - ls);
+        p.logprob[row] = bad || x_tok != x_tok ? nan : empty ? -INFINITY : log_p(x_tok);
     }
     if (R) {
         int have = 0;
@@ -441,7 +443,7 @@ __global__ void __launch_bounds__(LP_THREADS, 2) token_logprobs_kernel(const __g
             have += __popc(__ballot_sync(0xffffffffu, key != 0));
             if (!key) continue;
             p.top_id[(size_t)row * p.k + at] = (int)~(uint32_t)key;
-            p.top_logprob[(size_t)row * p.k + at] = bad ? nan : LP_LN2 * ((lp_value(key) - q.m) * c - ls);
+            p.top_logprob[(size_t)row * p.k + at] = bad ? nan : log_p(lp_value(key));
         }
         for (int b = 0; have < p.k && b < p.V; b += 32) {      // the others are -inf: the lowest indices of those
             const bool low = b + lane < p.V && LpVec<T>::one(x[b + lane]) == -INFINITY;
