@@ -979,16 +979,15 @@ int launch_rope_kv_append(const RopeParams& p, cudaStream_t s, bool pdl) {
 
 // picks the chunking, launches attention (+ merge when sequences span several chunks)
 int launch_paged_decode_attn(AttnParams p, int max_seq_hint, void* workspace, size_t workspace_bytes, cudaStream_t s, bool pdl, AttnChunks* unmerged = nullptr, bool beside = false) {
-    static DevOnce attr;
-    if (attr.need()) {
-        if (cuda_check(cudaFuncSetAttribute(paged_decode_attn_kernel<false, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, AT_SMEM), "attn smem")) return WF_ERR_CUDA;
-        if (cuda_check(cudaFuncSetAttribute(paged_decode_attn_kernel<true, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, AT_SMEM), "attn smem")) return WF_ERR_CUDA;
-        if (cuda_check(cudaFuncSetAttribute(paged_decode_attn_kernel<false, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, AT8_SMEM), "attn smem")) return WF_ERR_CUDA;
-        if (cuda_check(cudaFuncSetAttribute(paged_decode_attn_kernel<true, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, AT8_SMEM), "attn smem")) return WF_ERR_CUDA;
-        // (left to itself the driver gives an SM the shared memory that one of its kernels asks for, and the other's blocks wait)
-        if (cuda_check(cudaFuncSetAttribute(paged_decode_attn_kernel<false, false, true>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared), "attn smem") ||
-            cuda_check(cudaFuncSetAttribute(paged_decode_attn_kernel<false, false, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, AT_BESIDE_SMEM), "attn smem")) return WF_ERR_CUDA;
-    }
+    static DevMade attr;
+    if (int rc = attr.once([]() -> int {
+            auto smem = [](auto kernel, int bytes) { return cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "attn smem"); };
+            if (smem(paged_decode_attn_kernel<false, false>, AT_SMEM) || smem(paged_decode_attn_kernel<true, false>, AT_SMEM) || smem(paged_decode_attn_kernel<false, true>, AT8_SMEM) ||
+                smem(paged_decode_attn_kernel<true, true>, AT8_SMEM)) return WF_ERR_CUDA;
+            // (left to itself the driver gives an SM the shared memory that one of its kernels asks for, and the other's blocks wait)
+            return cuda_check(cudaFuncSetAttribute(paged_decode_attn_kernel<false, false, true>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared), "attn smem") ||
+                           smem(paged_decode_attn_kernel<false, false, true>, AT_BESIDE_SMEM) ? WF_ERR_CUDA : WF_OK;
+        })) return rc;
     const int max_blocks16 = (max_seq_hint + AT_BLK - 1) / AT_BLK;
     // Chunking of a sequence's KV stream over CTAs (large grids; small ones take the cluster form below).  Cost model, calibrated on
     // forced chunk counts, in units of one 16-token block of a CTA:

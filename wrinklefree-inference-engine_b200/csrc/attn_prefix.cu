@@ -514,7 +514,6 @@ DevMade g_px_attr;
 
 // [128][slot][page, layer, K | V, head], boxes of `box` slots x 128 bytes
 int px_encode(CUtensorMap* tm, const wf_kv_layout* kv, int box) {
-    if (!tc_encoder()) gemm_tc_init_attrs();
     EncodeTiledFn fn = tc_encoder();
     if (!fn) { set_error("wf_paged_prefix_attn: cuTensorMapEncodeTiled unavailable"); return WF_ERR_CUDA; }
     const cuuint64_t gdim[3] = {AT_D, (cuuint64_t)kv->page_size, (cuuint64_t)kv->max_pages * kv->layers * 2 * kv->kv_heads};

@@ -466,29 +466,32 @@ __global__ void __launch_bounds__(tc_threads(NU), 1) ternary_gemm_tc_kernel(cons
 }
 
 // ---- host side --------------------------------------------------------------------------------------------
-static EncodeTiledFn g_encode = nullptr;
-static DevOnce g_tc_attr;
-static int g_tc_nu = 0;
-EncodeTiledFn tc_encoder() { return g_encode; }
+static DevMade g_tc_attr;
+static std::atomic<int> g_tc_nu{0};
+
+EncodeTiledFn tc_encoder() {
+    static std::atomic<EncodeTiledFn> encoder{nullptr};
+    EncodeTiledFn e = encoder.load(std::memory_order_acquire);
+    if (e) return e;
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult qr;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &qr) == cudaSuccess && qr == cudaDriverEntryPointSuccess) e = (EncodeTiledFn)fn;
+    if (e) encoder.store(e, std::memory_order_release);        // the same from every thread
+    return e;
+}
 
 void gemm_tc_init_attrs() {
-    if (g_tc_attr.need()) {
+    g_tc_attr.once([]() -> int {                               // (a launch without them fails by itself)
         bool ok = cudaFuncSetAttribute(ternary_gemm_tc_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, TC_SMEM) == cudaSuccess;
         ok = ok && cudaFuncSetAttribute(ternary_gemm_tc_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, TC_SMEM) == cudaSuccess;
         ok = ok && cudaFuncSetAttribute(ternary_gemm_tc_kernel<2, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, TC_SMEM) == cudaSuccess;
         ok = ok && cudaFuncSetAttribute(ternary_gemm_tc_kernel<3>, cudaFuncAttributeMaxDynamicSharedMemorySize, TC_SMEM) == cudaSuccess;
-        (void)ok;
-    }
-    if (!g_encode) {
-        void* fn = nullptr;
-        cudaDriverEntryPointQueryResult qr;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &qr) == cudaSuccess && qr == cudaDriverEntryPointSuccess)
-            g_encode = (EncodeTiledFn)fn;
-    }
+        return ok ? WF_OK : WF_ERR_CUDA;
+    });
     if (!g_tc_nu) {
         const char* u = getenv("WF_TC_NU");
-        g_tc_nu = u ? atoi(u) : 2;     // two unpack groups: 18 warps at 112 registers (three groups = 22 warps at 88 spill)
-        if (g_tc_nu < 1 || g_tc_nu > 3) g_tc_nu = 2;
+        const int nu = u ? atoi(u) : 2;        // two unpack groups: 18 warps at 112 registers (three groups = 22 warps at 88 spill)
+        g_tc_nu = nu < 1 || nu > 3 ? 2 : nu;
     }
 }
 
@@ -499,7 +502,7 @@ static int launch_tc(const wf_linear_args* a, const EpiParams& ep, cudaStream_t 
     const cuuint64_t gstride[1] = {(cuuint64_t)a->ldq};
     const cuuint32_t box[2] = {TC_BK, TC_BN};
     const cuuint32_t estr[2] = {1, 1};
-    const CUresult cr = g_encode(&tmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, (void*)a->q, gdim, gstride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+    const CUresult cr = tc_encoder()(&tmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, (void*)a->q, gdim, gstride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (cr != CUDA_SUCCESS) { set_error("gemm_tc: cuTensorMapEncodeTiled failed (%d)", (int)cr); return WF_ERR_CUDA; }
     TcParams p;
@@ -520,7 +523,7 @@ static int launch_tc(const wf_linear_args* a, const EpiParams& ep, cudaStream_t 
 int launch_gemm_tc_red(const uint8_t* w_tile, int N, int K, const int8_t* q, int M, int ldq, int k_off, float* acc, int acc_ld,
                        cudaStream_t s, bool pdl) {
     gemm_tc_init_attrs();
-    if (!g_encode) { set_error("gemm_tc: tcgen05 path unavailable (driver entry point / smem attribute)"); return WF_ERR_CUDA; }
+    if (!tc_encoder()) { set_error("gemm_tc: tcgen05 path unavailable (driver entry point / smem attribute)"); return WF_ERR_CUDA; }
     if (M < 1 || M > TC_BN || K % WF_QK || k_off % WF_QK || ldq % 16 || acc_ld % 4 || N % 8) { set_error("gemm_tc_red: unsupported shape"); return WF_ERR_UNSUPPORTED; }
     constexpr int NU = 2;
     CUtensorMap tmap;
@@ -528,7 +531,7 @@ int launch_gemm_tc_red(const uint8_t* w_tile, int N, int K, const int8_t* q, int
     const cuuint64_t gstride[1] = {(cuuint64_t)ldq};
     const cuuint32_t box[2] = {TC_BK, TC_BN};
     const cuuint32_t estr[2] = {1, 1};
-    const CUresult cr = g_encode(&tmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, (void*)(q + k_off), gdim, gstride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+    const CUresult cr = tc_encoder()(&tmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, (void*)(q + k_off), gdim, gstride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (cr != CUDA_SUCCESS) { set_error("gemm_tc_red: cuTensorMapEncodeTiled failed (%d)", (int)cr); return WF_ERR_CUDA; }
     TcParams p;
@@ -570,7 +573,7 @@ static int launch_tc_split(const wf_linear_args* a, const EpiParams& ep, int ksp
     const cuuint64_t gstride[1] = {(cuuint64_t)a->ldq};
     const cuuint32_t box[2] = {TC_BK, TC_BN};
     const cuuint32_t estr[2] = {1, 1};
-    const CUresult cr = g_encode(&tmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, (void*)a->q, gdim, gstride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+    const CUresult cr = tc_encoder()(&tmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, (void*)a->q, gdim, gstride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (cr != CUDA_SUCCESS) { set_error("gemm_tc_split: cuTensorMapEncodeTiled failed (%d)", (int)cr); return WF_ERR_CUDA; }
     TcParams p;
@@ -621,7 +624,7 @@ static int choose_form(int M, int N, int K, int out_mode, int epi_flags, int* ks
 
 int launch_gemm_tc(const wf_linear_args* a, const EpiParams& ep, cudaStream_t s) {
     gemm_tc_init_attrs();
-    if (!g_encode) { set_error("gemm_tc: tcgen05 path unavailable (driver entry point / smem attribute)"); return WF_ERR_CUDA; }
+    if (!tc_encoder()) { set_error("gemm_tc: tcgen05 path unavailable (driver entry point / smem attribute)"); return WF_ERR_CUDA; }
     int ksplit;
     // (where the host memory that pairs report to cannot be had, the forms of this file, whose waits have no limit)
     if (choose_form(a->M, a->N, a->K, ep.out_mode, ep.epi_flags, &ksplit) && tc_wait_word()) return launch_gemm_tc_pair(a, ep, s);
