@@ -559,12 +559,14 @@ __global__ void __launch_bounds__(AT_WARPS * 32, I8 || BESIDE ? 3 : 2) paged_dec
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
         const float m_new = fmaxf(m_run, mx);
-        const float corr = fast_exp2(m_run - m_new);   // 0 on the first block (m_run = -inf)
+        // nothing but scores of -inf so far: weights of 0, not of 2^(inf - inf)  (the decode engine writes its own keys)
+        const float m_sub = !FUSED && m_new == -INFINITY ? 0.f : m_new;
+        const float corr = fast_exp2(m_run - m_sub);   // 0 on the first block (m_run = -inf)
         float psum = 0.f;
         uint32_t pa[4];
         {
-            const float p00 = fast_exp2(s[0][0] - m_new), p01 = fast_exp2(s[0][1] - m_new);
-            const float p10 = fast_exp2(s[1][0] - m_new), p11 = fast_exp2(s[1][1] - m_new);
+            const float p00 = fast_exp2(s[0][0] - m_sub), p01 = fast_exp2(s[0][1] - m_sub);
+            const float p10 = fast_exp2(s[1][0] - m_sub), p11 = fast_exp2(s[1][1] - m_sub);
             psum = (p00 + p01) + (p10 + p11);
             if (!I8) {
                 pa[0] = pack_bf16x2(p00, p01);   // A frag: row g, k = 2t,2t+1
