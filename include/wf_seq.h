@@ -209,7 +209,7 @@ int wf_seq_step(wf_seq_engine* e, int nseq, const int32_t* slots, const int32_t*
 int wf_seq_sample(wf_seq_engine* e, int nwant, float temperature, int top_k, float top_p, const float* uniforms_host, int32_t* next_host);
 /* Of each wanted row of the last step, softmax(logits / temperature) (temperature > 0): the log probability of tokens_host[row] (a token outside the vocabulary:
  * NaN), the entropy (nats), and the `top` (0..64) most likely tokens, most likely first, equal ones by id (top_logprob_host, top_id_host [nwant, top], null for
- * top = 0).  Logits of -inf have probability 0.  Synchronous. */
+ * top = 0).  Logits of -inf have probability 0.  As wf_seq_sample: the first nwant rows, at most as many as the last step wanted.  Synchronous. */
 int wf_seq_logprobs(wf_seq_engine* e, int nwant, const int32_t* tokens_host, int top, float temperature, float* logprob_host, float* entropy_host,
                     float* top_logprob_host, int32_t* top_id_host);
 void* wf_seq_logits_device(wf_seq_engine* e);

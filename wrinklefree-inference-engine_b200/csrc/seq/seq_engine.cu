@@ -151,7 +151,8 @@ struct wf_seq_engine {
     int key_splits = 0;               // of the tensor-core attention launched last (wf_seq_key_splits)
     int pair_path_max = 64;           // up to this many (token, expert) pairs the experts run as per-pair weight streams (WF_SEQ_PAIR_MAX)
     float* logits = nullptr;
-    size_t logits_rows = 0;
+    size_t logits_rows = 0;        // that the buffer holds
+    int head_rows = 0;             // that the last step left in it
     float* d_uniform = nullptr;
     int32_t* d_next = nullptr;
     size_t sample_rows = 0;
@@ -1179,7 +1180,7 @@ int run_head(wf_seq_engine* e, const StepView& v, int nwant) {
 }
 
 // layers + head of one step: eagerly, or (decode-only shapes seen before) as a captured graph
-int run_model(wf_seq_engine* e, const StepView& v, int nwant) {
+int run_step(wf_seq_engine* e, const StepView& v, int nwant) {
     int rc;
     const bool decode_only = v.b.n == v.b.nseq;
     if (!decode_only || v.b.n > e->graph_max || e->layer_tap || e->prof) {
@@ -1208,6 +1209,13 @@ int run_model(wf_seq_engine* e, const StepView& v, int nwant) {
         it = e->graphs.emplace(key, exec).first;
     }
     return cuda_check(cudaGraphLaunch(it->second, e->stream), "graph launch");
+}
+
+int run_model(wf_seq_engine* e, const StepView& v, int nwant) {
+    e->head_rows = 0;
+    const int rc = run_step(e, v, nwant);
+    if (!rc && nwant > 0) e->head_rows = nwant;
+    return rc;
 }
 
 }  // namespace
@@ -1856,13 +1864,13 @@ extern "C" int wf_seq_step(wf_seq_engine* e, int nseq, const int32_t* slots, con
     const long long l0 = launch_count();
     if ((rc = run_model(e, v, nwant))) return rc;
     if (launch_count() > l0) e->launches = (int)(launch_count() - l0);     // a graph replay launches what its capture counted
-    if ((rc = finish_step(e, "wf_seq_step", e->logits, logits_host, logits_host && nwant > 0 ? (size_t)nwant * e->cfg.vocab * 4 : 0))) return rc;
+    if ((rc = finish_step(e, "wf_seq_step", e->logits, logits_host, logits_host && nwant > 0 ? (size_t)nwant * e->cfg.vocab * 4 : 0))) { e->head_rows = 0; return rc; }
     commit_lengths(e, nseq, slots, counts);
     return WF_OK;
 }
 
 extern "C" int wf_seq_sample(wf_seq_engine* e, int nwant, float temperature, int top_k, float top_p, const float* uniforms_host, int32_t* next_host) {
-    if (!e || !next_host || nwant <= 0 || (size_t)nwant > e->logits_rows) { set_error("wf_seq_sample: no logits for %d rows", nwant); return WF_ERR_INVALID; }
+    if (!e || !next_host || nwant <= 0 || nwant > e->head_rows) { set_error("wf_seq_sample: no logits for %d rows", nwant); return WF_ERR_INVALID; }
     if ((size_t)nwant > e->sample_rows) {
         if (e->d_uniform) cudaFree(e->d_uniform);
         if (e->d_next) cudaFree(e->d_next);
@@ -1882,7 +1890,7 @@ extern "C" int wf_seq_sample(wf_seq_engine* e, int nwant, float temperature, int
 
 extern "C" int wf_seq_logprobs(wf_seq_engine* e, int nwant, const int32_t* tokens_host, int top, float temperature, float* logprob_host, float* entropy_host,
                                float* top_logprob_host, int32_t* top_id_host) {
-    if (!e || nwant <= 0 || (size_t)nwant > e->logits_rows) { set_error("wf_seq_logprobs: no logits for %d rows", nwant); return WF_ERR_INVALID; }
+    if (!e || nwant <= 0 || nwant > e->head_rows) { set_error("wf_seq_logprobs: no logits for %d rows", nwant); return WF_ERR_INVALID; }
     if (!tokens_host || !logprob_host || !entropy_host || (top > 0 && (!top_logprob_host || !top_id_host))) { set_error("wf_seq_logprobs: null pointer"); return WF_ERR_INVALID; }
     if (top < 0 || top > LP_TOP_MAX || top > e->cfg.vocab) { set_error("wf_seq_logprobs: top (%d) is 0 to %d, and at most the vocabulary", top, LP_TOP_MAX); return WF_ERR_INVALID; }
     const size_t n = (size_t)nwant, bytes = n * (3 + 2 * (size_t)top) * 4;
