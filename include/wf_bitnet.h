@@ -224,8 +224,9 @@ int wf_paged_decode_attn(const void* q, const wf_kv_layout* kv, int layer, const
 
 /* The same for a batch that shares a prefix: every sequence's keys are the first prefix_len tokens of the pages in prefix_table (ceil(prefix_len / page_size)
  * entries), read once for all, and then its own seq_lens[b] tokens as above (block_table and seq_lens name the own tokens only; slots count from 0 again).
- * prefix_len or max_blocks may be 0, seq_lens[b] too; a sequence without any key gets zeros.  At most 65535 sequences where max_blocks > 0.  q, out, the pool and the workspace are 16-byte aligned.  The workspace is
- * free to be used again as soon as the stream has passed the call. */
+ * prefix_len or max_blocks may be 0, seq_lens[b] too; a sequence without any key gets zeros.  At most 65535 sequences where max_blocks > 0, 2^24 rows of queries
+ * (B * H) and a prefix of 2^30 tokens; no workspace (0) for more.  q, out, the pool and the workspace are 16-byte aligned.  The workspace is free to be used again as
+ * soon as the stream has passed the call. */
 size_t wf_prefix_attn_workspace_bytes(int B, int H, int kv_heads, int max_seq, int prefix_len);
 int wf_paged_prefix_attn(const void* q, const wf_kv_layout* kv, int layer, const int32_t* prefix_table, int prefix_len, const int32_t* block_table, int max_blocks,
                          const int32_t* seq_lens, int B, int H, float scale, void* out, int out_dtype, void* workspace, size_t workspace_bytes, void* stream);

@@ -655,6 +655,11 @@ PxCut px_cut(int B, int H, int Hkv, int prefix) {
     return c;
 }
 
+// what the call refuses for its size alone, and has no workspace for (the last one: a grid's third dimension)
+const char* px_too_large(int B, int H, int prefix, bool own) {
+    return prefix > 1 << 30 ? "a prefix is at most 2^30 tokens" : (long long)B * H > 1 << 24 ? "at most 2^24 rows of queries" : own && B > 65535 ? "at most 65535 sequences with keys of their own" : nullptr;
+}
+
 }  // namespace
 
 }  // namespace wf
@@ -662,7 +667,7 @@ PxCut px_cut(int B, int H, int Hkv, int prefix) {
 using namespace wf;
 
 extern "C" size_t wf_prefix_attn_workspace_bytes(int B, int H, int kv_heads, int max_seq, int prefix_len) {
-    if (B <= 0 || H <= 0 || kv_heads <= 0) return 0;
+    if (B <= 0 || H <= 0 || kv_heads <= 0 || px_too_large(B, H, prefix_len, max_seq > 0)) return 0;
     return px_cut(B, H, kv_heads, prefix_len).bytes + attn_chunks_bytes(B, H, kv_heads, max_seq);
 }
 
@@ -670,11 +675,11 @@ extern "C" int wf_paged_prefix_attn(const void* q, const wf_kv_layout* kv, int l
                                     const int32_t* seq_lens, int B, int H, float scale, void* out, int out_dtype, void* workspace, size_t workspace_bytes, void* stream) {
     const char* who = "wf_paged_prefix_attn";
     if (prefix_len < 0 || max_blocks < 0 || B < 0 || H <= 0) { set_error("%s: bad size (B %d, H %d, prefix %d, blocks %d)", who, B, H, prefix_len, max_blocks); return WF_ERR_INVALID; }
+    if (const char* why = px_too_large(B, H, prefix_len, max_blocks > 0)) { set_error("%s: %s (%d sequences, %d heads, a prefix of %d)", who, why, B, H, prefix_len); return WF_ERR_UNSUPPORTED; }
     const bool pointers = B == 0 || (q && out && (prefix_len == 0 || prefix_table) && (max_blocks == 0 || (block_table && seq_lens)));
     if (int rc = check_decode_attn(kv, layer, H, out_dtype, pointers, who)) return rc;
     if (B == 0) return WF_OK;
-    if ((long long)max_blocks * kv->page_size > 0x7fffffff || prefix_len > 1 << 30 || (long long)B * H > (1 << 24)) { set_error("%s: a row of block_table of 2^31 tokens, a prefix of more than 2^30, or 2^24 rows of queries", who); return WF_ERR_UNSUPPORTED; }
-    if (max_blocks > 0 && B > 65535) { set_error("%s: at most 65535 sequences with keys of their own (got %d)", who, B); return WF_ERR_UNSUPPORTED; }       // a grid's third dimension
+    if ((long long)max_blocks * kv->page_size > 0x7fffffff) { set_error("%s: a row of block_table holds less than 2^31 tokens", who); return WF_ERR_UNSUPPORTED; }
     if (int rc = check_wait_word(who)) return rc;
     if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)kv->pool) & 15) { set_error("%s: q, out and the pool must be 16-byte aligned", who); return WF_ERR_INVALID; }
     const PxCut cut = px_cut(B, H, kv->kv_heads, prefix_len);

@@ -255,13 +255,13 @@ Tensor paged_prefix_attn(const Tensor& q, const Tensor& pool, int64_t max_pages,
     const Tensor pt = prefix_table.contiguous(), bt = block_table.contiguous(), sl = seq_lens.contiguous();
     const int B = (int)q.size(0), H = (int)q.size(1), D = (int)q.size(2), blocks = to_int(bt.size(1), "block_table"), pre = to_int(prefix_len, "prefix_len");
     to_int(bt.size(1) * page_size, "block_table");
-    Tensor out = fresh({B, H, D}, out_dtype);
     wf_kv_layout kv;
     memset(&kv, 0, sizeof kv);
     kv.pool = pool.data_ptr();
     kv.max_pages = (int)max_pages; kv.layers = (int)layers; kv.kv_heads = (int)kv_heads; kv.page_size = (int)page_size; kv.head_dim = (int)head_dim; kv.dtype = (int)kv_dtype;
-    // memory of this call's own: calls on other streams and captured graphs do not share it
-    Tensor ws = fresh({(int64_t)wf_prefix_attn_workspace_bytes(B, H, kv.kv_heads, blocks * kv.page_size, pre)}, at::kByte);
+    // memory of this call's own: calls on other streams and captured graphs do not share it (none for sizes that the call refuses)
+    const int64_t bytes = (int64_t)wf_prefix_attn_workspace_bytes(B, H, kv.kv_heads, blocks * kv.page_size, pre);
+    Tensor out = fresh({bytes || (blocks == 0 && pre == 0) ? B : 0, H, D}, out_dtype), ws = fresh({bytes}, at::kByte);
     check(wf_paged_prefix_attn(qc.data_ptr(), &kv, (int)layer, (const int32_t*)pt.data_ptr(), pre, (const int32_t*)bt.data_ptr(), blocks, (const int32_t*)sl.data_ptr(), B, H, (float)scale,
                                out.data_ptr(), code_of(out_dtype), ws.data_ptr(), (size_t)ws.numel(), stream()));
     return out;
@@ -283,7 +283,7 @@ std::vector<Tensor> paged_plan(const Tensor& seq_lens, const Tensor& new_lens, T
     TORCH_CHECK_VALUE(block_table.is_contiguous(), "block_table must be contiguous (it is written in place)");
     const Tensor sl = seq_lens.contiguous(), nl = new_lens.contiguous(), fp = free_pages.contiguous();
     const int rows = to_int(B, "block_table"), cap = to_int(max_tokens, "max_tokens"), page = to_int(page_size, "page_size");
-    const int64_t cap4 = (max_tokens + 3) / 4 * 4;         // every map starts on 16 bytes
+    const int64_t cap4 = cap > 1 << 30 ? 0 : (max_tokens + 3) / 4 * 4;      // every map starts on 16 bytes (the call refuses more than 2^30 tokens)
     const Tensor buf = fresh({4 * cap4 + 2 * B + 3}, at::kInt);
     const int64_t at[8] = {0, cap4, 2 * cap4, 3 * cap4, 4 * cap4, 4 * cap4 + B + 1, 4 * cap4 + 2 * B + 1, 4 * cap4 + 2 * B + 2};
     const int64_t len[8] = {max_tokens, max_tokens, max_tokens, max_tokens, B + 1, B, 1, 1};
@@ -329,9 +329,9 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor& logits, 
     const int n = to_int(x.size(0), "rows"), V = to_int(x.size(1), "vocab"), k = to_int(top, "top");
     const int64_t ld = n > 1 ? x.stride(0) : V;
     const Tensor& y = ld < V ? x.contiguous() : x;         // rows that overlap (an expanded row)
-    const int64_t m = n, mk = m * k;
+    const int64_t m = n, kk = k > 64 || k > V ? 0 : k, mk = m * kk;        // (the call refuses more)
     const Tensor buf = fresh({2 * (m + mk)}, at::kFloat);
-    Tensor lp = part_of(buf, at::kFloat, 0, {m}), ent = part_of(buf, at::kFloat, m, {m}), tlp = part_of(buf, at::kFloat, 2 * m, {m, k}), tid = part_of(buf, at::kInt, 2 * m + mk, {m, k});
+    Tensor lp = part_of(buf, at::kFloat, 0, {m}), ent = part_of(buf, at::kFloat, m, {m}), tlp = part_of(buf, at::kFloat, 2 * m, {m, kk}), tid = part_of(buf, at::kInt, 2 * m + mk, {m, kk});
     check(wf_token_logprobs(y.data_ptr(), dt, n, V, ld < V ? V : ld, (const int32_t*)tk.data_ptr(), k, (float)temperature, (float*)lp.data_ptr(), (float*)ent.data_ptr(),
                             (float*)tlp.data_ptr(), (int32_t*)tid.data_ptr(), stream()));
     return {lp, ent, tlp, tid};

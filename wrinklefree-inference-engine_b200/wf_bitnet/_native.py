@@ -66,8 +66,9 @@ class _Ctypes:
         with torch.cuda.device(q.device):
             qc = q.contiguous()
             qc = qc.clone() if qc.data_ptr() % 16 else qc
-            out = torch.empty(B, H, D, dtype=out_dtype, device=q.device)
-            ws = torch.empty(int(_lib.lib().wf_prefix_attn_workspace_bytes(B, H, kv_heads, bt.shape[1] * page_size, prefix_len)), dtype=torch.uint8, device=q.device)
+            nbytes = int(_lib.lib().wf_prefix_attn_workspace_bytes(B, H, kv_heads, bt.shape[1] * page_size, prefix_len))       # 0 for sizes that the call refuses: no memory for them
+            out = torch.empty(B if nbytes or not (bt.shape[1] or prefix_len) else 0, H, D, dtype=out_dtype, device=q.device)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
             layout = _lib.KvLayout(pool.data_ptr(), max_pages, layers, kv_heads, page_size, head_dim, kv_dtype)
             _lib.check(_lib.lib().wf_paged_prefix_attn(qc.data_ptr(), C.byref(layout), layer, pt.data_ptr(), prefix_len, bt.data_ptr(), bt.shape[1], sl.data_ptr(), B, H, float(scale),
                                                        out.data_ptr(), ops._DT[out_dtype], ws.data_ptr(), ws.numel(), ops._stream()))
@@ -90,7 +91,7 @@ class _Ctypes:
         if not (0 <= max_tokens <= 0x7fffffff and 0 <= page_size <= 0x7fffffff):
             raise ValueError("max_tokens or page_size out of range")
         with torch.cuda.device(block_table.device):
-            cap4 = (max_tokens + 3) // 4 * 4
+            cap4 = 0 if max_tokens > 1 << 30 else (max_tokens + 3) // 4 * 4          # (the call refuses more)
             buf = torch.empty(4 * cap4 + 2 * B + 3, dtype=torch.int32, device=block_table.device)
             at = (0, cap4, 2 * cap4, 3 * cap4, 4 * cap4, 4 * cap4 + B + 1, 4 * cap4 + 2 * B + 1, 4 * cap4 + 2 * B + 2)
             out = [buf[a:a + n] for a, n in zip(at, (max_tokens,) * 4 + (B + 1, B, 1, 1))]
@@ -139,7 +140,8 @@ class _Ctypes:
         with torch.cuda.device(logits.device):
             x = logits if (V <= 1 or logits.stride(1) == 1) and (n <= 1 or logits.stride(0) >= V) else logits.contiguous()
             lp, ent = (torch.empty(n, dtype=torch.float32, device=x.device) for _ in range(2))
-            tlp, tid = (torch.empty(n, top, dtype=t, device=x.device) for t in (torch.float32, torch.int32))
+            k = top if top <= min(64, V) else 0                                       # (the call refuses more)
+            tlp, tid = (torch.empty(n, k, dtype=t, device=x.device) for t in (torch.float32, torch.int32))
             _lib.check(_lib.lib().wf_token_logprobs(x.data_ptr(), dt, n, V, x.stride(0) if n > 1 else V, tk.data_ptr(), top, float(temperature), lp.data_ptr(), ent.data_ptr(),
                                                     tlp.data_ptr(), tid.data_ptr(), ops._stream()))
         return lp, ent, tlp, tid
