@@ -16,6 +16,7 @@
 //   head form the (padded) M=16 rows of mma.m16n8k16 bf16: S = Q K^T (fp32), online softmax in fp32 with
 //   exp2, O += P V.  Warps are merged through shared memory; chunks are merged by a second tiny kernel.
 #include <cuda_fp16.h>
+#include <float.h>
 #include <algorithm>
 
 #include "attn_chunks.cuh"
@@ -478,7 +479,9 @@ __global__ void __launch_bounds__(AT_WARPS * 32, I8 || BESIDE ? 3 : 2) paged_dec
     float o[16][4];
 #pragma unroll
     for (int j = 0; j < 16; ++j) { o[j][0] = 0.f; o[j][1] = 0.f; o[j][2] = 0.f; o[j][3] = 0.f; }
-    float m_run = -INFINITY, l_run = 0.f;   // row g (replicated over the 4 lanes of a group)
+    // row g (replicated over the 4 lanes of a group).  The maximum starts at the lowest float: where all scores so far are -inf their weights are 0, not 2^(inf - inf)
+    // (the decode engine writes its own keys; its chunks without work are known by -inf)
+    float m_run = FUSED ? -INFINITY : -FLT_MAX, l_run = 0.f;
     float c_run = 0.f, q_bias = 0.f;        // int8 KV: running sum of the f16 P operands (per lane); 1152 * sum_d q[g][d]
     if (I8) {
         float qs = 0.f;
@@ -559,14 +562,12 @@ __global__ void __launch_bounds__(AT_WARPS * 32, I8 || BESIDE ? 3 : 2) paged_dec
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
         const float m_new = fmaxf(m_run, mx);
-        // nothing but scores of -inf so far: weights of 0, not of 2^(inf - inf)  (the decode engine writes its own keys)
-        const float m_sub = !FUSED && m_new == -INFINITY ? 0.f : m_new;
-        const float corr = fast_exp2(m_run - m_sub);   // 0 on the first block (m_run = -inf)
+        const float corr = fast_exp2(m_run - m_new);   // 0 on the first block with a weight
         float psum = 0.f;
         uint32_t pa[4];
         {
-            const float p00 = fast_exp2(s[0][0] - m_sub), p01 = fast_exp2(s[0][1] - m_sub);
-            const float p10 = fast_exp2(s[1][0] - m_sub), p11 = fast_exp2(s[1][1] - m_sub);
+            const float p00 = fast_exp2(s[0][0] - m_new), p01 = fast_exp2(s[0][1] - m_new);
+            const float p10 = fast_exp2(s[1][0] - m_new), p11 = fast_exp2(s[1][1] - m_new);
             psum = (p00 + p01) + (p10 + p11);
             if (!I8) {
                 pa[0] = pack_bf16x2(p00, p01);   // A frag: row g, k = 2t,2t+1
