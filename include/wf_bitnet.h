@@ -192,7 +192,8 @@ int wf_rope_kv_append(const void* qkv, int B, int H, const wf_kv_layout* kv, int
 
 /* Block tables and slot maps of a step, on the GPU: the free list of KVCacheManager (tests/test_kv_cache_cpp.py:44-70; pages come off the end of the list) as a
  * stack in device memory, free_pages[0 .. *free_count) of pool_pages entries.  Request r (of rows <= 8192) has seq_lens[r] cached tokens, whose pages stand in
- * block_table[r][0 .. ceil(seq_lens[r] / page_size)), and new_lens[r] >= 0 new ones.  The pages that it still needs are taken off the stack, request after
+ * block_table[r][0 .. ceil(seq_lens[r] / page_size)), and new_lens[r] >= 0 new ones (behind a shared prefix, wf_paged_prefix_attn, these are the request's own
+ * tokens, and positions count from its first own one: a rotary embedding there adds the prefix's length).  The pages that it still needs are taken off the stack, request after
  * request and block after block, and written to its row of block_table (the other entries stay).  For every new token t, requests one after another:
  * token_rows[t], positions[t] (in its sequence), pages[t] and slots[t] (what wf_kv_scatter takes); entries from the last token up to max_tokens: -1, 0, -1, 0.
  * offsets[rows + 1]: first token of each request and their number; lens_out = seq_lens + new_lens; free_count_out = *free_count - pages taken.  Nothing of the
@@ -224,7 +225,8 @@ int wf_paged_decode_attn(const void* q, const wf_kv_layout* kv, int layer, const
 
 /* The same for a batch that shares a prefix: every sequence's keys are the first prefix_len tokens of the pages in prefix_table (ceil(prefix_len / page_size)
  * entries), read once for all, and then its own seq_lens[b] tokens as above (block_table and seq_lens name the own tokens only; slots count from 0 again).
- * prefix_len or max_blocks may be 0, seq_lens[b] too; a sequence without any key gets zeros.  At most 65535 sequences where max_blocks > 0, 2^24 rows of queries
+ * prefix_len or max_blocks may be 0, seq_lens[b] too; a sequence without any key, or with none but of -inf scores, gets zeros.  The prefix's weights enter their
+ * product with the values in bf16 (int8 pools: times the value's scale; there the own part and wf_paged_decode_attn have fp16).  At most 65535 sequences where max_blocks > 0, 2^24 rows of queries
  * (B * H) and a prefix of 2^30 tokens; no workspace (0) for more.  q, out, the pool and the workspace are 16-byte aligned.  The workspace is free to be used again as
  * soon as the stream has passed the call. */
 size_t wf_prefix_attn_workspace_bytes(int B, int H, int kv_heads, int max_seq, int prefix_len);
@@ -252,7 +254,7 @@ int wf_lm_head_argmax(const void* h, const void* E, int B, int V, int K, float* 
 /* Log probabilities from logits [rows, vocab] (dtype WF_F32 / WF_BF16 / WF_F16, rows row_stride elements apart), z = logits / temperature, temperature > 0, vocab at most 2^30:
  * logprob[r] = log softmax(z_r)[tokens[r]], entropy[r] = -sum p ln p (nats, in float whatever the dtype), and the `top` (0..64, at most vocab) largest logits of
  * each row, largest first, equal ones by index: top_id, top_logprob [rows, top].  Logits of -inf have probability 0.  A row with nothing above -inf: logprobs
- * -inf, entropy 0.  A row with +inf or NaN: all its floats NaN, NaN is no alternative (top_id -1 where the row has too few others).  A token outside
+ * -inf, entropy 0.  Tokens masked with the type's lowest value have large negative logprobs, -inf where a float does not hold them.  A row with +inf or NaN: all its floats NaN, NaN is no alternative (top_id -1 where the row has too few others).  A token outside
  * [0, vocab): logprob NaN.  One launch, no workspace. */
 int wf_token_logprobs(const void* logits, int dtype, int rows, int vocab, long long row_stride, const int32_t* tokens, int top, float temperature, float* logprob,
                       float* entropy, float* top_logprob, int32_t* top_id, void* stream);

@@ -5,9 +5,12 @@
 // product per key/value head, B * H / Hkv rows of queries against the prefix's keys, cut over the keys into splits.  The first part is bound by memory, the
 // second by the tensor cores' operand reads and the exponentials between their products: with a bf16 pool the prefix part is launched first and keeps to 161 KB of
 // shared memory and 2/3 of the registers, so that blocks of the own part run beside it on the same SMs (128 sequences, 32 and 8 heads, a prefix of 32768 and up to 512
-// own tokens: 98 us against 110 one after the other; 64 of 20 and 5 heads, 8192 and 300: 26.2 and 30.7; 256 of 32 and 8, 2048 and 128: 50 and 56; nowhere more than 1 %
-// slower from prefixes of 512 to 65536).
+// own tokens: 101 us against 119 one after the other, the own part first; 64 of 20 and 5 heads, 8192 and 300: 24.7 and 29.0; 256 of 32 and 8, 2048 and 128: 43.7 and 50.3;
+// 4 of 20 and 5, 2048 and 300: 10.5 and 11.1; 64 of 32 and 8 behind 512: 17.0 and 20.2, behind 65536: 99 and 109).  These are replays over the same inputs, medians of one
+// run; another GPU gave 92 for the first, and a call that finds its inputs changed takes 117.
 // With an int8 pool the prefix part needs all of an SM's shared memory and registers, and the own part goes first.
+//
+// Operands have 8 bits: weights go into the value product as bf16, with an int8 pool after the value's scale (the own part and paged_decode_attn have 11 bits of them there).
 #include "attn_chunks.cuh"
 #include "gemm_tc_common.cuh"
 #include "wf_bitnet.h"
@@ -62,7 +65,7 @@ constexpr int PX_THREADS = 12 * 32, PX_REGS = 112, PX_REGS_SOFTMAX = 128, PX_REG
 static_assert(2 * PX_REGS_SOFTMAX + PX_REGS_OTHERS == 3 * PX_REGS, "the softmax warpgroups take what the third one gives");
 // int8 pools: a ring of tiles as they lie in the pool, and one of converted tiles with their scales
 constexpr int PX_RAW = 3, PX_RAW_TILE = 2 * PX_KEYS * AT_D, PX_SC = 2 * PX_KEYS * 4, PX_STAGES8 = 3;
-constexpr int PX_CONV = 4;                             // converting warps (eight: as fast, at 34.4 us for 31 sequences of 64 and 8 heads over 16003 keys: shared memory is what is busy)
+constexpr int PX_CONV = 4;                             // converting warps (eight: as fast, at 34.4 us for 31 sequences of 64 and 8 heads over 16003 keys)
 constexpr int PX_SMEM8_USE = 2 * PX_QTILE + PX_STAGES8 * 2 * PX_TILE + PX_RAW * PX_RAW_TILE + PX_STAGES8 * PX_SC;
 constexpr int PX_SMEM8 = PX_SMEM8_USE + 1024;
 constexpr int PX_THREADS8 = (11 + PX_CONV) * 32, PX_REGS8 = 128;

@@ -28,7 +28,8 @@ namespace {
 constexpr int LP_THREADS = 512, LP_WARPS = LP_THREADS / 32;
 constexpr int LP_CAND = 2048;                         // candidates of a block
 // Blocks' lists of up to so many keys are joined by counting (n^2 / 32 reads of shared memory an SM), longer ones by bisection in each other list (a chain of reads):
-// eight lists of 20 take one row from 9.4 to 8.4 us, four of 64 took 33 rows from 8.8 to 10.3.
+// of one row of 128256, eight lists of 20 take 8.5 us counted and 9.4 otherwise, of 24 9.0 and 9.6, of 32 10.5 and 10.2, of 64 21.0 and 13.8; of 33 rows of 32000, four
+// lists of 24 take 7.6 and 7.8, of 32 8.0 both, of 64 10.8 and 9.2; of 64 rows, two lists of 24 8.1 both, of 32 8.5 and 8.2.
 constexpr int LP_FEW = 20;
 constexpr int LP_PEND = 64;                           // entries of a warp's buffer where a row is read again
 constexpr float LP_LN2 = 0.6931471805599453f, LP_LOG2E = 1.4426950408889634f;

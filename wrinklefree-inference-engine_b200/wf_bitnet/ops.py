@@ -320,7 +320,8 @@ def paged_prefix_attn(q: torch.Tensor, kv: PagedKV, layer: int, prefix_table: to
                       scale: Optional[float] = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """Decode attention of a batch that shares a prefix: sequence b's keys are the first `prefix_len` tokens of the pages in prefix_table (int32 [pages]),
     which are read once for the whole batch, and then seq_lens[b] tokens of its own pages, block_table[b] (int32 [B, blocks], blocks may be 0).
-    q: bf16 [B, H, D].  A sequence without any key gets zeros.  Otherwise as paged_decode_attn."""
+    q: bf16 [B, H, D].  A sequence without any key gets zeros.  The prefix's weights are rounded to bf16 (over an int8 cache times the value's scale, where the
+    own tokens' are fp16).  Otherwise as paged_decode_attn."""
     if out_dtype not in (torch.bfloat16, torch.float32):
         raise ValueError("out_dtype must be bfloat16 or float32")
     c = kv.c
@@ -329,9 +330,10 @@ def paged_prefix_attn(q: torch.Tensor, kv: PagedKV, layer: int, prefix_table: to
 
 
 class PagedPlan(NamedTuple):
-    """A step's tokens in the paged cache, all int32 on the GPU.  Of every token, requests one after another (-1, 0, -1, 0 behind the last one):"""
+    """A step's tokens in the paged cache, all int32 on the GPU, views of one buffer (clone `lens` and `free_count` to go on with them without keeping the
+    maps' memory).  Of every token, requests one after another (-1, 0, -1, 0 behind the last one):"""
     rows: torch.Tensor          # [max_tokens] its request (row of block_table)
-    positions: torch.Tensor     # [max_tokens] its position in the sequence
+    positions: torch.Tensor     # [max_tokens] its position in the sequence (behind a shared prefix: among its own tokens)
     pages: torch.Tensor         # [max_tokens] where it lies in the cache: what kv_scatter takes
     slots: torch.Tensor         # [max_tokens]
     offsets: torch.Tensor       # [B + 1] first token of each request, and the number of tokens
