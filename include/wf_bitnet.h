@@ -210,7 +210,8 @@ int wf_paged_plan(const int32_t* seq_lens, const int32_t* new_lens, int rows, in
                   int32_t* lens_out, int32_t* free_count_out, int32_t* status, void* stream);
 /* The way back: the requests with done[r] != 0 hand their ceil(seq_lens[r] / page_size) pages back, request after request and block after block, on top of the
  * stack (free_pages[*free_count ..]).  lens_out: 0 for them, seq_lens[r] for the others; free_count_out = *free_count + pages handed back.  Where the stack
- * would not hold them, or a length or the count is out of range, nothing is done and lens_out and free_count_out are the inputs. */
+ * would not hold them, or a length or the count is out of range, nothing is done and lens_out and free_count_out are the inputs.  Outputs overlap neither one another
+ * nor the inputs. */
 int wf_paged_release(const uint8_t* done, const int32_t* seq_lens, int rows, const int32_t* block_table, int max_blocks, int32_t* free_pages, int pool_pages,
                      const int32_t* free_count, int page_size, int32_t* lens_out, int32_t* free_count_out, void* stream);
 
@@ -225,6 +226,7 @@ int wf_paged_decode_attn(const void* q, const wf_kv_layout* kv, int layer, const
 
 /* The same for a batch that shares a prefix: every sequence's keys are the first prefix_len tokens of the pages in prefix_table (ceil(prefix_len / page_size)
  * entries), read once for all, and then its own seq_lens[b] tokens as above (block_table and seq_lens name the own tokens only; slots count from 0 again).
+ * The tables' entries for these tokens are pages of the pool; others are not used.
  * prefix_len or max_blocks may be 0, seq_lens[b] too; a sequence without any key, or with none but of -inf scores, gets zeros.  The prefix's weights enter their
  * product with the values in bf16 (int8 pools: times the value's scale; there the own part and wf_paged_decode_attn have fp16).  At most 65535 sequences where max_blocks > 0, 2^24 rows of queries
  * (B * H) and a prefix of 2^30 tokens; no workspace (0) for more.  q, out, the pool and the workspace are 16-byte aligned.  The workspace is free to be used again as
