@@ -191,7 +191,7 @@ int wf_rope_kv_append(const void* qkv, int B, int H, const wf_kv_layout* kv, int
                       int max_pos, void* q_out, void* stream);
 
 /* Block tables and slot maps of a step, on the GPU: the free list of KVCacheManager (tests/test_kv_cache_cpp.py:44-70; pages come off the end of the list) as a
- * stack in device memory, free_pages[0 .. *free_count) of pool_pages entries.  Request r (of rows <= 8192) has seq_lens[r] cached tokens, whose pages stand in
+ * stack in device memory, free_pages[0 .. *free_count) of pool_pages entries (at most 2^30).  Request r (of rows <= 8192) has seq_lens[r] cached tokens, whose pages stand in
  * block_table[r][0 .. ceil(seq_lens[r] / page_size)), and new_lens[r] >= 0 new ones (behind a shared prefix, wf_paged_prefix_attn, these are the request's own
  * tokens, and positions count from its first own one: a rotary embedding there adds the prefix's length).  The pages that it still needs are taken off the stack, request after
  * request and block after block, and written to its row of block_table (the other entries stay).  For every new token t, requests one after another:

@@ -170,6 +170,7 @@ int pl_check(const char* who, PlanParams& p) {
     if (p.rows < 0 || p.max_blocks < 0 || p.pool_pages < 0 || p.cap < 0) { set_error("%s: negative size", who); return WF_ERR_INVALID; }
     if (p.page <= 0) { set_error("%s: page_size must be positive (got %d)", who, p.page); return WF_ERR_INVALID; }
     if (p.cap > 1 << 30) { set_error("%s: max_tokens is at most 2^30 (got %d)", who, p.cap); return WF_ERR_UNSUPPORTED; }
+    if (p.pool_pages > 1 << 30) { set_error("%s: a free list is at most 2^30 entries (got %d)", who, p.pool_pages); return WF_ERR_UNSUPPORTED; }      // what a block's step adds to an index fits too
     if (p.rows > PL_MAX_ROWS) { set_error("%s: at most %d requests (got %d)", who, PL_MAX_ROWS, p.rows); return WF_ERR_UNSUPPORTED; }
     // with 2^(l-1) < page <= 2^l, mul = ceil(2^(31+l) / page) is below 2^32 and exceeds 2^(31+l) / page by less than 1: x * mul / 2^(31+l) is above x / page by less
     // than 2^-l <= 1 / page, which does not reach the next whole number

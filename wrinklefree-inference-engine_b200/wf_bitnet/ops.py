@@ -351,7 +351,7 @@ def paged_plan(seq_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torc
     (0: none).  Pages that it needs come off the end of the free list free_pages[:free_count] (the order of sgl_kernel.kvcache.PageAllocator) and are written to
     its row of block_table; the free list itself stays.  Go on with the plan's `lens` and `free_count`.  A step that does not fit (pages, max_tokens, columns of
     block_table; a length or the count out of range) is not planned at all: `status` says why, no token has a page, and `lens` and `free_count` are as before.
-    At most 8192 requests."""
+    At most 8192 requests, and a free list of 2^30 entries."""
     return PagedPlan(*_native.ops().paged_plan(seq_lens, new_lens, block_table, free_pages, free_count, page_size, max_tokens))
 
 
