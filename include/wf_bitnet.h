@@ -229,7 +229,7 @@ int wf_paged_decode_attn(const void* q, const wf_kv_layout* kv, int layer, const
  * The tables' entries for these tokens are pages of the pool; others are not used.
  * prefix_len or max_blocks may be 0, seq_lens[b] too; a sequence without any key, or with none but of -inf scores, gets zeros.  The prefix's weights enter their
  * product with the values in bf16 (int8 pools: times the value's scale; there the own part and wf_paged_decode_attn have fp16).  At most 65535 sequences where max_blocks > 0, 2^24 rows of queries
- * (B * H) and a prefix of 2^30 tokens; no workspace (0) for more.  q, out, the pool and the workspace are 16-byte aligned.  The workspace is free to be used again as
+ * (B * H), a prefix of 2^30 tokens (no workspace, 0, for more) and rows of block_table of 2^31 - 4096 tokens.  q, out, the pool and the workspace are 16-byte aligned.  The workspace is free to be used again as
  * soon as the stream has passed the call. */
 size_t wf_prefix_attn_workspace_bytes(int B, int H, int kv_heads, int max_seq, int prefix_len);
 int wf_paged_prefix_attn(const void* q, const wf_kv_layout* kv, int layer, const int32_t* prefix_table, int prefix_len, const int32_t* block_table, int max_blocks,

@@ -682,7 +682,8 @@ extern "C" int wf_paged_prefix_attn(const void* q, const wf_kv_layout* kv, int l
     const bool pointers = B == 0 || (q && out && (prefix_len == 0 || prefix_table) && (max_blocks == 0 || (block_table && seq_lens)));
     if (int rc = check_decode_attn(kv, layer, H, out_dtype, pointers, who)) return rc;
     if (B == 0) return WF_OK;
-    if ((long long)max_blocks * kv->page_size > 0x7fffffff) { set_error("%s: a row of block_table holds less than 2^31 tokens", who); return WF_ERR_UNSUPPORTED; }
+    // (a warp asks for pages a few blocks behind the last one)
+    if ((long long)max_blocks * kv->page_size > 0x80000000ll - 4096) { set_error("%s: a row of block_table holds at most 2^31 - 4096 tokens", who); return WF_ERR_UNSUPPORTED; }
     if (int rc = check_wait_word(who)) return rc;
     if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)kv->pool) & 15) { set_error("%s: q, out and the pool must be 16-byte aligned", who); return WF_ERR_INVALID; }
     const PxCut cut = px_cut(B, H, kv->kv_heads, prefix_len);
