@@ -268,7 +268,8 @@ class PagedKV:
 def kv_scatter(kv: PagedKV, k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, slots: torch.Tensor, layer: int) -> None:
     _need_cuda(k, v, pages, slots)
     T = pages.shape[0]
-    check(lib().wf_kv_scatter(kv.ref(), k.contiguous().data_ptr(), v.contiguous().data_ptr(), pages.data_ptr(), slots.data_ptr(), T, layer, _stream()))
+    k, v = k.contiguous(), v.contiguous()              # both alive until the launch: one that has been let go would lend its memory to the other
+    check(lib().wf_kv_scatter(kv.ref(), k.data_ptr(), v.data_ptr(), pages.data_ptr(), slots.data_ptr(), T, layer, _stream()))
 
 
 def kv_gather(kv: PagedKV, k_out: torch.Tensor, v_out: torch.Tensor, pages: torch.Tensor, slots: torch.Tensor, layer: int) -> None:
