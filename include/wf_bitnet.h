@@ -190,6 +190,18 @@ int wf_rope_kv_append(const void* qkv, int B, int H, const wf_kv_layout* kv, int
                       const int32_t* block_table, int max_blocks, const void* cos_tab, const void* sin_tab,
                       int max_pos, void* q_out, void* stream);
 
+/* What lies between the projection of a step's tokens and their attention, in one launch: qkv bf16 [tokens][(H + 2 Hkv) * D], rows row_stride numbers apart (a multiple of 4).
+ * Every query head is RMS-normed with q_norm, every key head with k_norm (gains [D] of norm_dtype WF_F32 or WF_BF16; null: not normed), x / sqrt(mean x^2 + eps) * gain, and
+ * rotated by positions[t]: of the first `rot` dims (a multiple of 8, 0: none) the pairs (i, i + rot / 2), or (2i, 2i + 1) where interleaved, (a, b) -> (a cos - b sin,
+ * a sin + b cos), cos and sin from row positions[t] of cos_tab, sin_tab [max_pos][rot / 2] (table_dtype WF_F32 or WF_BF16).  All in float, rounded once to bf16.  Queries go
+ * to q_out [tokens][H][D]; keys and values to (pages[t], slots[t], layer) of the cache, an int8 pool's codes as wf_kv_scatter makes them of the bf16 values.  A token whose
+ * page or slot is none of the pool's is not appended (wf_paged_plan's entries behind the last token); one whose position is not in [0, max_pos) is not either, and its
+ * queries are NaN.  head_dim 64, 128 or 256.  qkv, q_out, the pool, tables and gains are 16-byte aligned.  Of two tokens at the same
+ * place it is not determined what is kept. */
+int wf_norm_rope_kv_append(const void* qkv, long long row_stride, int tokens, int H, const wf_kv_layout* kv, int layer, const int32_t* positions, const int32_t* pages,
+                           const int32_t* slots, const void* cos_tab, const void* sin_tab, int table_dtype, int rot, int max_pos, const void* q_norm, const void* k_norm,
+                           int norm_dtype, float eps, int interleaved, void* q_out, void* stream);
+
 /* Block tables and slot maps of a step, on the GPU: the free list of KVCacheManager (tests/test_kv_cache_cpp.py:44-70; pages come off the end of the list) as a
  * stack in device memory, free_pages[0 .. *free_count) of pool_pages entries (at most 2^30).  Request r (of rows <= 8192) has seq_lens[r] cached tokens, whose pages stand in
  * block_table[r][0 .. ceil(seq_lens[r] / page_size)), and new_lens[r] >= 0 new ones (behind a shared prefix, wf_paged_prefix_attn, these are the request's own
@@ -235,6 +247,37 @@ size_t wf_prefix_attn_workspace_bytes(int B, int H, int kv_heads, int max_seq, i
 int wf_paged_prefix_attn(const void* q, const wf_kv_layout* kv, int layer, const int32_t* prefix_table, int prefix_len, const int32_t* block_table, int max_blocks,
                          const int32_t* seq_lens, int B, int H, float scale, void* out, int out_dtype, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- drafted tokens ------------ */
+
+/* Trees of drafts.  A sequence's new tokens of a step (offsets [rows + 1], of `tokens` rows, as wf_paged_plan has them) are its drafts, each behind the one that it follows:
+ * parents[t] is that one's place among the sequence's drafts, below its own; -1 (or any other number) follows the cached tokens alone.  Bit j of mask[t] (words of 64, ceil(max_nodes /
+ * 64) a token; max_nodes at most 256): the draft at place j is t itself or on its way up.  positions[t] = seq_lens[r] + the number of drafts above t.  Of a sequence with more
+ * than max_nodes drafts, or a length out of range: masks of 0, positions -1; of rows behind the last sequence: 0 and 0. */
+int wf_tree_plan(const int32_t* parents, const int32_t* offsets, const int32_t* seq_lens, int rows, int tokens, int max_nodes, uint64_t* mask, int32_t* positions, void* stream);
+
+/* Attention of drafts: q bf16 [tokens][H][D], sequence b's rows offsets[b] .. offsets[b + 1], its cached tokens 0 .. seq_lens[b] and its drafts behind them at seq_lens[b] + place
+ * (appended before: wf_norm_rope_kv_append, wf_kv_scatter) in the pages of block_table[b].  Row t sees every cached token, and the drafts whose bits are set in mask[t]
+ * [mask_words] (1 to 4; bits behind the last draft count for nothing; any pattern, not only a tree's).  out bf16 or f32 [tokens][H][D]; a row that sees no key, or none but of
+ * -inf scores, gets zeros; so do rows behind the last sequence, and those of sequences with more than 64 mask_words drafts.  What a row does not see has no weight, whatever
+ * it holds (NaN too).  Offsets rise; else the results mean nothing.  Weights enter their product with the values in bf16 (int8 pools: times the value's scale).  The tables' entries of
+ * the tokens in range are pages of the pool (others read as zeros).  At most 65536 sequences, 2^24 rows of queries (tokens * H), and rows of block_table of 2^31 - 4096 tokens.  q, out, the pool
+ * and the workspace are 16-byte aligned.  The workspace is free to be used again as soon as the stream has passed the call. */
+size_t wf_tree_attn_workspace_bytes(int B, int tokens, int H, int kv_heads, int mask_words);
+int wf_paged_tree_attn(const void* q, const wf_kv_layout* kv, int layer, const int32_t* block_table, int max_blocks, const int32_t* seq_lens, const int32_t* offsets,
+                       const uint64_t* mask, int mask_words, int B, int tokens, int H, float scale, void* out, int out_dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Which drafts are kept.  tokens[t] is draft t, targets[t] what the model has drawn behind it, parents as in wf_tree_plan.  A sequence's first draft (the token drawn last, not
+ * cached before this step) is kept; behind a kept draft the one that follows it with the token drawn there is (the lowest place of several).  accepted[b]: how many (0
+ * without drafts); path[offsets[b] + k]: the place of the k-th kept one (-1 behind the last, and in rows of no sequence); next[b]: what was drawn behind the last kept one (-1
+ * without drafts), the next step's first draft.  Keys and values of the kept drafts, of every layer, move to seq_lens[b] + k; lens_out = seq_lens + accepted; pages behind
+ * the last kept token go back on the stack free_pages[*free_count ..] of pool_pages entries (at most 2^30), sequence after sequence and block after block.  Where that cannot be
+ * done as a whole, status has the WF_PLAN_* bits of why (PAGES: the stack would not hold them; BLOCKS, LENGTH: a sequence beyond max_blocks pages, more than 256 drafts, or
+ * out of range; COUNT), nothing moves or is handed back, lens_out = seq_lens + the drafts and free_count_out = *free_count; accepted, path and next stand (sequences with more than
+ * 256 drafts: none kept).  At most 8192 rows.  Rows of a head are a multiple of 16 bytes.  The pool is 16-byte aligned.  Outputs overlap neither one another nor the inputs. */
+int wf_tree_accept(const int32_t* parents, const int32_t* tokens, const int32_t* targets, const int32_t* offsets, const int32_t* seq_lens, int rows, int n_tokens,
+                   const wf_kv_layout* kv, const int32_t* block_table, int max_blocks, int32_t* free_pages, int pool_pages, const int32_t* free_count, int32_t* accepted, int32_t* path,
+                   int32_t* next_tokens, int32_t* lens_out, int32_t* free_count_out, int32_t* status, void* stream);
+
 /* ---- glue around the linears -------------------------------------------- */
 
 /* rms_norm (direct_inference_full.py:181-184) with the reference's bf16 rounding points, fused
@@ -260,6 +303,34 @@ int wf_lm_head_argmax(const void* h, const void* E, int B, int V, int K, float* 
  * [0, vocab): logprob NaN.  One launch, no workspace. */
 int wf_token_logprobs(const void* logits, int dtype, int rows, int vocab, long long row_stride, const int32_t* tokens, int top, float temperature, float* logprob,
                       float* entropy, float* top_logprob, int32_t* top_id, void* stream);
+
+/* What requests ask of their logits before a token is drawn.  Row n (of `rows`) belongs to sequence b with offsets[b] <= n < offsets[b + 1], or to sequence n where offsets is null
+ * (sequences == rows then).  A token is seen where it stands in the first history_lens[b] of history[b] (null: all history_width), and drawn where it stands there at
+ * prompt_lens[b] or behind (null: from the start), once for each time.  For every token v, in float, rounded once:
+ *   seen or drafted: x > 0 ? x / repetition[b] : x * repetition[b];
+ *   - frequency[b] * (times drawn) - presence[b] where drawn;  + the last bias_values[b][i] with bias_ids[b][i] == v;  -inf where bit v % 32 of allowed[n][v / 32] is not set.
+ * Rows of drafts (node_mask [rows][mask_words], at most 4 words; node_tokens [rows]): the tokens node_tokens[offsets[b] + j] of the bits j in node_mask[n] are drawn once each,
+ * too.  Null pointers leave their part out; ids outside [0, vocab) are none.  Rows behind the last sequence are copied.  logits and out may be the same memory (with the same stride), or
+ * do not overlap.  At most 2^30 columns and rows, 65534 sequences, 65535 biases. */
+typedef struct wf_logits_args {
+    const void* logits;        /* [rows][vocab] of dtype WF_F32, WF_BF16 or WF_F16, rows row_stride elements apart */
+    void* out;                 /* the same type, rows out_stride elements apart */
+    int dtype, rows, vocab, sequences;
+    long long row_stride, out_stride;
+    const int32_t* offsets;    /* [sequences + 1] */
+    const int32_t* history;    /* [sequences][history_width], rows history_stride apart */
+    long long history_stride;
+    const int32_t *history_lens, *prompt_lens; /* [sequences] */
+    const float *repetition, *frequency, *presence; /* [sequences] */
+    const int32_t* bias_ids;   /* [sequences][bias_width] */
+    const float* bias_values;
+    const int32_t* allowed;    /* [rows][ceil(vocab / 32)], rows allowed_stride apart */
+    long long allowed_stride;
+    const int32_t* node_tokens;
+    const uint64_t* node_mask;
+    int history_width, bias_width, mask_words;
+} wf_logits_args;
+int wf_process_logits(const wf_logits_args* args, void* stream);
 
 /* ---- decode engine (the whole step of scripts/direct_inference_full.py:267-302) --- */
 

@@ -20,6 +20,7 @@
 #include <algorithm>
 
 #include "attn_chunks.cuh"
+#include "kv8.cuh"
 #include "fused_common.cuh"
 
 namespace wf {
@@ -68,16 +69,6 @@ __device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// per-(token, head) symmetric int8 quantisation, the reference's arithmetic (kv_cache.py:198-218) at token granularity:
-// scale = 127 / absmax (absmax < 1e-6 -> 1), code = clamp(round(x * scale), -127, 127), stored dequant scale = absmax / 127
-__device__ __forceinline__ float kv8_inv(float& amax) {
-    if (amax < 1e-6f) amax = 1.0f;
-    return __fdiv_rn(127.0f, amax);
-}
-__device__ __forceinline__ int kv8_code(float x, float inv) { return (int)fminf(fmaxf(rintf(__fmul_rn(x, inv)), -127.f), 127.f); }
-__device__ __forceinline__ uint8_t kv8_store(float x, float inv) { return (uint8_t)(kv8_code(x, inv) + 128); }   // offset binary
-__device__ __forceinline__ float kv8_scale(float amax) { return __fdiv_rn(amax, 127.0f); }
-
 // ex2.approx: one MUFU instead of exp2f()'s range-scaling sequence; exp2(-inf) = 0, 2 ulp — far inside the 16-bit rounding of P
 __device__ __forceinline__ float fast_exp2(float x) {
     float y;

@@ -43,6 +43,16 @@ class KvLayout(C.Structure):
     ]
 
 
+class LogitsArgs(C.Structure):
+    _fields_ = [
+        ("logits", C.c_void_p), ("out", C.c_void_p), ("dtype", C.c_int), ("rows", C.c_int), ("vocab", C.c_int), ("sequences", C.c_int),
+        ("row_stride", C.c_longlong), ("out_stride", C.c_longlong), ("offsets", C.c_void_p), ("history", C.c_void_p), ("history_stride", C.c_longlong),
+        ("history_lens", C.c_void_p), ("prompt_lens", C.c_void_p), ("repetition", C.c_void_p), ("frequency", C.c_void_p), ("presence", C.c_void_p),
+        ("bias_ids", C.c_void_p), ("bias_values", C.c_void_p), ("allowed", C.c_void_p), ("allowed_stride", C.c_longlong),
+        ("node_tokens", C.c_void_p), ("node_mask", C.c_void_p), ("history_width", C.c_int), ("bias_width", C.c_int), ("mask_words", C.c_int),
+    ]
+
+
 class ModelConfig(C.Structure):
     _fields_ = [
         ("hidden", C.c_int), ("layers", C.c_int), ("heads", C.c_int), ("kv_heads", C.c_int), ("head_dim", C.c_int),
@@ -89,6 +99,12 @@ SYMBOLS = {
     "wf_prefix_attn_workspace_bytes": (_sz, [_i] * 5),
     "wf_paged_prefix_attn": (_i, [_vp, C.POINTER(KvLayout), _i, _vp, _i, _vp, _i, _vp, _i, _i, _f, _vp, _i, _vp, _sz, _vp]),
     "wf_token_logprobs": (_i, [_vp, _i, _i, _i, C.c_longlong, _vp, _i, _f, _vp, _vp, _vp, _vp, _vp]),
+    "wf_norm_rope_kv_append": (_i, [_vp, C.c_longlong, _i, _i, C.POINTER(KvLayout), _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _i, _f, _i, _vp, _vp]),
+    "wf_tree_plan": (_i, [_vp, _vp, _vp, _i, _i, _i, _vp, _vp, _vp]),
+    "wf_tree_attn_workspace_bytes": (_sz, [_i] * 5),
+    "wf_paged_tree_attn": (_i, [_vp, C.POINTER(KvLayout), _i, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _f, _vp, _i, _vp, _sz, _vp]),
+    "wf_tree_accept": (_i, [_vp] * 5 + [_i, _i, C.POINTER(KvLayout), _vp, _i, _vp, _i] + [_vp] * 8),
+    "wf_process_logits": (_i, [C.POINTER(LogitsArgs), _vp]),
     "wf_rmsnorm_quant": (_i, [_vp, _vp, _f, _i, _i, _vp, _vp, _vp, _vp, _vp]),
     "wf_embed": (_i, [_vp, _vp, _i, _i, _vp, _vp]),
     "wf_lm_head_workspace_bytes": (_sz, [_i, _i]),

@@ -290,6 +290,18 @@ def rope_kv_append(qkv: torch.Tensor, H: int, kv: PagedKV, layer: int, positions
     return q_out
 
 
+def norm_rope_kv_append(qkv: torch.Tensor, H: int, kv: PagedKV, layer: int, positions: torch.Tensor, pages: torch.Tensor, slots: torch.Tensor, cos_tab: torch.Tensor,
+                        sin_tab: torch.Tensor, q_norm: Optional[torch.Tensor] = None, k_norm: Optional[torch.Tensor] = None, eps: float = 1e-6, interleaved: bool = False) -> torch.Tensor:
+    """Queries and keys of a step's tokens normed head by head and rotated, queries returned (bf16 [T, H, D]), keys and values appended to the cache, in one launch.
+    qkv: bf16 [T, (H + 2 Hkv) * D], any row stride.  positions, pages, slots: int32 [T] (paged_plan's; of drafts, tree_plan's positions).  cos_tab, sin_tab: float32 or
+    bf16 [max_pos, R / 2] for the first R dims of a head (a multiple of 8), pairs (i, i + R / 2), or (2i, 2i + 1) with interleaved.  q_norm, k_norm: gains of an RMS
+    norm over the head, float32 or bf16 [D], or None.  In float, rounded once to bf16; an int8 cache then quantises as kv_scatter does.  A token whose page or slot is
+    outside the cache is not appended; one whose position is outside the tables is not either, and its queries are NaN.  Head sizes 64, 128 and 256."""
+    c = kv.c
+    return _native.ops().norm_rope_kv_append(qkv, H, kv.raw if kv.dtype == torch.int8 else kv.pool, c.max_pages, c.layers, c.kv_heads, c.page_size, c.head_dim, c.dtype, layer, positions,
+                                             pages, slots, cos_tab, sin_tab, q_norm, k_norm, eps, interleaved)
+
+
 _attn_ws = {}
 
 
@@ -363,6 +375,55 @@ def paged_release(done: torch.Tensor, seq_lens: torch.Tensor, block_table: torch
     return _native.ops().paged_release(done, seq_lens, block_table, free_pages, free_count, page_size)
 
 
+# ----------------------------------------------------------------------------------------- drafted tokens
+class TreePlan(NamedTuple):
+    """Masks and positions of a step's drafts (of rows behind the last sequence 0 and 0)."""
+    mask: torch.Tensor          # int64 [T, ceil(max_nodes / 64)]: bit j for the draft at place j of the sequence, the row's own and those on its way up
+    positions: torch.Tensor     # int32 [T] cached tokens + drafts above it
+
+
+def tree_plan(parents: torch.Tensor, offsets: torch.Tensor, seq_lens: torch.Tensor, max_nodes: int = 64) -> TreePlan:
+    """Trees of drafts: the new tokens of a sequence (offsets int32 [B + 1], paged_plan's), each behind the one that it follows; parents int32 [T] has that one's place
+    among the sequence's drafts, -1 for those that follow the seq_lens[b] cached tokens alone.  A chain (i - 1) makes a causal mask.  At most max_nodes <= 256
+    drafts a sequence (one with more has masks of 0 and positions -1)."""
+    return TreePlan(*_native.ops().tree_plan(parents, offsets, seq_lens, max_nodes))
+
+
+def paged_tree_attn(q: torch.Tensor, kv: PagedKV, layer: int, block_table: torch.Tensor, seq_lens: torch.Tensor, offsets: torch.Tensor, mask: torch.Tensor,
+                    scale: Optional[float] = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """Attention of drafts over the paged cache: q bf16 [T, H, D], the rows of sequence b are offsets[b] to offsets[b + 1]; it has seq_lens[b] cached tokens and its
+    drafts' keys and values behind them (norm_rope_kv_append or kv_scatter has put them there).  Row t sees every cached token, and the drafts whose bits mask[t] has
+    (int64 [T, words], tree_plan's or any other pattern over up to 64 * words drafts, words <= 4).  A row that sees no key gets zeros, as do rows behind the last
+    sequence.  Weights are rounded to bf16 (over an int8 cache times the value's scale)."""
+    if out_dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError("out_dtype must be bfloat16 or float32")
+    c = kv.c
+    return _native.ops().paged_tree_attn(q, kv.raw if kv.dtype == torch.int8 else kv.pool, c.max_pages, c.layers, c.kv_heads, c.page_size, c.head_dim, c.dtype, layer, block_table,
+                                         seq_lens, offsets, mask, 1.0 / (q.shape[-1] ** 0.5) if scale is None else scale, out_dtype)
+
+
+class TreeAccept(NamedTuple):
+    """What a verified step keeps, all int32."""
+    accepted: torch.Tensor      # [B] drafts kept, the first one (the token drawn last) among them
+    path: torch.Tensor          # [T] from offsets[b] on: the places of the kept ones, -1 behind them
+    next_tokens: torch.Tensor   # [B] drawn behind the last kept one (-1 for sequences without drafts)
+    lens: torch.Tensor          # [B] seq_lens + accepted
+    free_count: torch.Tensor    # [1] pages on the free list now
+    status: torch.Tensor        # [1] 0, or why nothing was moved or handed back (PLAN_*, ORed)
+
+
+def tree_accept(parents: torch.Tensor, tokens: torch.Tensor, targets: torch.Tensor, offsets: torch.Tensor, seq_lens: torch.Tensor, kv: PagedKV, block_table: torch.Tensor,
+                free_pages: torch.Tensor, free_count: torch.Tensor) -> TreeAccept:
+    """Keeps the drafts that the model agrees with: tokens[t] is draft t, targets[t] what was drawn behind it (greedily, or from the model's distribution, whose own the
+    result then is).  The first draft of a sequence is kept; behind a kept one, the draft that follows it with the token drawn there (of several the lowest).  Keys and
+    values of the kept drafts move up behind the cached tokens in every layer, and pages behind the last of them go back on the free list (free_pages is written
+    in place, in paged_release's order).  Go on with `lens`, `free_count` and `next_tokens`.  What does not fit is not done at all: `status` says why, and lens
+    is then seq_lens + the drafts.  At most 8192 sequences of 256 drafts."""
+    c = kv.c
+    return TreeAccept(*_native.ops().tree_accept(parents, tokens, targets, offsets, seq_lens, kv.raw if kv.dtype == torch.int8 else kv.pool, c.max_pages, c.layers, c.kv_heads, c.page_size,
+                                                 c.head_dim, c.dtype, block_table, free_pages, free_count))
+
+
 # ----------------------------------------------------------------------------------------- glue
 def embed(table: torch.Tensor, tokens: torch.Tensor) -> torch.Tensor:
     _need_cuda(table, tokens)
@@ -390,3 +451,19 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, tem
     top_ids int32 [N, top]).  Logits of -inf have probability 0; a row of nothing else has logprobs -inf and entropy 0; a row with +inf or NaN has NaN; a token
     outside [0, V) has NaN."""
     return _native.ops().token_logprobs(logits, tokens, top, temperature)
+
+
+def process_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = None, history_lens: Optional[torch.Tensor] = None, prompt_lens: Optional[torch.Tensor] = None,
+                   repetition: Optional[torch.Tensor] = None, frequency: Optional[torch.Tensor] = None, presence: Optional[torch.Tensor] = None,
+                   bias_ids: Optional[torch.Tensor] = None, bias_values: Optional[torch.Tensor] = None, allowed: Optional[torch.Tensor] = None, offsets: Optional[torch.Tensor] = None,
+                   node_tokens: Optional[torch.Tensor] = None, node_mask: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Penalties, biases and grammar masks on logits (f32, bf16 or f16 [N, V], any row stride) before a token is drawn, in one pass; returns `out` (new memory, or the
+    tensor given, which may be `logits` itself).  Row n is sequence n's, or with offsets (int32 [B + 1]) that of the sequence b whose rows offsets[b] to offsets[b + 1] it is
+    among (rows behind the last one are copied).  Of each sequence:
+      history int32 [B, L], its first history_lens[b] tokens (None: L): the prompt's, up to prompt_lens[b] (None: none), and those drawn since.  Tokens in it: x / repetition[b]
+      where x > 0, else x * repetition[b]; drawn ones also - frequency[b] * times - presence[b] (float32 [B] each).
+      bias_ids int32 [B, n], bias_values float32 [B, n]: added; of entries of the same id the last one counts.
+    Of each row: allowed int32 [N, ceil(V / 32)], bit v % 32 of word v // 32 for token v: the others become -inf.
+    Rows of drafts: node_tokens int32 [N] and node_mask int64 [N, words] (tree_plan's): the drafts whose bits a row has count as drawn.  Ids outside [0, V) are none."""
+    new = _native.ops().process_logits(logits, history, history_lens, prompt_lens, repetition, frequency, presence, bias_ids, bias_values, allowed, offsets, node_tokens, node_mask, out)
+    return new if out is None else out
