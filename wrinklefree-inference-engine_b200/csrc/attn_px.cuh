@@ -93,10 +93,9 @@ __device__ __forceinline__ uint64_t px_add2(uint64_t a, uint64_t b) { uint64_t v
 __device__ __forceinline__ float px_ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ float px_max(float a, float b) { float y; asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b)); return y; }     // NaN stays NaN
 // 2^x of two numbers on the multiply-add units: x = i + f, |f| <= 1/2, by adding 1.5 * 2^23; 2^f by its minimax polynomial of degree 3 (Remez; off by 7.5e-5 at
-// most, a 50th of what the rounding of a weight to bf16 may be); i goes into the exponent.  Below 2^-126: 2^-126 or less.  The special function unit gives 16 values a
+// most, a 50th of what the rounding of a weight to bf16 may be); i goes into the exponent.  Below 2^-126: 0.  The special function unit gives 16 values a
 // clock and SM; one pair in PX_POLY takes this way: 74.4 us for a prefix of 32768 under 128 sequences with one in 8, 71.5 in 4, 71.7 in 3, 72.3 in 2, 79 without.
 constexpr int PX_POLY = 4;
-template <bool FLUSH>
 __device__ __forceinline__ void px_exp2_poly(uint64_t x, float& e0, float& e1) {
     const uint64_t magic = px_pair(0x4b400000u, 0x4b400000u), minus_magic = px_pair(0xcb400000u, 0xcb400000u), minus1 = px_pair(0xbf800000u, 0xbf800000u);
     constexpr float c0 = 0.9999280571937561f, c1 = 0.6932609677314758f, c2 = 0.2426111251115799f, c3 = 0.0551716685295105f;
@@ -109,11 +108,10 @@ __device__ __forceinline__ void px_exp2_poly(uint64_t x, float& e0, float& e1) {
     y = px_fma2(y, f, px_pair(__float_as_uint(c0), __float_as_uint(c0)));
     e0 = __uint_as_float((uint32_t)y + ((uint32_t)t << 23));
     e1 = __uint_as_float((uint32_t)(y >> 32) + ((uint32_t)(t >> 32) << 23));
-    if (FLUSH) {                                          // what is left below 2^-126 becomes 0, so that hidden keys have no weight at all
-        uint64_t z;
-        asm("add.rn.ftz.f32x2 %0, %1, %2;" : "=l"(z) : "l"(px_pair(__float_as_uint(e0), __float_as_uint(e1))), "l"(0ull));
-        px_unpair(z, e0, e1);
-    }
+    // what is left below 2^-126 becomes 0, so that hidden keys and those of -inf scores have no weight at all
+    uint64_t z;
+    asm("add.rn.ftz.f32x2 %0, %1, %2;" : "=l"(z) : "l"(px_pair(__float_as_uint(e0), __float_as_uint(e1))), "l"(0ull));
+    px_unpair(z, e0, e1);
 }
 template <int N> __device__ __forceinline__ void px_regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N) : "memory"); }
 template <int N> __device__ __forceinline__ void px_regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N) : "memory"); }
@@ -425,7 +423,7 @@ __device__ __forceinline__ void px_block(const CUtensorMap& tmap, const P& p, un
                 const uint64_t x = px_fma2(px_pair(s[2 * c], s[2 * c + 1]), unit2, nm2);
                 float e0, e1;
                 if (c % PX_POLY == PX_POLY - 1) {
-                    px_exp2_poly<TREE>(x, e0, e1);
+                    px_exp2_poly(x, e0, e1);
                 } else {
                     px_unpair(x, e0, e1);
                     e0 = px_ex2(e0); e1 = px_ex2(e1);
