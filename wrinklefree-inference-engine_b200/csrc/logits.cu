@@ -4,13 +4,16 @@
 // y - f c - p [c > 0], then + bias, then -inf where the grammar does not allow v; in float, rounded once to the logits' type.  Entries that nothing of it concerns are
 // copied as they are (left alone where the result goes over the logits).
 //
-// A block has a slice of the vocabulary of one sequence: it counts the sequence's history into a table in shared memory (whole numbers: the order of the atomics does not
-// show) and then takes its share of the sequence's rows, a warp or several to a row.  Rows of drafted tokens differ by what each one's own past adds, up to 256
-// tokens: those of the slice stand in a short list of the warp's, and in a bitmap beside the table's.  Only where a bitmap or the mask has something to say is an
-// entry more than copied.
+// A block has a run of a sequence's logits, row after row.  It first notes the tokens there that the history, the drafts or a bias concerns: a bitmap, the number of them in
+// front of each word of it, and so the place of each token's own word (times drawn, whether seen) in a list as long as there are such tokens.  All of it are whole numbers whose
+// order of arrival does not show.  Meanwhile the first logits are on their way: each warp moves chunks of 2 KB through a ring of its own in shared memory, three deep,
+// changes its listed tokens there, a lane each, and masks on the way out.  A draft's own past, which differs from row to row, is the common bits of its mask and of a set
+// of drafts for each listed token.
 //
-// Bound by memory: each logit is read and written once; a masked vector is not read at all.
+// Bound by memory: each logit is read and written once; masked vectors are not read.
 #include <cuda_fp16.h>
+
+#include <algorithm>
 
 #include "common.cuh"
 #include "wf_bitnet.h"
@@ -19,17 +22,23 @@ namespace wf {
 
 namespace {
 
-typedef unsigned long long u64;
-
-constexpr int LG_THREADS = 256, LG_WARPS = LG_THREADS / 32;
-constexpr int LG_SLICE = 4096;                         // tokens of a slice at most
-constexpr int LG_NODES = 256;                          // drafts of a sequence at most
-constexpr int LG_AHEAD = 4;                            // vectors of a lane under way together
-constexpr uint32_t LG_SEEN = 0x80000000u;
+constexpr int LG_WARPS = 12, LG_THREADS = 32 * LG_WARPS;
+constexpr int LG_CHUNK = 2048, LG_STAGES = 2;          // bytes of a warp's chunk, and chunks of its ring
+constexpr int LG_SHORT = 512;                          // bytes of a chunk where there is little to read, and warps would have none
+constexpr int lg_ring(int bytes) { return LG_WARPS * LG_STAGES * (bytes + 16); }
+constexpr int LG_SLICE = 131072, LG_ENTRIES = 8192;    // columns that a block's bitmap has, and entries of a list, at most
+constexpr int LG_BLOCKS = 2;                           // blocks of an SM
+constexpr int LG_TABLE_COST = 28;                      // what a block's table takes, in chunks' times
+constexpr int LG_MIN_RUN = 2;                          // chunks of a block at least
+constexpr int LG_NODES = 256;                          // drafts of a sequence at most: a thread each
+static_assert(LG_NODES <= LG_THREADS, "");
+constexpr uint32_t LG_SEEN = 0x80000000u, LG_DRAFT = 0x40000000u, LG_TIMES = 0x3fffffffu;      // of an entry's word: in the history, a draft, times drawn
 
 struct LogitsParams {
     wf_logits_args a;
-    int slice, row_parts;
+    int slice, groups;             // columns of a slice (a multiple of a chunk; nearly always all there are), and blocks of each slice
+    int run;                       // chunks of a block
+    int entries, tables;
 };
 
 template <typename T> struct LgType;
@@ -46,176 +55,345 @@ template <> struct LgType<__half> {
     static __device__ __forceinline__ __half put(float v) { return __float2half_rn(v); }
 };
 
-// n <= 32 bits from bit `at` of the words on
-__device__ __forceinline__ uint32_t lg_bits(const uint32_t* w, int at, int n) {
-    uint32_t v = w[at >> 5] >> (at & 31);
-    if ((at & 31) + n > 32) v |= w[(at >> 5) + 1] << (32 - (at & 31));
-    return n < 32 ? v & ((1u << n) - 1u) : v;
-}
+__device__ __forceinline__ void lg_async16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
 
-template <typename T>
-__global__ void __launch_bounds__(LG_THREADS) process_logits_kernel(const __grid_constant__ LogitsParams p) {
-    constexpr int E = 16 / (int)sizeof(T);
-    extern __shared__ __align__(16) uint32_t lg_smem[];
-    __shared__ uint32_t past_bits[LG_WARPS][LG_SLICE / 32];
-    __shared__ uint16_t past_list[LG_WARPS][LG_NODES];
+template <typename T, int BYTES>
+__global__ void __launch_bounds__(LG_THREADS, LG_BLOCKS) process_logits_kernel(const __grid_constant__ LogitsParams p) {
+    constexpr int E = 16 / (int)sizeof(T), CHUNK = BYTES / (int)sizeof(T), GROUPS = CHUNK / 32, VECS = BYTES / 512;
+    extern __shared__ __align__(16) unsigned char lg_smem[];
+    __shared__ uint32_t mask_s[LG_WARPS][LG_STAGES][GROUPS];
+    __shared__ int warp_n[LG_WARPS], found[4];
+    __shared__ float bias_s[LG_THREADS];
     const wf_logits_args& a = p.a;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    uint32_t* count = lg_smem;                         // [slice] drawn so often; LG_SEEN: there before
-    uint32_t* touched = count + p.slice;               // [slice / 32] a bit per entry that the history or a bias concerns
-    uint16_t* bias_at = reinterpret_cast<uint16_t*>(touched + p.slice / 32);      // [slice] its bias, from 1
-    const int lo = blockIdx.x * p.slice, hi = min(a.vocab, lo + p.slice);
-    const int b = blockIdx.y;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, words = p.slice / 32;
+    uint32_t* entry = reinterpret_cast<uint32_t*>(lg_smem + lg_ring(BYTES));          // [entries]
+    uint32_t* touched = entry + p.entries;             // [words] a bit per token that has an entry
+    uint32_t* same = touched + words;                  // [drafts][2 words of mask] the drafts of the same token, by one of them
+    uint16_t* bias = reinterpret_cast<uint16_t*>(same + 128 * a.mask_words * a.mask_words);    // [entries] the place of its bias among the sequence's, from 1
+    uint16_t* token_of = bias + (a.bias_ids ? p.entries : 0);          // [entries] the token, from the first column's (mod 2^16: a chunk's tokens are near one another)
+    uint16_t* front = token_of + p.entries;            // [words + 1] entries in front of a word's first
+    uint8_t* draft_of = reinterpret_cast<uint8_t*>(front + words + 2);         // [entries] the draft that stands for the token
+    const int slice = blockIdx.x / p.groups, group = blockIdx.x - slice * p.groups;
+    const int s_lo = slice * p.slice, s_hi = min(a.vocab, s_lo + p.slice), per_row = (s_hi - s_lo + CHUNK - 1) / CHUNK;
     pdl_wait_prior();
     pdl_launch_dependents();
-    int r0, r1;                                        // this block's rows
+    // this block's sequence (a.sequences: rows behind the last one), its rows first .. end, and its run of their chunks
+    int b, first, end, part;
     if (a.offsets) {
-        const int end = a.sequences > 0 ? min(max(a.offsets[a.sequences], 0), a.rows) : 0;
-        r0 = b < a.sequences ? min(max(a.offsets[b], 0), a.rows) : end;
-        r1 = b < a.sequences ? max(min(a.offsets[b + 1], a.rows), r0) : a.rows;
+        int before = 0;                                // runs of the sequences in front
+        b = -1;
+        for (int s0 = 0; s0 <= a.sequences; s0 += LG_THREADS) {
+            const int s = s0 + tid;
+            int from = 0, to = 0;
+            if (s <= a.sequences) {
+                from = a.sequences > 0 ? min(max(a.offsets[s], 0), a.rows) : 0;
+                to = s < a.sequences ? max(min(a.offsets[s + 1], a.rows), from) : a.rows;
+            }
+            const int n = (int)(((long long)(to - from) * per_row + p.run - 1) / p.run);
+            int in = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) { const int z = __shfl_up_sync(0xffffffffu, in, o); if (lane >= o) in += z; }
+            if (lane == 31) warp_n[warp] = in;
+            __syncthreads();
+            int total = 0, base = before;
+#pragma unroll
+            for (int w = 0; w < LG_WARPS; ++w) { if (w < warp) base += warp_n[w]; total += warp_n[w]; }
+            const int at = group - base - (in - n);
+            if (at >= 0 && at < n) { found[0] = s; found[1] = from; found[2] = to; found[3] = at; }
+            before += total;
+            __syncthreads();
+            if (group < before) { b = found[0]; first = found[1]; end = found[2]; part = found[3]; break; }
+        }
+        if (b < 0) return;                             // (the same in all threads)
     } else {
-        r0 = min(b, a.rows);
-        r1 = b < a.sequences ? min(b + 1, a.rows) : a.rows;
+        const int parts = (per_row + p.run - 1) / p.run;
+        b = first = group / parts;
+        end = b + 1;
+        part = group - b * parts;
+        if (b >= a.rows) return;
     }
-    const int first = r0, per = (r1 - r0 + p.row_parts - 1) / p.row_parts;
-    r0 += min(r1 - r0, per * (int)blockIdx.z);
-    r1 = min(r1, r0 + per);
-    if (r0 >= r1) return;
-    const bool none = b >= a.sequences;                // rows behind the last sequence
-    if (none && a.out == a.logits) return;
-    const bool tables = !none && (a.history || a.bias_ids);
+    const bool none = b >= a.sequences, tables = !none && p.tables, masked = !none && a.allowed, in_place = a.logits == a.out;
+    if (in_place && !tables && !masked) return;
+    // its first row and chunk there, how many chunks, and the columns that they have
+    const long long at0 = (long long)part * p.run;
+    const int row0 = first + (int)(at0 / per_row), col0 = (int)(at0 % per_row);
+    const int chunks = (int)min((long long)p.run, (long long)(end - first) * per_row - at0);
+    const bool one_row = col0 + chunks <= per_row;
+    const int lo = one_row ? s_lo + col0 * CHUNK : s_lo, hi = one_row ? min(s_hi, lo + chunks * CHUNK) : s_hi;
+    const uint32_t ring = smem_u32(lg_smem) + warp * LG_STAGES * (BYTES + 16);
+    T* const ring_p = reinterpret_cast<T*>(lg_smem + warp * LG_STAGES * (BYTES + 16));
+    constexpr int STEP = (BYTES + 16) / (int)sizeof(T);
+
+    // a warp's chunks are every eighth of the block's
+    struct Chunk { int left, row, col; };              // chunks of the block from this one on (none: 0 or less), its row and place there
+    auto step = [&](Chunk& c) { c.left -= LG_WARPS; c.col += LG_WARPS; while (c.col >= per_row) { c.col -= per_row; ++c.row; } };
+    auto from_of = [&](const Chunk& c) { return s_lo + c.col * CHUNK; };
+    auto in_of = [&](const Chunk& c) { return reinterpret_cast<const T*>(a.logits) + (size_t)c.row * a.row_stride + from_of(c); };
+    Chunk ahead{chunks - warp, row0, col0 + warp};     // the chunk whose mask is asked for next
+    while (ahead.col >= per_row) { ahead.col -= per_row; ++ahead.row; }
+    Chunk asked = ahead, now = ahead;                  // whose logits are; the one to change
+    // the mask's word of this lane's 32 tokens; bits behind the last token are 0
+    auto mask_of = [&](const Chunk& c) -> uint32_t {
+        const int n = s_hi - from_of(c) - lane * 32;
+        if (c.left <= 0 || lane >= GROUPS || n <= 0) return 0u;
+        const uint32_t valid = n < 32 ? (1u << n) - 1u : ~0u;
+        return masked ? reinterpret_cast<const uint32_t*>(a.allowed)[(size_t)c.row * a.allowed_stride + (from_of(c) >> 5) + lane] & valid : valid;
+    };
+    // Asks for a chunk: its 16-byte vectors from the boundary at or in front of its first token on (a row may begin anywhere), but for those that the mask hides
+    auto ask = [&](const Chunk& c, uint32_t word, int stage) {
+        if (lane < GROUPS) mask_s[warp][stage][lane] = word;
+        if (c.left > 0 && !in_place) {
+            const T* x = in_of(c);
+            const int off = (int)((uintptr_t)x % 16 / sizeof(T)), n = min(CHUNK, s_hi - from_of(c));
+            const uint32_t dst = ring + stage * (BYTES + 16);
+            if (off == 0 && n == CHUNK) {              // the usual case: a vector's bits lie in one word, and words a whole number of lanes apart
+                const T* xl = x + lane * E;
+#pragma unroll
+                for (int u = 0; u < VECS; ++u) {
+                    const uint32_t bits = masked ? __shfl_sync(0xffffffffu, word, u * E + lane * E / 32) >> (lane * E & 31) & ((1u << E) - 1u) : 1u;
+                    if (bits) lg_async16(dst + lane * 16 + u * 512, xl + u * 32 * E);
+                }
+            } else
+#pragma unroll
+            for (int u = 0; u < VECS + 1; ++u) {
+                const int vec = u * 32 + lane, t0 = vec * E - off;             // its first token; in an aligned row the others are in the same word
+                const uint32_t w0 = __shfl_sync(0xffffffffu, word, max(t0, 0) / 32), w1 = __shfl_sync(0xffffffffu, word, min(t0 + E - 1, CHUNK - 1) / 32);
+                if (t0 < n && (!masked || (off ? (w0 | w1) != 0u : (w0 >> (t0 & 31) & ((1u << E) - 1u)) != 0u))) lg_async16(dst + vec * 16, x + t0);
+                if (u == VECS - 1 && !off) break;                               // (the last vector only where the row begins inside one)
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    uint32_t next[LG_STAGES];                          // a chunk's mask is asked for three chunks ahead of its logits
+#pragma unroll
+    for (int i = 0; i < LG_STAGES; ++i) { next[i] = mask_of(ahead); step(ahead); }
+#pragma unroll
+    for (int i = 0; i < LG_STAGES - 1; ++i) {
+        ask(asked, next[i], i);
+        step(asked);
+        next[i] = mask_of(ahead);
+        step(ahead);
+    }
+    float rep = 1.f, freq = 0.f, pres = 0.f;
     if (tables) {
-        for (int i = tid; i < p.slice + p.slice / 32 + p.slice / 2; i += LG_THREADS) lg_smem[i] = 0u;
+        // what comes from memory is asked for at once: the first biases and the drafts, a thread each, lengths and weights
+        const int n_b = a.bias_ids ? a.bias_width : 0, n_nodes = a.node_mask ? min(end - first, 64 * a.mask_words) : 0;
+        const int32_t *h = a.history + (size_t)b * a.history_stride, *ids = a.bias_ids + (size_t)b * a.bias_width;
+        const int my_id = tid < n_b ? ids[tid] : -1, my_node = tid < n_nodes ? a.node_tokens[first + tid] : -1;
+        const float my_bias = tid < n_b ? a.bias_values[(size_t)b * a.bias_width + tid] : 0.f;
+        if (a.repetition) rep = a.repetition[b];
+        if (a.frequency) freq = a.frequency[b];
+        if (a.presence) pres = a.presence[b];
+        const int n_h = !a.history ? 0 : min(max(a.history_lens ? a.history_lens[b] : a.history_width, 0), a.history_width), drawn = a.prompt_lens ? a.prompt_lens[b] : 0;
+        const int used = (hi - lo + 31) / 32;          // words of the bitmap
+        for (int i = tid; i < (p.entries + used + 3) / 4; i += LG_THREADS) reinterpret_cast<uint4*>(entry)[i] = make_uint4(0u, 0u, 0u, 0u);      // (and the bitmap behind it)
+        for (int i = tid; a.bias_ids && i < p.entries / 8; i += LG_THREADS) reinterpret_cast<uint4*>(bias)[i] = make_uint4(0u, 0u, 0u, 0u);
+        auto history = [&](auto token) {               // every token of it that lies in the run's columns, with its place
+            const int n4 = (uintptr_t)h % 16 ? 0 : n_h / 4;
+            auto in = [&](int v, int i) { if (v >= lo && v < hi) token(v - lo, i); };
+            for (int i = tid; i < n4; i += LG_THREADS * 4) {
+                int4 v[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) v[u] = i + u * LG_THREADS < n4 ? reinterpret_cast<const int4*>(h)[i + u * LG_THREADS] : make_int4(-1, -1, -1, -1);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int k = 4 * (i + u * LG_THREADS);
+                    in(v[u].x, k); in(v[u].y, k + 1); in(v[u].z, k + 2); in(v[u].w, k + 3);
+                }
+            }
+            for (int i = 4 * n4 + tid; i < n_h; i += LG_THREADS) in(h[i], i);
+        };
+        auto biases = [&](auto each) {
+            if (my_id >= lo && my_id < hi) each(my_id - lo, tid);
+            for (int i = tid + LG_THREADS; i < n_b; i += LG_THREADS) { const int v = ids[i]; if (v >= lo && v < hi) each(v - lo, i); }
+        };
+        auto touch = [&](int v) {
+            const uint32_t bit = 1u << (v & 31);
+            if (!(*(volatile uint32_t*)&touched[v >> 5] & bit)) atomicOr(&touched[v >> 5], bit);
+        };
+        const bool draft = my_node >= lo && my_node < hi;
+        bias_s[tid] = my_bias;
         __syncthreads();
-        if (a.history) {
-            const int32_t* h = a.history + (size_t)b * a.history_stride;
-            const int n = min(max(a.history_lens ? a.history_lens[b] : a.history_width, 0), a.history_width), drawn = a.prompt_lens ? a.prompt_lens[b] : 0;
-            for (int i = tid; i < n; i += LG_THREADS) {
-                const int v = h[i];
-                if (v < lo || v >= hi) continue;
-                if (i >= drawn) atomicAdd(&count[v - lo], 1u);
-                atomicOr(&count[v - lo], LG_SEEN);
-                atomicOr(&touched[(v - lo) >> 5], 1u << ((v - lo) & 31));
-            }
+        history([&](int v, int) { touch(v); });
+        if (draft) touch(my_node - lo);
+        biases([&](int v, int) { touch(v); });
+        __syncthreads();
+        {                                              // entries in front of every word
+            const int each = (used + LG_THREADS - 1) / LG_THREADS, w0 = min(used, tid * each), w1 = min(used, w0 + each);
+            int n = 0;
+            for (int w = w0; w < w1; ++w) n += __popc(touched[w]);
+            int in = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) { const int z = __shfl_up_sync(0xffffffffu, in, o); if (lane >= o) in += z; }
+            if (lane == 31) warp_n[warp] = in;
+            __syncthreads();
+            int at = in - n;
+#pragma unroll
+            for (int w = 0; w < LG_WARPS; ++w) if (w < warp) at += warp_n[w];
+            for (int w = w0; w < w1; ++w) { front[w] = (uint16_t)at; at += __popc(touched[w]); }
+            if (tid == LG_THREADS - 1) front[used] = (uint16_t)at;
         }
-        if (a.bias_ids) {
-            // entries of an id in order: the last one counts, and it is the one that no later one of the same id follows
-            for (int i = tid; i < a.bias_width; i += LG_THREADS) {
-                const int v = a.bias_ids[(size_t)b * a.bias_width + i];
-                if (v < lo || v >= hi) continue;
-                bool last = true;
-                for (int j = i + 1; j < a.bias_width && last; ++j) last = a.bias_ids[(size_t)b * a.bias_width + j] != v;
-                if (last) {
-                    bias_at[v - lo] = (uint16_t)(i + 1);
-                    atomicOr(&touched[(v - lo) >> 5], 1u << ((v - lo) & 31));
-                }
-            }
+        for (int i = tid; i < n_nodes * 2 * a.mask_words; i += LG_THREADS) same[i] = 0u;
+        __syncthreads();
+        auto place = [&](int v) {
+            const int e = front[v >> 5] + __popc(touched[v >> 5] & ((1u << (v & 31)) - 1u));
+            token_of[e] = (uint16_t)v;
+            return e;
+        };
+        history([&](int v, int i) {
+            uint32_t* e = &entry[place(v)];
+            if (!(*(volatile uint32_t*)e & LG_SEEN)) atomicOr(e, LG_SEEN);
+            if (i >= drawn) atomicAdd(e, 1u);
+        });
+        int my_entry = -1;
+        if (draft) {                                   // drafts of the same token: the one whose number is left, whichever, stands for all
+            my_entry = place(my_node - lo);
+            atomicOr(&entry[my_entry], LG_DRAFT);
+            draft_of[my_entry] = (uint8_t)tid;
+        }
+        bool more;                                     // of biases of the same token the last one counts: those that find an earlier one there write again
+        do {
+            more = false;
+            biases([&](int v, int i) { const int e = place(v); if (bias[e] <= i) { bias[e] = (uint16_t)(i + 1); more = true; } });
+        } while (__syncthreads_or(more));
+        if (a.node_mask) {
+            if (draft) atomicOr(&same[draft_of[my_entry] * 2 * a.mask_words + (tid >> 5)], 1u << (tid & 31));
+            __syncthreads();
         }
     }
-    const bool nodes = !none && a.node_mask;
-    if (nodes)
-        for (int i = lane; i < p.slice / 32; i += 32) past_bits[warp][i] = 0u;
-    __syncthreads();
-    const float rep = !none && a.repetition ? a.repetition[b] : 1.f, freq = !none && a.frequency ? a.frequency[b] : 0.f, pres = !none && a.presence ? a.presence[b] : 0.f;
-    const int rows = r1 - r0, of_row = rows >= LG_WARPS ? 1 : rows >= 4 ? 2 : rows >= 2 ? 4 : 8;       // warps of a row
-    const int share = p.slice / of_row;
-    for (int unit = warp; unit < rows * of_row; unit += LG_WARPS) {
-        const int row = r0 + unit / of_row, slo = lo + unit % of_row * share, shi = min(hi, slo + share);
-        if (slo >= shi) continue;
-        int past = 0;
-        if (nodes) {                                   // what this draft's own past adds in the slice
-            for (int w = 0; w < a.mask_words; ++w) {
-                const u64 seen = a.node_mask[(size_t)row * a.mask_words + w];
+    uint4 neg;                                         // -inf all over
+    {
+        alignas(16) T q[E];
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const int j = w * 64 + half * 32 + lane;
-                    int v = -1;
-                    if ((seen >> (half * 32 + lane) & 1) && first + j < a.rows) v = a.node_tokens[first + j];
-                    const bool in = v >= slo && v < shi;
-                    const unsigned who = __ballot_sync(0xffffffffu, in);
-                    if (in) {
-                        past_list[warp][past + __popc(who & ((1u << lane) - 1u))] = (uint16_t)(v - lo);
-                        atomicOr(&past_bits[warp][(v - lo) >> 5], 1u << ((v - lo) & 31));
-                    }
-                    past += __popc(who);
-                }
+        for (int i = 0; i < E; ++i) q[i] = LgType<T>::put(-INFINITY);
+        neg = *reinterpret_cast<const uint4*>(q);
+    }
+    auto change = [&](int stage) {
+        const T* x = in_of(now);
+        const int from = from_of(now), n = min(CHUNK, s_hi - from), off = in_place ? 0 : (int)((uintptr_t)x % 16 / sizeof(T));
+        T* y = reinterpret_cast<T*>(a.out) + (size_t)now.row * a.out_stride + from;
+        T* s = in_place ? y : ring_p + stage * STEP + off;                     // the chunk's tokens
+        const uint32_t* keep_s = mask_s[warp][stage];
+        int e0 = 0, e1 = 0;                            // its entries
+        if (tables) { e0 = front[(from - lo) >> 5]; e1 = front[(from - lo + n + 31) >> 5]; }
+        asm volatile("cp.async.wait_group %0;" ::"n"(LG_STAGES - 2) : "memory");
+        __syncwarp();
+        for (int e = e0 + lane; e < e1; e += 32) {
+            const int v = (uint16_t)(token_of[e] - (from - lo));
+            const uint32_t w = entry[e], biased = a.bias_ids ? bias[e] : 0;
+            uint32_t times = w & LG_TIMES;
+            if (!(keep_s[v >> 5] >> (v & 31) & 1u)) continue;
+            if (w & LG_DRAFT) {                        // drafts of this token in the row's own past
+                const uint32_t* past = reinterpret_cast<const uint32_t*>(a.node_mask + (size_t)now.row * a.mask_words);
+                for (int i = 0; i < 2 * a.mask_words; ++i) times += __popc(same[draft_of[e] * 2 * a.mask_words + i] & past[i]);
             }
-            __syncwarp();
+            const bool seen = times || (w & LG_SEEN);
+            float z = LgType<T>::get(s[v]);
+            if (seen) z = z > 0.f ? __fdiv_rn(z, rep) : z * rep;
+            z -= freq * (float)times + (times ? pres : 0.f);
+            if (biased) z += biased <= LG_THREADS ? bias_s[biased - 1] : a.bias_values[(size_t)b * a.bias_width + biased - 1];
+            if (seen || biased) s[v] = LgType<T>::put(z);              // (else a draft that is not in this row's past)
         }
-        const T* x = reinterpret_cast<const T*>(a.logits) + (size_t)row * a.row_stride;
-        T* y = reinterpret_cast<T*>(a.out) + (size_t)row * a.out_stride;
-        const uint32_t* ok = !none && a.allowed ? reinterpret_cast<const uint32_t*>(a.allowed) + (size_t)row * a.allowed_stride : nullptr;
-        const bool in_place = (const void*)x == (const void*)y;
-        auto concerned = [&](int v, int n) -> uint32_t { return (tables ? lg_bits(touched, v - lo, n) : 0u) | (past ? lg_bits(past_bits[warp], v - lo, n) : 0u); };
-        auto value = [&](float z, int v) -> float {
-            const uint32_t c0 = tables ? count[v - lo] : 0u;
-            uint32_t c = c0 & ~LG_SEEN;
-            for (int i = 0; i < past; ++i) c += past_list[warp][i] == (uint16_t)(v - lo);
-            if (c0 | c) z = z > 0.f ? __fdiv_rn(z, rep) : z * rep;
-            z -= freq * (float)c + (c ? pres : 0.f);
-            if (tables && a.bias_ids) {
-                const int i = bias_at[v - lo];
-                if (i) z += a.bias_values[(size_t)b * a.bias_width + i - 1];
-            }
-            return z;
-        };
+        __syncwarp();
         auto one = [&](int v) {
-            const bool keep = !ok || (ok[v >> 5] >> (v & 31) & 1u);
-            const bool work = concerned(v, 1);
-            if (keep && !work && in_place) return;
-            y[v] = !keep ? LgType<T>::put(-INFINITY) : work ? LgType<T>::put(value(LgType<T>::get(x[v]), v)) : x[v];
+            if (!(keep_s[v >> 5] >> (v & 31) & 1u)) y[v] = LgType<T>::put(-INFINITY);
+            else if (!in_place) y[v] = s[v];
         };
-        // vectors between the row's 16-byte boundaries, entries one by one in front of and behind them (all of them where the two rows lie differently to it)
-        const int off = (int)((uintptr_t)(x + slo) % 16 / sizeof(T));
-        int va = min(shi, slo + (off ? E - off : 0)), ve = va + (shi - va) / E * E;
-        if (((uintptr_t)x ^ (uintptr_t)y) & 15) va = ve = shi;
-        for (int v = slo + lane; v < va; v += 32) one(v);
-        for (int v = ve + lane; v < shi; v += 32) one(v);
-        for (int v = va + lane * E; v < ve; v += 32 * E * LG_AHEAD) {
-            uint32_t keep[LG_AHEAD], work[LG_AHEAD];
-            uint4 q[LG_AHEAD];
+        constexpr uint32_t ALL = (1u << E) - 1u;
+        if (!masked && in_place) {
+        } else if (!in_place && off == 0 && n == CHUNK && !((uintptr_t)y & 15)) {              // the usual case
+            const uint32_t keep_l = masked && lane < GROUPS ? keep_s[lane] : 0u;
+            const T* sl = s + lane * E;
+            T* yl = y + lane * E;
 #pragma unroll
-            for (int u = 0; u < LG_AHEAD; ++u) {
-                const int at = v + u * 32 * E;
-                keep[u] = at >= ve ? 0u : ok ? lg_bits(ok, at, E) : (1u << E) - 1u;
-            }
+            for (int u = 0; u < VECS; ++u) {
+                const uint32_t keep = masked ? __shfl_sync(0xffffffffu, keep_l, u * E + lane * E / 32) >> (lane * E & 31) & ALL : ALL;
+                alignas(16) T q[E];
+                if (keep == 0u) { *reinterpret_cast<uint4*>(yl + u * 32 * E) = neg; continue; }
+                *reinterpret_cast<uint4*>(q) = *reinterpret_cast<const uint4*>(sl + u * 32 * E);
+                if (keep != ALL) {
 #pragma unroll
-            for (int u = 0; u < LG_AHEAD; ++u) {
-                const int at = v + u * 32 * E;
-                work[u] = keep[u] ? concerned(at, E) : 0u;
-                if (keep[u] && (work[u] || !in_place || keep[u] != (1u << E) - 1u)) q[u] = *reinterpret_cast<const uint4*>(x + at);
-            }
-#pragma unroll
-            for (int u = 0; u < LG_AHEAD; ++u) {
-                const int at = v + u * 32 * E;
-                if (at >= ve) break;
-                if (in_place && !work[u] && keep[u] == (1u << E) - 1u) continue;
-                if (keep[u] != (1u << E) - 1u) {
-                    alignas(16) T e[E];
-                    *reinterpret_cast<uint4*>(e) = keep[u] ? q[u] : make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-                    for (int k = 0; k < E; ++k)
-                        if (!(keep[u] >> k & 1u)) e[k] = LgType<T>::put(-INFINITY);
-                    q[u] = *reinterpret_cast<const uint4*>(e);
+                    for (int i = 0; i < E; ++i) if (!(keep >> i & 1u)) q[i] = LgType<T>::put(-INFINITY);
                 }
-                *reinterpret_cast<uint4*>(y + at) = q[u];
-                for (uint32_t m = work[u] & keep[u]; m; m &= m - 1u) {         // few: read again, and stored behind their vector by the thread that stored it
-                    const int v1 = at + __ffs(m) - 1;
-                    y[v1] = LgType<T>::put(value(LgType<T>::get(x[v1]), v1));
-                }
+                *reinterpret_cast<uint4*>(yl + u * 32 * E) = *reinterpret_cast<const uint4*>(q);
             }
+        } else if (!in_place && (((uintptr_t)x ^ (uintptr_t)y) & 15)) {        // the rows lie differently to 16 bytes
+            for (int v = lane; v < n; v += 32) one(v);
+        } else {
+            const int lead = (int)((uintptr_t)y % 16 / sizeof(T)), va = min(n, lead ? E - lead : 0), ve = va + (n - va) / E * E;
+#pragma unroll
+            for (int u = 0; u < VECS; ++u) {
+                const int v = va + (u * 32 + lane) * E;
+                if (v >= ve) break;
+                uint32_t keep = ALL;
+                if (masked) {
+                    keep = keep_s[v >> 5] >> (v & 31);
+                    if ((v & 31) + E > 32) keep |= keep_s[(v >> 5) + 1] << (32 - (v & 31));
+                    keep &= ALL;
+                }
+                if (in_place && keep == ALL) continue;
+                alignas(16) T q[E];
+                if (keep) *reinterpret_cast<uint4*>(q) = *reinterpret_cast<const uint4*>(s + v);
+                if (keep != ALL) {
+#pragma unroll
+                    for (int i = 0; i < E; ++i) if (!(keep >> i & 1u)) q[i] = LgType<T>::put(-INFINITY);
+                }
+                *reinterpret_cast<uint4*>(y + v) = *reinterpret_cast<const uint4*>(q);
+            }
+            if (lane < va) one(lane);
+            if (ve + lane < n) one(ve + lane);
         }
-        if (past) {
-            __syncwarp();
-            for (int i = lane; i < past; i += 32) past_bits[warp][past_list[warp][i] >> 5] = 0u;
-            __syncwarp();
+        __syncwarp();                                  // the stage is free
+    };
+    while (now.left > 0) {
+#pragma unroll
+        for (int stage = 0; stage < LG_STAGES; ++stage) {
+            if (now.left <= 0) break;
+            change(stage);
+            step(now);
+            constexpr int LAST = LG_STAGES - 1;
+            const int free = (stage + LAST) % LG_STAGES;               // (left by the chunk before)
+            ask(asked, next[free], free);
+            step(asked);
+            next[free] = mask_of(ahead);
+            step(ahead);
+            __syncwarp();                              // (its mask too)
         }
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
+DevMade g_lg_attr;
+// entries of words, and of biases and drafts where there are any; bitmap, fronts; the drafts' sets
+int lg_smem_bytes(int bytes, int slice, int entries, int mask_words, bool biases) {
+    return lg_ring(bytes) + entries * (6 + (biases ? 2 : 0) + (mask_words ? 1 : 0)) + slice / 8 + slice / 16 + 4 + 512 * mask_words * mask_words;
 }
 
 template <typename T>
-cudaError_t lg_launch(const LogitsParams& p, dim3 grid, cudaStream_t s) {
-    return launch_pdl(process_logits_kernel<T>, grid, LG_THREADS, (size_t)p.slice * 4 + p.slice / 8 + p.slice * 2, s, p);
+cudaError_t lg_launch(const LogitsParams& p, int bytes, dim3 grid, cudaStream_t s) {
+    const size_t smem = (size_t)lg_smem_bytes(bytes, p.slice, p.entries, p.a.mask_words, p.a.bias_ids != nullptr);
+    return bytes == LG_SHORT ? launch_pdl(process_logits_kernel<T, LG_SHORT>, grid, LG_THREADS, smem, s, p) : launch_pdl(process_logits_kernel<T, LG_CHUNK>, grid, LG_THREADS, smem, s, p);
+}
+template <typename T>
+int lg_attrs(const char* who) {
+    auto set = [&](auto kernel, int bytes) { return cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, lg_smem_bytes(bytes, LG_SLICE, LG_ENTRIES, LG_NODES / 64, true)), who); };
+    return set(process_logits_kernel<T, LG_SHORT>, LG_SHORT) || set(process_logits_kernel<T, LG_CHUNK>, LG_CHUNK) ? WF_ERR_CUDA : WF_OK;
+}
+
+// How many chunks a block takes.  The time of a run in units of what a chunk takes at the memory's rate over all blocks (about 0.19 us): every round of blocks costs its
+// table, and its chunks at least half of that each (what one block alone moves); all of them the memory's rate; and the last block ends half a run behind the others.
+int lg_run(long long rows, long long seqs, long long per_row, long long wave, bool tables, bool whole_rows) {
+    const long long all = rows * per_row, own = (rows + seqs - 1) / seqs * per_row;           // of all, and of a sequence on average
+    long long best = 0, least = 0;
+    auto look = [&](long long run) {
+        if (run < LG_MIN_RUN || run > 1 << 30) return;
+        const long long groups = whole_rows ? (per_row + run - 1) / run * rows : (all + run - 1) / run + (own % run ? seqs / 2 : 0), rounds = (groups + wave - 1) / wave;
+        const long long cost = 2 * rounds * (tables ? LG_TABLE_COST : 4) + std::max(rounds * run, 2 * all / wave) + run;
+        if (!best || cost < least) { best = run; least = cost; }
+    };
+    for (int k = 1; k <= 16; ++k) look((4 * all + k * wave - 1) / (k * wave));
+    for (int k = 1; k <= 16; ++k) look((own + k - 1) / k);
+    return best ? (int)best : LG_MIN_RUN;
 }
 
 }  // namespace
@@ -237,12 +415,14 @@ extern "C" int wf_process_logits(const wf_logits_args* args, void* stream) {
     if (!a.offsets && a.sequences != a.rows) { set_error("%s: %d rows of %d sequences want offsets", who, a.rows, a.sequences); return WF_ERR_INVALID; }
     if (a.sequences > 65534) { set_error("%s: at most 65534 sequences (got %d)", who, a.sequences); return WF_ERR_UNSUPPORTED; }
     if (a.history_width < 0 || a.bias_width < 0 || a.mask_words < 0) { set_error("%s: negative width", who); return WF_ERR_INVALID; }
+    if (a.history_width > 1 << 29) { set_error("%s: a history is at most 2^29 tokens (got %d)", who, a.history_width); return WF_ERR_UNSUPPORTED; }
     if (a.bias_width > 65535) { set_error("%s: at most 65535 biases a sequence (got %d)", who, a.bias_width); return WF_ERR_UNSUPPORTED; }
     if (a.mask_words > LG_NODES / 64) { set_error("%s: at most %d drafts a sequence (got %d words of mask)", who, LG_NODES, a.mask_words); return WF_ERR_UNSUPPORTED; }
     if (a.rows == 0) return WF_OK;
     if (a.history_width == 0) a.history = nullptr;
     if (a.bias_width == 0) a.bias_ids = nullptr;
     if (a.mask_words == 0) a.node_mask = nullptr;
+    if (!a.node_mask) a.mask_words = 0;
     if (!a.logits || !a.out || (a.bias_ids && !a.bias_values) || (a.node_mask && !a.node_tokens)) { set_error("%s: null pointer", who); return WF_ERR_INVALID; }
     if (a.history && a.history_stride < a.history_width && a.sequences > 1) { set_error("%s: history stride %lld below its width %d", who, a.history_stride, a.history_width); return WF_ERR_INVALID; }
     if (a.allowed && a.rows > 1 && a.allowed_stride < (a.vocab + 31) / 32) { set_error("%s: mask stride %lld below its %d words", who, a.allowed_stride, (a.vocab + 31) / 32); return WF_ERR_INVALID; }
@@ -250,16 +430,27 @@ extern "C" int wf_process_logits(const wf_logits_args* args, void* stream) {
     const int es = a.dtype == WF_F32 ? 4 : 2;
     if ((uintptr_t)a.logits % es || (uintptr_t)a.out % es) { set_error("%s: logits are not aligned to their type", who); return WF_ERR_INVALID; }
     if ((uintptr_t)a.node_mask & 7) { set_error("%s: the drafts' masks must be 8-byte aligned", who); return WF_ERR_INVALID; }
-    // slices as wide as leave the GPU two blocks an SM, and shares of a sequence's rows where even whole sequences do not
-    p.slice = LG_SLICE;
-    const long long groups = (long long)a.sequences + (a.offsets ? 1 : 0);
-    auto blocks = [&](int slice) { return ((long long)a.vocab + slice - 1) / slice * groups; };
-    while (p.slice > 512 && blocks(p.slice) < 2ll * sm_count()) p.slice /= 2;
-    p.row_parts = 1;
-    const long long most = a.offsets ? ((long long)a.rows + a.sequences) / (a.sequences + 1) : 1;      // rows of a sequence, about
-    while (p.row_parts < 32 && p.row_parts * 2 * LG_WARPS <= most && blocks(p.slice) * p.row_parts < 4ll * sm_count()) p.row_parts *= 2;
-    const dim3 grid((unsigned)((a.vocab + p.slice - 1) / p.slice), (unsigned)(groups ? groups : 1), (unsigned)p.row_parts);
+    // Entries of a list are at most what the sequence brings, and at most the columns of a slice
+    const long long brings = (a.history ? a.history_width : 0ll) + (a.bias_ids ? a.bias_width : 0) + (a.node_mask ? 64 * a.mask_words : 0);
+    p.tables = brings > 0;
+    // short chunks where the others would not give every warp of an SM one
+    const int bytes = (long long)a.rows * a.vocab * es < (long long)LG_WARPS * sm_count() * LG_CHUNK ? LG_SHORT : LG_CHUNK, chunk = bytes / es;
+    const long long most = brings > LG_ENTRIES ? LG_ENTRIES : LG_SLICE;
+    p.slice = (int)((a.vocab < most ? a.vocab : most) + 511) / 512 * 512;
+    const long long slices = ((long long)a.vocab + p.slice - 1) / p.slice, per_row = p.slice / chunk;
+    const long long seqs = a.offsets ? a.sequences + 1ll : a.sequences;
+    const int full = lg_smem_bytes(bytes, p.slice, (int)(std::min(brings, (long long)p.slice) + 7) / 8 * 8, a.mask_words, a.bias_ids != nullptr);
+    const long long wave = std::max((full + 6144 <= 113 * 1024 ? LG_BLOCKS : 1) * sm_count() / slices, 1ll);
+    p.run = lg_run(a.rows, a.offsets && a.sequences ? a.sequences : seqs, per_row, wave, p.tables, !a.offsets);
+    const long long all = a.rows * per_row;
+    const long long groups = a.offsets ? (all + p.run - 1) / p.run + seqs : (per_row + p.run - 1) / p.run * seqs;        // every sequence's last run may be short
+    const long long columns = a.offsets ? p.slice : std::min((long long)p.slice, (long long)p.run * chunk);
+    p.entries = (int)(std::min(brings, columns) + 7) / 8 * 8;
+    if (groups * slices > 0x7fffffffll || groups > 0x7fffffffll) { set_error("%s: too many rows and columns (%d, %d)", who, a.rows, a.vocab); return WF_ERR_UNSUPPORTED; }
+    p.groups = (int)groups;
+    if (int rc = g_lg_attr.once([&]() -> int { return lg_attrs<float>(who) || lg_attrs<__nv_bfloat16>(who) || lg_attrs<__half>(who) ? WF_ERR_CUDA : WF_OK; })) return rc;
+    const dim3 grid((unsigned)(groups * slices));
     cudaStream_t s = (cudaStream_t)stream;
-    const cudaError_t e = a.dtype == WF_F32 ? lg_launch<float>(p, grid, s) : a.dtype == WF_BF16 ? lg_launch<__nv_bfloat16>(p, grid, s) : lg_launch<__half>(p, grid, s);
+    const cudaError_t e = a.dtype == WF_F32 ? lg_launch<float>(p, bytes, grid, s) : a.dtype == WF_BF16 ? lg_launch<__nv_bfloat16>(p, bytes, grid, s) : lg_launch<__half>(p, bytes, grid, s);
     return launch_check(e, who);
 }
