@@ -6,7 +6,7 @@
 // 128 columns of output; the scores of a group's next tile are under way while a tile's weights are computed:
 //   * more than 128 rows: a group per 128 rows, and every tile serves both;
 //   * up to 128 rows: both groups have the same rows and every other tile; their results are joined in shared memory at the end.
-// Warp 8 loads keys and values by TMA into rings of 64-key tiles (a box of 64 dims per run of keys inside a page); one thread of warps 9 and 10 each issues a
+// Warps 8 and 11 load keys and values by TMA into rings of 64-key tiles (a box of 64 dims per run of keys inside a page); one thread of warps 9 and 10 each issues a
 // group's S = Q K^T (both operands in shared memory) and O += P V (P in TMEM): a wait of one group leaves the other's products running.  The output is rescaled
 // only when a row's maximum has grown by more than 2^8 since the scale was last fixed (exact: the sum carries the same scale).
 // Weights are rounded to bf16, as the products' operands (off by 2^-8 of a weight at most; sums, maxima and outputs are fp32).
@@ -52,7 +52,7 @@ static_assert(2 * PX_REGS_SOFTMAX + PX_REGS_OTHERS == 3 * PX_REGS, "the softmax 
 constexpr int PX_RAW = 3, PX_RAW_TILE = 2 * PX_KEYS * AT_D, PX_SC = 2 * PX_KEYS * 4, PX_STAGES8 = 3;
 constexpr int PX_CONV = 4;                             // converting warps (eight: as fast, at 34.4 us for 31 sequences of 64 and 8 heads over 16003 keys)
 constexpr int PX_SMEM8_USE = 2 * PX_QTILE + PX_STAGES8 * 2 * PX_TILE + PX_RAW * PX_RAW_TILE + PX_STAGES8 * PX_SC;
-constexpr int PX_SMEM8 = PX_SMEM8_USE + 1024;
+constexpr int PX_SMEM8 = PX_SMEM8_USE + 1024, PX_SMEM8_FULL = PX_SMEM8 + PX_SC;      // (one group's queries: their place is one more tile's)
 constexpr int PX_THREADS8 = (11 + PX_CONV) * 32, PX_REGS8 = 128;
 static_assert(PX_SMEM <= 226 * 1024 && PX_SMEM8 <= 226 * 1024 && PX_SMEM_FULL + 1024 <= 226 * 1024, "one block's shared memory");
 constexpr unsigned long long PX_LIMIT_NS = 1000000000ull;
@@ -147,9 +147,10 @@ __device__ __forceinline__ void px_block(const CUtensorMap& tmap, const P& p, un
     const bool alt = rows - row0 <= PX_ROWS;              // the groups have the same rows and every other tile
     const int nt = (key1 - key0 + PX_KEYS - 1) / PX_KEYS;
     const int fix_row = key1 - key0 - (nt - 1) * PX_KEYS;  // rows of the last value tile from here on hold no key: zeroed (a weight of zero times NaN is NaN)
-    const int nst = TREE && !I8 ? (PX_SMEM_FULL - (alt ? 1 : 2) * PX_QTILE) / (2 * PX_TILE) : p.stages, hop = alt ? 2 : 1;           // tiles of a ring; from one tile of a group to its next
+    const int nst = !TREE ? p.stages : I8 ? (alt ? PX_STAGES8 + 1 : PX_STAGES8) : (PX_SMEM_FULL - (alt ? 1 : 2) * PX_QTILE) / (2 * PX_TILE);          // tiles of a ring
+    const int hop = alt ? 2 : 1;                           // from one tile of a group to its next
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    const uint32_t q_s = base, k_s = I8 ? base + 2 * PX_QTILE : base + (TREE ? PX_SMEM_FULL : PX_SMEM_USE) - 2 * nst * PX_TILE, v_s = k_s + nst * PX_TILE;
+    const uint32_t q_s = base, k_s = I8 ? base + (TREE && alt ? 1 : 2) * PX_QTILE : base + (TREE ? PX_SMEM_FULL : PX_SMEM_USE) - 2 * nst * PX_TILE, v_s = k_s + nst * PX_TILE;
     const uint32_t raw_s = v_s + nst * PX_TILE, sc_s = raw_s + PX_RAW * PX_RAW_TILE;       // int8: the pool's tiles; 64 scales of keys and 64 of values of every converted tile
 
     if (tid == 0) {
@@ -157,7 +158,7 @@ __device__ __forceinline__ void px_block(const CUtensorMap& tmap, const P& p, un
             mbar_init(&q_full[i], 4); mbar_init(&o_full[i], 1); mbar_init(&o_end[i], 1); mbar_init(&drained[i], 1);
             for (int u = 0; u < 2; ++u) { mbar_init(&s_full[i][u], 1); mbar_init(&p_full[i][u], 4); }
         }
-        for (int u = 0; u < (TREE ? PX_STAGES_FULL : PX_STAGES); ++u) { mbar_init(&kv_full[u], I8 ? PX_CONV : 1); mbar_init(&kv_empty[u], alt ? 1 : 2); }
+        for (int u = 0; u < (TREE ? PX_STAGES_FULL : PX_STAGES); ++u) { mbar_init(&kv_full[u], I8 ? PX_CONV : 2); mbar_init(&kv_empty[u], alt ? 1 : 2); }
         for (int u = 0; u < PX_RAW; ++u) { mbar_init(&raw_full[u], 1); mbar_init(&raw_empty[u], PX_CONV); }
         mbar_init(&tail_full, 1);
         fence_mbar_init();
@@ -174,37 +175,41 @@ __device__ __forceinline__ void px_block(const CUtensorMap& tmap, const P& p, un
     if (!TREE) wait();                                     // (a tree's block has waited for its lengths)
     pdl_launch_dependents();
 
-    if (!I8 && warp == 11) {
+    if (warp == 8 || (!I8 && warp == 11)) {
         if (!I8 && !FULL) px_regs_dec<PX_REGS_OTHERS>();
-    } else if (warp == 8) {
-        if (!I8 && !FULL) px_regs_dec<PX_REGS_OTHERS>();
-        // ------------------------------------------------------------ producer: lanes 0..3 the boxes of keys, 4..7 of values
-        const int kv = lane >> 2 & 1, off = (lane & 3) * p.box;
-        const int depth = I8 ? PX_RAW : nst, step = I8 ? PX_RAW_TILE : PX_TILE;
+        // ------------------------------------------------------------ producers: warp 8 the boxes of keys and warp 11 those of values, lanes 0..3 (int8: warp 8 all, 4..7 the values')
+        const int kv = I8 ? lane >> 2 & 1 : warp == 11, off = (lane & 3) * p.box;
+        const int depth = I8 ? PX_RAW : nst, tile_bytes = I8 ? PX_RAW_TILE : PX_TILE;
         const uint32_t ring = (I8 ? raw_s + kv * PX_KEYS * AT_D : kv ? v_s : k_s) + off * 128;
         uint64_t *const fulls = I8 ? raw_full : kv_full, *const empties = I8 ? raw_empty : kv_empty;
-        auto here = [&](int i) { return lane < 8 && off < PX_KEYS && key0 + i * PX_KEYS + off < key1; };       // this lane's box of tile i holds keys
-        auto page_of = [&](int i) { return here(i) ? ldcg_i32(table + (key0 + i * PX_KEYS + off) / p.page_size) : 0; };
+        const bool boxed = lane < (I8 ? 8 : 4) && off < PX_KEYS;
+        // this lane's box: its place in a page, and that page's among the range's.  The warp holds 32 entries of the table from `held` on, and the 32 behind them
+        const int first_page = key0 / p.page_size, pages = (key1 - 1) / p.page_size - first_page + 1, per_page = p.layers * 2 * p.Hkv, block0 = (p.layer * 2 + kv) * p.Hkv + kvh;
+        int slot = key0 - first_page * p.page_size + off, at = 0, held = 0;
+        auto entry = [&](int i) { return i < pages ? ldcg_i32(table + first_page + i) : 0; };
+        int entries = entry(lane), behind = entry(32 + lane);
         bool ok = true;
         int st = 0, lap = 0, i = 0;
-        int page = page_of(0), page1 = page_of(1), page2 = page_of(2), page3 = page_of(3);      // a tile's entry is asked for four tiles ahead
         for (; i < nt; ++i) {
-            const int next = page_of(i + 4);
-            const bool mine = here(i), tail = !I8 && i == nt - 1 && fix_row < PX_KEYS;
+            while (slot >= p.page_size) { slot -= p.page_size; ++at; }
+            const int lead = __shfl_sync(0xffffffffu, at, 0);              // (box 0 is the first)
+            if (lead - held >= 32) { entries = behind; held += 32; behind = entry(held + 32 + lane); }
+            const int page0 = __shfl_sync(0xffffffffu, entries, (at - held) & 31), page1 = __shfl_sync(0xffffffffu, behind, (at - held) & 31), page = at - held < 32 ? page0 : page1;
+            const bool mine = boxed && key0 + i * PX_KEYS + off < key1, tail = !I8 && kv && i == nt - 1 && fix_row < PX_KEYS;
             const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, mine));
             uint64_t* full = tail ? &tail_full : &fulls[st];
             if (lap && !px_wait_warp(&empties[st], (uint32_t)((lap & 1) ^ 1))) { ok = false; break; }
             if (lane == 0) mbar_expect_tx(full, boxes * (uint32_t)((I8 ? 1 : 2) * p.box * 128));
             __syncwarp();
             if (mine) {
-                const int slot = (key0 + i * PX_KEYS + off) % p.page_size, block = ((page * p.layers + p.layer) * 2 + kv) * p.Hkv + kvh;
+                const int block = page * per_page + block0;
 #pragma unroll
                 for (int h = 0; h < (I8 ? 1 : 2); ++h)
                     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-                                 ::"r"(ring + st * step + h * PX_HALF), "l"(&tmap), "r"(h * 64), "r"(slot), "r"(block), "r"(smem_u32(full)) : "memory");
+                                 ::"r"(ring + st * tile_bytes + h * PX_HALF), "l"(&tmap), "r"(h * 64), "r"(slot), "r"(block), "r"(smem_u32(full)) : "memory");
             }
             __syncwarp();
-            page = page1; page1 = page2; page2 = page3; page3 = next;
+            slot += PX_KEYS;
             // the other tiles wait until the queries are there, which would queue behind them (the ring's first filling takes all SMs' bandwidth)
             if (i == 1) { px_wait_warp(&q_full[0], 0); if (!alt) px_wait_warp(&q_full[1], 0); }
             if (tail) {                                    // its keyless value rows are cleared before the tile is handed on
@@ -222,7 +227,7 @@ __device__ __forceinline__ void px_block(const CUtensorMap& tmap, const P& p, un
         if (!ok) {                                        // the block leaves early, but not before its copies have landed
             if (lane == 0) *(volatile int*)p.err = 16;
             for (int u = max(0, i - depth); u < i; ++u)
-                if (I8 || u < nt - 1 || fix_row == PX_KEYS) px_wait_warp(&fulls[u % depth], (uint32_t)((u / depth) & 1));
+                if (I8 || !kv || u < nt - 1 || fix_row == PX_KEYS) px_wait_warp(&fulls[u % depth], (uint32_t)((u / depth) & 1));
         }
     } else if (I8 && warp >= 11) {
         // ------------------------------------------------------------ converters: codes to bf16 in the operands' layout, scales beside them

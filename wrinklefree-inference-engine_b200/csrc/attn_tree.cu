@@ -347,9 +347,9 @@ extern "C" int wf_paged_tree_attn(const void* q, const wf_kv_layout* kv, int lay
     if (int rc = px_encode(&tm, kv, p.box, who)) return rc;
     if (int rc = g_tx_attr.once([&]() -> int {
             return cuda_check(cudaFuncSetAttribute(tree_attn_tc_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, PX_SMEM_FULL + 1024), who) ||
-                           cuda_check(cudaFuncSetAttribute(tree_attn_tc_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, PX_SMEM8), who) ? WF_ERR_CUDA : WF_OK;
+                           cuda_check(cudaFuncSetAttribute(tree_attn_tc_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, PX_SMEM8_FULL), who) ? WF_ERR_CUDA : WF_OK;
         })) return rc;
-    const cudaError_t e = p.scales ? launch_pdl(tree_attn_tc_kernel<true>, dim3((unsigned)z.blocks), PX_THREADS8, PX_SMEM8, s, tm, p)
+    const cudaError_t e = p.scales ? launch_pdl(tree_attn_tc_kernel<true>, dim3((unsigned)z.blocks), PX_THREADS8, PX_SMEM8_FULL, s, tm, p)
                                    : launch_pdl(tree_attn_tc_kernel<false>, dim3((unsigned)z.blocks), PX_THREADS, PX_SMEM_FULL + 1024, s, tm, p);
     if (int rc = launch_check(e, "tree_attn_tc")) return rc;
     const long long rows = (long long)tokens * p.G;
