@@ -50,10 +50,12 @@ constexpr int PX_THREADS = 12 * 32, PX_REGS = 112, PX_REGS_SOFTMAX = 128, PX_REG
 static_assert(2 * PX_REGS_SOFTMAX + PX_REGS_OTHERS == 3 * PX_REGS, "the softmax warpgroups take what the third one gives");
 // int8 pools: a ring of tiles as they lie in the pool, and one of converted tiles with their scales
 constexpr int PX_RAW = 3, PX_RAW_TILE = 2 * PX_KEYS * AT_D, PX_SC = 2 * PX_KEYS * 4, PX_STAGES8 = 3;
-constexpr int PX_CONV = 4;                             // converting warps (eight: as fast, at 34.4 us for 31 sequences of 64 and 8 heads over 16003 keys)
+constexpr int PX_CONV = 4;                             // converting warps of a tile; two such sets take the tiles in turn
+constexpr int PX_CONV0 = 12;                           // the first of them
 constexpr int PX_SMEM8_USE = 2 * PX_QTILE + PX_STAGES8 * 2 * PX_TILE + PX_RAW * PX_RAW_TILE + PX_STAGES8 * PX_SC;
 constexpr int PX_SMEM8 = PX_SMEM8_USE + 1024, PX_SMEM8_FULL = PX_SMEM8 + PX_SC;      // (one group's queries: their place is one more tile's)
-constexpr int PX_THREADS8 = (11 + PX_CONV) * 32, PX_REGS8 = 128;
+constexpr int PX_THREADS8 = (PX_CONV0 + 2 * PX_CONV) * 32, PX_REGS8 = 96, PX_REGS8_SOFTMAX = 128, PX_REGS8_OTHERS = 72;
+static_assert(2 * PX_REGS8_SOFTMAX + 3 * PX_REGS8_OTHERS <= 5 * PX_REGS8, "the softmax warpgroups take what the three others give");
 static_assert(PX_SMEM <= 226 * 1024 && PX_SMEM8 <= 226 * 1024 && PX_SMEM_FULL + 1024 <= 226 * 1024, "one block's shared memory");
 constexpr unsigned long long PX_LIMIT_NS = 1000000000ull;
 constexpr float PX_LAZY = 8.f;
@@ -175,8 +177,8 @@ __device__ __forceinline__ void px_block(const CUtensorMap& tmap, const P& p, un
     if (!TREE) wait();                                     // (a tree's block has waited for its lengths)
     pdl_launch_dependents();
 
+    if (warp >= 8) { if (I8) px_regs_dec<PX_REGS8_OTHERS>(); else if (!FULL) px_regs_dec<PX_REGS_OTHERS>(); }
     if (warp == 8 || (!I8 && warp == 11)) {
-        if (!I8 && !FULL) px_regs_dec<PX_REGS_OTHERS>();
         // ------------------------------------------------------------ producers: warp 8 the boxes of keys and warp 11 those of values, lanes 0..3 (int8: warp 8 all, 4..7 the values')
         const int kv = I8 ? lane >> 2 & 1 : warp == 11, off = (lane & 3) * p.box;
         const int depth = I8 ? PX_RAW : nst, tile_bytes = I8 ? PX_RAW_TILE : PX_TILE;
@@ -229,28 +231,36 @@ __device__ __forceinline__ void px_block(const CUtensorMap& tmap, const P& p, un
             for (int u = max(0, i - depth); u < i; ++u)
                 if (I8 || !kv || u < nt - 1 || fix_row == PX_KEYS) px_wait_warp(&fulls[u % depth], (uint32_t)((u / depth) & 1));
         }
-    } else if (I8 && warp >= 11) {
-        // ------------------------------------------------------------ converters: codes to bf16 in the operands' layout, scales beside them
+    } else if (I8 && warp == 11) {                        // only fills its warpgroup
+    } else if (I8 && warp >= PX_CONV0) {
+        // ------------------------------------------------------------ converters: codes to bf16 in the operands' layout, scales beside them; every other tile a set of four warps
         // A thread takes 16 codes of a row at a time.  A quarter of a warp takes four pieces of rows r and r ^ 5: both the swizzled pieces that it reads and those
         // that it writes lie in different banks.
-        const int x = tid - 11 * 32, w = warp - 11;
+        const int set = (warp - PX_CONV0) / PX_CONV, x = tid - (PX_CONV0 + set * PX_CONV) * 32, w = (warp - PX_CONV0) % PX_CONV;
         const int pc = (lane & 3) + 4 * (lane >> 3 & 1), flip = lane >> 2 & 1 ? 5 : 0;
         const int skv = x >> 6, sj = x & 63;               // this thread's scale: of keys or values, of which key
-        auto page_of = [&](int i) { const int j = key0 + i * PX_KEYS + sj; return i < nt && j < key1 ? ldcg_i32(table + j / p.page_size) : -1; };
-        auto scale_of = [&](int i, int page) {
+        // a scale is asked for a tile of this set ahead, its page two; their places are counted on from tile to tile
+        const int page_size = p.page_size, per_page = p.layers * 2 * p.Hkv, block0 = (p.layer * 2 + skv) * p.Hkv + kvh;
+        int key = key0 + set * PX_KEYS + sj, at = key / page_size, slot = key - at * page_size;
+        int page_now = key < key1 ? ldcg_i32(table + at) : -1, slot_now = slot;
+        auto next_page = [&]() { key += 2 * PX_KEYS; slot += 2 * PX_KEYS; while (slot >= page_size) { slot -= page_size; ++at; } return key < key1 ? ldcg_i32(table + at) : -1; };
+        auto scale_at = [&](int page, int s) {
             float v = 0.f;
             if (page >= 0 && page < p.max_pages)           // what is no page reads as zeros, as the copies do
-                asm volatile("ld.global.cg.f32 %0, [%1];" : "=f"(v) : "l"(p.scales + ((((size_t)page * p.layers + p.layer) * 2 + skv) * p.Hkv + kvh) * p.page_size + (key0 + i * PX_KEYS + sj) % p.page_size));
+                asm volatile("ld.global.cg.f32 %0, [%1];" : "=f"(v) : "l"(p.scales + (size_t)(page * per_page + block0) * page_size + s));
             return v;
         };
+        float sc = scale_at(page_now, slot_now);
+        int page1 = next_page(), slot1 = slot;
+        int page2 = next_page(), slot2 = slot;
         bool ok = true;
-        int st = 0, lap = 0, rs = 0, rlap = 0;
-        // a scale is asked for one tile ahead, its page two tiles before that
-        int page1 = page_of(1), page2 = page_of(2);
-        float sc = scale_of(0, page_of(0));
-        for (int i = 0; i < nt; ++i) {
-            const float sc_next = scale_of(i + 1, page1);
-            page1 = page2; page2 = page_of(i + 3);
+        int st = set % nst, rs = set, rlap = 0, lap = 0;
+        for (int i = set; i < nt; i += 2) {
+            const float sc_next = scale_at(page1, slot1);
+            page1 = page2; slot1 = slot2;
+            page2 = next_page(); slot2 = slot;
+            // The tile before in this place of either ring was the other set's: a phase of its barriers is told from the one two before only once that tile is converted
+            if (rlap && !px_wait_warp(&raw_empty[rs], (uint32_t)((rlap - 1) & 1))) { ok = false; break; }
             if (!px_wait_warp(&raw_full[rs], (uint32_t)(rlap & 1)) || (lap && !px_wait_warp(&kv_empty[st], (uint32_t)((lap & 1) ^ 1)))) { ok = false; break; }
             asm volatile("st.shared.f32 [%0], %1;" ::"r"(sc_s + st * PX_SC + x * 4), "f"(sc) : "memory");
 #pragma unroll
@@ -286,12 +296,11 @@ __device__ __forceinline__ void px_block(const CUtensorMap& tmap, const P& p, un
             __syncwarp();
             if (lane == 0) { mbar_arrive(&kv_full[st]); mbar_arrive(&raw_empty[rs]); }
             sc = sc_next;
-            if (++st == nst) { st = 0; ++lap; }
-            if (++rs == PX_RAW) { rs = 0; ++rlap; }
+            if ((st += 2) >= nst) { st -= nst; ++lap; }
+            if ((rs += 2) >= PX_RAW) { rs -= PX_RAW; ++rlap; }
         }
         if (!ok && lane == 0) *(volatile int*)p.err = 19;
     } else if (warp == 9 || warp == 10) {
-        if (!I8 && !FULL) px_regs_dec<PX_REGS_OTHERS>();
         // ------------------------------------------------------------ a group's products
         const int t = warp - 9, tiles = alt ? (nt - t + 1) / 2 : nt;
         uint32_t elected;
@@ -336,7 +345,7 @@ __device__ __forceinline__ void px_block(const CUtensorMap& tmap, const P& p, un
         if (elected) px_commit(&drained[t]);              // nor while a product still reads shared memory or TMEM
         px_wait_warp(&drained[t], 0);
     } else {
-        if (!I8 && !FULL) px_regs_inc<PX_REGS_SOFTMAX>();
+        if (I8) px_regs_inc<PX_REGS8_SOFTMAX>(); else if (!FULL) px_regs_inc<PX_REGS_SOFTMAX>();
         // ------------------------------------------------------------ softmax: a thread per row
         const int t = warp >> 2, tr = (warp & 3) * 32 + lane, r = row0 + (alt ? 0 : t * PX_ROWS) + tr;
         const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;

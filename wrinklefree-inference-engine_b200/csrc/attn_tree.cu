@@ -175,7 +175,7 @@ struct TxParams {
 
     // Row r's weighted values of columns c and c + 1 again, by the whole warp (c is the lane's own), over the keys that it sees alone; m: its maximum
     template <bool I8>
-    __device__ __noinline__ float2 row_again(const PxWork& w, int r, float m, float, int c) const {
+    __device__ __forceinline__ float2 row_again(const PxWork& w, int r, float m, float, int c) const {
         const int lane = threadIdx.x & 31;
         float2 sum = make_float2(0.f, 0.f);
         if (m == -INFINITY) return sum;
