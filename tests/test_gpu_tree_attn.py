@@ -215,6 +215,40 @@ def test_rows_taken_again_are_right():
 
 
 @pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("n", [20, 200])
+def test_a_row_that_sees_nothing_beside_a_hidden_nan(n, int8):
+    """with one block a tile and with several: zeros, whatever the hidden value is"""
+    from wf_bitnet import ops
+    empty = torch.arange(n) % 3 == 1
+    bits = tree_bits(n, torch.Generator().manual_seed(4))
+    bits[:, 0] = True
+    bits[empty] = False
+    a, _ = case([0], [n], 8, 2, 16, int8, 6, bits=[bits])
+    target = a["kv"].scales if int8 else a["kv"].pool
+    target[a["block_table"][0, 0].long(), a["layer"], 1, :, 0] = math.nan
+    out = ops.paged_tree_attn(**a, out_dtype=torch.float32)[:n]
+    assert bool((out[empty.cuda()] == 0).all()) and bool(out[~empty.cuda()].isnan().all())
+
+
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("wide", [False, True])
+def test_many_short_sequences(wide, int8):
+    """a block has many row tiles one after another, of one group's rows and (wide) of two groups', some sequences without any"""
+    g = torch.Generator().manual_seed(11 + wide)
+    nodes = torch.randint(0, 6, (300,), generator=g).tolist()
+    ctx = torch.randint(0, 140, (300,), generator=g).tolist()
+    if wide:
+        for b in range(0, 300, 7):
+            nodes[b] = int(torch.randint(33, 130, (1,), generator=g))
+    check(*case(ctx, nodes, 8, 2, 16, int8, 12, pad=2000))
+
+
+@pytest.mark.parametrize("int8", [False, True])
+def test_a_long_sequence_among_short_ones(int8):
+    check(*case([3, 0, 30011, 64, 7, 9000], [1, 9, 40, 0, 100, 2], 16, 2, 64, int8, 13))
+
+
+@pytest.mark.parametrize("int8", [False, True])
 def test_sequences_without_drafts_and_with_too_many(int8):
     from wf_bitnet import ops
     a, bits = case([50, 20, 30], [0, 70, 9], 8, 2, 16, int8, 3)

@@ -76,7 +76,7 @@ def test_tree_attention_workspace():
     for B, T, H, Hkv, words in ((1, 1, 1, 1, 1), (8, 480, 20, 5, 1), (64, 9000, 64, 8, 4)):
         n = L.wf_tree_attn_workspace_bytes(B, T, H, Hkv, words)
         rows = min(256, -(-64 * words * H // Hkv // 32) * 32)
-        assert 8 * B + 2 * sms * rows * 130 * 4 <= n <= 8 * B + 256 + 2 * sms * rows * 130 * 4
+        assert 2 * sms * rows * 130 * 4 < n <= 2 * sms * (rows * 130 * 4 + 64) + 256
 
 
 def test_accept():

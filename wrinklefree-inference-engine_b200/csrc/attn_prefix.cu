@@ -33,8 +33,8 @@ struct PxParams {
     int behind_own;                // the kernel before is this call's own part, which has waited for what both read
     int* err;                      // the wait word
 
-    template <typename Wait>
-    __device__ __forceinline__ PxWork work(Wait) const {
+    struct Walk {};
+    __device__ __forceinline__ PxWork first(Walk&) const {
         PxWork w;
         w.rows = B * G;
         const int pairs = (w.rows + 2 * PX_ROWS - 1) / (2 * PX_ROWS), pr = blockIdx.x % pairs, split = blockIdx.x / pairs / Hkv;
@@ -46,6 +46,7 @@ struct PxParams {
         w.part = split * Hkv + w.kvh;
         w.part_row0 = 0;
         w.ctx = 0;
+        w.narrow = 0;
         w.table = table;
         return w;
     }

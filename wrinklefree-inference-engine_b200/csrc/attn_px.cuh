@@ -34,6 +34,7 @@ struct PxWork {
     int first;                     // the token of row 0
     int part, part_row0;           // where its results go, and the row that stands there first (part < 0: straight into the output)
     int ctx;                       // trees: keys in front of the drafts
+    int narrow;                    // trees: no share of the call has rows of a second group, whose queries' place is one more tile's
     const int32_t* table;
 };
 
@@ -53,7 +54,7 @@ constexpr int PX_RAW = 3, PX_RAW_TILE = 2 * PX_KEYS * AT_D, PX_SC = 2 * PX_KEYS 
 constexpr int PX_CONV = 4;                             // converting warps of a tile; two such sets take the tiles in turn
 constexpr int PX_CONV0 = 12;                           // the first of them
 constexpr int PX_SMEM8_USE = 2 * PX_QTILE + PX_STAGES8 * 2 * PX_TILE + PX_RAW * PX_RAW_TILE + PX_STAGES8 * PX_SC;
-constexpr int PX_SMEM8 = PX_SMEM8_USE + 1024, PX_SMEM8_FULL = PX_SMEM8 + PX_SC;      // (one group's queries: their place is one more tile's)
+constexpr int PX_SMEM8 = PX_SMEM8_USE + 1024, PX_SMEM8_FULL = PX_SMEM8 + PX_SC;      // (a tile instead of the second group's queries)
 constexpr int PX_THREADS8 = (PX_CONV0 + 2 * PX_CONV) * 32, PX_REGS8 = 96, PX_REGS8_SOFTMAX = 128, PX_REGS8_OTHERS = 72;
 static_assert(2 * PX_REGS8_SOFTMAX + 3 * PX_REGS8_OTHERS <= 5 * PX_REGS8, "the softmax warpgroups take what the three others give");
 static_assert(PX_SMEM <= 226 * 1024 && PX_SMEM8 <= 226 * 1024 && PX_SMEM_FULL + 1024 <= 226 * 1024, "one block's shared memory");
@@ -136,34 +137,74 @@ __device__ __forceinline__ u64 px_sight(const u64* words, int count, int rel, in
     return n < 64 ? see & ((1ull << n) - 1ull) : see;
 }
 
+// such a share, and what follows from it
+struct PxSeg : PxWork {
+    bool alt;                      // the groups have the same rows and every other tile
+    int nt, fix_row;               // tiles; rows of the last value tile from here on hold no key: zeroed (a weight of zero times NaN is NaN)
+    int nst, hop;                  // tiles of a ring; from one tile of a group to its next
+    uint32_t q_s, k_s, v_s, raw_s, sc_s;       // int8: the pool's tiles; 64 scales of keys and 64 of values of every converted tile
+};
+template <bool I8, typename P>
+__device__ __forceinline__ PxSeg px_seg(const PxWork& w, const P& p, uint32_t base) {
+    constexpr bool TREE = P::TREE;
+    PxSeg g;
+    static_cast<PxWork&>(g) = w;
+    g.alt = w.rows - w.row0 <= PX_ROWS;
+    g.nt = (w.key1 - w.key0 + PX_KEYS - 1) / PX_KEYS;
+    g.fix_row = w.key1 - w.key0 - (g.nt - 1) * PX_KEYS;
+    const int queries = TREE && w.narrow ? 1 : 2;
+    g.nst = I8 ? PX_STAGES8 + 2 - queries : TREE ? PX_STAGES_FULL + 1 - queries : p.stages;
+    g.hop = g.alt ? 2 : 1;
+    g.q_s = base;
+    g.k_s = I8 || TREE ? base + queries * PX_QTILE : base + PX_SMEM_USE - 2 * g.nst * PX_TILE;
+    g.v_s = g.k_s + g.nst * PX_TILE;
+    g.raw_s = g.v_s + g.nst * PX_TILE;
+    g.sc_s = g.raw_s + PX_RAW * PX_RAW_TILE;
+    return g;
+}
+
+// a place in a ring and the parity of its lap
+struct PxAt {
+    int st = 0;
+    uint32_t par = 0;
+    __device__ __forceinline__ void step(int n, int size) { st += n; while (st >= size) { st -= size; par ^= 1u; } }
+    __device__ __forceinline__ void leap(int n, int size) { st += n; const int laps = st / size; st -= laps * size; par ^= (uint32_t)laps & 1u; }
+    __device__ __forceinline__ PxAt after(int n, int size) const { PxAt a = *this; a.step(n, size); return a; }
+};
+
+// A block's work: one share (the shared prefix), or, for trees, shares one after another.  Between two of those nothing is drained: warp 8 says what comes next as soon as it has
+// asked for a share's last keys, and each role takes it up when it is through with its own part, the rings and their phases running on.
 template <bool I8, typename P, typename Wait>
 __device__ __forceinline__ void px_block(const CUtensorMap& tmap, const P& p, unsigned char* smem_raw, Wait wait) {
     constexpr bool TREE = P::TREE, FULL = TREE;            // FULL: the block has its SM to itself
-    __shared__ __align__(8) uint64_t q_full[2], kv_full[TREE ? PX_STAGES_FULL : PX_STAGES], kv_empty[TREE ? PX_STAGES_FULL : PX_STAGES], tail_full, raw_full[PX_RAW], raw_empty[PX_RAW], s_full[2][2], p_full[2][2], o_full[2], o_end[2], drained[2];
+    constexpr int STAGES = TREE ? PX_STAGES_FULL : PX_STAGES;
+    constexpr int TAKERS = I8 ? 2 + 8 + 2 * PX_CONV : 3 + 8;        // warps that are told of a share
+    __shared__ __align__(8) uint64_t q_full[3], kv_full[STAGES], kv_empty[STAGES], tail_full, raw_full[PX_RAW], raw_empty[PX_RAW], s_full[2][2], p_full[2][2], o_full[2], o_end[2], drained[2],
+        joint, w_full[2], w_empty[2];
     __shared__ uint32_t tmem_base_s;
+    __shared__ PxWork w_s[2];
+    __shared__ typename P::Walk walk_s;
+    __shared__ int failed_s;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const PxWork w = p.work(wait);                // this block's rows and keys
-    if (w.rows <= 0) return;                               // (the same in all threads)
-    const int rows = w.rows, kvh = w.kvh, row0 = w.row0, key0 = w.key0, key1 = w.key1;
-    const int32_t* table = w.table;
-    const bool alt = rows - row0 <= PX_ROWS;              // the groups have the same rows and every other tile
-    const int nt = (key1 - key0 + PX_KEYS - 1) / PX_KEYS;
-    const int fix_row = key1 - key0 - (nt - 1) * PX_KEYS;  // rows of the last value tile from here on hold no key: zeroed (a weight of zero times NaN is NaN)
-    const int nst = !TREE ? p.stages : I8 ? (alt ? PX_STAGES8 + 1 : PX_STAGES8) : (PX_SMEM_FULL - (alt ? 1 : 2) * PX_QTILE) / (2 * PX_TILE);          // tiles of a ring
-    const int hop = alt ? 2 : 1;                           // from one tile of a group to its next
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    const uint32_t q_s = base, k_s = I8 ? base + (TREE && alt ? 1 : 2) * PX_QTILE : base + (TREE ? PX_SMEM_FULL : PX_SMEM_USE) - 2 * nst * PX_TILE, v_s = k_s + nst * PX_TILE;
-    const uint32_t raw_s = v_s + nst * PX_TILE, sc_s = raw_s + PX_RAW * PX_RAW_TILE;       // int8: the pool's tiles; 64 scales of keys and 64 of values of every converted tile
-
     if (tid == 0) {
+        failed_s = 0;
+        for (int i = 0; i < STAGES; ++i) { mbar_init(&kv_full[i], I8 ? PX_CONV : 2); mbar_init(&kv_empty[i], 2); }
+        for (int i = 0; i < PX_RAW; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], PX_CONV); }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&q_full[i], 4); mbar_init(&o_full[i], 1); mbar_init(&o_end[i], 1); mbar_init(&drained[i], 1);
-            for (int u = 0; u < 2; ++u) { mbar_init(&s_full[i][u], 1); mbar_init(&p_full[i][u], 4); }
+            mbar_init(&q_full[i], 4); mbar_init(&o_full[i], 1); mbar_init(&o_end[i], 1); mbar_init(&drained[i], 1); mbar_init(&w_full[i], 1); mbar_init(&w_empty[i], TAKERS);
+            for (int k = 0; k < 2; ++k) { mbar_init(&s_full[i][k], 1); mbar_init(&p_full[i][k], 4); }
         }
-        for (int u = 0; u < (TREE ? PX_STAGES_FULL : PX_STAGES); ++u) { mbar_init(&kv_full[u], I8 ? PX_CONV : 2); mbar_init(&kv_empty[u], alt ? 1 : 2); }
-        for (int u = 0; u < PX_RAW; ++u) { mbar_init(&raw_full[u], 1); mbar_init(&raw_empty[u], PX_CONV); }
+        mbar_init(&q_full[2], 4);
         mbar_init(&tail_full, 1);
+        mbar_init(&joint, 8);
         fence_mbar_init();
+    }
+    if (TREE) wait();
+    if (warp == 8) {
+        typename P::Walk walk;
+        const PxWork w = p.first(walk);
+        if (lane == 0) { w_s[0] = w; walk_s = walk; }
     }
     if (warp == 9) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_s)), "n"(512) : "memory");
@@ -176,12 +217,46 @@ __device__ __forceinline__ void px_block(const CUtensorMap& tmap, const P& p, un
     const uint32_t tmem = tmem_base_s;
     if (!TREE) wait();                                     // (a tree's block has waited for its lengths)
     pdl_launch_dependents();
+    auto fail = [&](int code) { if (lane == 0) { *(volatile int*)p.err = code; *(volatile int*)&failed_s = 1; } };
+    // A role's part of the shares; run(share, its number): whether all went well
+    auto shares = [&](auto run) {
+        if constexpr (!TREE) {
+            run(px_seg<I8>(w_s[0], p, base), 0);
+        } else {
+            for (int sh = 0;; ++sh) {
+                PxWork& said = w_s[sh & 1];
+                const uint32_t par = (uint32_t)(sh >> 1 & 1);
+                if (sh > 0) {
+                    if (warp == 8) {                       // what comes next: said where all have taken up the share before last
+                        typename P::Walk walk = walk_s;
+                        PxWork w = p.next(walk);           // (the same in all lanes)
+                        if (!px_wait_warp(&w_empty[sh & 1], par ^ 1u)) { fail(20); break; }
+                        if (*(volatile int*)&failed_s) w.rows = 0;
+                        if (lane == 0) { said = w; walk_s = walk; mbar_arrive(&w_full[sh & 1]); }
+                        __syncwarp();
+                    } else if (!px_wait_warp(&w_full[sh & 1], par)) { fail(21); break; }
+                } else if (warp == 8 && lane == 0) mbar_arrive(&w_full[0]);
+                const PxWork w = said;
+                __syncwarp();
+                if (warp != 8 && lane == 0) mbar_arrive(&w_empty[sh & 1]);
+                if (w.rows <= 0 || !run(px_seg<I8>(w, p, base), sh)) break;
+            }
+        }
+    };
 
     if (warp >= 8) { if (I8) px_regs_dec<PX_REGS8_OTHERS>(); else if (!FULL) px_regs_dec<PX_REGS_OTHERS>(); }
     if (warp == 8 || (!I8 && warp == 11)) {
+        PxAt at_ring;
+        int depth = 1;
+        uint32_t tail_par = 0;
+        shares([&](const PxSeg& g, int sh) {
+        const int kvh = g.kvh, key0 = g.key0, key1 = g.key1, nt = g.nt, fix_row = g.fix_row, nst = g.nst;
+        const uint32_t k_s = g.k_s, v_s = g.v_s, raw_s = g.raw_s;
+        const int32_t* table = g.table;
         // ------------------------------------------------------------ producers: warp 8 the boxes of keys and warp 11 those of values, lanes 0..3 (int8: warp 8 all, 4..7 the values')
         const int kv = I8 ? lane >> 2 & 1 : warp == 11, off = (lane & 3) * p.box;
-        const int depth = I8 ? PX_RAW : nst, tile_bytes = I8 ? PX_RAW_TILE : PX_TILE;
+        depth = I8 ? PX_RAW : nst;
+        const int tile_bytes = I8 ? PX_RAW_TILE : PX_TILE;
         const uint32_t ring = (I8 ? raw_s + kv * PX_KEYS * AT_D : kv ? v_s : k_s) + off * 128;
         uint64_t *const fulls = I8 ? raw_full : kv_full, *const empties = I8 ? raw_empty : kv_empty;
         const bool boxed = lane < (I8 ? 8 : 4) && off < PX_KEYS;
@@ -191,8 +266,8 @@ __device__ __forceinline__ void px_block(const CUtensorMap& tmap, const P& p, un
         auto entry = [&](int i) { return i < pages ? ldcg_i32(table + first_page + i) : 0; };
         int entries = entry(lane), behind = entry(32 + lane);
         bool ok = true;
-        int st = 0, lap = 0, i = 0;
-        for (; i < nt; ++i) {
+        for (int i = 0; i < nt; ++i) {
+            const int st = at_ring.st;
             while (slot >= p.page_size) { slot -= p.page_size; ++at; }
             const int lead = __shfl_sync(0xffffffffu, at, 0);              // (box 0 is the first)
             if (lead - held >= 32) { entries = behind; held += 32; behind = entry(held + 32 + lane); }
@@ -200,7 +275,7 @@ __device__ __forceinline__ void px_block(const CUtensorMap& tmap, const P& p, un
             const bool mine = boxed && key0 + i * PX_KEYS + off < key1, tail = !I8 && kv && i == nt - 1 && fix_row < PX_KEYS;
             const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, mine));
             uint64_t* full = tail ? &tail_full : &fulls[st];
-            if (lap && !px_wait_warp(&empties[st], (uint32_t)((lap & 1) ^ 1))) { ok = false; break; }
+            if (!px_wait_warp(&empties[st], at_ring.par ^ 1u)) { ok = false; break; }       // (the first lap finds every place empty)
             if (lane == 0) mbar_expect_tx(full, boxes * (uint32_t)((I8 ? 1 : 2) * p.box * 128));
             __syncwarp();
             if (mine) {
@@ -212,10 +287,12 @@ __device__ __forceinline__ void px_block(const CUtensorMap& tmap, const P& p, un
             }
             __syncwarp();
             slot += PX_KEYS;
-            // the other tiles wait until the queries are there, which would queue behind them (the ring's first filling takes all SMs' bandwidth)
-            if (i == 1) { px_wait_warp(&q_full[0], 0); if (!alt) px_wait_warp(&q_full[1], 0); }
+            // the first share's other tiles wait until the queries are there, which would queue behind them (the ring's first filling takes all SMs' bandwidth)
+            if (i == 1 && sh == 0) { px_wait_warp(&q_full[g.alt ? 2 : 0], 0); if (!g.alt) px_wait_warp(&q_full[1], 0); }
+            at_ring.step(1, depth);
             if (tail) {                                    // its keyless value rows are cleared before the tile is handed on
-                ok = px_wait_warp(&tail_full, 0);
+                ok = px_wait_warp(&tail_full, tail_par);
+                tail_par ^= 1u;
                 for (int c = lane; ok && c < (PX_KEYS - fix_row) * 16; c += 32) {
                     const int h = c / ((PX_KEYS - fix_row) * 8), r = c - h * (PX_KEYS - fix_row) * 8;
                     asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(v_s + st * PX_TILE + h * PX_HALF + (fix_row * 8 + r) * 16), "r"(0u) : "memory");
@@ -224,15 +301,19 @@ __device__ __forceinline__ void px_block(const CUtensorMap& tmap, const P& p, un
                 __syncwarp();
                 if (ok && lane == 0) mbar_arrive(&kv_full[st]);
             }
-            if (++st == depth) { st = 0; ++lap; }
         }
-        if (!ok) {                                        // the block leaves early, but not before its copies have landed
-            if (lane == 0) *(volatile int*)p.err = 16;
-            for (int u = max(0, i - depth); u < i; ++u)
-                if (I8 || !kv || u < nt - 1 || fix_row == PX_KEYS) px_wait_warp(&fulls[u % depth], (uint32_t)((u / depth) & 1));
-        }
+        if (!ok) fail(16);
+        return ok;
+        });
+        // a block that leaves early does so only when its copies have landed (places never used: the phase before the first)
+        for (int u = 0; u < depth; ++u, at_ring.step(1, depth)) px_wait_warp(&(I8 ? raw_full : kv_full)[at_ring.st], at_ring.par ^ 1u);
     } else if (I8 && warp == 11) {                        // only fills its warpgroup
     } else if (I8 && warp >= PX_CONV0) {
+        PxAt raw0, kv0;                                    // where a share begins in either ring
+        shares([&](const PxSeg& g, int) {
+        const int kvh = g.kvh, key0 = g.key0, key1 = g.key1, nt = g.nt, nst = g.nst;
+        const uint32_t k_s = g.k_s, v_s = g.v_s, raw_s = g.raw_s, sc_s = g.sc_s;
+        const int32_t* table = g.table;
         // ------------------------------------------------------------ converters: codes to bf16 in the operands' layout, scales beside them; every other tile a set of four warps
         // A thread takes 16 codes of a row at a time.  A quarter of a warp takes four pieces of rows r and r ^ 5: both the swizzled pieces that it reads and those
         // that it writes lie in different banks.
@@ -254,14 +335,14 @@ __device__ __forceinline__ void px_block(const CUtensorMap& tmap, const P& p, un
         int page1 = next_page(), slot1 = slot;
         int page2 = next_page(), slot2 = slot;
         bool ok = true;
-        int st = set % nst, rs = set, rlap = 0, lap = 0;
+        PxAt raw = raw0.after(set, PX_RAW), kvt = kv0.after(set, nst);
         for (int i = set; i < nt; i += 2) {
             const float sc_next = scale_at(page1, slot1);
             page1 = page2; slot1 = slot2;
             page2 = next_page(); slot2 = slot;
+            const int rs = raw.st, st = kvt.st;
             // The tile before in this place of either ring was the other set's: a phase of its barriers is told from the one two before only once that tile is converted
-            if (rlap && !px_wait_warp(&raw_empty[rs], (uint32_t)((rlap - 1) & 1))) { ok = false; break; }
-            if (!px_wait_warp(&raw_full[rs], (uint32_t)(rlap & 1)) || (lap && !px_wait_warp(&kv_empty[st], (uint32_t)((lap & 1) ^ 1)))) { ok = false; break; }
+            if (!px_wait_warp(&raw_empty[rs], raw.par ^ 1u) || !px_wait_warp(&raw_full[rs], raw.par) || !px_wait_warp(&kv_empty[st], kvt.par ^ 1u)) { ok = false; break; }
             asm volatile("st.shared.f32 [%0], %1;" ::"r"(sc_s + st * PX_SC + x * 4), "f"(sc) : "memory");
 #pragma unroll
             for (int kv = 0; kv < 2; ++kv) {
@@ -296,56 +377,82 @@ __device__ __forceinline__ void px_block(const CUtensorMap& tmap, const P& p, un
             __syncwarp();
             if (lane == 0) { mbar_arrive(&kv_full[st]); mbar_arrive(&raw_empty[rs]); }
             sc = sc_next;
-            if ((st += 2) >= nst) { st -= nst; ++lap; }
-            if ((rs += 2) >= PX_RAW) { rs -= PX_RAW; ++rlap; }
+            kvt.step(2, nst);
+            raw.step(2, PX_RAW);
         }
-        if (!ok && lane == 0) *(volatile int*)p.err = 19;
+        raw0.leap(nt, PX_RAW);
+        kv0.leap(nt, nst);
+        if (!ok) fail(19);
+        return ok;
+        });
     } else if (warp == 9 || warp == 10) {
-        // ------------------------------------------------------------ a group's products
-        const int t = warp - 9, tiles = alt ? (nt - t + 1) / 2 : nt;
+        PxAt kv0;                                          // where a share begins in the ring
+        int tile0 = 0;                                     // tiles of the group's in the shares before: its buffers go on in turn
+        uint32_t q_alt = 0, q_two = 0;                     // parities of the shares of one group's rows and of two groups' (who waits for a barrier waits for all of its phases)
         uint32_t elected;
         asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(elected));
+        shares([&](const PxSeg& g, int) {
+        const int nt = g.nt, nst = g.nst, hop = g.hop;
+        const uint32_t q_s = g.q_s, k_s = g.k_s, v_s = g.v_s;
+        const bool alt = g.alt;
+        // ------------------------------------------------------------ a group's products
+        const int t = warp - 9, tiles = alt ? (nt - t + 1) / 2 : nt;
         constexpr uint32_t idesc_s = px_idesc(PX_KEYS, 0), idesc_o = px_idesc(AT_D, 1);
         const uint64_t qd = px_desc(q_s + (alt ? 0 : t) * PX_QTILE, 16), kd0 = px_desc(k_s, 16), vd0 = px_desc(v_s, PX_HALF);
         const uint32_t s_t = tmem + t * 256, o_t = s_t + 128;
-        int kst = alt ? t : 0, vst = kst;
-        uint32_t par = 0;
-        bool ok = px_wait_warp(&q_full[alt ? 0 : t], 0);
+        PxAt kt = kv0.after(alt ? t : 0, nst), vt = kt;
+        bool ok = px_wait_warp(&q_full[alt ? 2 : t], alt ? q_alt : q_two);
+        if (alt) q_alt ^= 1u; else q_two ^= 1u;
         for (int n = -1; n < tiles && ok; ++n) {
+            const int now = tile0 + n, next = now + 1;
             if (n + 1 < tiles) {                          // the next tile's scores, into the buffer that the values before last have left
-                if (!px_wait_warp(&kv_full[kst], par)) { ok = false; break; }
+                if (!px_wait_warp(&kv_full[kt.st], kt.par)) { ok = false; break; }
                 tc_fence_after();
                 if (elected) {
-                    const uint64_t kd = kd0 + (uint64_t)(kst * (PX_TILE >> 4));
+                    const uint64_t kd = kd0 + (uint64_t)(kt.st * (PX_TILE >> 4));
 #pragma unroll
                     for (int ks = 0; ks < 8; ++ks)
-                        px_mma_ss(s_t + ((n + 1) & 1) * PX_KEYS, qd + (uint64_t)((ks >> 2) * (PX_QHALF >> 4) + (ks & 3) * 2), kd + (uint64_t)((ks >> 2) * (PX_HALF >> 4) + (ks & 3) * 2), idesc_s,
+                        px_mma_ss(s_t + (next & 1) * PX_KEYS, qd + (uint64_t)((ks >> 2) * (PX_QHALF >> 4) + (ks & 3) * 2), kd + (uint64_t)((ks >> 2) * (PX_HALF >> 4) + (ks & 3) * 2), idesc_s,
                                   ks ? 1u : 0u);
-                    px_commit(&s_full[t][(n + 1) & 1]);
+                    px_commit(&s_full[t][next & 1]);
                 }
                 __syncwarp();
-                if ((kst += hop) >= nst) { kst -= nst; par ^= 1; }
+                kt.step(hop, nst);
             }
             if (n >= 0) {
-                if (!px_wait_warp(&p_full[t][n & 1], (uint32_t)((n >> 1) & 1))) { ok = false; break; }
+                if (!px_wait_warp(&p_full[t][now & 1], (uint32_t)(now >> 1 & 1))) { ok = false; break; }
                 tc_fence_after();
                 if (elected) {
-                    const uint64_t vd = vd0 + (uint64_t)(vst * (PX_TILE >> 4));
+                    const uint64_t vd = vd0 + (uint64_t)(vt.st * (PX_TILE >> 4));
 #pragma unroll
-                    for (int ks = 0; ks < PX_KEYS / 16; ++ks) px_mma_ts(o_t, s_t + (n & 1) * PX_KEYS + ks * 8, vd + (uint64_t)(ks * 128), idesc_o, n || ks ? 1u : 0u);   // 16 keys = 2048 bytes
+                    for (int ks = 0; ks < PX_KEYS / 16; ++ks) px_mma_ts(o_t, s_t + (now & 1) * PX_KEYS + ks * 8, vd + (uint64_t)(ks * 128), idesc_o, n || ks ? 1u : 0u);   // 16 keys = 2048 bytes
                     px_commit(n == tiles - 1 ? &o_end[t] : &o_full[t]);
-                    px_commit(&kv_empty[vst]);
+                    px_commit(&kv_empty[vt.st]);
+                    if (alt) px_commit(&kv_empty[vt.st]);  // (for the other group, which does not read it)
                 }
                 __syncwarp();
-                if ((vst += hop) >= nst) vst -= nst;
+                vt.step(hop, nst);
             }
         }
-        if (!ok && lane == 0) *(volatile int*)p.err = 17;
+        if (tiles == 0 && elected) px_commit(&o_end[t]);
         __syncwarp();
-        if (elected) px_commit(&drained[t]);              // nor while a product still reads shared memory or TMEM
-        px_wait_warp(&drained[t], 0);
+        kv0.leap(nt, nst);
+        tile0 += tiles;
+        if (!ok) fail(17);
+        return ok;
+        });
+        __syncwarp();
+        if (elected) px_commit(&drained[warp - 9]);       // nor while a product still reads shared memory or TMEM
+        px_wait_warp(&drained[warp - 9], 0);
     } else {
         if (I8) px_regs_inc<PX_REGS8_SOFTMAX>(); else if (!FULL) px_regs_inc<PX_REGS_SOFTMAX>();
+        PxAt kv0;                                          // as the products'
+        int tile0 = 0;
+        uint32_t o_par = 0;                                // the parity of the shares' o_full before
+        shares([&](const PxSeg& w, int sh) {
+        const int rows = w.rows, kvh = w.kvh, row0 = w.row0, key0 = w.key0, key1 = w.key1, nt = w.nt, fix_row = w.fix_row, nst = w.nst, hop = w.hop;
+        const uint32_t q_s = w.q_s, sc_s = w.sc_s;
+        const bool alt = w.alt;
         // ------------------------------------------------------------ softmax: a thread per row
         const int t = warp >> 2, tr = (warp & 3) * 32 + lane, r = row0 + (alt ? 0 : t * PX_ROWS) + tr;
         const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
@@ -373,26 +480,27 @@ __device__ __forceinline__ void px_block(const CUtensorMap& tmap, const P& p, un
                              "r"(v[i].x ^ sign), "r"(v[i].y ^ sign), "r"(v[i].z ^ sign), "r"(v[i].w ^ sign) : "memory");
             fence_proxy_async();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&q_full[t]);
+            if (lane == 0) mbar_arrive(&q_full[alt ? 2 : t]);
         }
         const u64* mask_row = nullptr;                     // the row's drafts
         if constexpr (TREE) mask_row = r_ok ? p.mask + (size_t)(w.first + r / p.G) * p.words : nullptr;
         float m_ref = -INFINITY, l = 0.f;                 // scores in units of log 2
-        int sst = alt ? t : 0;                             // int8: the converted tile that holds the scales
+        PxAt sc_at = kv0.after(alt ? t : 0, nst);          // int8: the converted tile that holds the scales
         bool ok = true;
         for (int n = 0; n < tiles && ok; ++n) {
-            const uint32_t s_n = s_t + (n & 1) * PX_KEYS;
-            if (!px_wait_warp(&s_full[t][n & 1], (uint32_t)((n >> 1) & 1))) { ok = false; break; }
+            const int buf = (tile0 + n) & 1;
+            const uint32_t s_n = s_t + buf * PX_KEYS;
+            if (!px_wait_warp(&s_full[t][buf], (uint32_t)((tile0 + n) >> 1 & 1))) { ok = false; break; }
             tc_fence_after();
             if (idle) {
-                if (lane == 0) mbar_arrive(&p_full[t][n & 1]);
+                if (lane == 0) mbar_arrive(&p_full[t][buf]);
                 continue;
             }
             uint32_t s[PX_KEYS];
             TC_LD32(s_n, (s + 0));
             TC_LD32(s_n + 32, (s + 32));
             asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-            const uint32_t sc_n = sc_s + (I8 ? sst * PX_SC : 0);
+            const uint32_t sc_n = sc_s + (I8 ? sc_at.st * PX_SC : 0);
             if (I8) {                                     // the keys' scales; those of keys that are none are 0
 #pragma unroll
                 for (int c = 0; c < PX_KEYS; c += 4) {
@@ -401,7 +509,7 @@ __device__ __forceinline__ void px_block(const CUtensorMap& tmap, const P& p, un
                     const uint64_t a = px_mul2(px_pair(s[c], s[c + 1]), px_pair(k[0], k[1])), b = px_mul2(px_pair(s[c + 2], s[c + 3]), px_pair(k[2], k[3]));
                     s[c] = (uint32_t)a; s[c + 1] = (uint32_t)(a >> 32); s[c + 2] = (uint32_t)b; s[c + 3] = (uint32_t)(b >> 32);
                 }
-                if ((sst += hop) >= nst) sst -= nst;
+                sc_at.step(hop, nst);
             }
             const int tile = n * hop + (alt ? t : 0);
             if constexpr (TREE) {                         // a tile that reaches the drafts: those that the row's mask has, and no key behind the last one
@@ -451,7 +559,7 @@ __device__ __forceinline__ void px_block(const CUtensorMap& tmap, const P& p, un
             }
             TC_ST32(s_n, s);
             if (n > 0 && __any_sync(0xffffffffu, corr != 1.f)) {
-                if (!px_wait_warp(&o_full[t], (uint32_t)((n - 1) & 1))) { ok = false; break; }      // the scores above came behind all values but the last tile's
+                if (!px_wait_warp(&o_full[t], o_par ^ (uint32_t)((n - 1) & 1))) { ok = false; break; }      // the scores above came behind all values but the last tile's
                 tc_fence_after();
 #pragma unroll 1
                 for (int c = 0; c < AT_D; c += 32) {
@@ -466,36 +574,37 @@ __device__ __forceinline__ void px_block(const CUtensorMap& tmap, const P& p, un
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[t][n & 1]);
+            if (lane == 0) mbar_arrive(&p_full[t][buf]);
             float l0, l1;
             px_unpair(px_add2(ls[0], ls[1]), l0, l1);
             l += l0 + l1;
         }
-        // ---- the group's output.  Groups of the same rows hand each other a half of the columns through the ring, when no product reads it any more, and each
-        // finishes the half that it keeps
+        if (tiles > 0) o_par ^= (uint32_t)(tiles - 1) & 1u;
+        tile0 += tiles;
+        kv0.leap(nt, nst);
+        // ---- the group's output.  Groups of the same rows tell each other their maxima and sums, and each finishes a half of the columns: its lanes of tensor memory are the
+        // other's too
         const bool joined = alt && nt > 1;
-        if (ok && tiles > 0) ok = px_wait_warp(&o_end[t], 0);
-        if (joined && ok) ok = px_wait_warp(&o_end[1 - t], 0);
+        if (ok) ok = px_wait_warp(&o_end[t], (uint32_t)(sh & 1));
         tc_fence_after();
-        const uint32_t ml_s = k_s + 2 * PX_ROWS * 256 + tr * 8;
-        const uint32_t mine = k_s + (uint32_t)t * PX_ROWS * 256 + tr * 16, theirs = k_s + (uint32_t)(1 - t) * PX_ROWS * 256 + tr * 16;
-        if (joined && ok && !idle) {
-            uint32_t o[64];
-            TC_LD32(o_t + (1 - t) * 64, (o + 0));
-            TC_LD32(o_t + (1 - t) * 64 + 32, (o + 32));
-            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-            for (int k = 0; k < 64; k += 4)
-                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(mine + (k >> 2) * PX_ROWS * 16), "r"(o[k]), "r"(o[k + 1]), "r"(o[k + 2]), "r"(o[k + 3]) : "memory");
-            asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(ml_s + t * PX_ROWS * 8), "f"(m_ref), "f"(l) : "memory");
+        if (joined) {                                      // (by way of tensor memory, where the group's scores were)
+            if (ok && !idle) {
+                asm volatile("tcgen05.st.sync.aligned.32x32b.x2.b32 [%0], {%1, %2};" ::"r"(s_t), "f"(m_ref), "f"(l) : "memory");
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (ok && lane == 0) mbar_arrive(&joint);
+            if (ok) ok = px_wait_warp(&joint, 0);
+            tc_fence_after();
         }
-        if (joined) asm volatile("bar.sync 1, 256;" ::: "memory");
         if (ok && !idle && (t == 0 || joined || !alt)) {
             float4* dst = reinterpret_cast<float4*>(p.part_o) + (size_t)w.part * 32 * p.rows_p + (r - w.part_row0);      // rows side by side: a warp's stores are whole lines
             float f0 = 1.f, f1 = 0.f;
             if (joined) {
                 float2 ml;
-                asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(ml.x), "=f"(ml.y) : "r"(ml_s + (1 - t) * PX_ROWS * 8) : "memory");
+                asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0, %1}, [%2];" : "=f"(ml.x), "=f"(ml.y) : "r"(tmem + (1 - t) * 256 + lane_base) : "memory");
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
                 const float m = fmaxf(m_ref, ml.x);
                 f0 = m_ref == -INFINITY ? 0.f : px_ex2(m_ref - m);
                 f1 = ml.x == -INFINITY ? 0.f : px_ex2(ml.x - m);
@@ -510,14 +619,14 @@ __device__ __forceinline__ void px_block(const CUtensorMap& tmap, const P& p, un
                 TC_LD32(o_t + c + 32, (o + 32));
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
                 if (joined) {
+                    const uint32_t theirs = tmem + (1 - t) * 256 + 128 + lane_base + c;
 #pragma unroll
-                    for (int k = 0; k < 64; k += 4) {
-                        float4 w;
-                        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(w.x), "=f"(w.y), "=f"(w.z), "=f"(w.w) : "r"(theirs + (k >> 2) * PX_ROWS * 16) : "memory");
-                        o[k] = __float_as_uint(fmaf(__uint_as_float(o[k]), f0, w.x * f1));
-                        o[k + 1] = __float_as_uint(fmaf(__uint_as_float(o[k + 1]), f0, w.y * f1));
-                        o[k + 2] = __float_as_uint(fmaf(__uint_as_float(o[k + 2]), f0, w.z * f1));
-                        o[k + 3] = __float_as_uint(fmaf(__uint_as_float(o[k + 3]), f0, w.w * f1));
+                    for (int h = 0; h < 64; h += 32) {
+                        uint32_t x[32];
+                        TC_LD32(theirs + h, x);
+                        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) o[h + k] = __float_as_uint(fmaf(__uint_as_float(o[h + k]), f0, __uint_as_float(x[k]) * f1));
                     }
                 }
                 bool mine_ok = r_ok;
@@ -531,7 +640,7 @@ __device__ __forceinline__ void px_block(const CUtensorMap& tmap, const P& p, un
                     for (; again; again &= again - 1u) {
                         const int who = __ffs(again) - 1, rr = r - lane + who;
                         const float2 v = p.template row_again<I8>(w, rr, __shfl_sync(0xffffffffu, m_ref, who), unit, c + 2 * lane);
-                        const float inv = 1.f / __shfl_sync(0xffffffffu, l, who);
+                        const float l_who = __shfl_sync(0xffffffffu, l, who), inv = l_who > 0.f ? 1.f / l_who : 0.f;
                         if (w.part < 0) p.store2(w, rr, c + 2 * lane, v.x * inv, v.y * inv);
                         else reinterpret_cast<float2*>(p.part_o)[(((size_t)w.part * 32 + ((c + 2 * lane) >> 2)) * p.rows_p + (rr - w.part_row0)) * 2 + (lane & 1)] = v;
                     }
@@ -547,7 +656,15 @@ __device__ __forceinline__ void px_block(const CUtensorMap& tmap, const P& p, un
             }
             if (r_ok && (t == 0 || !alt) && (!TREE || w.part >= 0)) reinterpret_cast<float2*>(p.part_ml)[(size_t)w.part * p.rows_p + (r - w.part_row0)] = make_float2(m_ref, l);
         }
-        if (!ok && lane == 0) *(volatile int*)p.err = 18;
+        if (TREE && joined && ok) {                       // nor does a group go on while the other still reads its results
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&joint);
+            ok = px_wait_warp(&joint, 1);
+        }
+        if (!ok) fail(18);
+        return ok;
+        });
     }
     __syncwarp();
     tc_fence_before();
