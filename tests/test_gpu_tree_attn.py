@@ -317,6 +317,21 @@ def test_the_same_page_twice():
     check(a, bits)
 
 
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("page", [-1, 40000, 2**29, 2**31 - 1, -2**31])
+def test_what_is_no_page_reads_as_zeros(page, int8):
+    """numbers beyond the pool, 2^29 among them, which times the 8 heads' rows of a page here is 0 in 32 bits"""
+    from wf_bitnet import ops
+    a, _ = case([96, 40], [10, 10], 8, 2, 16, int8)
+    blank = int(a["block_table"][0, 3])
+    a["kv"].pool[blank] = 128 if int8 else 0
+    if int8:
+        a["kv"].scales[blank] = 0.0
+    want = ops.paged_tree_attn(**a)
+    a["block_table"][0, 3] = page
+    assert torch.equal(ops.paged_tree_attn(**a), want)
+
+
 def test_a_table_that_ends_inside_the_drafts():
     """the keys end with the table's row: nothing behind it is read"""
     from wf_bitnet import ops

@@ -279,7 +279,7 @@ __device__ __forceinline__ void px_block(const CUtensorMap& tmap, const P& p, un
             if (lane == 0) mbar_expect_tx(full, boxes * (uint32_t)((I8 ? 1 : 2) * p.box * 128));
             __syncwarp();
             if (mine) {
-                const int block = page * per_page + block0;
+                const int block = (unsigned)page < (unsigned)p.max_pages ? page * per_page + block0 : -1;      // what is no page reads as zeros
 #pragma unroll
                 for (int h = 0; h < (I8 ? 1 : 2); ++h)
                     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"

@@ -6,7 +6,7 @@
 //
 // A block has a run of a sequence's logits, row after row.  It first notes the tokens there that the history, the drafts or a bias concerns: a bitmap, the number of them in
 // front of each word of it, and so the place of each token's own word (times drawn, whether seen) in a list as long as there are such tokens.  All of it are whole numbers whose
-// order of arrival does not show.  Meanwhile the first logits are on their way: each warp moves chunks of 2 KB through a ring of its own in shared memory, three deep,
+// order of arrival does not show.  Meanwhile the first logits are on their way: each warp moves chunks of 2 KB (of 512 bytes where there are few) through a ring of two in shared memory,
 // changes its listed tokens there, a lane each, and masks on the way out.  A draft's own past, which differs from row to row, is the common bits of its mask and of a set
 // of drafts for each listed token.
 //
