@@ -7,8 +7,8 @@
 //
 // Bound by memory: (2 H + 4 Hkv) D 2 bytes a token are read and written once.  D / 8 lanes have a head, each the 8 numbers of four pairs, so that the rotation is a
 // lane's own business: with pairs (i, i + R/2) lane l < R/8 has 4l.. and R/2 + 4l.. of the head (8 bytes each), the others 8 in a row.  A warp has a token, where there are
-// many, and asks for the next heads ahead of working on these: 16384 tokens of 32 + 8 heads 79.5 us (5.1 TB/s; the bytes alone 62), without that 88, with twice as many heads a
-// time 87, with warps that go on from token to token 94.
+// many, and asks for the next heads ahead of working on these: 16384 tokens of 32 + 8 heads 73.5 us (5.5 TB/s; the bytes alone 62), in blocks of 256 threads 79 (the last ones run
+// alone), of 64 76; without the loads ahead 88, with twice as many heads a time 87, with half a token 84, with warps that go on from token to token 94.
 #include "attn_chunks.cuh"
 #include "kv8.cuh"
 #include "wf_bitnet.h"
@@ -34,7 +34,7 @@ struct AppendParams {
     int chunk, chunks;                                 // heads of a warp's share of a token, and shares of a token
 };
 
-constexpr int QA_THREADS = 256;
+constexpr int QA_THREADS = 128;
 constexpr int QA_AHEAD = 2;                            // rounds of heads whose loads are under way while as many are worked on
 
 __device__ __forceinline__ void qa_load4(const void* tab, int bf16, size_t at, float (&v)[4]) {
@@ -46,6 +46,14 @@ __device__ __forceinline__ void qa_load4(const void* tab, int bf16, size_t at, f
         v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w;
     }
 }
+
+// two floats at a time
+typedef unsigned long long u64;
+__device__ __forceinline__ u64 qa_pair(float a, float b) { u64 v; asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); return v; }
+__device__ __forceinline__ float qa_lo(u64 v) { return __uint_as_float((uint32_t)v); }
+__device__ __forceinline__ float qa_hi(u64 v) { return __uint_as_float((uint32_t)(v >> 32)); }
+__device__ __forceinline__ u64 qa_mul(u64 a, u64 b) { u64 v; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b)); return v; }
+__device__ __forceinline__ u64 qa_fma(u64 a, u64 b, u64 c) { u64 v; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c)); return v; }
 
 // A warp takes `chunk` heads of one token, 32 / (D / 8) at a time.
 template <int D, bool I8, bool PAIRS>
@@ -76,10 +84,16 @@ __global__ void __launch_bounds__(QA_THREADS) norm_rope_append_kernel(const __gr
     ask(h0);
     const bool bad = pos < 0 || pos >= p.max_pos;
     const bool held = !bad && page >= 0 && page < p.max_pages && slot >= 0 && slot < p.page_size;
-    float cs[4] = {1.f, 1.f, 1.f, 1.f}, sn[4] = {0.f, 0.f, 0.f, 0.f}, g[2][8];
-    if (turned && !bad) {
-        qa_load4(p.cos_tab, p.tab_bf16, (size_t)pos * (p.rot / 2) + 4 * l, cs);
-        qa_load4(p.sin_tab, p.tab_bf16, (size_t)pos * (p.rot / 2) + 4 * l, sn);
+    // what belongs to the lane's pairs, two pairs in a word: (0, 1) and (2, 3); of gains the pairs' first and second numbers'
+    u64 cs[2], sn[2], minus_sn[2], ga[2][2], gb[2][2];
+    {
+        float c[4] = {1.f, 1.f, 1.f, 1.f}, s[4] = {0.f, 0.f, 0.f, 0.f};
+        if (turned && !bad) {
+            qa_load4(p.cos_tab, p.tab_bf16, (size_t)pos * (p.rot / 2) + 4 * l, c);
+            qa_load4(p.sin_tab, p.tab_bf16, (size_t)pos * (p.rot / 2) + 4 * l, s);
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) { cs[k] = qa_pair(c[2 * k], c[2 * k + 1]); sn[k] = qa_pair(s[2 * k], s[2 * k + 1]); minus_sn[k] = qa_pair(-s[2 * k], -s[2 * k + 1]); }
     }
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
@@ -87,8 +101,14 @@ __global__ void __launch_bounds__(QA_THREADS) norm_rope_append_kernel(const __gr
         float a[4] = {1.f, 1.f, 1.f, 1.f}, b[4] = {1.f, 1.f, 1.f, 1.f};
         if (gain) { qa_load4(gain, p.norm_bf16, c0, a); qa_load4(gain, p.norm_bf16, c1, b); }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) { g[w][k] = a[k]; g[w][4 + k] = b[k]; }
+        for (int k = 0; k < 2; ++k) {
+            ga[w][k] = !PAIRS ? qa_pair(a[2 * k], a[2 * k + 1]) : k ? qa_pair(b[0], b[2]) : qa_pair(a[0], a[2]);
+            gb[w][k] = !PAIRS ? qa_pair(b[2 * k], b[2 * k + 1]) : k ? qa_pair(b[1], b[3]) : qa_pair(a[1], a[3]);
+        }
     }
+    __nv_bfloat16* const q = p.q_out + (size_t)t * p.H * D;
+    const size_t row0 = held ? ((size_t)page * p.layers + p.layer) * 2 * p.Hkv * p.page_size + slot : 0;       // the keys' first head's; values' heads follow the keys'
+    const bool norms = p.q_norm || p.k_norm;
     for (int hb = h0; hb < h1; hb += AT_ONCE * QA_AHEAD) {
 #pragma unroll
         for (int u = 0; u < QA_AHEAD; ++u) { in[u][0] = ahead[u][0]; in[u][1] = ahead[u][1]; }
@@ -98,36 +118,50 @@ __global__ void __launch_bounds__(QA_THREADS) norm_rope_append_kernel(const __gr
             const int h = hb + u * AT_ONCE + sub, which = h < p.H ? 0 : h < p.H + p.Hkv ? 1 : 2;     // query, key, value
             if (hb + u * AT_ONCE >= h1) break;
             uint2 o0 = in[u][0], o1 = in[u][1];
-            float x[8] = {bf16lo(o0.x), bf16hi(o0.x), bf16lo(o0.y), bf16hi(o0.y), bf16lo(o1.x), bf16hi(o1.x), bf16lo(o1.y), bf16hi(o1.y)};
-            float ss = 0.f;
+            u64 a[2], b[2];                                // the lane's pairs
 #pragma unroll
-            for (int k = 0; k < 8; ++k) ss = fmaf(x[k], x[k], ss);
+            for (int k = 0; k < 2; ++k) {
+                const uint32_t one = k ? o0.y : o0.x, two = k ? o1.y : o1.x, even = k ? o1.x : o0.x, odd = k ? o1.y : o0.y;
+                a[k] = PAIRS ? qa_pair(bf16lo(even), bf16lo(odd)) : qa_pair(bf16lo(one), bf16hi(one));
+                b[k] = PAIRS ? qa_pair(bf16hi(even), bf16hi(odd)) : qa_pair(bf16lo(two), bf16hi(two));
+            }
+            float inv = 1.f;
+            if (norms && hb + u * AT_ONCE < p.H + p.Hkv) { // (not for values alone)
+                const u64 sq = qa_fma(b[1], b[1], qa_fma(b[0], b[0], qa_fma(a[1], a[1], qa_mul(a[0], a[0]))));
+                float ss = qa_lo(sq) + qa_hi(sq);
 #pragma unroll
-            for (int o = LANES / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                for (int o = LANES / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                inv = rsqrtf(ss * (1.f / D) + p.eps);
+            }
             if (which < 2) {
                 if (which ? p.k_norm != nullptr : p.q_norm != nullptr) {
-                    const float inv = rsqrtf(ss * (1.f / D) + p.eps);
+                    const u64 inv2 = qa_pair(inv, inv);
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) x[k] = x[k] * inv * (which ? g[1][k] : g[0][k]);
+                    for (int k = 0; k < 2; ++k) {
+                        a[k] = qa_mul(qa_mul(a[k], inv2), which ? ga[1][k] : ga[0][k]);
+                        b[k] = qa_mul(qa_mul(b[k], inv2), which ? gb[1][k] : gb[0][k]);
+                    }
                 }
                 if (turned) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const int i = PAIRS ? 2 * k : k, j = PAIRS ? 2 * k + 1 : 4 + k;
-                        const float a = x[i], b = x[j];
-                        x[i] = fmaf(a, cs[k], -b * sn[k]);
-                        x[j] = fmaf(a, sn[k], b * cs[k]);
+                    for (int k = 0; k < 2; ++k) {
+                        const u64 x = qa_fma(a[k], cs[k], qa_mul(b[k], minus_sn[k])), y = qa_fma(a[k], sn[k], qa_mul(b[k], cs[k]));
+                        a[k] = x; b[k] = y;
                     }
                 }
-                o0 = make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]));
-                o1 = make_uint2(pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
+                if (PAIRS) {
+                    o0 = make_uint2(pack_bf16x2(qa_lo(a[0]), qa_lo(b[0])), pack_bf16x2(qa_hi(a[0]), qa_hi(b[0])));
+                    o1 = make_uint2(pack_bf16x2(qa_lo(a[1]), qa_lo(b[1])), pack_bf16x2(qa_hi(a[1]), qa_hi(b[1])));
+                } else {
+                    o0 = make_uint2(pack_bf16x2(qa_lo(a[0]), qa_hi(a[0])), pack_bf16x2(qa_lo(a[1]), qa_hi(a[1])));
+                    o1 = make_uint2(pack_bf16x2(qa_lo(b[0]), qa_hi(b[0])), pack_bf16x2(qa_lo(b[1]), qa_hi(b[1])));
+                }
                 if (bad) o0 = o1 = make_uint2(0x7fff7fffu, 0x7fff7fffu);       // NaN: there is no such position
             }
             if (which == 0) {
                 if (h < h1) {
-                    __nv_bfloat16* q = p.q_out + ((size_t)t * p.H + h) * D;
-                    *reinterpret_cast<uint2*>(q + c0) = o0;
-                    *reinterpret_cast<uint2*>(q + c1) = o1;
+                    *reinterpret_cast<uint2*>(q + (size_t)h * D + c0) = o0;
+                    *reinterpret_cast<uint2*>(q + (size_t)h * D + c1) = o1;
                 }
             }
             if (I8) {
@@ -139,7 +173,7 @@ __global__ void __launch_bounds__(QA_THREADS) norm_rope_append_kernel(const __gr
                 for (int o = LANES / 2; o; o >>= 1) am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, o));
                 if (which > 0 && h < h1 && held) {
                     const float inv = kv8_inv(am);
-                    const size_t row = ((((size_t)page * p.layers + p.layer) * 2 + (which - 1)) * p.Hkv + (h - p.H - (which - 1) * p.Hkv)) * p.page_size + slot;
+                    const size_t row = row0 + (size_t)(h - p.H) * p.page_size;
                     uchar4 a, b;
                     a.x = kv8_store(y[0], inv); a.y = kv8_store(y[1], inv); a.z = kv8_store(y[2], inv); a.w = kv8_store(y[3], inv);
                     b.x = kv8_store(y[4], inv); b.y = kv8_store(y[5], inv); b.z = kv8_store(y[6], inv); b.w = kv8_store(y[7], inv);
@@ -148,7 +182,7 @@ __global__ void __launch_bounds__(QA_THREADS) norm_rope_append_kernel(const __gr
                     if (l == 0) p.scales[row] = kv8_scale(am);
                 }
             } else if (which > 0 && h < h1 && held) {
-                const size_t row = ((((size_t)page * p.layers + p.layer) * 2 + (which - 1)) * p.Hkv + (h - p.H - (which - 1) * p.Hkv)) * p.page_size + slot;
+                const size_t row = row0 + (size_t)(h - p.H) * p.page_size;
                 __nv_bfloat16* kv = reinterpret_cast<__nv_bfloat16*>(p.pool) + row * D;
                 *reinterpret_cast<uint2*>(kv + c0) = o0;
                 *reinterpret_cast<uint2*>(kv + c1) = o1;
