@@ -215,6 +215,30 @@ def test_rows_taken_again_are_right():
 
 
 @pytest.mark.parametrize("int8", [False, True])
+def test_hidden_values_behind_a_long_context(int8):
+    """values of several drafts that are not finite, some in one column alone; every row has the numbers of the clean ones, or what is not finite, where the formula has them"""
+    from wf_bitnet import ops
+    ctx, n = 60000, 60
+    a, bits = case([ctx, 100], [n, 9], 16, 2, 16, int8, 21)
+    clean = ops.paged_tree_attn(**a, out_dtype=torch.float32)
+    spoilt = torch.zeros(n, D, dtype=torch.bool)
+    for j, columns, value in ((7, slice(None), math.nan), (23, slice(5, 6), math.inf), (59, slice(64, 130), -math.inf)):
+        page, slot = a["block_table"][0, (ctx + j) // 16].long(), (ctx + j) % 16
+        if int8:
+            a["kv"].scales[page, a["layer"], 1, :, slot] = value
+            columns = slice(None)
+        else:
+            a["kv"].pool[page, a["layer"], 1, :, slot, columns] = value
+        spoilt[:, columns] |= bits[0][:, j, None]
+    out = ops.paged_tree_attn(**a, out_dtype=torch.float32)
+    s = spoilt[:, None].expand(n, 16, D).cuda()
+    assert not out[:n][s].isfinite().any()
+    # the clean result has the hidden value's own (a weight of one in 60000 of a value of at most 6) where this one has none
+    assert bool(((out[:n] - clean[:n])[~s].abs() <= 2.0**-7 * 4).all())
+    assert torch.equal(out[n:n + 9], clean[n:n + 9])
+
+
+@pytest.mark.parametrize("int8", [False, True])
 @pytest.mark.parametrize("n", [20, 200])
 def test_a_row_that_sees_nothing_beside_a_hidden_nan(n, int8):
     """with one block a tile and with several: zeros, whatever the hidden value is"""

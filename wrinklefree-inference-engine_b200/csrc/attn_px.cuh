@@ -5,8 +5,10 @@
 // head).  Two softmax groups of four warps, a thread per row, each have two score buffers of 64 TMEM columns, which their weights (bf16) overwrite in place, and
 // 128 columns of output; the scores of a group's next tile are under way while a tile's weights are computed:
 //   * more than 128 rows: a group per 128 rows, and every tile serves both;
-//   * up to 128 rows: both groups have the same rows and every other tile; their results are joined in shared memory at the end.
-// Warps 8 and 11 load keys and values by TMA into rings of 64-key tiles (a box of 64 dims per run of keys inside a page); one thread of warps 9 and 10 each issues a
+//   * up to 128 rows: both groups have the same rows and every other tile; their results are joined at the end: a thread's lane of tensor memory is
+//     that of the other group's thread with the same row too, and each finishes a half of the columns.
+// Warps 8 and 11 load keys and values by TMA into rings of 64-key tiles (a box of 64 dims per run of keys inside a page; of int8 pools warp 8 both, into a ring of codes from which two
+// sets of four warps convert every other tile: one set took 3300 clocks a tile, two 1700, of which a set's own 2000 of 4000 are the conversion); one thread of warps 9 and 10 each issues a
 // group's S = Q K^T (both operands in shared memory) and O += P V (P in TMEM): a wait of one group leaves the other's products running.  The output is rescaled
 // only when a row's maximum has grown by more than 2^8 since the scale was last fixed (exact: the sum carries the same scale).
 // Weights are rounded to bf16, as the products' operands (off by 2^-8 of a weight at most; sums, maxima and outputs are fp32).
@@ -179,12 +181,13 @@ __device__ __forceinline__ void px_block(const CUtensorMap& tmap, const P& p, un
     constexpr bool TREE = P::TREE, FULL = TREE;            // FULL: the block has its SM to itself
     constexpr int STAGES = TREE ? PX_STAGES_FULL : PX_STAGES;
     constexpr int TAKERS = I8 ? 2 + 8 + 2 * PX_CONV : 3 + 8;        // warps that are told of a share
-    __shared__ __align__(8) uint64_t q_full[3], kv_full[STAGES], kv_empty[STAGES], tail_full, raw_full[PX_RAW], raw_empty[PX_RAW], s_full[2][2], p_full[2][2], o_full[2], o_end[2], drained[2],
+    __shared__ __align__(8) uint64_t q_full[3], kv_full[STAGES], kv_empty[STAGES], tail_full[2], raw_full[PX_RAW], raw_empty[PX_RAW], s_full[2][2], p_full[2][2], o_full[2], o_end[2], drained[2],
         joint, w_full[2], w_empty[2];
     __shared__ uint32_t tmem_base_s;
     __shared__ PxWork w_s[2];
     __shared__ typename P::Walk walk_s;
     __shared__ int failed_s;
+    __shared__ uint32_t hidden_s[TREE ? 4 : 1][8];         // of the shares of late, a bit for each draft whose values are not all finite
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     if (tid == 0) {
@@ -196,7 +199,7 @@ __device__ __forceinline__ void px_block(const CUtensorMap& tmap, const P& p, un
             for (int k = 0; k < 2; ++k) { mbar_init(&s_full[i][k], 1); mbar_init(&p_full[i][k], 4); }
         }
         mbar_init(&q_full[2], 4);
-        mbar_init(&tail_full, 1);
+        for (int i = 0; i < 2; ++i) mbar_init(&tail_full[i], 1);
         mbar_init(&joint, 8);
         fence_mbar_init();
     }
@@ -248,11 +251,15 @@ __device__ __forceinline__ void px_block(const CUtensorMap& tmap, const P& p, un
     if (warp == 8 || (!I8 && warp == 11)) {
         PxAt at_ring;
         int depth = 1;
-        uint32_t tail_par = 0;
+        int tails = 0;                                     // tiles of values that were looked at before they were handed on: they take two barriers in turn
         shares([&](const PxSeg& g, int sh) {
         const int kvh = g.kvh, key0 = g.key0, key1 = g.key1, nt = g.nt, fix_row = g.fix_row, nst = g.nst;
         const uint32_t k_s = g.k_s, v_s = g.v_s, raw_s = g.raw_s;
         const int32_t* table = g.table;
+        if (TREE && !I8 && warp == 11) {                   // (who was told of this share has told that it is through with the one three before)
+            if (lane < 8) hidden_s[sh & 3][lane] = 0u;
+            __syncwarp();
+        }
         // ------------------------------------------------------------ producers: warp 8 the boxes of keys and warp 11 those of values, lanes 0..3 (int8: warp 8 all, 4..7 the values')
         const int kv = I8 ? lane >> 2 & 1 : warp == 11, off = (lane & 3) * p.box;
         depth = I8 ? PX_RAW : nst;
@@ -263,23 +270,78 @@ __device__ __forceinline__ void px_block(const CUtensorMap& tmap, const P& p, un
         // this lane's box: its place in a page, and that page's among the range's.  The warp holds 32 entries of the table from `held` on, and the 32 behind them
         const int first_page = key0 / p.page_size, pages = (key1 - 1) / p.page_size - first_page + 1, per_page = p.layers * 2 * p.Hkv, block0 = (p.layer * 2 + kv) * p.Hkv + kvh;
         int slot = key0 - first_page * p.page_size + off, at = 0, held = 0;
-        auto entry = [&](int i) { return i < pages ? ldcg_i32(table + first_page + i) : 0; };
+        auto entry = [&](int i) { return i < pages ? (int)min((unsigned)ldcg_i32(table + first_page + i), (unsigned)p.max_pages) : 0; };       // what is no page reads as zeros: behind the last
         int entries = entry(lane), behind = entry(32 + lane);
         bool ok = true;
+        int waiting = 0, first_st = 0;                     // such tiles whose copies have been asked for, and the place of the first of them
+        auto hand_on = [&](int i) {                        // tile i
+            const uint32_t v = v_s + first_st * PX_TILE;
+            const int st = first_st, rows = i == nt - 1 ? fix_row : PX_KEYS;
+            if (++first_st == depth) first_st = 0;
+            --waiting;
+            if (!px_wait_warp(&tail_full[tails & 1], (uint32_t)(tails >> 1 & 1))) return false;
+            ++tails;
+            // rows without a key are cleared
+            for (int c = lane; c < (PX_KEYS - rows) * 16; c += 32) {
+                const int h = c / ((PX_KEYS - rows) * 8), r = c - h * (PX_KEYS - rows) * 8;
+                asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(v + h * PX_HALF + (rows * 8 + r) * 16), "r"(0u) : "memory");
+            }
+            if constexpr (TREE) {
+                // Values of drafts that are not finite become 0 (a weight of 0 times them is NaN for rows that do not see them), and their drafts are noted: rows that do see
+                // them get them at the end
+                const int first = key0 + i * PX_KEYS - g.ctx, r0 = max(-first, 0), n16 = (rows - r0) * 8;
+                auto place = [&](int c) { const int h = c >= n16; return v + h * PX_HALF + (r0 * 8 + c - h * n16) * 16; };
+                for (int c0 = lane; c0 < 2 * n16; c0 += 4 * 32) {
+                    uint32_t y[4][4], odd = 0;
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        y[u][0] = y[u][1] = y[u][2] = y[u][3] = 0u;
+                        if (c0 + u * 32 < 2 * n16)
+                            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(y[u][0]), "=r"(y[u][1]), "=r"(y[u][2]), "=r"(y[u][3]) : "r"(place(c0 + u * 32)) : "memory");
+                    }
+#pragma unroll
+                    for (int u = 0; u < 4; ++u)            // an exponent of ones carries into the sign's place
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) odd |= (y[u][k] & 0x7f807f80u) + 0x00800080u;
+                    if (!(odd & 0x80008000u)) continue;
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        uint32_t any = 0;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const uint32_t top = ((y[u][k] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+                            any |= top;
+                            y[u][k] &= ~((top >> 15) * 0xffffu);
+                        }
+                        if (any) {
+                            const int c = c0 + u * 32, d = first + ((r0 * 8 + c - (c >= n16) * n16) >> 3);
+                            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(place(c)), "r"(y[u][0]), "r"(y[u][1]), "r"(y[u][2]), "r"(y[u][3]) : "memory");
+                            if (d < 256) atomicOr(&hidden_s[sh & 3][d >> 5], 1u << (d & 31));
+                        }
+                    }
+                }
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&kv_full[st]);
+            return true;
+        };
         for (int i = 0; i < nt; ++i) {
             const int st = at_ring.st;
             while (slot >= p.page_size) { slot -= p.page_size; ++at; }
             const int lead = __shfl_sync(0xffffffffu, at, 0);              // (box 0 is the first)
             if (lead - held >= 32) { entries = behind; held += 32; behind = entry(held + 32 + lane); }
             const int page0 = __shfl_sync(0xffffffffu, entries, (at - held) & 31), page1 = __shfl_sync(0xffffffffu, behind, (at - held) & 31), page = at - held < 32 ? page0 : page1;
-            const bool mine = boxed && key0 + i * PX_KEYS + off < key1, tail = !I8 && kv && i == nt - 1 && fix_row < PX_KEYS;
+            const int reach = TREE ? key0 + (i + 1) * PX_KEYS - g.ctx : 0;         // trees: the tile's last drafts
+            const bool mine = boxed && key0 + i * PX_KEYS + off < key1, tail = !I8 && kv && ((i == nt - 1 && fix_row < PX_KEYS) || reach > 0);
             const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, mine));
-            uint64_t* full = tail ? &tail_full : &fulls[st];
+            if (tail && waiting == 2 && !hand_on(i - 2)) { ok = false; break; }
+            uint64_t* full = tail ? &tail_full[(tails + waiting) & 1] : &fulls[st];
             if (!px_wait_warp(&empties[st], at_ring.par ^ 1u)) { ok = false; break; }       // (the first lap finds every place empty)
             if (lane == 0) mbar_expect_tx(full, boxes * (uint32_t)((I8 ? 1 : 2) * p.box * 128));
             __syncwarp();
             if (mine) {
-                const int block = (unsigned)page < (unsigned)p.max_pages ? page * per_page + block0 : -1;      // what is no page reads as zeros
+                const int block = page * per_page + block0;
 #pragma unroll
                 for (int h = 0; h < (I8 ? 1 : 2); ++h)
                     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
@@ -290,18 +352,9 @@ __device__ __forceinline__ void px_block(const CUtensorMap& tmap, const P& p, un
             // the first share's other tiles wait until the queries are there, which would queue behind them (the ring's first filling takes all SMs' bandwidth)
             if (i == 1 && sh == 0) { px_wait_warp(&q_full[g.alt ? 2 : 0], 0); if (!g.alt) px_wait_warp(&q_full[1], 0); }
             at_ring.step(1, depth);
-            if (tail) {                                    // its keyless value rows are cleared before the tile is handed on
-                ok = px_wait_warp(&tail_full, tail_par);
-                tail_par ^= 1u;
-                for (int c = lane; ok && c < (PX_KEYS - fix_row) * 16; c += 32) {
-                    const int h = c / ((PX_KEYS - fix_row) * 8), r = c - h * (PX_KEYS - fix_row) * 8;
-                    asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(v_s + st * PX_TILE + h * PX_HALF + (fix_row * 8 + r) * 16), "r"(0u) : "memory");
-                }
-                fence_proxy_async();
-                __syncwarp();
-                if (ok && lane == 0) mbar_arrive(&kv_full[st]);
-            }
+            if (tail && !waiting++) first_st = st;
         }
+        while (waiting) ok = hand_on(nt - waiting) && ok;
         if (!ok) fail(16);
         return ok;
         });
@@ -557,6 +610,17 @@ __device__ __forceinline__ void px_block(const CUtensorMap& tmap, const P& p, un
                 }
                 s[c] = pack_bf16x2(e0, e1);
             }
+            if constexpr (TREE && I8) {                    // a hidden key has no weight, whatever its values' scale
+                const int at = key0 + tile * PX_KEYS;
+                if (at + PX_KEYS > w.ctx) {
+                    const u64 see = px_sight(mask_row, p.words, at - w.ctx, key1 - at);
+#pragma unroll
+                    for (int c = 0; c < PX_KEYS / 2; ++c) {
+                        const uint32_t two = (uint32_t)(see >> (2 * c & 32)) >> (2 * c & 31);
+                        s[c] &= (two & 1u) * 0xffffu | (two & 2u) * 0x7fff8000u;
+                    }
+                }
+            }
             TC_ST32(s_n, s);
             if (n > 0 && __any_sync(0xffffffffu, corr != 1.f)) {
                 if (!px_wait_warp(&o_full[t], o_par ^ (uint32_t)((n - 1) & 1))) { ok = false; break; }      // the scores above came behind all values but the last tile's
@@ -629,30 +693,31 @@ __device__ __forceinline__ void px_block(const CUtensorMap& tmap, const P& p, un
                         for (int k = 0; k < 32; ++k) o[h + k] = __float_as_uint(fmaf(__uint_as_float(o[h + k]), f0, __uint_as_float(x[k]) * f1));
                     }
                 }
-                bool mine_ok = r_ok;
-                if constexpr (TREE) {
-                    // a value that is not finite under a key that the row does not see has made the row NaN (its weight of 0 times it): such rows are taken again
-                    float bad = 0.f;
+                if constexpr (TREE && !I8) {               // drafts' values that are not finite, for the rows that see them
+                    uint32_t noted = 0;
 #pragma unroll
-                    for (int k = 0; k < 64; ++k) bad = fmaf(__uint_as_float(o[k]), 0.f, bad);
-                    unsigned again = key1 > w.ctx ? __ballot_sync(0xffffffffu, r_ok && bad != 0.f && m_ref < INFINITY && l < INFINITY) : 0u;
-                    mine_ok = r_ok && !(again >> lane & 1u);
-                    for (; again; again &= again - 1u) {
-                        const int who = __ffs(again) - 1, rr = r - lane + who;
-                        const float2 v = p.template row_again<I8>(w, rr, __shfl_sync(0xffffffffu, m_ref, who), unit, c + 2 * lane);
-                        const float l_who = __shfl_sync(0xffffffffu, l, who), inv = l_who > 0.f ? 1.f / l_who : 0.f;
-                        if (w.part < 0) p.store2(w, rr, c + 2 * lane, v.x * inv, v.y * inv);
-                        else reinterpret_cast<float2*>(p.part_o)[(((size_t)w.part * 32 + ((c + 2 * lane) >> 2)) * p.rows_p + (rr - w.part_row0)) * 2 + (lane & 1)] = v;
+                    for (int k = 0; k < 8; ++k) noted |= hidden_s[sh & 3][k];
+                    unsigned rows_of = noted ? __ballot_sync(0xffffffffu, r_ok && m_ref != -INFINITY && p.sees_any(w, r, hidden_s[sh & 3])) : 0u;
+                    for (; rows_of; rows_of &= rows_of - 1u) {
+                        const int who = __ffs(rows_of) - 1;
+                        const float2 v = p.hidden_values(w, r - lane + who, hidden_s[sh & 3], __shfl_sync(0xffffffffu, m_ref, who), c + 2 * lane);
+#pragma unroll
+                        for (int k = 0; k < 64; ++k) {
+                            const float x = __shfl_sync(0xffffffffu, k & 1 ? v.y : v.x, k >> 1);
+                            if (lane == who) o[k] = __float_as_uint(__uint_as_float(o[k]) + x);
+                        }
                     }
+                }
+                if constexpr (TREE) {
                     if (w.part < 0) {
                         const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;      // no key: zeros; NaN stays
-                        if (mine_ok) p.store64(w, r, c, o, inv);
+                        if (r_ok) p.store64(w, r, c, o, inv);
                         continue;
                     }
                 }
 #pragma unroll
                 for (int k = 0; k < 64; k += 4)
-                    if (mine_ok) dst[(size_t)((c + k) >> 2) * p.rows_p] = make_float4(__uint_as_float(o[k]), __uint_as_float(o[k + 1]), __uint_as_float(o[k + 2]), __uint_as_float(o[k + 3]));
+                    if (r_ok) dst[(size_t)((c + k) >> 2) * p.rows_p] = make_float4(__uint_as_float(o[k]), __uint_as_float(o[k + 1]), __uint_as_float(o[k + 2]), __uint_as_float(o[k + 3]));
             }
             if (r_ok && (t == 0 || !alt) && (!TREE || w.part >= 0)) reinterpret_cast<float2*>(p.part_ml)[(size_t)w.part * p.rows_p + (r - w.part_row0)] = make_float2(m_ref, l);
         }
@@ -678,6 +743,7 @@ __device__ __forceinline__ void px_block(const CUtensorMap& tmap, const P& p, un
 
 // [128][slot][page, layer, K | V, head], boxes of `box` slots x 128 bytes
 inline int px_encode(CUtensorMap* tm, const wf_kv_layout* kv, int box, const char* who) {
+    if (((long long)kv->max_pages + 1) * kv->layers * 2 * kv->kv_heads > 0x7fffffffll) { set_error("%s: a pool of at most 2^31 heads' rows of pages", who); return WF_ERR_UNSUPPORTED; }
     EncodeTiledFn fn = tc_encoder();
     if (!fn) { set_error("%s: cuTensorMapEncodeTiled unavailable", who); return WF_ERR_CUDA; }
     const cuuint64_t gdim[3] = {AT_D, (cuuint64_t)kv->page_size, (cuuint64_t)kv->max_pages * kv->layers * 2 * kv->kv_heads};

@@ -14,8 +14,9 @@
 // Bound by the memory where rows are few (the 48: 0.73 us for a tile of 64 keys an SM, 6.4 TB/s), by a tile's softmax and the products' turns on the tensor cores where there are
 // 256 (1500 of 2000 clocks are exponentials, maxima and sums), by the conversion of codes for int8 pools (1700).
 //
-// A row that sees no key gets zeros.  A value that is not finite under a key that a row does not see would make it NaN (0 times it): such rows, found by their result, are
-// computed again key by key.
+// A row that sees no key gets zeros.  A value that is not finite under a key that a row does not see would make it NaN (0 times it): among the drafts' values the warp that loads them
+// looks for such ones, puts zeros there and notes the drafts; rows that do see them get them at the end.  (Rows found by their
+// NaN and computed again key by key would keep the block's other roles waiting for longer than their limit behind long contexts.)
 #include <algorithm>
 
 #include "attn_px.cuh"
@@ -186,11 +187,6 @@ struct TxParams {
         return w;
     }
 
-    __device__ __forceinline__ void store2(const PxWork& w, int r, int c, float x, float y) const {
-        const size_t at = (((size_t)w.first + r / G) * H + w.kvh * G + r % G) * AT_D + c;
-        if (out_dtype == WF_BF16) reinterpret_cast<uint32_t*>(out)[at / 2] = pack_bf16x2(x, y);
-        else reinterpret_cast<float2*>(out)[at / 2] = make_float2(x, y);
-    }
     __device__ __forceinline__ void store64(const PxWork& w, int r, int c, const uint32_t (&o)[64], float inv) const {
         const size_t at = (((size_t)w.first + r / G) * H + w.kvh * G + r % G) * AT_D + c;
         auto v = [&](int i) { return __uint_as_float(o[i]) * inv; };
@@ -206,40 +202,31 @@ struct TxParams {
         }
     }
 
-    // Row r's weighted values of columns c and c + 1 again, by the whole warp (c is the lane's own), over the keys that it sees alone; m: its maximum
-    template <bool I8>
-    __device__ __forceinline__ float2 row_again(const PxWork& w, int r, float m, float, int c) const {
+    // whether row r sees any of the drafts noted
+    __device__ __forceinline__ bool sees_any(const PxWork& w, int r, const uint32_t* noted) const {
+        const u64* sees = mask + (size_t)(w.first + r / G) * words;
+        u64 any = 0;
+        for (int i = 0; i < words; ++i) any |= sees[i] & ((u64)noted[2 * i + 1] << 32 | noted[2 * i]);
+        return any != 0;
+    }
+    // Row r's weighted values of columns c and c + 1, by the whole warp (c is the lane's own), of those drafts and of the values among them that are not finite; m: its maximum
+    __device__ __forceinline__ float2 hidden_values(const PxWork& w, int r, const uint32_t* noted, float m, int c) const {
         const int lane = threadIdx.x & 31;
         float2 sum = make_float2(0.f, 0.f);
-        if (m == -INFINITY) return sum;
         const u64* sees = mask + (size_t)(w.first + r / G) * words;
         const uint2 qw = *(reinterpret_cast<const uint2*>(q + (((size_t)w.first + r / G) * H + w.kvh * G + r % G) * AT_D) + lane);
         const float x[4] = {bf16lo(qw.x), bf16hi(qw.x), bf16lo(qw.y), bf16hi(qw.y)};
-        for (int j = w.key0; j < w.key1; ++j) {
-            const int d = j - w.ctx;
-            if (d >= 0 && !(sees[d >> 6] >> (d & 63) & 1ull)) continue;
-            const int page = w.table[j / page_size];
-            float k[4] = {0.f, 0.f, 0.f, 0.f}, v0 = 0.f, v1 = 0.f;
-            if (page >= 0 && page < max_pages) {       // what is no page reads as zeros
+        for (int i = 0; i < words; ++i)
+            for (u64 which = sees[i] & ((u64)noted[2 * i + 1] << 32 | noted[2 * i]); which; which &= which - 1ull) {
+                const int j = w.ctx + i * 64 + __ffsll((long long)which) - 1, page = w.table[j / page_size];      // (of a page: what is none reads as zeros)
                 const size_t kr = ((((size_t)page * layers + layer) * 2) * Hkv + w.kvh) * page_size + j % page_size, vr = kr + (size_t)Hkv * page_size;
-                if (I8) {
-                    const uchar4 a = *(reinterpret_cast<const uchar4*>(reinterpret_cast<const uint8_t*>(pool) + kr * AT_D) + lane);
-                    const uchar2 b = *reinterpret_cast<const uchar2*>(reinterpret_cast<const uint8_t*>(pool) + vr * AT_D + c);
-                    const float ks = scales[kr], vs = scales[vr];
-                    k[0] = ((int)a.x - 128) * ks; k[1] = ((int)a.y - 128) * ks; k[2] = ((int)a.z - 128) * ks; k[3] = ((int)a.w - 128) * ks;
-                    v0 = ((int)b.x - 128) * vs; v1 = ((int)b.y - 128) * vs;
-                } else {
-                    const uint2 a = *(reinterpret_cast<const uint2*>(reinterpret_cast<const __nv_bfloat16*>(pool) + kr * AT_D) + lane);
-                    const uint32_t b = *reinterpret_cast<const uint32_t*>(reinterpret_cast<const __nv_bfloat16*>(pool) + vr * AT_D + c);
-                    k[0] = bf16lo(a.x); k[1] = bf16hi(a.x); k[2] = bf16lo(a.y); k[3] = bf16hi(a.y);
-                    v0 = bf16lo(b); v1 = bf16hi(b);
-                }
+                const uint2 a = *(reinterpret_cast<const uint2*>(reinterpret_cast<const __nv_bfloat16*>(pool) + kr * AT_D) + lane);
+                const uint32_t b = *reinterpret_cast<const uint32_t*>(reinterpret_cast<const __nv_bfloat16*>(pool) + vr * AT_D + c);
+                const float s = warp_sum(x[0] * bf16lo(a.x) + x[1] * bf16hi(a.x) + x[2] * bf16lo(a.y) + x[3] * bf16hi(a.y));
+                const float e = exp2f((scale_log2e == 0.f ? 0.f : s * scale_log2e) - m);
+                if (!isfinite(bf16lo(b))) sum.x += e * bf16lo(b);
+                if (!isfinite(bf16hi(b))) sum.y += e * bf16hi(b);
             }
-            const float s = warp_sum(x[0] * k[0] + x[1] * k[1] + x[2] * k[2] + x[3] * k[3]);
-            const float e = exp2f((scale_log2e == 0.f ? 0.f : s * scale_log2e) - m);
-            sum.x = fmaf(e, v0, sum.x);
-            sum.y = fmaf(e, v1, sum.y);
-        }
         return sum;
     }
 };
