@@ -10,6 +10,14 @@ F64 = torch.float64
 TYPES = [torch.float32, torch.bfloat16, torch.float16]
 
 
+@pytest.fixture(autouse=True)
+def used_memory():
+    """what is allocated next has been written before, so that an entry that a kernel leaves out shows"""
+    if torch.cuda.is_available():
+        kept = [torch.full((n // 4,), float("nan"), device="cuda") for n in [1 << 28] + [1 << 19] * 64]
+        del kept
+
+
 def pack(ok):
     """bool [n, V] -> int32 words"""
     n, V = ok.shape
@@ -244,3 +252,31 @@ def test_refusals():
     with pytest.raises(NotImplementedError):
         ops.process_logits(**{**a, "node_mask": torch.zeros(5, 5, dtype=torch.int64, device="cuda")})
     assert ops.process_logits(a["logits"][:0]).shape == (0, 100)
+
+
+def test_out_between_the_rows_and_over_them():
+    from wf_bitnet import ops
+    x = torch.randn(5, 2000, device="cuda")
+    bias = dict(bias_ids=torch.full((5, 1), 7, dtype=torch.int32, device="cuda"), bias_values=torch.ones(5, 1, device="cuda"))
+    want = ops.process_logits(x[:, :1000], **bias)
+    ops.process_logits(x[:, :1000], out=x[:, 1000:], **bias)
+    assert torch.equal(x[:, 1000:], want)
+    for out in (x[:, 1:1001], x[:, 999:1999]):
+        with pytest.raises(ValueError):
+            ops.process_logits(x[:, :1000], out=out, **bias)
+    y = x.view(10, 1000)
+    with pytest.raises(ValueError):
+        ops.process_logits(y[:9], out=y[1:], bias_ids=bias["bias_ids"].repeat(2, 1)[:9], bias_values=bias["bias_values"].repeat(2, 1)[:9])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [513, 1500, 9000, 32003, 32700, 70001])
+@pytest.mark.parametrize("rows", [[60] * 5, [1] * 40, [200, 3, 90]])
+def test_every_entry_is_written(rows, V, dtype):
+    """vocabularies whose last chunk is short, with rows enough for the longer chunks"""
+    from wf_bitnet import ops
+    a = case(rows, V, dtype, L=300, bias=9, nodes=len(set(rows)) > 1, tail=1 if len(rows) == 3 else 0)
+    mine = a["logits"].clone()
+    ops.process_logits(**{**a, "logits": mine}, out=mine)
+    out = ops.process_logits(**a, out=torch.full_like(mine, math.nan))
+    assert torch.equal(out, mine)

@@ -106,7 +106,8 @@ def test_logits():
         return L.wf_process_logits(C.byref(a), None)
     for bad in (dict(rows=-1), dict(vocab=0), dict(sequences=-1), dict(dtype=_lib.WF_I8), dict(row_stride=63), dict(out_stride=63), dict(sequences=3), dict(history_width=-1), dict(bias_width=-1),
                 dict(mask_words=-1), dict(logits=None), dict(out=None), dict(bias_values=None), dict(node_tokens=None), dict(history_stride=4), dict(allowed_stride=1), dict(logits=P + 2), dict(out=P + 3),
-                dict(node_mask=P + 4), dict(out=P, out_stride=128)):
+                dict(node_mask=P + 4), dict(out=P, out_stride=128), dict(out=P + 4), dict(out=P + 256), dict(out=P - 252), dict(out=P + 256, out_stride=128),
+                dict(out=P + 252, row_stride=128, out_stride=128), dict(out=P - 252, row_stride=128, out_stride=128)):
         assert call(**bad) == BAD, bad
         assert b"wf_process_logits" in L.wf_last_error()
     for bad in (dict(vocab=(1 << 30) + 1, row_stride=1 << 40, out_stride=1 << 40), dict(rows=(1 << 30) + 1, sequences=(1 << 30) + 1), dict(rows=65535, sequences=65535), dict(bias_width=65536),

@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(LG_THREADS, LG_BLOCKS) process_logits_kernel(c
     T* const ring_p = reinterpret_cast<T*>(lg_smem + warp * LG_STAGES * (BYTES + 16));
     constexpr int STEP = (BYTES + 16) / (int)sizeof(T);
 
-    // a warp's chunks are every eighth of the block's
+    // a warp's chunks are every twelfth of the block's
     struct Chunk { int left, row, col; };              // chunks of the block from this one on (none: 0 or less), its row and place there
     auto step = [&](Chunk& c) { c.left -= LG_WARPS; c.col += LG_WARPS; while (c.col >= per_row) { c.col -= per_row; ++c.row; } };
     auto from_of = [&](const Chunk& c) { return s_lo + c.col * CHUNK; };
@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(LG_THREADS, LG_BLOCKS) process_logits_kernel(c
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    uint32_t next[LG_STAGES];                          // a chunk's mask is asked for three chunks ahead of its logits
+    uint32_t next[LG_STAGES];                          // a chunk's mask is asked for a ring ahead of its logits
 #pragma unroll
     for (int i = 0; i < LG_STAGES; ++i) { next[i] = mask_of(ahead); step(ahead); }
 #pragma unroll
@@ -276,7 +276,7 @@ __global__ void __launch_bounds__(LG_THREADS, LG_BLOCKS) process_logits_kernel(c
         const uint32_t* keep_s = mask_s[warp][stage];
         int e0 = 0, e1 = 0;                            // its entries
         if (tables) { e0 = front[(from - lo) >> 5]; e1 = front[(from - lo + n + 31) >> 5]; }
-        asm volatile("cp.async.wait_group %0;" ::"n"(LG_STAGES - 2) : "memory");
+        asm volatile("cp.async.wait_group %0;" ::"n"(LG_STAGES - 1) : "memory");
         __syncwarp();
         for (int e = e0 + lane; e < e1; e += 32) {
             const int v = (uint16_t)(token_of[e] - (from - lo));
@@ -349,15 +349,14 @@ __global__ void __launch_bounds__(LG_THREADS, LG_BLOCKS) process_logits_kernel(c
 #pragma unroll
         for (int stage = 0; stage < LG_STAGES; ++stage) {
             if (now.left <= 0) break;
-            change(stage);
-            step(now);
             constexpr int LAST = LG_STAGES - 1;
             const int free = (stage + LAST) % LG_STAGES;               // (left by the chunk before)
             ask(asked, next[free], free);
             step(asked);
             next[free] = mask_of(ahead);
             step(ahead);
-            __syncwarp();                              // (its mask too)
+            change(stage);
+            step(now);
         }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -396,6 +395,15 @@ int lg_run(long long rows, long long seqs, long long per_row, long long wave, bo
     return best ? (int)best : LG_MIN_RUN;
 }
 
+// whether rows of the one have bytes of rows of the other (rows of the same stride may lie between each other)
+bool lg_overlap(uintptr_t x, uintptr_t y, const wf_logits_args& a, int es) {
+    const unsigned long long row = (unsigned long long)a.vocab * es, sx = (unsigned long long)a.row_stride * es, sy = (unsigned long long)a.out_stride * es, n = a.rows - 1;
+    if (x + n * sx + row <= y || y + n * sy + row <= x) return false;
+    if (n == 0 || sx != sy) return true;
+    const unsigned long long off = (x > y ? x - y : y - x) % sx;
+    return off < row || sx - off < row;
+}
+
 }  // namespace
 
 }  // namespace wf
@@ -428,6 +436,7 @@ extern "C" int wf_process_logits(const wf_logits_args* args, void* stream) {
     if (a.allowed && a.rows > 1 && a.allowed_stride < (a.vocab + 31) / 32) { set_error("%s: mask stride %lld below its %d words", who, a.allowed_stride, (a.vocab + 31) / 32); return WF_ERR_INVALID; }
     if (a.logits == a.out && a.rows > 1 && a.row_stride != a.out_stride) { set_error("%s: the same memory with row strides %lld and %lld", who, a.row_stride, a.out_stride); return WF_ERR_INVALID; }
     const int es = a.dtype == WF_F32 ? 4 : 2;
+    if (a.logits != a.out && lg_overlap((uintptr_t)a.logits, (uintptr_t)a.out, a, es)) { set_error("%s: out overlaps the logits without being them", who); return WF_ERR_INVALID; }
     if ((uintptr_t)a.logits % es || (uintptr_t)a.out % es) { set_error("%s: logits are not aligned to their type", who); return WF_ERR_INVALID; }
     if ((uintptr_t)a.node_mask & 7) { set_error("%s: the drafts' masks must be 8-byte aligned", who); return WF_ERR_INVALID; }
     // Entries of a list are at most what the sequence brings, and at most the columns of a slice
@@ -437,7 +446,7 @@ extern "C" int wf_process_logits(const wf_logits_args* args, void* stream) {
     const int bytes = (long long)a.rows * a.vocab * es < (long long)LG_WARPS * sm_count() * LG_CHUNK ? LG_SHORT : LG_CHUNK, chunk = bytes / es;
     const long long most = brings > LG_ENTRIES ? LG_ENTRIES : LG_SLICE;
     p.slice = (int)((a.vocab < most ? a.vocab : most) + 511) / 512 * 512;
-    const long long slices = ((long long)a.vocab + p.slice - 1) / p.slice, per_row = p.slice / chunk;
+    const long long slices = ((long long)a.vocab + p.slice - 1) / p.slice, per_row = (p.slice + chunk - 1) / chunk;
     const long long seqs = a.offsets ? a.sequences + 1ll : a.sequences;
     const int full = lg_smem_bytes(bytes, p.slice, (int)(std::min(brings, (long long)p.slice) + 7) / 8 * 8, a.mask_words, a.bias_ids != nullptr);
     const long long wave = std::max((full + 6144 <= 113 * 1024 ? LG_BLOCKS : 1) * sm_count() / slices, 1ll);
