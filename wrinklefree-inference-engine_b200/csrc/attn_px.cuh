@@ -100,6 +100,7 @@ __device__ __forceinline__ float px_max(float a, float b) { float y; asm("max.Na
 // 2^x of two numbers on the multiply-add units: x = i + f, |f| <= 1/2, by adding 1.5 * 2^23; 2^f by its minimax polynomial of degree 3 (Remez; off by 7.5e-5 at
 // most, a 50th of what the rounding of a weight to bf16 may be); i goes into the exponent.  Below 2^-126: 0.  The special function unit gives 16 values a
 // clock and SM; one pair in PX_POLY takes this way: 74.4 us for a prefix of 32768 under 128 sequences with one in 8, 71.5 in 4, 71.7 in 3, 72.3 in 2, 79 without.
+// Int8 pools: none, for their conversion wants the issue slots (31 sequences of 25 drafts over 8000: 188 us, with one in 4 200, in 2 215).
 constexpr int PX_POLY = 4;
 __device__ __forceinline__ void px_exp2_poly(uint64_t x, float& e0, float& e1) {
     const uint64_t magic = px_pair(0x4b400000u, 0x4b400000u), minus_magic = px_pair(0xcb400000u, 0xcb400000u), minus1 = px_pair(0xbf800000u, 0xbf800000u);
@@ -349,8 +350,9 @@ __device__ __forceinline__ void px_block(const CUtensorMap& tmap, const P& p, un
             }
             __syncwarp();
             slot += PX_KEYS;
-            // the first share's other tiles wait until the queries are there, which would queue behind them (the ring's first filling takes all SMs' bandwidth)
-            if (i == 1 && sh == 0) { px_wait_warp(&q_full[g.alt ? 2 : 0], 0); if (!g.alt) px_wait_warp(&q_full[1], 0); }
+            // the first share's other tiles wait until the queries are there, which would queue behind them (the ring's first filling takes all SMs' bandwidth); not a tree's bf16
+            // tiles, whose block has more shares to come (48 sequences of 12 drafts: 134 us, waiting 136; int8, waiting, 200 for 205)
+            if (i == 1 && sh == 0 && (!TREE || I8)) { px_wait_warp(&q_full[g.alt ? 2 : 0], 0); if (!g.alt) px_wait_warp(&q_full[1], 0); }
             at_ring.step(1, depth);
             if (tail && !waiting++) first_st = st;
         }
@@ -597,7 +599,7 @@ __device__ __forceinline__ void px_block(const CUtensorMap& tmap, const P& p, un
             for (int c = 0; c < PX_KEYS / 2; ++c) {       // columns (2c, 2c + 1) go to s[c], an entry whose score has been read
                 const uint64_t x = px_fma2(px_pair(s[2 * c], s[2 * c + 1]), unit2, nm2);
                 float e0, e1;
-                if (c % PX_POLY == PX_POLY - 1) {
+                if (!I8 && c % PX_POLY == PX_POLY - 1) {
                     px_exp2_poly(x, e0, e1);
                 } else {
                     px_unpair(x, e0, e1);
