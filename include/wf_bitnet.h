@@ -196,7 +196,7 @@ int wf_rope_kv_append(const void* qkv, int B, int H, const wf_kv_layout* kv, int
  * a sin + b cos), cos and sin from row positions[t] of cos_tab, sin_tab [max_pos][rot / 2] (table_dtype WF_F32 or WF_BF16).  All in float, rounded once to bf16.  Queries go
  * to q_out [tokens][H][D]; keys and values to (pages[t], slots[t], layer) of the cache, an int8 pool's codes as wf_kv_scatter makes them of the bf16 values.  A token whose
  * page or slot is none of the pool's is not appended (wf_paged_plan's entries behind the last token); one whose position is not in [0, max_pos) is not either, and its
- * queries are NaN.  head_dim 64, 128 or 256.  qkv, q_out, the pool, tables and gains are 16-byte aligned.  Of two tokens at the same
+ * queries are NaN.  head_dim 64, 128 or 256 (int8 pools: 128).  qkv, q_out, the pool, tables and gains are 16-byte aligned.  Of two tokens at the same
  * place it is not determined what is kept. */
 int wf_norm_rope_kv_append(const void* qkv, long long row_stride, int tokens, int H, const wf_kv_layout* kv, int layer, const int32_t* positions, const int32_t* pages,
                            const int32_t* slots, const void* cos_tab, const void* sin_tab, int table_dtype, int rot, int max_pos, const void* q_norm, const void* k_norm,

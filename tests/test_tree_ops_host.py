@@ -46,7 +46,7 @@ def test_append():
                 dict(out=P + 8), dict(qn=P + 4), dict(cos=P + 8), dict(kv=dict(pool=None)), dict(kv=dict(kv_heads=0)), dict(kv=dict(pool=P + 4))):
         assert call(**bad) == BAD, bad
         assert b"wf_norm_rope_kv_append" in L.wf_last_error()
-    for bad in (dict(rot=12), dict(kv=dict(head_dim=96)), dict(kv=dict(dtype=_lib.WF_F32)), dict(H=1 << 21, ld=1 << 40), dict(T=(1 << 30) + 1)):
+    for bad in (dict(rot=12), dict(kv=dict(head_dim=96)), dict(rot=64, ld=768, kv=dict(head_dim=64, dtype=_lib.WF_I8)), dict(ld=8192, kv=dict(head_dim=256, dtype=_lib.WF_I8)), dict(kv=dict(dtype=_lib.WF_F32)), dict(H=1 << 21, ld=1 << 40), dict(T=(1 << 30) + 1)):
         assert call(**bad) == NO, bad
     assert call(T=0, qkv=None, out=None) == _lib.WF_OK
 

@@ -212,6 +212,7 @@ extern "C" int wf_norm_rope_kv_append(const void* qkv, long long row_stride, int
     if (kv->dtype != WF_BF16 && kv->dtype != WF_I8) { set_error("%s: pool must be bf16 or int8", who); return WF_ERR_UNSUPPORTED; }
     const int D = kv->head_dim;
     if (D != 64 && D != 128 && D != 256) { set_error("%s: head_dim must be 64, 128 or 256 (got %d)", who, D); return WF_ERR_UNSUPPORTED; }
+    if (kv->dtype == WF_I8 && D != 128) { set_error("%s: int8 pools need head_dim 128 (got %d)", who, D); return WF_ERR_UNSUPPORTED; }
     if (layer < 0 || layer >= kv->layers) { set_error("%s: layer %d out of range", who, layer); return WF_ERR_INVALID; }
     if (rot < 0 || rot > D || max_pos < 0) { set_error("%s: %d rotated dims of %d, %d positions", who, rot, D, max_pos); return WF_ERR_INVALID; }
     if (rot % 8) { set_error("%s: the rotated dims must be a multiple of 8 (got %d)", who, rot); return WF_ERR_UNSUPPORTED; }
@@ -244,8 +245,8 @@ extern "C" int wf_norm_rope_kv_append(const void* qkv, long long row_stride, int
     if (blocks > 0x7fffffffll) { set_error("%s: too many tokens and heads", who); return WF_ERR_UNSUPPORTED; }
     cudaStream_t s = (cudaStream_t)stream;
     const bool i8 = p.scales != nullptr;
-    const cudaError_t e = D == 64 ? (i8 ? qa_launch<64, true>(p, interleaved, (unsigned)blocks, s) : qa_launch<64, false>(p, interleaved, (unsigned)blocks, s))
+    const cudaError_t e = D == 64 ? qa_launch<64, false>(p, interleaved, (unsigned)blocks, s)
                         : D == 128 ? (i8 ? qa_launch<128, true>(p, interleaved, (unsigned)blocks, s) : qa_launch<128, false>(p, interleaved, (unsigned)blocks, s))
-                                   : (i8 ? qa_launch<256, true>(p, interleaved, (unsigned)blocks, s) : qa_launch<256, false>(p, interleaved, (unsigned)blocks, s));
+                                   : qa_launch<256, false>(p, interleaved, (unsigned)blocks, s);
     return launch_check(e, who);
 }

@@ -296,7 +296,7 @@ def norm_rope_kv_append(qkv: torch.Tensor, H: int, kv: PagedKV, layer: int, posi
     qkv: bf16 [T, (H + 2 Hkv) * D], any row stride.  positions, pages, slots: int32 [T] (paged_plan's; of drafts, tree_plan's positions).  cos_tab, sin_tab: float32 or
     bf16 [max_pos, R / 2] for the first R dims of a head (a multiple of 8), pairs (i, i + R / 2), or (2i, 2i + 1) with interleaved.  q_norm, k_norm: gains of an RMS
     norm over the head, float32 or bf16 [D], or None.  In float, rounded once to bf16; an int8 cache then quantises as kv_scatter does.  A token whose page or slot is
-    outside the cache is not appended; one whose position is outside the tables is not either, and its queries are NaN.  Head sizes 64, 128 and 256."""
+    outside the cache is not appended; one whose position is outside the tables is not either, and its queries are NaN.  Head sizes 64, 128 and 256 (an int8 cache: 128)."""
     c = kv.c
     return _native.ops().norm_rope_kv_append(qkv, H, kv.raw if kv.dtype == torch.int8 else kv.pool, c.max_pages, c.layers, c.kv_heads, c.page_size, c.head_dim, c.dtype, layer, positions,
                                              pages, slots, cos_tab, sin_tab, q_norm, k_norm, eps, interleaved)
