@@ -434,3 +434,20 @@ def test_graphs_and_streams_side_by_side(int8):
         torch.cuda.synchronize()
         for a, o in zip(cases, outs):
             assert torch.equal(o, ops.paged_tree_attn(**a))
+
+
+@pytest.mark.parametrize("int8", [False, True])
+def test_tiles_of_one_group_and_of_two_in_turn(int8):
+    """row tiles of up to 128 rows beside wider ones, in rings of an odd number of tiles: three streams at a time, the same bits every time"""
+    from wf_bitnet import ops
+    a, bits = case([115, 9035, 0, 2681, 5288, 1809, 0, 5982, 3300], [145, 252, 249, 86, 128, 52, 122, 173, 74], 64, 8, 32, int8, 31, pad=60)
+    want = check(a, bits)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    for _ in range(40):
+        got = []
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(ops.paged_tree_attn(**a))
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, want) for x in got)

@@ -100,7 +100,7 @@ __device__ __forceinline__ float px_max(float a, float b) { float y; asm("max.Na
 // 2^x of two numbers on the multiply-add units: x = i + f, |f| <= 1/2, by adding 1.5 * 2^23; 2^f by its minimax polynomial of degree 3 (Remez; off by 7.5e-5 at
 // most, a 50th of what the rounding of a weight to bf16 may be); i goes into the exponent.  Below 2^-126: 0.  The special function unit gives 16 values a
 // clock and SM; one pair in PX_POLY takes this way: 74.4 us for a prefix of 32768 under 128 sequences with one in 8, 71.5 in 4, 71.7 in 3, 72.3 in 2, 79 without.
-// Int8 pools: none, for their conversion wants the issue slots (31 sequences of 25 drafts over 8000: 188 us, with one in 4 200, in 2 215).
+// Int8 pools: none, for their conversion wants the issue slots (31 sequences of 25 drafts over 8000: 193 us, with one in 4 204, in 2 218).
 constexpr int PX_POLY = 4;
 __device__ __forceinline__ void px_exp2_poly(uint64_t x, float& e0, float& e1) {
     const uint64_t magic = px_pair(0x4b400000u, 0x4b400000u), minus_magic = px_pair(0xcb400000u, 0xcb400000u), minus1 = px_pair(0xbf800000u, 0xbf800000u);
@@ -455,13 +455,23 @@ __device__ __forceinline__ void px_block(const CUtensorMap& tmap, const P& p, un
         constexpr uint32_t idesc_s = px_idesc(PX_KEYS, 0), idesc_o = px_idesc(AT_D, 1);
         const uint64_t qd = px_desc(q_s + (alt ? 0 : t) * PX_QTILE, 16), kd0 = px_desc(k_s, 16), vd0 = px_desc(v_s, PX_HALF);
         const uint32_t s_t = tmem + t * 256, o_t = s_t + 128;
-        PxAt kt = kv0.after(alt ? t : 0, nst), vt = kt;
+        PxAt kt = kv0, vt = kv0.after(alt ? t : 0, nst);
+        // The other group's tiles are looked at and given back too: who waits for some of a barrier's phases alone takes the phase two before for the one it waits for
+        int seen = 0;
+        auto pass_by = [&](int upto) {
+            for (; seen < upto; ++seen, kt.step(1, nst)) {
+                if (!px_wait_warp(&kv_full[kt.st], kt.par)) return false;
+                if (lane == 0) mbar_arrive(&kv_empty[kt.st]);
+                __syncwarp();
+            }
+            return true;
+        };
         bool ok = px_wait_warp(&q_full[alt ? 2 : t], alt ? q_alt : q_two);
         if (alt) q_alt ^= 1u; else q_two ^= 1u;
         for (int n = -1; n < tiles && ok; ++n) {
             const int now = tile0 + n, next = now + 1;
             if (n + 1 < tiles) {                          // the next tile's scores, into the buffer that the values before last have left
-                if (!px_wait_warp(&kv_full[kt.st], kt.par)) { ok = false; break; }
+                if (!pass_by(alt ? 2 * (n + 1) + t : n + 1) || !px_wait_warp(&kv_full[kt.st], kt.par)) { ok = false; break; }
                 tc_fence_after();
                 if (elected) {
                     const uint64_t kd = kd0 + (uint64_t)(kt.st * (PX_TILE >> 4));
@@ -472,7 +482,8 @@ __device__ __forceinline__ void px_block(const CUtensorMap& tmap, const P& p, un
                     px_commit(&s_full[t][next & 1]);
                 }
                 __syncwarp();
-                kt.step(hop, nst);
+                kt.step(1, nst);
+                ++seen;
             }
             if (n >= 0) {
                 if (!px_wait_warp(&p_full[t][now & 1], (uint32_t)(now >> 1 & 1))) { ok = false; break; }
@@ -483,12 +494,12 @@ __device__ __forceinline__ void px_block(const CUtensorMap& tmap, const P& p, un
                     for (int ks = 0; ks < PX_KEYS / 16; ++ks) px_mma_ts(o_t, s_t + (now & 1) * PX_KEYS + ks * 8, vd + (uint64_t)(ks * 128), idesc_o, n || ks ? 1u : 0u);   // 16 keys = 2048 bytes
                     px_commit(n == tiles - 1 ? &o_end[t] : &o_full[t]);
                     px_commit(&kv_empty[vt.st]);
-                    if (alt) px_commit(&kv_empty[vt.st]);  // (for the other group, which does not read it)
                 }
                 __syncwarp();
                 vt.step(hop, nst);
             }
         }
+        ok = ok && pass_by(nt);
         if (tiles == 0 && elected) px_commit(&o_end[t]);
         __syncwarp();
         kv0.leap(nt, nst);
