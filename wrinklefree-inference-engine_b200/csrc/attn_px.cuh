@@ -596,9 +596,10 @@ __device__ __forceinline__ void px_block(const CUtensorMap& tmap, const P& p, un
                 for (int k = 0; k < 4; ++k) mx4[k] = px_max(px_max(mx4[k], __uint_as_float(s[c + k])), __uint_as_float(s[c + 4 + k]));
             const float mx = px_max(px_max(mx4[0], mx4[1]), px_max(mx4[2], mx4[3])) * unit;
             float corr = 1.f;
-            if (!(mx <= m_ref + PX_LAZY)) {               // also the first time anything is seen, and NaN
-                corr = m_ref == -INFINITY ? 0.f : px_ex2(m_ref - mx);
-                m_ref = mx;
+            if (!(mx <= m_ref + PX_LAZY)) {               // also the first time anything is seen, and NaN, which stays: who joins parts takes -inf for one without weights
+                const float top = px_max(m_ref, mx);
+                corr = m_ref == -INFINITY ? 0.f : px_ex2(m_ref - top);
+                m_ref = top;
                 l *= corr;
             }
             // a row with a score of +inf or NaN has no weights but NaN
@@ -682,7 +683,7 @@ __device__ __forceinline__ void px_block(const CUtensorMap& tmap, const P& p, un
                 float2 ml;
                 asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0, %1}, [%2];" : "=f"(ml.x), "=f"(ml.y) : "r"(tmem + (1 - t) * 256 + lane_base) : "memory");
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                const float m = fmaxf(m_ref, ml.x);
+                const float m = px_max(m_ref, ml.x);      // (-inf is no weight in either group; a maximum that is NaN stays)
                 f0 = m_ref == -INFINITY ? 0.f : px_ex2(m_ref - m);
                 f1 = ml.x == -INFINITY ? 0.f : px_ex2(ml.x - m);
                 l = l * f0 + ml.y * f1;

@@ -313,8 +313,8 @@ __global__ void __launch_bounds__(TX_MERGE, 2) tree_merge_kernel(const __grid_co
                 float4 v[TX_MERGE_COLS];
 #pragma unroll
                 for (int k = 0; k < TX_MERGE_COLS; ++k) v[k] = reinterpret_cast<const float4*>(p.part_o)[((size_t)part * 32 + col + k) * p.rows_p + r];
-                // a part of nothing has no weight, whatever stands there
-                const float m = fmaxf(M, ml.x), f0 = M == -INFINITY ? 0.f : exp2f(M - m), f1 = ml.x == -INFINITY ? 0.f : exp2f(ml.x - m);
+                // a part of nothing (-inf) has no weight, whatever stands there; a maximum that is NaN is none of those, and stays NaN to the end
+                const float m = px_max(M, ml.x), f0 = M == -INFINITY ? 0.f : exp2f(M - m), f1 = ml.x == -INFINITY ? 0.f : exp2f(ml.x - m);
                 const bool nothing = ml.x == -INFINITY;
                 L = nothing ? L : L * f0 + ml.y * f1;
 #pragma unroll
@@ -348,7 +348,7 @@ __global__ void __launch_bounds__(TX_MERGE, 2) tree_merge_kernel(const __grid_co
         if (r < tile.rows) {                           // a warp finishes four columns
             float m = -INFINITY;
 #pragma unroll
-            for (int w = 0; w < WARPS; ++w) m = fmaxf(m, ml_s[w][lane].x);
+            for (int w = 0; w < WARPS; ++w) m = px_max(m, ml_s[w][lane].x);
             float l = 0.f;
             float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
