@@ -252,7 +252,7 @@ int wf_paged_prefix_attn(const void* q, const wf_kv_layout* kv, int layer, const
 /* Trees of drafts.  A sequence's new tokens of a step (offsets [rows + 1], of `tokens` rows, as wf_paged_plan has them) are its drafts, each behind the one that it follows:
  * parents[t] is that one's place among the sequence's drafts, below its own; -1 (or any other number) follows the cached tokens alone.  Bit j of mask[t] (words of 64, ceil(max_nodes /
  * 64) a token; max_nodes at most 256): the draft at place j is t itself or on its way up.  positions[t] = seq_lens[r] + the number of drafts above t.  Of a sequence with more
- * than max_nodes drafts, or a length out of range: masks of 0, positions -1; of rows behind the last sequence: 0 and 0. */
+ * than max_nodes drafts, or a length out of range: masks of 0, positions -1; of rows of no sequence (in front of the first one or behind the last): 0 and 0. */
 int wf_tree_plan(const int32_t* parents, const int32_t* offsets, const int32_t* seq_lens, int rows, int tokens, int max_nodes, uint64_t* mask, int32_t* positions, void* stream);
 
 /* Attention of drafts: q bf16 [tokens][H][D], sequence b's rows offsets[b] .. offsets[b + 1], its cached tokens 0 .. seq_lens[b] and its drafts behind them at seq_lens[b] + place

@@ -46,7 +46,7 @@ __global__ void __launch_bounds__(64 * W) tree_plan_kernel(const __grid_constant
     pdl_launch_dependents();
     int first, n;
     tr_span(p.offsets, blockIdx.x, p.tokens, first, n);
-    const int len = p.seq[blockIdx.x], end = min(max(p.offsets[p.rows], 0), p.tokens);
+    const int len = p.seq[blockIdx.x], front = p.offsets[0], end = min(max(p.offsets[p.rows], 0), p.tokens);
     const bool fits = n <= p.max_nodes && len >= 0 && len <= 0x7fffffff - TR_MAX;
     if (fits) {
         int up = -1;
@@ -83,10 +83,14 @@ __global__ void __launch_bounds__(64 * W) tree_plan_kernel(const __grid_constant
             p.positions[first + k] = -1;
         }
     }
-    for (int k = end + blockIdx.x * 64 * W + i; k < p.tokens; k += gridDim.x * 64 * W) {       // rows of no sequence
-        for (int w = 0; w < W; ++w) p.mask[(size_t)k * W + w] = 0ull;
-        p.positions[k] = 0;
-    }
+    auto nothing = [&](int from, int to) {             // rows of no sequence
+        for (int k = from + blockIdx.x * 64 * W + i; k < to; k += gridDim.x * 64 * W) {
+            for (int w = 0; w < W; ++w) p.mask[(size_t)k * W + w] = 0ull;
+            p.positions[k] = 0;
+        }
+    };
+    nothing(0, min(front, end));
+    nothing(end, p.tokens);
 }
 
 struct AcceptParams {

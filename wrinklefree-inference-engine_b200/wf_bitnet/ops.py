@@ -377,7 +377,7 @@ def paged_release(done: torch.Tensor, seq_lens: torch.Tensor, block_table: torch
 
 # ----------------------------------------------------------------------------------------- drafted tokens
 class TreePlan(NamedTuple):
-    """Masks and positions of a step's drafts (of rows behind the last sequence 0 and 0)."""
+    """Masks and positions of a step's drafts (of rows in front of the first sequence and behind the last one 0 and 0)."""
     mask: torch.Tensor          # int64 [T, ceil(max_nodes / 64)]: bit j for the draft at place j of the sequence, the row's own and those on its way up
     positions: torch.Tensor     # int32 [T] cached tokens + drafts above it
 
