@@ -154,8 +154,12 @@ __global__ void __launch_bounds__(AC_WARPS * 32) tree_accept_kernel(const __grid
             p.next[b] = kept ? want[last] : -1;
         }
     }
-    const int end = p.rows ? min(max(p.offsets[p.rows], 0), p.n_tokens) : 0;
-    for (int k = end + blockIdx.x * blockDim.x + threadIdx.x; k < p.n_tokens; k += gridDim.x * blockDim.x) p.path[k] = -1;
+    const int front = p.offsets[0], end = p.rows ? min(max(p.offsets[p.rows], 0), p.n_tokens) : 0;
+    auto nothing = [&](int from, int to) {             // rows of no sequence
+        for (int k = from + blockIdx.x * blockDim.x + threadIdx.x; k < to; k += gridDim.x * blockDim.x) p.path[k] = -1;
+    };
+    nothing(0, min(front, end));
+    nothing(end, p.n_tokens);
 }
 
 __device__ __forceinline__ int ac_blocks(int tokens, int page) { return (int)(((unsigned)tokens + page - 1) / page); }

@@ -405,7 +405,7 @@ def paged_tree_attn(q: torch.Tensor, kv: PagedKV, layer: int, block_table: torch
 class TreeAccept(NamedTuple):
     """What a verified step keeps, all int32."""
     accepted: torch.Tensor      # [B] drafts kept, the first one (the token drawn last) among them
-    path: torch.Tensor          # [T] from offsets[b] on: the places of the kept ones, -1 behind them
+    path: torch.Tensor          # [T] from offsets[b] on: the places of the kept ones, -1 behind them and in rows of no sequence
     next_tokens: torch.Tensor   # [B] drawn behind the last kept one (-1 for sequences without drafts)
     lens: torch.Tensor          # [B] seq_lens + accepted
     free_count: torch.Tensor    # [1] pages on the free list now
