@@ -310,7 +310,7 @@ int wf_token_logprobs(const void* logits, int dtype, int rows, int vocab, long l
  *   seen or drafted: x > 0 ? x / repetition[b] : x * repetition[b];
  *   - frequency[b] * (times drawn) - presence[b] where drawn;  + the last bias_values[b][i] with bias_ids[b][i] == v;  -inf where bit v % 32 of allowed[n][v / 32] is not set.
  * Rows of drafts (node_mask [rows][mask_words], at most 4 words; node_tokens [rows]): the tokens node_tokens[offsets[b] + j] of the bits j in node_mask[n] are drawn once each,
- * too.  Null pointers leave their part out; ids outside [0, vocab) are none.  Rows behind the last sequence are copied.  logits and out may be the same memory (with the same stride), or
+ * too.  Null pointers leave their part out; ids outside [0, vocab) are none.  Rows of no sequence (in front of the first one or behind the last) are copied.  logits and out may be the same memory (with the same stride), or
  * do not overlap.  At most 2^30 columns and rows, 65534 sequences, 65535 biases. */
 typedef struct wf_logits_args {
     const void* logits;        /* [rows][vocab] of dtype WF_F32, WF_BF16 or WF_F16, rows row_stride elements apart */

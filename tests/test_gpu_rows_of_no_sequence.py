@@ -1,8 +1,11 @@
 """Offsets that begin behind row 0: the rows in front of the first sequence are of no sequence, as those behind the last one are."""
+import math
+
 import numpy as np
 import pytest
 import torch
 
+from test_gpu_logits import case as logits_case
 from test_gpu_tree_plan import forest, i32
 
 pytestmark = pytest.mark.gpu
@@ -58,3 +61,48 @@ def test_acceptance(lead):
     for x, y in zip((a.accepted, a.next_tokens, a.lens, a.free_count, a.status), (want.accepted, want.next_tokens, want.lens, want.free_count, want.status)):
         assert torch.equal(x, y)
     assert torch.equal(kv.pool, kv0.pool) and torch.equal(free, free0) and int(a.status) == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("V", [1, 100, 1003, 32003, 140000])
+@pytest.mark.parametrize("rows", [[3], [2, 0, 5], [60, 1, 9]])
+@pytest.mark.parametrize("lead", [1, 7, 70])
+def test_logits(lead, rows, V, dtype):
+    """copied, whatever their masks say; in place left as they are"""
+    from wf_bitnet import ops
+    a = logits_case(rows, V, dtype, L=40, nodes=True, tail=2, seed=lead)
+    want = ops.process_logits(**a)
+    g = torch.Generator(device="cuda").manual_seed(lead)
+    more = dict(a)
+    more["logits"] = torch.cat([torch.randn(lead, V, generator=g, device="cuda").to(dtype), a["logits"]])
+    more["allowed"] = torch.cat([torch.zeros(lead, a["allowed"].shape[1], dtype=torch.int32, device="cuda"), a["allowed"]])
+    more["node_mask"] = torch.cat([torch.full((lead, a["node_mask"].shape[1]), -1, device="cuda"), a["node_mask"]])
+    more["node_tokens"] = torch.cat([torch.zeros(lead, dtype=torch.int32, device="cuda"), a["node_tokens"]])
+    more["offsets"] = a["offsets"] + lead
+    out = ops.process_logits(**more)
+    assert torch.equal(out[:lead], more["logits"][:lead]) and torch.equal(out[lead:], want)
+    out = ops.process_logits(**more, out=torch.full_like(out, math.nan))
+    assert torch.equal(out[:lead], more["logits"][:lead]) and torch.equal(out[lead:], want)
+    mine = more["logits"].clone()
+    ops.process_logits(**{**more, "logits": mine}, out=mine)
+    assert torch.equal(mine, out)
+
+
+def test_logits_of_no_sequence_at_all():
+    from wf_bitnet import ops
+    x = torch.randn(300, 999, device="cuda")
+    for offsets in ([0], [300], [9], [1000, 1000]):
+        assert torch.equal(ops.process_logits(x, offsets=i32(offsets), out=torch.full_like(x, math.nan)), x)
+
+
+def test_attention():
+    from test_gpu_tree_attn import case
+    from wf_bitnet import ops
+    a, _ = case([70, 3], [9, 30], 8, 2, 16, pad=0)
+    want = ops.paged_tree_attn(**a)
+    lead = 37
+    a["q"] = torch.cat([torch.randn(lead, 8, 128, device="cuda").to(torch.bfloat16), a["q"]])
+    a["mask"] = torch.cat([torch.full((lead, a["mask"].shape[1]), -1, device="cuda"), a["mask"]])
+    a["offsets"] = a["offsets"] + lead
+    out = ops.paged_tree_attn(**a)
+    assert not out[:lead].any() and torch.equal(out[lead:], want)

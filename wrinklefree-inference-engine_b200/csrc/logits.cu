@@ -78,17 +78,19 @@ __global__ void __launch_bounds__(LG_THREADS, LG_BLOCKS) process_logits_kernel(c
     const int s_lo = slice * p.slice, s_hi = min(a.vocab, s_lo + p.slice), per_row = (s_hi - s_lo + CHUNK - 1) / CHUNK;
     pdl_wait_prior();
     pdl_launch_dependents();
-    // this block's sequence (a.sequences: rows behind the last one), its rows first .. end, and its run of their chunks
+    // this block's sequence (a.sequences: rows behind the last one, a.sequences + 1: in front of the first one), its rows first .. end, and its run of their chunks
     int b, first, end, part;
     if (a.offsets) {
         int before = 0;                                // runs of the sequences in front
         b = -1;
-        for (int s0 = 0; s0 <= a.sequences; s0 += LG_THREADS) {
+        for (int s0 = 0; s0 <= a.sequences + 1; s0 += LG_THREADS) {
             const int s = s0 + tid;
             int from = 0, to = 0;
             if (s <= a.sequences) {
                 from = a.sequences > 0 ? min(max(a.offsets[s], 0), a.rows) : 0;
                 to = s < a.sequences ? max(min(a.offsets[s + 1], a.rows), from) : a.rows;
+            } else if (s == a.sequences + 1 && a.sequences > 0) {
+                to = min(max(a.offsets[0], 0), a.rows);
             }
             const int n = (int)(((long long)(to - from) * per_row + p.run - 1) / p.run);
             int in = n;
@@ -448,7 +450,7 @@ extern "C" int wf_process_logits(const wf_logits_args* args, void* stream) {
     const long long most = brings > LG_ENTRIES ? LG_ENTRIES : LG_SLICE;
     p.slice = (int)((a.vocab < most ? a.vocab : most) + 511) / 512 * 512;
     const long long slices = ((long long)a.vocab + p.slice - 1) / p.slice, per_row = (p.slice + chunk - 1) / chunk;
-    const long long seqs = a.offsets ? a.sequences + 1ll : a.sequences;
+    const long long seqs = a.offsets ? a.sequences + 2ll : a.sequences;            // (and the rows behind the last one, and in front of the first)
     const int full = lg_smem_bytes(bytes, p.slice, (int)(std::min(brings, (long long)p.slice) + 7) / 8 * 8, a.mask_words, a.bias_ids != nullptr);
     const long long wave = std::max((full + 6144 <= 113 * 1024 ? LG_BLOCKS : 1) * sm_count() / slices, 1ll);
     p.run = lg_run(a.rows, a.offsets && a.sequences ? a.sequences : seqs, per_row, wave, p.tables, !a.offsets);

@@ -459,7 +459,7 @@ def process_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = No
                    node_tokens: Optional[torch.Tensor] = None, node_mask: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Penalties, biases and grammar masks on logits (f32, bf16 or f16 [N, V], any row stride) before a token is drawn, in one pass; returns `out` (new memory, or the
     tensor given, which may be `logits` itself).  Row n is sequence n's, or with offsets (int32 [B + 1]) that of the sequence b whose rows offsets[b] to offsets[b + 1] it is
-    among (rows behind the last one are copied).  Of each sequence:
+    among (rows in front of the first one and behind the last are copied).  Of each sequence:
       history int32 [B, L], its first history_lens[b] tokens (None: L): the prompt's, up to prompt_lens[b] (None: none), and those drawn since.  Tokens in it: x / repetition[b]
       where x > 0, else x * repetition[b]; drawn ones also - frequency[b] * times - presence[b] (float32 [B] each).
       bias_ids int32 [B, n], bias_values float32 [B, n]: added; of entries of the same id the last one counts.
