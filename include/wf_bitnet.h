@@ -273,7 +273,7 @@ int wf_paged_tree_attn(const void* q, const wf_kv_layout* kv, int layer, const i
  * the last kept token go back on the stack free_pages[*free_count ..] of pool_pages entries (at most 2^30), sequence after sequence and block after block.  Where that cannot be
  * done as a whole, status has the WF_PLAN_* bits of why (PAGES: the stack would not hold them; BLOCKS, LENGTH: a sequence beyond max_blocks pages, more than 256 drafts, or
  * out of range; COUNT), nothing moves or is handed back, lens_out = seq_lens + the drafts and free_count_out = *free_count; accepted, path and next stand (sequences with more than
- * 256 drafts: none kept).  At most 8192 rows.  Rows of a head are a multiple of 16 bytes.  The pool is 16-byte aligned.  Outputs overlap neither one another nor the inputs. */
+ * 256 drafts: none kept).  Offsets rise; else the results mean nothing.  At most 8192 rows.  Rows of a head are a multiple of 16 bytes.  The pool is 16-byte aligned.  Outputs overlap neither one another nor the inputs. */
 int wf_tree_accept(const int32_t* parents, const int32_t* tokens, const int32_t* targets, const int32_t* offsets, const int32_t* seq_lens, int rows, int n_tokens,
                    const wf_kv_layout* kv, const int32_t* block_table, int max_blocks, int32_t* free_pages, int pool_pages, const int32_t* free_count, int32_t* accepted, int32_t* path,
                    int32_t* next_tokens, int32_t* lens_out, int32_t* free_count_out, int32_t* status, void* stream);

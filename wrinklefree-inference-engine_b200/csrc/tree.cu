@@ -224,7 +224,8 @@ __global__ void __launch_bounds__(AC_THREADS) tree_move_kernel(const __grid_cons
     tr_span(p.offsets, b, p.n_tokens, first, n);
     int moved = 0;
     for (int k = tid; k < kept; k += AC_THREADS) {
-        const int j = p.path[first + k];
+        int j = p.path[first + k];
+        if (j < k || j >= n) j = k;                    // (where offsets do not rise, another sequence may have written there: no place outside this one's drafts is looked up)
         path_s[k] = j;
         const int from = len + j, to = len + k;
         const int fp = p.table[(size_t)b * p.max_blocks + from / p.page_size], tp = p.table[(size_t)b * p.max_blocks + to / p.page_size];
