@@ -260,7 +260,8 @@ int wf_tree_plan(const int32_t* parents, const int32_t* offsets, const int32_t* 
  * [mask_words] (1 to 4; bits behind the last draft count for nothing; any pattern, not only a tree's).  out bf16 or f32 [tokens][H][D]; a row that sees no key, or none but of
  * -inf scores, gets zeros; so do rows behind the last sequence, and those of sequences with more than 64 mask_words drafts.  What a row does not see has no weight, whatever
  * it holds (NaN too).  Offsets rise; else the results mean nothing.  Weights enter their product with the values in bf16 (int8 pools: times the value's scale).  The tables' entries of
- * the tokens in range are pages of the pool (others read as zeros).  At most 65536 sequences, 2^24 rows of queries (tokens * H), and rows of block_table of 2^31 - 4096 tokens.  q, out, the pool
+ * the tokens in range are pages of the pool (others read as zeros).  head_dim 128, pages of a multiple of 16 tokens, bf16 or int8 pools, H a multiple of kv_heads and at most 8 times as
+ * many, as wf_paged_decode_attn has them.  A NaN in a query, or in a key that a row sees, makes the row NaN.  At most 65536 sequences, 2^24 rows of queries (tokens * H), and rows of block_table of 2^31 - 4096 tokens.  q, out, the pool
  * and the workspace are 16-byte aligned.  The workspace is free to be used again as soon as the stream has passed the call. */
 size_t wf_tree_attn_workspace_bytes(int B, int tokens, int H, int kv_heads, int mask_words);
 int wf_paged_tree_attn(const void* q, const wf_kv_layout* kv, int layer, const int32_t* block_table, int max_blocks, const int32_t* seq_lens, const int32_t* offsets,

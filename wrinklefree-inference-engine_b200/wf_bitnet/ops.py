@@ -394,7 +394,8 @@ def paged_tree_attn(q: torch.Tensor, kv: PagedKV, layer: int, block_table: torch
     """Attention of drafts over the paged cache: q bf16 [T, H, D], the rows of sequence b are offsets[b] to offsets[b + 1]; it has seq_lens[b] cached tokens and its
     drafts' keys and values behind them (norm_rope_kv_append or kv_scatter has put them there).  Row t sees every cached token, and the drafts whose bits mask[t] has
     (int64 [T, words], tree_plan's or any other pattern over up to 64 * words drafts, words <= 4).  A row that sees no key gets zeros, as do rows behind the last
-    sequence.  Weights are rounded to bf16 (over an int8 cache times the value's scale)."""
+    sequence.  Weights are rounded to bf16 (over an int8 cache times the value's scale).  Heads of 128, at most 8 query heads a key/value head, pages of a multiple of 16
+    tokens, bf16 and int8 caches, as paged_decode_attn; norm_rope_kv_append and tree_accept take more."""
     if out_dtype not in (torch.bfloat16, torch.float32):
         raise ValueError("out_dtype must be bfloat16 or float32")
     c = kv.c
