@@ -29,7 +29,7 @@ struct PxParams {
     float scale_log2e;
     float *part_o, *part_ml;       // [splits][Hkv][AT_D / 4][rows][4], [splits][Hkv][rows][2], rows = B * G up to the next multiple of 32
     int rows_p;                    // those rows
-    int box, stages;               // keys per TMA box (a power of two that divides the page); key and value tiles in flight
+    int box, stages;               // keys per TMA box (a power of two that divides the page); key and value tiles in flight (bf16 pools)
     int behind_own;                // the kernel before is this call's own part, which has waited for what both read
     int* err;                      // the wait word
 
@@ -248,7 +248,7 @@ extern "C" int wf_paged_prefix_attn(const void* q, const wf_kv_layout* kv, int l
         const bool i8 = p.scales != nullptr;
         p.box = 16;
         while (p.box < PX_KEYS && kv->page_size % (2 * p.box) == 0) p.box *= 2;
-        p.stages = i8 ? PX_STAGES8 : (PX_SMEM_USE - (rows <= PX_ROWS ? 1 : 2) * PX_QTILE) / (2 * PX_TILE);
+        p.stages = (PX_SMEM_USE - (rows <= PX_ROWS ? 1 : 2) * PX_QTILE) / (2 * PX_TILE);
         p.err = tc_wait_word();
         if (!p.err) { set_error("%s: no wait word", who); return WF_ERR_CUDA; }
         CUtensorMap tm;

@@ -49,7 +49,7 @@ constexpr int PX_STAGES = 4;
 constexpr int PX_SMEM_FULL = 224 * 1024, PX_STAGES_FULL = 6;           // the same of a block that shares its SM with no other
 // A block of the own part wants 64 KB and 168 registers a thread of the same SM.  Registers are had from quarters of an SM, three warps of this kernel and one of that
 // on each: (3 x 112 + 168) x 32 of 16384.  The softmax warps take 16 of what the others leave (at 112 for all they spill, 84 us instead of 73).
-constexpr int PX_THREADS = 12 * 32, PX_REGS = 112, PX_REGS_SOFTMAX = 128, PX_REGS_OTHERS = 80;         // (warp 11 only fills its warpgroup)
+constexpr int PX_THREADS = 12 * 32, PX_REGS = 112, PX_REGS_SOFTMAX = 128, PX_REGS_OTHERS = 80;         // (with int8 pools warp 11 only fills its warpgroup)
 static_assert(2 * PX_REGS_SOFTMAX + PX_REGS_OTHERS == 3 * PX_REGS, "the softmax warpgroups take what the third one gives");
 // int8 pools: a ring of tiles as they lie in the pool, and one of converted tiles with their scales
 constexpr int PX_RAW = 3, PX_RAW_TILE = 2 * PX_KEYS * AT_D, PX_SC = 2 * PX_KEYS * 4, PX_STAGES8 = 3;
@@ -156,7 +156,8 @@ __device__ __forceinline__ PxSeg px_seg(const PxWork& w, const P& p, uint32_t ba
     g.nt = (w.key1 - w.key0 + PX_KEYS - 1) / PX_KEYS;
     g.fix_row = w.key1 - w.key0 - (g.nt - 1) * PX_KEYS;
     const int queries = TREE && w.narrow ? 1 : 2;
-    g.nst = I8 ? PX_STAGES8 + 2 - queries : TREE ? PX_STAGES_FULL + 1 - queries : p.stages;
+    if constexpr (I8 || TREE) g.nst = (I8 ? PX_STAGES8 + 1 : PX_STAGES_FULL) + 1 - queries;
+    else g.nst = p.stages;
     g.hop = g.alt ? 2 : 1;
     g.q_s = base;
     g.k_s = I8 || TREE ? base + queries * PX_QTILE : base + PX_SMEM_USE - 2 * g.nst * PX_TILE;

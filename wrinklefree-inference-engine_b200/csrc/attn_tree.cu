@@ -61,7 +61,7 @@ struct TxParams {
     int rows_p;
     void* out;
     int out_dtype;
-    int box, stages;
+    int box;
     int* err;
 
     __device__ __forceinline__ TxSeq seq(int b) const {
@@ -430,7 +430,6 @@ extern "C" int wf_paged_tree_attn(const void* q, const wf_kv_layout* kv, int lay
     p.out = out; p.out_dtype = out_dtype;
     p.box = 16;
     while (p.box < PX_KEYS && kv->page_size % (2 * p.box) == 0) p.box *= 2;
-    p.stages = PX_STAGES8;
     p.err = tc_wait_word();
     if (!p.err) { set_error("%s: no wait word", who); return WF_ERR_CUDA; }
     CUtensorMap tm;

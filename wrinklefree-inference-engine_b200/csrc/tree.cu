@@ -24,7 +24,7 @@ constexpr int TR_WORDS = TR_MAX / 64;
 
 struct TreePlanParams {
     const int32_t *parents, *offsets, *seq;
-    int rows, tokens, words, max_nodes;
+    int rows, tokens, max_nodes;
     u64* mask;
     int32_t* positions;
 };
@@ -280,16 +280,17 @@ extern "C" int wf_tree_plan(const int32_t* parents, const int32_t* offsets, cons
     if (tokens == 0) return WF_OK;
     if (!mask || !positions || !offsets || (rows > 0 && (!parents || !seq_lens))) { set_error("%s: null pointer", who); return WF_ERR_INVALID; }
     if ((uintptr_t)mask & 7) { set_error("%s: the mask must be 8-byte aligned", who); return WF_ERR_INVALID; }
+    const int words = (max_nodes + 63) / 64;
     TreePlanParams p = {};
-    p.parents = parents; p.offsets = offsets; p.seq = seq_lens; p.rows = rows; p.tokens = tokens; p.max_nodes = max_nodes; p.words = (max_nodes + 63) / 64;
+    p.parents = parents; p.offsets = offsets; p.seq = seq_lens; p.rows = rows; p.tokens = tokens; p.max_nodes = max_nodes;
     p.mask = (u64*)mask; p.positions = positions;
     if (rows == 0) {                                   // no sequence: rows of none
-        if (int rc = cuda_check(cudaMemsetAsync(mask, 0, (size_t)tokens * p.words * 8, (cudaStream_t)stream), who)) return rc;
+        if (int rc = cuda_check(cudaMemsetAsync(mask, 0, (size_t)tokens * words * 8, (cudaStream_t)stream), who)) return rc;
         return cuda_check(cudaMemsetAsync(positions, 0, (size_t)tokens * 4, (cudaStream_t)stream), who);
     }
     cudaStream_t s = (cudaStream_t)stream;
     const dim3 grid((unsigned)rows);
-    switch (p.words) {
+    switch (words) {
         case 1: return launch_check(launch_pdl(tree_plan_kernel<1>, grid, 64, 0, s, p), who);
         case 2: return launch_check(launch_pdl(tree_plan_kernel<2>, grid, 128, 0, s, p), who);
         case 3: return launch_check(launch_pdl(tree_plan_kernel<3>, grid, 192, 0, s, p), who);
