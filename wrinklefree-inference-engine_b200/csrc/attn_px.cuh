@@ -352,7 +352,7 @@ __device__ __forceinline__ void px_block(const CUtensorMap& tmap, const P& p, un
             __syncwarp();
             slot += PX_KEYS;
             // the first share's other tiles wait until the queries are there, which would queue behind them (the ring's first filling takes all SMs' bandwidth); not a tree's bf16
-            // tiles, whose block has more shares to come (48 sequences of 12 drafts: 134 us, waiting 136; int8, waiting, 200 for 205)
+            // tiles, whose block has more shares to come (48 sequences of 12 drafts: 134 us, waiting 136; over int8 pools waiting took 31 sequences of 25 from 205 to 200 when it was tried)
             if (i == 1 && sh == 0 && (!TREE || I8)) { px_wait_warp(&q_full[g.alt ? 2 : 0], 0); if (!g.alt) px_wait_warp(&q_full[1], 0); }
             at_ring.step(1, depth);
             if (tail && !waiting++) first_st = st;

@@ -9,7 +9,7 @@
 // is written straight to the output; of the others every block has at most two, one that it ends and one that it begins, whose results go to its two parts of the
 // workspace, and the second kernel joins them.  (A block per tile and split instead, in waves, with 10 us a block before its first product and behind its last, against 4 us from
 // one tile to the next: 48 sequences of 12 drafts over up to 4096 keys 177 us instead of 134, 8 of 250 over up to 16384 with 64 heads 670 instead of 629, 31 of 25 over int8 241
-// instead of 213, now 207.)
+// instead of 213; with what came since, 193.)
 //
 // Bound by the memory where rows are few (the 48: 0.73 us for a tile of 64 keys an SM, 6.4 TB/s), by a tile's softmax and the products' turns on the tensor cores where there are
 // 256 (1500 of 2000 clocks are exponentials, maxima and sums), by the conversion of codes for int8 pools (1650).
